@@ -63,3 +63,84 @@ def _fwd_backward(ctx, dY, dmeans, drstds):
 
 
 torch.library.register_autograd("gnb200::fwd", _fwd_backward, setup_context=_fwd_setup_context)
+
+
+# ---------------------------------------------------------------------------------------------- token rows
+
+
+def _none_of(t):
+    return t.new_empty((0,))
+
+
+@torch.library.register_fake("gnb200::rms_fwd")
+def _rms_fwd_fake(x, residual, weight, eps, offset):
+    s = _none_of(x) if residual is None else torch.empty_like(residual, memory_format=torch.contiguous_format)
+    return torch.empty_like(x, memory_format=torch.contiguous_format), s, x.new_empty(x.shape[:-1], dtype=torch.float32)
+
+
+@torch.library.register_fake("gnb200::rms_bwd")
+def _rms_bwd_fake(dy, dsum, sum, weight, rstd, offset):
+    ds = _none_of(sum) if sum.dtype == dy.dtype else torch.empty_like(sum, memory_format=torch.contiguous_format)
+    return torch.empty_like(dy, memory_format=torch.contiguous_format), ds, _none_of(sum) if weight is None else torch.empty_like(weight)
+
+
+@torch.library.register_fake("gnb200::rms_quant")
+def _rms_quant_fake(x, residual, weight, eps, offset, block, format):
+    q = x.new_empty(x.shape, dtype=torch.float8_e4m3fn if format == 0 else torch.int8)
+    scales = (x.shape[-1] + block - 1) // block if block else 1
+    s = _none_of(x) if residual is None else torch.empty_like(residual, memory_format=torch.contiguous_format)
+    return q, x.new_empty(x.shape[:-1] + (scales,), dtype=torch.float32), s
+
+
+@torch.library.register_fake("gnb200::rotary")
+def _rotary_fake(q, k, positions, inv_freq, sections, q_weight, k_weight, eps, offset, interleaved):
+    contiguous = torch.contiguous_format
+    return torch.empty_like(q, memory_format=contiguous), _none_of(q) if k is None else torch.empty_like(k, memory_format=contiguous)
+
+
+@torch.library.register_fake("gnb200::rotary_bwd")
+def _rotary_bwd_fake(dq, dk, q, k, positions, inv_freq, sections, q_weight, k_weight, eps, offset, interleaved):
+    contiguous = torch.contiguous_format
+    return (torch.empty_like(dq, memory_format=contiguous), _none_of(dq) if dk is None else torch.empty_like(dk, memory_format=contiguous),
+            _none_of(dq) if q_weight is None else torch.empty_like(q_weight), _none_of(dq) if k_weight is None else torch.empty_like(k_weight))
+
+
+def _rms_setup_context(ctx, inputs, output):
+    x, residual, weight, _, offset = inputs
+    _, s, rstd = output
+    ctx.has_residual = residual is not None
+    ctx.offset = offset
+    ctx.save_for_backward(s if ctx.has_residual else x, weight, rstd)
+    ctx.mark_non_differentiable(rstd) if ctx.has_residual else ctx.mark_non_differentiable(rstd, s)
+
+
+def _rms_backward(ctx, dy, ds, drstd):
+    s, weight, rstd = ctx.saved_tensors
+    dx, dres, dw = torch.ops.gnb200.rms_bwd(dy, ds if ctx.has_residual else None, s, weight, rstd, ctx.offset)
+    if not ctx.has_residual:
+        dres = None
+    elif s.dtype == dx.dtype:
+        dres = dx
+    return dx, dres, None if weight is None else dw, None, None
+
+
+torch.library.register_autograd("gnb200::rms_fwd", _rms_backward, setup_context=_rms_setup_context)
+
+
+def _rotary_setup_context(ctx, inputs, output):
+    q, k, positions, inv_freq, ctx.sections, q_weight, k_weight, ctx.eps, ctx.offset, ctx.interleaved = inputs
+    ctx.has_k = k is not None
+    ctx.save_for_backward(q, k, positions, inv_freq, q_weight, k_weight)
+    if not ctx.has_k:
+        ctx.mark_non_differentiable(output[1])
+
+
+def _rotary_backward(ctx, dq, dk):
+    q, k, positions, inv_freq, q_weight, k_weight = ctx.saved_tensors
+    gq, gk, gqw, gkw = torch.ops.gnb200.rotary_bwd(dq, dk if ctx.has_k else None, q, k, positions, inv_freq, ctx.sections, q_weight, k_weight,
+                                                   ctx.eps, ctx.offset, ctx.interleaved)
+    return (gq, gk if ctx.has_k else None, None, None, None, None if q_weight is None else gqw, None if k_weight is None else gkw,
+            None, None, None)
+
+
+torch.library.register_autograd("gnb200::rotary", _rotary_backward, setup_context=_rotary_setup_context)

@@ -93,6 +93,38 @@ lib.gnb200_describe_plan.argtypes = [_c_int64, _c_int64, _c_int64, _c_int64, cty
 lib.gnb200_launch_count.restype = ctypes.c_int
 lib.gnb200_launch_count.argtypes = [_c_int64, _c_int64, _c_int64, _c_int64, ctypes.c_int, ctypes.c_int]
 
+QUANT_E4M3, QUANT_INT8 = 0, 1
+POS_CODES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+_c_int = ctypes.c_int
+_c_double = ctypes.c_double
+lib.gnb200_rms_fwd.restype = _c_int
+lib.gnb200_rms_fwd.argtypes = [_c_void_p, _c_int64, _c_void_p, _c_int64, _c_void_p, _c_int64, _c_int64, _c_double, _c_double, _c_int, _c_int,
+                               _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p]
+lib.gnb200_rms_fwd_8bit.restype = _c_int
+lib.gnb200_rms_fwd_8bit.argtypes = lib.gnb200_rms_fwd.argtypes[:12] + [_c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p]
+lib.gnb200_rms_bwd_workspace_bytes.restype = ctypes.c_size_t
+lib.gnb200_rms_bwd_workspace_bytes.argtypes = [_c_int64, _c_int64, _c_int, _c_int]
+lib.gnb200_rms_bwd.restype = _c_int
+lib.gnb200_rms_bwd.argtypes = [_c_void_p, _c_int64, _c_void_p, _c_int64, _c_void_p, _c_int64, _c_void_p, _c_void_p, _c_int64, _c_int64, _c_double,
+                               _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, ctypes.c_size_t, _c_void_p]
+
+
+class RotaryArgs(ctypes.Structure):
+    """gnb200_rotary_args"""
+    _fields_ = [("batch", _c_int64), ("tokens", _c_int64), ("q_heads", _c_int64), ("k_heads", _c_int64), ("head_dim", _c_int64),
+                ("positions", _c_void_p), ("pos_stride", _c_int64 * 3), ("pos_type", _c_int), ("axes", _c_int), ("sections", _c_int * 8),
+                ("inv_freq", _c_void_p), ("q_weight", _c_void_p), ("k_weight", _c_void_p), ("q_weight_dtype", _c_int),
+                ("k_weight_dtype", _c_int), ("eps", _c_double), ("offset", _c_double), ("interleaved", _c_int), ("dtype", _c_int)]
+
+
+_c_strides = ctypes.POINTER(_c_int64)
+lib.gnb200_rotary_fwd.restype = _c_int
+lib.gnb200_rotary_fwd.argtypes = [ctypes.POINTER(RotaryArgs), _c_void_p, _c_strides, _c_void_p, _c_strides, _c_void_p, _c_void_p, _c_void_p]
+lib.gnb200_rotary_bwd_workspace_bytes.restype = ctypes.c_size_t
+lib.gnb200_rotary_bwd_workspace_bytes.argtypes = [ctypes.POINTER(RotaryArgs)]
+lib.gnb200_rotary_bwd.restype = _c_int
+lib.gnb200_rotary_bwd.argtypes = [ctypes.POINTER(RotaryArgs)] + [_c_void_p, _c_strides] * 4 + [_c_void_p] * 5 + [ctypes.c_size_t, _c_void_p]
+
 
 class Gnb200Error(RuntimeError):
     """A C-ABI call returned a non-zero status."""

@@ -23,8 +23,9 @@ CORE_LIB = os.path.join(LIB_DIR, "libgnb200.so")
 TORCH_LIB = os.path.join(LIB_DIR, "gnb200_torch.so")
 PYTHON_LIB = os.path.join(LIB_DIR, "gnb200_python.so")
 
-CUDA_SOURCES = ["gn_fwd.cu", "gn_bwd.cu", "gn_wave.cu", "gn_resident.cu", "gn_nchw.cu", "gn_f64.cu", "gn_plan.cu", "gn_capi.cu", "gn_static_scratch.cu"]
-CUDA_HEADERS = ["gn_common.cuh", "gn_math.cuh", "gn_async.cuh", "gn_reduce.cuh", "gn_peer.cuh", "gn_kernels.h", os.path.join(INCLUDE_DIR, "gnb200.h")]
+CUDA_SOURCES = ["gn_fwd.cu", "gn_bwd.cu", "gn_wave.cu", "gn_resident.cu", "gn_nchw.cu", "gn_f64.cu", "gn_rms.cu", "gn_rotary.cu", "gn_plan.cu", "gn_capi.cu", "gn_static_scratch.cu"]
+TORCH_SOURCES = ["gn_torch.cpp", "gn_torch_tokens.cpp"]
+CUDA_HEADERS = ["gn_common.cuh", "gn_math.cuh", "gn_async.cuh", "gn_reduce.cuh", "gn_peer.cuh", "gn_tokens.cuh", "gn_kernels.h", os.path.join(INCLUDE_DIR, "gnb200.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC"]
 
@@ -67,7 +68,7 @@ def _core_digest():
 
 
 def _torch_digest():
-    return _digest(["gn_torch.cpp", "gn_torch.h", os.path.join(INCLUDE_DIR, "gnb200.h")])
+    return _digest(TORCH_SOURCES + ["gn_torch.h", os.path.join(INCLUDE_DIR, "gnb200.h")])
 
 
 def _python_digest():
@@ -113,7 +114,7 @@ def build_core(verbose=False, extra_flags=()):
     return CORE_LIB
 
 
-def _build_binding(source, lib_path, libs, verbose):
+def _build_binding(sources, lib_path, libs, verbose):
     from torch.utils import cpp_extension as ce
 
     os.makedirs(LIB_DIR, exist_ok=True)
@@ -122,7 +123,7 @@ def _build_binding(source, lib_path, libs, verbose):
     for p in ce.include_paths() + [sysconfig.get_paths()["include"], os.path.join(cuda_home, "include")]:
         inc += ["-isystem", p]
     torch_lib = ce.library_paths()[0]
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", os.path.join(CSRC, source), "-o", lib_path,
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared"] + [os.path.join(CSRC, s) for s in sources] + ["-o", lib_path,
            "-DTORCH_API_INCLUDE_EXTENSION_H"] + inc + [
         "-L", torch_lib, "-L", LIB_DIR] + libs + ["-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + torch_lib]
     if verbose:
@@ -131,13 +132,13 @@ def _build_binding(source, lib_path, libs, verbose):
 
 
 def build_torch(verbose=False):
-    _build_binding("gn_torch.cpp", TORCH_LIB, ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-lgnb200"], verbose)
+    _build_binding(TORCH_SOURCES, TORCH_LIB, ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-lgnb200"], verbose)
     _write_stamp(TORCH_LIB, _torch_digest())
     return TORCH_LIB
 
 
 def build_python(verbose=False):
-    _build_binding("gn_python.cpp", PYTHON_LIB, ["-lc10", "-ltorch_cpu", "-ltorch_python", "-l:gnb200_torch.so"], verbose)
+    _build_binding(["gn_python.cpp"], PYTHON_LIB, ["-lc10", "-ltorch_cpu", "-ltorch_python", "-l:gnb200_torch.so"], verbose)
     _write_stamp(PYTHON_LIB, _python_digest())
     return PYTHON_LIB
 

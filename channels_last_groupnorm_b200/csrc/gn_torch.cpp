@@ -280,16 +280,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> call_fwd(const at::Tensor& X, con
 // transform, tracer, lazy negation, profiler) and its tensor has the storage order that the kernels want; every other call
 // goes through the ops as before.  The kernels, their arguments and the results' sizes and strides are the same.
 // ------------------------------------------------------------------------------------------------
-bool only_cuda_sees(std::initializer_list<const at::Tensor*> tensors) {
-  static const c10::DispatchKeySet allowed =
-      c10::autograd_dispatch_keyset_with_ADInplaceOrView | c10::autocast_dispatch_keyset |
-      c10::DispatchKeySet({c10::DispatchKey::BackendSelect, c10::DispatchKey::CUDA, c10::DispatchKey::AutogradCUDA});
-  c10::DispatchKeySet ks;
-  for (const at::Tensor* t : tensors) ks = ks | t->key_set();
-  const auto tls = c10::impl::tls_local_dispatch_key_set();
-  ks = (ks | tls.included_) - tls.excluded_;
-  return (ks.raw_repr() & ~allowed.raw_repr()) == 0 && !at::hasCallbacks();
-}
+using gnb200_ops::only_cuda_sees;
 
 // Storage of a plain tensor of rank >= 3, by the rules of flatten() and layout_of(); false where it would be copied.
 struct Dense {
@@ -510,6 +501,17 @@ at::Tensor group_norm_act_plain(const at::Tensor& X, const at::Tensor& weight, c
 }
 
 }  // namespace
+
+bool gnb200_ops::only_cuda_sees(std::initializer_list<const at::Tensor*> tensors) {
+  static const c10::DispatchKeySet allowed =
+      c10::autograd_dispatch_keyset_with_ADInplaceOrView | c10::autocast_dispatch_keyset |
+      c10::DispatchKeySet({c10::DispatchKey::BackendSelect, c10::DispatchKey::CUDA, c10::DispatchKey::AutogradCUDA});
+  c10::DispatchKeySet ks;
+  for (const at::Tensor* t : tensors) ks = ks | t->key_set();
+  const auto tls = c10::impl::tls_local_dispatch_key_set();
+  ks = (ks | tls.included_) - tls.excluded_;
+  return (ks.raw_repr() & ~allowed.raw_repr()) == 0 && !at::hasCallbacks();
+}
 
 at::Tensor gnb200_ops::group_norm_act_direct(const at::Tensor& X, const at::Tensor& weight, const at::Tensor& bias, int64_t G,
                                              double eps, int64_t act) {

@@ -224,6 +224,72 @@ int gnb200_allreduce_param_grads(float* dgamma_dbeta_f32, void* dgamma, void* db
                                  const void* const* peer_bufs, int rank, int world, void* stream);
 
 /*
+ * Token rows: what stands around the attention and feed-forward blocks of transformers.  No counterparts in the reference.
+ * Rows are C contiguous elements; a row stride (in elements) may be larger, as for slices of a wider tensor.  Pointers that are
+ * 16-byte aligned, with strides and C that are multiples of a 16-byte vector, take the vector kernels, all others single elements.
+ * Types are those of x: GNB200_F32 / F16 / BF16; the residual (and `sum`) and the weight may be fp32 beside 16-bit x.
+ *
+ * gnb200_rms_fwd: root-mean-square norm with the residual's addition.
+ *   s = x + residual (residual may be NULL: s = x), y = s * rstd * (offset + weight) (weight may be NULL: y = s * rstd),
+ *   rstd = 1 / sqrt(mean(s^2) + eps) per row.  Writes y (contiguous), `sum` = s rounded once to the residual's type (contiguous, only
+ *   with a residual) and rstd (rows floats, may be NULL).  s is not rounded before the norm.
+ * gnb200_rms_fwd_8bit: the same with y as 8-bit codes q and fp32 scales, y = q * scale: scale = max |y| / 448 (e4m3) or / 127
+ *   (int8), at least 2^-126, one per row (block 0: `rows` floats) or per block of 32, 64 or 128 channels (rows x ceil(C / block)
+ *   floats).  A NaN makes the scale of its block NaN.
+ * gnb200_rms_bwd: dy and, where the sum was used, dsum (may be NULL) are the gradients of y and sum; `sum` is what the forward
+ *   stored, or x where there was no residual.  With n = sum * rstd and g = dy * (offset + weight) it writes
+ *   d = dsum + rstd * (g - n * mean(g * n)), the gradient of x and of the residual, to dx in dy's type and, where the sum has
+ *   another type, to dsum_out in the sum's (NULL otherwise); and dweight = sum over rows of dy * n (NULL: not wanted) in the
+ *   weight's type, added in a fixed order.  The workspace is needed only for dweight.
+ */
+enum { GNB200_E4M3 = 0, GNB200_INT8 = 1 };
+int gnb200_rms_fwd(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight,
+                   int64_t rows, int64_t C, double eps, double offset, int dtype, int residual_dtype, int weight_dtype,
+                   void* y, void* sum, float* rstd, void* stream);
+int gnb200_rms_fwd_8bit(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight,
+                        int64_t rows, int64_t C, double eps, double offset, int dtype, int residual_dtype, int weight_dtype,
+                        int block, int format, void* q, float* scale, void* sum, void* stream);
+size_t gnb200_rms_bwd_workspace_bytes(int64_t rows, int64_t C, int dtype, int sum_dtype);
+int gnb200_rms_bwd(const void* dy, int64_t dy_stride, const void* dsum, int64_t dsum_stride, const void* sum,
+                   int64_t sum_stride, const void* weight, const float* rstd, int64_t rows, int64_t C, double offset,
+                   int dtype, int sum_dtype, int weight_dtype, void* dx, void* dsum_out, void* dweight,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Rotary positions with several axes on queries and keys (batch x tokens x heads x head_dim, any strides with contiguous
+ * channels), with the root-mean-square norm of each head in front where there is a weight: n = x * rstd * (offset + weight),
+ * rstd over the head's channels; q and k each have a weight or none.  The first 2 * pairs channels of a head are turned, pairs = the
+ * sum of the sections; pair i is channels (i, i + pairs), or (2 i, 2 i + 1) where interleaved, and turns by
+ * position[axis] * inv_freq[i], the first sections[0] pairs by axis 0, the next sections[1] by axis 1, and so on.  The other
+ * channels pass.  Outputs are contiguous, of the inputs' type.  Strides are those of batch, token and head, in elements; of the
+ * positions, of batch, token and axis.  A tensor with 0 heads is left out.
+ * gnb200_rotary_bwd: dq, dk are the gradients of the outputs; q and k (what the forward got) are read only where there is a weight,
+ * whose gradients (in its type, in a fixed order) then need the workspace.
+ */
+enum { GNB200_POS_I32 = 0, GNB200_POS_I64 = 1, GNB200_POS_F32 = 2 };
+typedef struct gnb200_rotary_args {
+  int64_t batch, tokens, q_heads, k_heads, head_dim;
+  const void* positions;
+  int64_t pos_stride[3];
+  int pos_type;
+  int axes;         /* 1 .. 8 */
+  int sections[8];  /* pairs of each axis */
+  const float* inv_freq;
+  const void *q_weight, *k_weight; /* NULL: no norm */
+  int q_weight_dtype, k_weight_dtype;
+  double eps, offset;
+  int interleaved;
+  int dtype;
+} gnb200_rotary_args;
+int gnb200_rotary_fwd(const gnb200_rotary_args* args, const void* q, const int64_t* q_stride, const void* k,
+                      const int64_t* k_stride, void* q_out, void* k_out, void* stream);
+size_t gnb200_rotary_bwd_workspace_bytes(const gnb200_rotary_args* args);
+int gnb200_rotary_bwd(const gnb200_rotary_args* args, const void* dq, const int64_t* dq_stride, const void* dk,
+                      const int64_t* dk_stride, const void* q, const int64_t* q_stride, const void* k, const int64_t* k_stride,
+                      void* dq_out, void* dk_out, void* dq_weight, void* dk_weight, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/*
  * Describes the launch plan chosen for a problem ("fwd fused k=4 cw=64 ..."; the plans are fused,
  * twopass, wave and resident, the last with the plan that takes over where its grid cannot be
  * resident: "fallback=twopass"), for logs, tests and benchmarks.  Writes at most buf_len bytes including the terminating NUL; returns the
