@@ -79,7 +79,7 @@ def _rms_fwd_fake(x, residual, weight, eps, offset):
 
 
 @torch.library.register_fake("gnb200::rms_bwd")
-def _rms_bwd_fake(dy, dsum, sum, weight, rstd, offset):
+def _rms_bwd_fake(dy, dsum, sum, addend, weight, rstd, offset):
     ds = _none_of(sum) if sum.dtype == dy.dtype else torch.empty_like(sum, memory_format=torch.contiguous_format)
     return torch.empty_like(dy, memory_format=torch.contiguous_format), ds, _none_of(sum) if weight is None else torch.empty_like(weight)
 
@@ -110,13 +110,15 @@ def _rms_setup_context(ctx, inputs, output):
     _, s, rstd = output
     ctx.has_residual = residual is not None
     ctx.offset = offset
-    ctx.save_for_backward(s if ctx.has_residual else x, weight, rstd)
+    # (as the native node: x and the residual again where the stored sum is rounded and the weight's gradient wanted)
+    again = ctx.has_residual and residual.dtype != torch.float32 and weight is not None and weight.requires_grad
+    ctx.save_for_backward(residual if again else s if ctx.has_residual else x, x if again else None, weight, rstd)
     ctx.mark_non_differentiable(rstd) if ctx.has_residual else ctx.mark_non_differentiable(rstd, s)
 
 
 def _rms_backward(ctx, dy, ds, drstd):
-    s, weight, rstd = ctx.saved_tensors
-    dx, dres, dw = torch.ops.gnb200.rms_bwd(dy, ds if ctx.has_residual else None, s, weight, rstd, ctx.offset)
+    s, addend, weight, rstd = ctx.saved_tensors
+    dx, dres, dw = torch.ops.gnb200.rms_bwd(dy, ds if ctx.has_residual else None, s, addend, weight, rstd, ctx.offset)
     if not ctx.has_residual:
         dres = None
     elif s.dtype == dx.dtype:

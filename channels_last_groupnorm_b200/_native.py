@@ -105,7 +105,7 @@ lib.gnb200_rms_fwd_8bit.argtypes = lib.gnb200_rms_fwd.argtypes[:12] + [_c_int, _
 lib.gnb200_rms_bwd_workspace_bytes.restype = ctypes.c_size_t
 lib.gnb200_rms_bwd_workspace_bytes.argtypes = [_c_int64, _c_int64, _c_int, _c_int]
 lib.gnb200_rms_bwd.restype = _c_int
-lib.gnb200_rms_bwd.argtypes = [_c_void_p, _c_int64, _c_void_p, _c_int64, _c_void_p, _c_int64, _c_void_p, _c_void_p, _c_int64, _c_int64, _c_double,
+lib.gnb200_rms_bwd.argtypes = [_c_void_p, _c_int64, _c_void_p, _c_int64, _c_void_p, _c_int64, _c_void_p, _c_int64, _c_void_p, _c_void_p, _c_int64, _c_int64, _c_double,
                                _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, ctypes.c_size_t, _c_void_p]
 
 

@@ -288,11 +288,11 @@ __global__ void __launch_bounds__(kMostThreads) rms_fwd_any_kernel(const RmsFwd 
 // Backward
 // ---------------------------------------------------------------------------------------------
 struct RmsBwd {
-  const void *dy, *dsum, *sum, *weight;
+  const void *dy, *dsum, *sum, *addend, *weight;  // s = sum, or sum + addend (dy's type) where the stored sum was rounded to 16 bits
   const float* rstd;
   void *dx, *dsum_out;  // the same gradient in dy's type and, where sum has another type, in sum's
   float* part;          // one row of C floats per CTA, or NULL
-  long long rows, dy_stride, ds_stride, s_stride;
+  long long rows, dy_stride, ds_stride, s_stride, a_stride;
   int C, lanes, w_dtype;
   float offset, inv_c;
 };
@@ -308,13 +308,15 @@ __global__ void __launch_bounds__(WARP ? kWarpThreads : kMostThreads) rms_bwd_ke
   long long row = blockIdx.x * per_cta + (WARP ? (int)threadIdx.x / lanes : 0);
   grid_dep_launch_dependents();
   const Tx* dy = static_cast<const Tx*>(p.dy);
+  const Tx* add = static_cast<const Tx*>(p.addend);
   const Ts *ds = static_cast<const Ts*>(p.dsum), *sum = static_cast<const Ts*>(p.sum);
-  Pack<Tx, VE> yv[V];
+  Pack<Tx, VE> yv[V], av[V];
   Pack<Ts, VE> sv[V], dv[V];
   float rn = 0.f;
   auto ask = [&](long long at) {
     fetch<Tx, VE, V>(yv, dy + at * p.dy_stride, first, lanes, nvec);
     fetch<Ts, VE, V>(sv, sum + at * p.s_stride, first, lanes, nvec);
+    if (add) fetch<Tx, VE, V>(av, add + at * p.a_stride, first, lanes, nvec);
     if (ds) fetch<Ts, VE, V>(dv, ds + at * p.ds_stride, first, lanes, nvec);
     rn = p.rstd[at];
   };
@@ -338,6 +340,12 @@ __global__ void __launch_bounds__(WARP ? kWarpThreads : kMostThreads) rms_bwd_ke
       if (live && first + v * lanes < nvec) {
         unpack<Tx, VE>(yv[v], g[v]);
         unpack<Ts, VE>(sv[v], n[v]);
+        if (add) {
+          float f[VE];
+          unpack<Tx, VE>(av[v], f);
+#pragma unroll
+          for (int e = 0; e < VE; ++e) n[v][e] += f[e];
+        }
         if (ds) unpack<Ts, VE>(dv[v], d[v]);
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
@@ -400,9 +408,10 @@ __global__ void __launch_bounds__(kMostThreads) rms_bwd_any_kernel(const RmsBwd 
     const Tx* dy = static_cast<const Tx*>(p.dy) + row * p.dy_stride;
     const Ts* sum = static_cast<const Ts*>(p.sum) + row * p.s_stride;
     const Ts* ds = p.dsum ? static_cast<const Ts*>(p.dsum) + row * p.ds_stride : nullptr;
+    const Tx* add = p.addend ? static_cast<const Tx*>(p.addend) + row * p.a_stride : nullptr;
     const float rstd = p.rstd[row];
     auto g_at = [&](int i) { return load_param<Tx>(dy, i) * (p.weight ? p.offset + param_at(p.weight, p.w_dtype, i, 1.f) : 1.f); };
-    auto n_at = [&](int i) { return load_param<Ts>(sum, i) * rstd; };
+    auto n_at = [&](int i) { return (load_param<Ts>(sum, i) + (add ? load_param<Tx>(add, i) : 0.f)) * rstd; };
     float dot = 0.f;
     for (int i = threadIdx.x; i < p.C; i += blockDim.x) dot = fmaf(g_at(i), n_at(i), dot);
     const float c = cta_sum(dot, slots, turn) * p.inv_c;
@@ -417,9 +426,11 @@ __global__ void __launch_bounds__(kMostThreads) rms_bwd_any_kernel(const RmsBwd 
   // (a second look at the CTA's own rows, one channel per thread)
   for (int i = threadIdx.x; i < p.C; i += blockDim.x) {
     float t = 0.f;
-    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x)
-      t = fmaf(load_param<Tx>(static_cast<const Tx*>(p.dy) + row * p.dy_stride, i),
-               load_param<Ts>(static_cast<const Ts*>(p.sum) + row * p.s_stride, i) * p.rstd[row], t);
+    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+      float s = load_param<Ts>(static_cast<const Ts*>(p.sum) + row * p.s_stride, i);
+      if (p.addend) s += load_param<Tx>(static_cast<const Tx*>(p.addend) + row * p.a_stride, i);
+      t = fmaf(load_param<Tx>(static_cast<const Tx*>(p.dy) + row * p.dy_stride, i), s * p.rstd[row], t);
+    }
     p.part[(long long)blockIdx.x * p.C + i] = t;
   }
 }
@@ -646,7 +657,7 @@ size_t gnb200_rms_bwd_workspace_bytes(int64_t rows, int64_t C, int dtype, int su
 }
 
 int gnb200_rms_bwd(const void* dy, int64_t dy_stride, const void* dsum, int64_t dsum_stride, const void* sum, int64_t sum_stride,
-                   const void* weight, const float* rstd, int64_t rows, int64_t C, double offset, int dtype, int sum_dtype,
+                   const void* addend, int64_t addend_stride, const void* weight, const float* rstd, int64_t rows, int64_t C, double offset, int dtype, int sum_dtype,
                    int weight_dtype, void* dx, void* dsum_out, void* dweight, void* workspace, size_t workspace_bytes, void* stream) {
   const char* name = "gnb200_rms_bwd";
   if (!weight) weight_dtype = dtype;
@@ -661,12 +672,13 @@ int gnb200_rms_bwd(const void* dy, int64_t dy_stride, const void* dsum, int64_t 
   if (dsum_out && sum_dtype == dtype)
     return report_error(GNB200_ERR_INVALID_ARGUMENT, "%s: dsum_out is for a sum of another type than dy", name);
   RmsBwd p = {};
-  p.dy = dy, p.dsum = dsum, p.sum = sum, p.weight = weight, p.rstd = rstd, p.dx = dx, p.dsum_out = dsum_out;
-  p.rows = rows, p.dy_stride = dy_stride, p.ds_stride = dsum_stride, p.s_stride = sum_stride;
+  p.dy = dy, p.dsum = dsum, p.sum = sum, p.addend = addend, p.weight = weight, p.rstd = rstd, p.dx = dx, p.dsum_out = dsum_out;
+  p.rows = rows, p.dy_stride = dy_stride, p.ds_stride = dsum_stride, p.s_stride = sum_stride, p.a_stride = addend_stride;
   p.C = (int)C, p.w_dtype = weight_dtype, p.offset = (float)offset, p.inv_c = (float)(1.0 / (double)C);
   const int full = dtype == GNB200_F32 ? 4 : 8;
-  const bool aligned = on16(dy) && on16(dsum) && on16(sum) && on16(dx) && on16(dsum_out) && dy_stride % full == 0 &&
-                       sum_stride % full == 0 && (!dsum || dsum_stride % full == 0);
+  const bool aligned = on16(dy) && on16(dsum) && on16(sum) && on16(addend) && on16(dx) && on16(dsum_out) &&
+                       dy_stride % full == 0 && sum_stride % full == 0 && (!dsum || dsum_stride % full == 0) &&
+                       (!addend || addend_stride % full == 0);
   unsigned grid = 0;
   if (dweight) {
     cudaError_t err = launch_rms_bwd(p, dtype, sum_dtype, aligned, s, &grid, true);

@@ -1,7 +1,8 @@
 // torch binding of the operators on token rows: torch.ops.gnb200.{rms_fwd, rms_bwd, rms_quant, rotary, rotary_bwd} over the C ABI,
 // and the plain calls with their autograd nodes.
 //   rms_fwd(x, residual?, weight?, eps, offset) -> (y, sum, rstd)       sum is empty without a residual
-//   rms_bwd(dy, dsum?, sum, weight?, rstd, offset) -> (dx, dsum_out, dweight)    dsum_out, dweight empty where there are none
+//   rms_bwd(dy, dsum?, sum, addend?, weight?, rstd, offset) -> (dx, dsum_out, dweight)    s = sum + addend; dsum_out, dweight empty where
+//                                                                                      there are none
 //   rms_quant(x, residual?, weight?, eps, offset, block, format) -> (codes, scales, sum)
 //   rotary(q, k?, positions, inv_freq, sections, q_weight?, k_weight?, eps, offset, interleaved) -> (q, k)
 //   rotary_bwd(dq, dk?, q, k?, positions, ...) -> (dq, dk, dq_weight, dk_weight)
@@ -122,8 +123,8 @@ RmsOut rms_forward(const Tensor& x, const Tensor& weight, const Tensor& residual
 struct RmsGrads {
   Tensor dx, dsum, dweight;  // dsum undefined where it would be dx
 };
-RmsGrads rms_backward(const Tensor& dy, const Tensor& dsum, const Tensor& sum, const Tensor& weight, const Tensor& rstd, double offset,
-                      bool want_dsum, bool want_dweight) {
+RmsGrads rms_backward(const Tensor& dy, const Tensor& dsum, const Tensor& sum, const Tensor& addend, const Tensor& weight, const Tensor& rstd,
+                      double offset, bool want_dsum, bool want_dweight) {
   TORCH_CHECK(dy.device().is_cuda(), "gnb200: dy must be a CUDA tensor; this package has no CPU path");
   TORCH_CHECK(dtype_code(dy.scalar_type()) >= 0 && dy.dim() >= 1 && dy.size(-1) >= 1, "gnb200: dy must be (*, channels) in float32, float16 or bfloat16");
   TORCH_CHECK(sum.sizes() == dy.sizes() && sum.device() == dy.device() &&
@@ -131,6 +132,8 @@ RmsGrads rms_backward(const Tensor& dy, const Tensor& dsum, const Tensor& sum, c
               "gnb200: sum must match dy in sizes and device and have its dtype or float32");
   TORCH_CHECK(!dsum.defined() || (dsum.sizes() == sum.sizes() && dsum.device() == sum.device() && dsum.scalar_type() == sum.scalar_type()),
               "gnb200: dsum must match sum in sizes, dtype and device");
+  TORCH_CHECK(!addend.defined() || (addend.sizes() == dy.sizes() && addend.device() == dy.device() && addend.scalar_type() == dy.scalar_type()),
+              "gnb200: addend must match dy in sizes, dtype and device");
   const int64_t C = dy.size(-1), rows = dy.numel() / C;
   TORCH_CHECK(rstd.scalar_type() == at::kFloat && rstd.is_contiguous() && rstd.numel() == rows && rstd.device() == dy.device(),
               "gnb200: rstd must be the tensor returned by gnb200::rms_fwd for this input");
@@ -138,8 +141,8 @@ RmsGrads rms_backward(const Tensor& dy, const Tensor& dsum, const Tensor& sum, c
                                     (weight.scalar_type() == dy.scalar_type() || weight.scalar_type() == at::kFloat)),
               "gnb200: weight must be a contiguous vector of one element per channel in the dtype of dy or float32");
   c10::cuda::CUDAGuard guard(dy.device());
-  int64_t dy_stride = C, ds_stride = C, s_stride = C;
-  const Tensor dyr = as_rows(dy, &dy_stride), dsr = as_rows(dsum, &ds_stride), sr = as_rows(sum, &s_stride);
+  int64_t dy_stride = C, ds_stride = C, s_stride = C, a_stride = C;
+  const Tensor dyr = as_rows(dy, &dy_stride), dsr = as_rows(dsum, &ds_stride), sr = as_rows(sum, &s_stride), ar = as_rows(addend, &a_stride);
   const int dtype = code_of(dy), sum_dtype = code_of(sum);
   RmsGrads out;
   out.dx = empty_like_sizes(dy.sizes(), dy.scalar_type(), dy);
@@ -152,8 +155,8 @@ RmsGrads rms_backward(const Tensor& dy, const Tensor& dsum, const Tensor& sum, c
     ws_bytes = gnb200_rms_bwd_workspace_bytes(rows, C, dtype, sum_dtype);
     if (ws_bytes) ws = empty_like_sizes({(int64_t)ws_bytes}, at::kByte, dy);
   }
-  check_status(gnb200_rms_bwd(data(dyr), dy_stride, data(dsr), ds_stride, data(sr), s_stride, data(weight), rstd.const_data_ptr<float>(), rows,
-                              C, offset, dtype, sum_dtype, code_of(weight), out.dx.mutable_data_ptr(),
+  check_status(gnb200_rms_bwd(data(dyr), dy_stride, data(dsr), ds_stride, data(sr), s_stride, data(ar), a_stride, data(weight),
+                              rstd.const_data_ptr<float>(), rows, C, offset, dtype, sum_dtype, code_of(weight), out.dx.mutable_data_ptr(),
                               out.dsum.defined() ? out.dsum.mutable_data_ptr() : nullptr,
                               want_dweight ? out.dweight.mutable_data_ptr() : nullptr, ws_bytes ? ws.mutable_data_ptr() : nullptr, ws_bytes,
                               c10::cuda::getCurrentCUDAStream().stream()));
@@ -166,9 +169,9 @@ std::tuple<Tensor, Tensor, Tensor> rms_fwd_op(const Tensor& x, const OptTensor& 
   RmsOut o = rms_forward(x, value(weight), value(residual), eps, offset, true, 0, -1);
   return {o.y, o.sum.defined() ? o.sum : none_of(x), o.rstd};
 }
-std::tuple<Tensor, Tensor, Tensor> rms_bwd_op(const Tensor& dy, const OptTensor& dsum, const Tensor& sum, const OptTensor& weight,
-                                              const Tensor& rstd, double offset) {
-  RmsGrads g = rms_backward(dy, value(dsum), sum, value(weight), rstd, offset, true, true);
+std::tuple<Tensor, Tensor, Tensor> rms_bwd_op(const Tensor& dy, const OptTensor& dsum, const Tensor& sum, const OptTensor& addend,
+                                              const OptTensor& weight, const Tensor& rstd, double offset) {
+  RmsGrads g = rms_backward(dy, value(dsum), sum, value(addend), value(weight), rstd, offset, true, true);
   return {g.dx, g.dsum.defined() ? g.dsum : none_of(sum), g.dweight.defined() ? g.dweight : none_of(sum)};
 }
 std::tuple<Tensor, Tensor, Tensor> rms_quant_op(const Tensor& x, const OptTensor& residual, const OptTensor& weight, double eps, double offset,
@@ -190,7 +193,10 @@ struct RmsFunction : torch::autograd::Function<RmsFunction> {
     const Tensor residual = value(residual_arg), weight = value(weight_arg);
     RmsOut o = rms_forward(x, weight, residual, eps, offset, true, 0, -1);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({residual.defined() ? o.sum : x, weight, o.rstd});
+    // The stored sum of a 16-bit stream is rounded: good enough for the gradient of x, whose terms are rounded alike, but it would cost
+    // the weight's gradient, a sum in fp32 over all rows, what its 16 bits lack.  There the backward adds x and the residual again.
+    const bool again = residual.defined() && residual.scalar_type() != at::kFloat && weight.defined() && weight.requires_grad();
+    ctx->save_for_backward({again ? residual : residual.defined() ? o.sum : x, again ? x : Tensor(), weight, o.rstd});
     ctx->saved_data["offset"] = offset;
     ctx->saved_data["x_type"] = (int64_t)x.scalar_type();
     ctx->saved_data["residual"] = residual.defined();
@@ -200,7 +206,7 @@ struct RmsFunction : torch::autograd::Function<RmsFunction> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &dy = grads[0], dsum = grads.size() > 1 ? grads[1] : Tensor();
-    const Tensor &sum = saved[0], &weight = saved[1], &rstd = saved[2];
+    const Tensor &sum = saved[0], &addend = saved[1], &weight = saved[2], &rstd = saved[3];
     const auto x_type = (at::ScalarType)ctx->saved_data["x_type"].toInt();
     const double offset = ctx->saved_data["offset"].toDouble();
     const bool residual = ctx->saved_data["residual"].toBool();
@@ -216,13 +222,13 @@ struct RmsFunction : torch::autograd::Function<RmsFunction> {
     }
     if (c10::GradMode::is_enabled()) {  // a graph of the backward is asked for: through the dispatcher, as any op without a second derivative
       static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("gnb200::rms_bwd", "").typed<decltype(rms_bwd_op)>();
-      auto [dx, ds, dw] = op.call(dy, opt(dsum), sum, opt(weight), rstd, offset);
+      auto [dx, ds, dw] = op.call(dy, opt(dsum), sum, opt(addend), opt(weight), rstd, offset);
       out[0] = dx;
       if (want_dsum) out[1] = sum.scalar_type() == x_type ? dx : ds;
       if (want_dweight) out[2] = dw;
       return out;
     }
-    RmsGrads g = rms_backward(dy, dsum, sum, weight, rstd, offset, want_dsum, want_dweight);
+    RmsGrads g = rms_backward(dy, dsum, sum, addend, weight, rstd, offset, want_dsum, want_dweight);
     out[0] = g.dx;
     if (want_dsum) out[1] = g.dsum.defined() ? g.dsum : g.dx;
     out[2] = g.dweight;
@@ -496,7 +502,7 @@ std::tuple<Tensor, Tensor> gnb200_ops::rotary_direct(const Tensor& q, const Tens
 
 TORCH_LIBRARY_FRAGMENT(gnb200, m) {
   m.def("rms_fwd(Tensor x, Tensor? residual, Tensor? weight, float eps, float offset) -> (Tensor, Tensor, Tensor)");
-  m.def("rms_bwd(Tensor dy, Tensor? dsum, Tensor sum, Tensor? weight, Tensor rstd, float offset) -> (Tensor, Tensor, Tensor)");
+  m.def("rms_bwd(Tensor dy, Tensor? dsum, Tensor sum, Tensor? addend, Tensor? weight, Tensor rstd, float offset) -> (Tensor, Tensor, Tensor)");
   m.def("rms_quant(Tensor x, Tensor? residual, Tensor? weight, float eps, float offset, int block, int format) -> (Tensor, Tensor, Tensor)");
   m.def("rotary(Tensor q, Tensor? k, Tensor positions, Tensor inv_freq, int[] sections, Tensor? q_weight, Tensor? k_weight, float eps, "
         "float offset, bool interleaved) -> (Tensor, Tensor)");

@@ -236,8 +236,9 @@ int gnb200_allreduce_param_grads(float* dgamma_dbeta_f32, void* dgamma, void* db
  * gnb200_rms_fwd_8bit: the same with y as 8-bit codes q and fp32 scales, y = q * scale: scale = max |y| / 448 (e4m3) or / 127
  *   (int8), at least 2^-126, one per row (block 0: `rows` floats) or per block of 32, 64 or 128 channels (rows x ceil(C / block)
  *   floats).  A NaN makes the scale of its block NaN.
- * gnb200_rms_bwd: dy and, where the sum was used, dsum (may be NULL) are the gradients of y and sum; `sum` is what the forward
- *   stored, or x where there was no residual.  With n = sum * rstd and g = dy * (offset + weight) it writes
+ * gnb200_rms_bwd: dy and, where the sum was used, dsum (may be NULL) are the gradients of y and sum; s is `sum`, what the forward
+ *   stored, or x where there was no residual; or, with an addend in dy's type (otherwise NULL), sum + addend: the residual and x, for
+ *   a gradient of the weight that is as exact as the forward where the stored sum is rounded to 16 bits.  With n = s * rstd and g = dy * (offset + weight) it writes
  *   d = dsum + rstd * (g - n * mean(g * n)), the gradient of x and of the residual, to dx in dy's type and, where the sum has
  *   another type, to dsum_out in the sum's (NULL otherwise); and dweight = sum over rows of dy * n (NULL: not wanted) in the
  *   weight's type, added in a fixed order.  The workspace is needed only for dweight.
@@ -251,7 +252,7 @@ int gnb200_rms_fwd_8bit(const void* x, int64_t x_stride, const void* residual, i
                         int block, int format, void* q, float* scale, void* sum, void* stream);
 size_t gnb200_rms_bwd_workspace_bytes(int64_t rows, int64_t C, int dtype, int sum_dtype);
 int gnb200_rms_bwd(const void* dy, int64_t dy_stride, const void* dsum, int64_t dsum_stride, const void* sum,
-                   int64_t sum_stride, const void* weight, const float* rstd, int64_t rows, int64_t C, double offset,
+                   int64_t sum_stride, const void* addend, int64_t addend_stride, const void* weight, const float* rstd, int64_t rows, int64_t C, double offset,
                    int dtype, int sum_dtype, int weight_dtype, void* dx, void* dsum_out, void* dweight,
                    void* workspace, size_t workspace_bytes, void* stream);
 

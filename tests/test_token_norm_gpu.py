@@ -56,17 +56,20 @@ def test_forward_rows(rows, c):
 
 
 @pytest.mark.parametrize("c", WIDTHS)
-@pytest.mark.parametrize("dtype,residual,weight", [(F32, F32, F32), (BF16, BF16, F32), (F16, F32, F16), (BF16, None, BF16), (F32, None, None)])
+@pytest.mark.parametrize("dtype,residual,weight", [(F32, F32, F32), (BF16, BF16, F32), (F16, F32, F16), (BF16, None, BF16), (F32, None, None),
+                                                   (F16, F16, None)])
 def test_backward(c, dtype, residual, weight, rows=7):
     x, w, r, dy, ds = _inputs(rows, c, dtype, residual, weight, grads=True)
     leaves = [t.requires_grad_(True) for t in (x, r, w) if t is not None]
     out = pkg.rms_norm(x, w, r, 1e-5, 0.25)
     outs, cots = ((out,), (dy,)) if r is None else (out, (dy, ds))
     grads = list(torch.autograd.grad(outs, leaves, cots))
-    stored = (x if r is None else out[1]).detach().double()
+    # a 16-bit sum whose weight needs no gradient is taken as it was stored
+    as_stored = r is not None and w is None and residual != F32
+    stored = x.detach().double() if r is None else out[1].detach().double() if as_stored else x.detach().double() + r.detach().double()
     _, _, rstd = ref.rms(x.detach(), None, None if r is None else r.detach(), 1e-5, 0.0)
     d, dw, size, wsize = ref.rms_grads(dy, ds, stored, rstd, None if w is None else w.detach(), 0.25)
-    # against the stored sum; dot product as the sum of squares above, and the terms' own operations
+    # the dot product as the sum of squares above, and the terms' own operations
     fp32 = 2 * FORWARD
     dx = grads.pop(0)
     assert dx.dtype == dtype

@@ -79,7 +79,7 @@ def test_rms_refusals_of_the_c_abi():
     bwd = nt.lib.gnb200_rms_bwd
 
     def back(dy=one, rstd=one, dw=None, w=None, ds_out=None, rows=2):
-        return bwd(dy, 8, None, 8, one, 8, w, rstd, rows, 8, 0.0, 0, 0, 0, one, ds_out, dw, None, 0, None)
+        return bwd(dy, 8, None, 8, one, 8, None, 8, w, rstd, rows, 8, 0.0, 0, 0, 0, one, ds_out, dw, None, 0, None)
 
     assert back(dy=None) == -1 and back(rstd=None) == -1
     assert back(dw=one) == -1  # a gradient of no weight
