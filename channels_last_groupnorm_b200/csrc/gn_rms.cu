@@ -29,18 +29,20 @@ struct RmsFwd {
   void *y, *sum;  // y: or the codes
   float *rstd, *scale;
   long long rows, x_stride, r_stride;
-  int C, lanes, w_dtype, block, blocks, format;
+  int C, lanes, stages, stage_bytes, w_dtype, block, blocks, format;
   float eps, offset, inv_c;
 };
 
 // ---------------------------------------------------------------------------------------------
 // 8-bit codes
 // ---------------------------------------------------------------------------------------------
+// (the product and the reciprocal are an ulp or two off the quotients, some 2^-22 of a code's rounding step of 2^-4; the division's
+// slow path would be most of the instructions of a small block)
 __device__ __forceinline__ float scale_of(uint32_t most, int format) {
-  const float largest = format == GNB200_E4M3 ? 448.f : 127.f;
-  const float s = __uint_as_float(most) / largest;
+  const float s = __uint_as_float(most) * (format == GNB200_E4M3 ? 1.f / 448.f : 1.f / 127.f);
   return s < kSmallestScale ? kSmallestScale : s;  // (a NaN stays)
 }
+__device__ __forceinline__ float inverse_of(float scale) { return __fdividef(1.f, scale); }
 template <int VE>
 __device__ __forceinline__ void store_codes(uint8_t* p, const float (&f)[VE], float inverse, int format) {
   Pack<uint8_t, VE> c;
@@ -70,15 +72,37 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float (&f)[VE], fl
 }
 
 // ---------------------------------------------------------------------------------------------
-// Forward
+// Rows in shared memory
 // ---------------------------------------------------------------------------------------------
+// Bytes of a tensor's row in a stage: 16-byte chunks, and one more where rows start between chunk boundaries.
+__host__ __device__ constexpr int segment_bytes(int C, int size, bool aligned) { return aligned ? C * size : (C * size + 30) / 16 * 16; }
+
+// Copies a row, 16 bytes a lane, from the chunk boundary at or before its first byte.  That boundary lies in the row's own allocation
+// (which starts on one), and the last copy ends with the row: nothing outside of the tensor's allocation is read.
 template <typename T, int VE, int V>
-__device__ __forceinline__ void fetch(Pack<T, VE> (&out)[V], const T* row, int first, int step, int nvec) {
+__device__ __forceinline__ void ask_row(char* stage, const T* row, int C, int first, int step) {
+  const uint32_t dst = smem_addr(stage);
+  if constexpr (VE > 1) {
+    constexpr int kParts = sizeof(T) * VE / 16;  // 32 bytes where 8 floats stand beside 8 halves
+    const int nvec = C / VE;
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int at = first + v * step;
-    if (at < nvec) out[v] = load_vec<T, VE>(row + (long long)at * VE);
+    for (int v = 0; v < V; ++v) {
+      const int at = first + v * step;
+      if (at < nvec) {
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) cp_async16(dst + (at * kParts + i) * 16, reinterpret_cast<const char*>(row + (long long)at * VE) + i * 16);
+      }
+    }
+  } else {
+    const int skew = (int)(reinterpret_cast<uintptr_t>(row) & 15), bytes = skew + C * (int)sizeof(T);
+    const char* src = reinterpret_cast<const char*>(row) - skew;
+    for (int at = first * 16; at < bytes; at += step * 16) cp_async16_part(dst + at, src + at, min(16, bytes - at));
   }
+}
+// where the row begins in the stage
+template <typename T, int VE>
+__device__ __forceinline__ const T* row_in(const char* stage, const T* row) {
+  return reinterpret_cast<const T*>(stage + (VE > 1 ? 0 : (reinterpret_cast<uintptr_t>(row) & 15)));
 }
 
 // (offset + w) of this thread's channels
@@ -90,73 +114,149 @@ __device__ __forceinline__ void fetch_weight(float (&w)[V][VE], const void* p, i
 #pragma unroll
     for (int e = 0; e < VE; ++e) w[v][e] = 1.f;
     if (p != nullptr && at < nvec) {
+      params_at<VE>(p, dtype, (long long)at * VE, w[v]);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) w[v][e] = offset + param_at(p, dtype, (long long)at * VE + e, 1.f);
+      for (int e = 0; e < VE; ++e) w[v][e] += offset;
     }
   }
 }
 
-template <typename Tx, typename Ts, int VE, int V, bool WARP, bool Q>
-__global__ void __launch_bounds__(WARP ? kWarpThreads : kMostThreads) rms_fwd_kernel(const RmsFwd p) {
-  __shared__ float slots[2][32];
-  __shared__ uint32_t most[VE == 1 && Q ? V * (kMostThreads / 32) : 32];
-  const int lanes = WARP ? p.lanes : (int)blockDim.x;
-  const int first = WARP ? (int)threadIdx.x & (lanes - 1) : (int)threadIdx.x;
-  const int nvec = p.C / VE;
-  const long long per_cta = WARP ? kWarpThreads / lanes : 1;
-  const long long step = per_cta * gridDim.x;
-  long long row = blockIdx.x * per_cta + (WARP ? (int)threadIdx.x / lanes : 0);
-  const Tx* x = static_cast<const Tx*>(p.x);
-  const Ts* r = static_cast<const Ts*>(p.residual);
-  Pack<Tx, VE> xv[V];
-  Pack<Ts, VE> rv[V];
-  if (row < p.rows) {
-    fetch<Tx, VE, V>(xv, x + row * p.x_stride, first, lanes, nvec);
-    if (r) fetch<Ts, VE, V>(rv, r + row * p.r_stride, first, lanes, nvec);
+// How the rows are dealt out: this thread's place in its row's group, the group's rows and its stages.  A group is a power-of-two number
+// of lanes of one warp (WARP), a team of whole warps (TEAMS) or the CTA.
+template <int VE, bool WARP, bool TEAMS>
+struct Place {
+  int lanes, first, nvec, group;
+  long long per_cta, base, row, step;
+  char* stages;
+  __device__ __forceinline__ Place(int C, int row_lanes, int stage_bytes, int nstages, char* smem) {
+    lanes = WARP || TEAMS ? row_lanes : (int)blockDim.x;
+    group = WARP || TEAMS ? (int)threadIdx.x / lanes : 0;
+    first = (int)threadIdx.x - group * lanes;
+    nvec = C / VE;
+    per_cta = WARP || TEAMS ? (int)blockDim.x / lanes : 1;
+    base = blockIdx.x * per_cta + (WARP ? 0 : group);  // (a warp's groups take their turns together, teams each for themselves)
+    row = blockIdx.x * per_cta + group;
+    step = per_cta * gridDim.x;
+    stages = smem + (long long)group * stage_bytes * nstages;
   }
-  float w[V][VE];
-  fetch_weight<VE, V>(w, p.weight, p.w_dtype, p.offset, first, lanes, nvec);
-  int turn = 0;
-  // (every thread of a warp takes the same number of turns: the shuffles want all lanes)
-  for (long long base = blockIdx.x * per_cta; base < p.rows; base += step, row += step) {
-    const bool live = row < p.rows;
-    float s[V][VE];
-    float sq = 0.f;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      if (live && first + v * lanes < nvec) {
-        unpack<Tx, VE>(xv[v], s[v]);
-        if (r) {
-          float f[VE];
-          unpack<Ts, VE>(rv[v], f);
-#pragma unroll
-          for (int e = 0; e < VE; ++e) s[v][e] += f[e];
-        }
+  // copies that other lanes waited for become visible
+  __device__ __forceinline__ void meet() const {
+    if constexpr (VE == 1) {
+      if constexpr (WARP)
+        __syncwarp();
+      else
+        team_barrier<TEAMS>(lanes, group);
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------------------------
+// Forward
+// ---------------------------------------------------------------------------------------------
+// What a thread holds of the row that comes next: registers where a few vectors do, otherwise the stages.
+template <typename Tx, typename Ts, int VE, int V, bool WARP>
+constexpr bool kStaged = VE == 1 || (!WARP && V * VE * (sizeof(Tx) + sizeof(Ts)) > 64);
+
+template <typename Tx, typename Ts, int VE, int V, bool WARP, bool Q, bool RES>
+__global__ void __launch_bounds__(WARP ? kWarpThreads : kMostThreads) rms_fwd_kernel(const RmsFwd p) {
+  constexpr bool STAGED = kStaged<Tx, Ts, VE, V, WARP>;
+  extern __shared__ __align__(16) char smem[];
+  __shared__ TeamSlots slots;
+  __shared__ uint32_t most[VE == 1 && Q ? V * (kMostThreads / 32) : 32];
+  Place<VE, WARP, false> at(p.C, p.lanes, p.stage_bytes, p.stages, smem);
+  const int lanes = at.lanes, first = at.first, nvec = at.nvec;
+  const int r_at = segment_bytes(p.C, sizeof(Tx), VE > 1);
+  const Tx* next_x = static_cast<const Tx*>(p.x) + at.row * p.x_stride;  // the next row to be asked for
+  const Ts* next_r = RES ? static_cast<const Ts*>(p.residual) + at.row * p.r_stride : nullptr;
+  const long long x_step = at.step * p.x_stride, r_step = RES ? at.step * p.r_stride : 0;
+  long long asked = at.row;
+  int ask_stage = 0, stage = 0;
+  Pack<Tx, VE> xv[STAGED ? 1 : V];
+  Pack<Ts, VE> rv[STAGED || !RES ? 1 : V];
+  auto ask = [&]() {
+    if (asked < p.rows) {
+      if constexpr (STAGED) {
+        char* s = at.stages + ask_stage * p.stage_bytes;
+        ask_row<Tx, VE, V>(s, next_x, p.C, first, lanes);
+        if constexpr (RES) ask_row<Ts, VE, V>(s + r_at, next_r, p.C, first, lanes);
       } else {
 #pragma unroll
-        for (int e = 0; e < VE; ++e) s[v][e] = 0.f;
+        for (int v = 0; v < V; ++v) {
+          const int i = first + v * lanes;
+          if (i < nvec) {
+            xv[v] = load_vec<Tx, VE>(next_x + i * VE);
+            if constexpr (RES) rv[v] = load_vec<Ts, VE>(next_r + i * VE);
+          }
+        }
       }
+    }
+    if constexpr (STAGED) {
+      cp_async_commit();
+      ask_stage = ask_stage + 1 == p.stages ? 0 : ask_stage + 1;
+    }
+    next_x += x_step;
+    next_r += r_step;
+    asked += at.step;
+  };
+  ask();
+  if constexpr (STAGED)
+    for (int i = 1; i < p.stages; ++i) ask();
+  float w[V][VE];
+  fetch_weight<VE, V>(w, p.weight, p.w_dtype, p.offset, first, lanes, nvec);
+  if constexpr (!WARP) clear<false>(slots, lanes, 0, first);
+  int turn = 0;
+  long long row = at.row;
+  uintptr_t x_skew = reinterpret_cast<uintptr_t>(static_cast<const Tx*>(p.x) + row * p.x_stride), r_skew = 0;
+  if constexpr (RES) r_skew = reinterpret_cast<uintptr_t>(static_cast<const Ts*>(p.residual) + row * p.r_stride);
+  // (every thread of a warp takes the same number of turns: the shuffles want all lanes)
+  for (long long base = at.base; base < p.rows; base += at.step, row += at.step) {
+    const bool live = !WARP || row < p.rows;
+    const char* here = nullptr;
+    if constexpr (STAGED) {
+      cp_async_wait_dyn8(p.stages - 1);
+      at.meet();
+      here = at.stages + stage * p.stage_bytes;
+      stage = stage + 1 == p.stages ? 0 : stage + 1;
+    }
+    const Tx* xs = reinterpret_cast<const Tx*>(here + (VE > 1 ? 0 : (x_skew & 15)));
+    const Ts* rs = reinterpret_cast<const Ts*>(here + r_at + (VE > 1 ? 0 : (r_skew & 15)));
+    x_skew += x_step * sizeof(Tx);
+    r_skew += r_step * sizeof(Ts);
+    Ts* sum = static_cast<Ts*>(p.sum) + row * p.C;
+    float s[V][VE];
+    float sq[2] = {0.f, 0.f};
 #pragma unroll
-      for (int e = 0; e < VE; ++e) sq = fmaf(s[v][e], s[v][e], sq);
-    }
-    const long long next = row + step;
-    if (next < p.rows) {
-      fetch<Tx, VE, V>(xv, x + next * p.x_stride, first, lanes, nvec);
-      if (r) fetch<Ts, VE, V>(rv, r + next * p.r_stride, first, lanes, nvec);
-    }
-    if (r && live) {
-      Ts* out = static_cast<Ts*>(p.sum) + row * p.C;
+    for (int v = 0; v < V; ++v) {
+      const int i = first + v * lanes;
 #pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (first + v * lanes < nvec) store_vec<Ts, VE>(out + (first + v * lanes) * VE, pack<Ts, VE>(s[v]));
+      for (int e = 0; e < VE; ++e) s[v][e] = 0.f;
+      if (live && i < nvec) {
+        if constexpr (STAGED)
+          unpack<Tx, VE>(load_vec<Tx, VE>(xs + i * VE), s[v]);
+        else
+          unpack<Tx, VE>(xv[v], s[v]);
+        if constexpr (RES) {
+          float f[VE];
+          if constexpr (STAGED)
+            unpack<Ts, VE>(load_vec<Ts, VE>(rs + i * VE), f);
+          else
+            unpack<Ts, VE>(rv[v], f);
+          add_each(s[v], f);
+          store_vec<Ts, VE>(sum + i * VE, pack<Ts, VE>(s[v]));
+        }
+      }
+      dot_each(sq, s[v], s[v]);
     }
-    sq = WARP ? lanes_sum(sq, lanes) : cta_sum(sq, slots, turn);
-    const float rstd = 1.f / sqrtf(fmaf(sq, p.inv_c, p.eps));
+    if constexpr (VE > 1) ask();  // (a lane's own chunks: read, so free)
+    const float all_sq = WARP ? lanes_sum(sq[0] + sq[1], lanes) : team_sum<false>(sq[0] + sq[1], slots, turn, lanes, 0);
+    if constexpr (VE == 1) ask();  // (behind the sum's barrier, or its shuffles, every lane has read the row)
+    const float rstd = __frsqrt_rn(fmaf(all_sq, p.inv_c, p.eps));
     if (p.rstd && live && first == 0) p.rstd[row] = rstd;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-#pragma unroll
-      for (int e = 0; e < VE; ++e) s[v][e] = s[v][e] * rstd * w[v][e];
+    for (int v = 0; v < V; ++v) {
+      scale_each(s[v], rstd);
+      mul_each(s[v], w[v]);
+    }
     if constexpr (!Q) {
       if (live) {
         Tx* out = static_cast<Tx*>(p.y) + row * p.C;
@@ -180,7 +280,7 @@ __global__ void __launch_bounds__(WARP ? kWarpThreads : kMostThreads) rms_fwd_ke
 #pragma unroll
         for (int v = 0; v < V; ++v) all = max(all, m[v]);
         all = WARP ? lanes_max(all, lanes) : cta_max(all, most);
-        const float scale = scale_of(all, p.format), inverse = 1.f / scale;
+        const float scale = scale_of(all, p.format), inverse = inverse_of(scale);
         if (live && first == 0) p.scale[row] = scale;
 #pragma unroll
         for (int v = 0; v < V; ++v)
@@ -190,11 +290,36 @@ __global__ void __launch_bounds__(WARP ? kWarpThreads : kMostThreads) rms_fwd_ke
         const int share = p.block / VE, among = min(share, WARP ? lanes : 32);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const int at = first + v * lanes;
-          const float scale = scale_of(lanes_max(m[v], among), p.format), inverse = 1.f / scale;
-          if (live && at < nvec) {
-            if (at % share == 0) p.scale[row * p.blocks + at / share] = scale;
-            store_codes<VE>(out + at * VE, s[v], inverse, p.format);
+          const int i = first + v * lanes;
+          const float scale = scale_of(lanes_max(m[v], among), p.format), inverse = inverse_of(scale);
+          if (live && i < nvec) {
+            if (i % share == 0) p.scale[row * p.blocks + i / share] = scale;
+            store_codes<VE>(out + i * VE, s[v], inverse, p.format);
+          }
+        }
+      } else if constexpr (WARP) {
+        // single elements in one warp: turn v holds channels v * lanes and on; a block is one, two or four turns of a whole warp (a row
+        // of fewer lanes has one turn's worth of channels a lane and one block)
+        const int share = max(1, p.block / lanes);
+        uint32_t all = 0;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const int in = v % share;
+          all = in == 0 ? m[v] : max(all, m[v]);
+          m[v] = all;  // over the block so far
+        }
+#pragma unroll
+        for (int v = V - 1; v >= 0; --v) {
+          const int last = min(v / share * share + share, V) - 1;  // the block's last turn has seen all of it
+          if (v != last) m[v] = m[v + 1];
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const int i = first + v * lanes;
+          const float scale = scale_of(lanes_max(m[v], lanes), p.format);
+          if (live && i < nvec) {
+            if (i % p.block == 0) p.scale[row * p.blocks + i / p.block] = scale;
+            store_codes<1>(out + i, s[v], inverse_of(scale), p.format);
           }
         }
       } else {
@@ -202,20 +327,20 @@ __global__ void __launch_bounds__(WARP ? kWarpThreads : kMostThreads) rms_fwd_ke
         const int nwarps = lanes >> 5, warp = first >> 5, share = p.block / 32;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const uint32_t mv = __reduce_max_sync(0xffffffffu, m[v]);
+          const uint32_t mv = lanes_max(m[v], 32);
           if ((first & 31) == 0) most[v * nwarps + warp] = mv;
         }
         __syncthreads();
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const int at = first + v * lanes;
-          if (at < nvec) {
-            const int from = at / p.block * share, to = min(from + share, V * nwarps);
+          const int i = first + v * lanes;
+          if (i < nvec) {
+            const int from = i / p.block * share, to = min(from + share, V * nwarps);
             uint32_t all = 0;
-            for (int i = from; i < to; ++i) all = max(all, most[i]);
+            for (int k = from; k < to; ++k) all = max(all, most[k]);
             const float scale = scale_of(all, p.format);
-            if (at % p.block == 0) p.scale[row * p.blocks + at / p.block] = scale;
-            store_codes<1>(out + at, s[v], 1.f / scale, p.format);
+            if (i % p.block == 0) p.scale[row * p.blocks + i / p.block] = scale;
+            store_codes<1>(out + i, s[v], inverse_of(scale), p.format);
           }
         }
       }
@@ -226,8 +351,9 @@ __global__ void __launch_bounds__(WARP ? kWarpThreads : kMostThreads) rms_fwd_ke
 // Rows of any length: one CTA per row, element by element, read once for the sum and once more for each thing that needs it.
 template <typename Tx, typename Ts, bool Q>
 __global__ void __launch_bounds__(kMostThreads) rms_fwd_any_kernel(const RmsFwd p) {
-  __shared__ float slots[2][32];
+  __shared__ TeamSlots slots;
   __shared__ uint32_t most[32];
+  clear<false>(slots, blockDim.x, 0, threadIdx.x);
   int turn = 0;
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const Tx* x = static_cast<const Tx*>(p.x) + row * p.x_stride;
@@ -243,8 +369,8 @@ __global__ void __launch_bounds__(kMostThreads) rms_fwd_any_kernel(const RmsFwd 
       sq = fmaf(s, s, sq);
       if (r) static_cast<Ts*>(p.sum)[row * p.C + i] = store_param<Ts>(s);
     }
-    sq = cta_sum(sq, slots, turn);
-    const float rstd = 1.f / sqrtf(fmaf(sq, p.inv_c, p.eps));
+    sq = team_sum<false>(sq, slots, turn, blockDim.x, 0);
+    const float rstd = __frsqrt_rn(fmaf(sq, p.inv_c, p.eps));
     if (p.rstd && threadIdx.x == 0) p.rstd[row] = rstd;
     auto y_at = [&](int i) { return sum_at(i) * rstd * (p.weight ? p.offset + param_at(p.weight, p.w_dtype, i, 1.f) : 1.f); };
     if constexpr (!Q) {
@@ -254,7 +380,7 @@ __global__ void __launch_bounds__(kMostThreads) rms_fwd_any_kernel(const RmsFwd 
       if (p.block == 0) {
         uint32_t m = 0;
         for (int i = threadIdx.x; i < p.C; i += blockDim.x) m = max(m, magnitude(y_at(i)));
-        const float scale = scale_of(cta_max(m, most), p.format), inverse = 1.f / scale;
+        const float scale = scale_of(cta_max(m, most), p.format), inverse = inverse_of(scale);
         if (threadIdx.x == 0) p.scale[row] = scale;
         for (int i = threadIdx.x; i < p.C; i += blockDim.x) {
           const float f[1] = {y_at(i)};
@@ -271,7 +397,7 @@ __global__ void __launch_bounds__(kMostThreads) rms_fwd_any_kernel(const RmsFwd 
             f[v][0] = in < p.block && i < p.C ? y_at(i) : 0.f;
             m = max(m, magnitude(f[v][0]));
           }
-          const float scale = scale_of(__reduce_max_sync(0xffffffffu, m), p.format), inverse = 1.f / scale;
+          const float scale = scale_of(lanes_max(m, 32), p.format), inverse = inverse_of(scale);
           if (lane == 0) p.scale[row * p.blocks + b] = scale;
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
@@ -287,121 +413,152 @@ __global__ void __launch_bounds__(kMostThreads) rms_fwd_any_kernel(const RmsFwd 
 // ---------------------------------------------------------------------------------------------
 // Backward
 // ---------------------------------------------------------------------------------------------
+// CTA sizes: the more rows a CTA takes at once, the fewer rows of partial sums there are to add up afterwards
+template <int VE, bool WARP>
+constexpr bool kTeams = VE > 1 && !WARP;
+constexpr int bwd_threads(int ve, int v) { return ve > 1 && ve * v <= 8 ? 1024 : 512; }
+
 struct RmsBwd {
   const void *dy, *dsum, *sum, *addend, *weight;  // s = sum, or sum + addend (dy's type) where the stored sum was rounded to 16 bits
   const float* rstd;
   void *dx, *dsum_out;  // the same gradient in dy's type and, where sum has another type, in sum's
   float* part;          // one row of C floats per CTA, or NULL
   long long rows, dy_stride, ds_stride, s_stride, a_stride;
-  int C, lanes, w_dtype;
+  int C, lanes, stages, stage_bytes, w_dtype;
   float offset, inv_c;
 };
 
-template <typename Tx, typename Ts, int VE, int V, bool WARP>
-__global__ void __launch_bounds__(WARP ? kWarpThreads : kMostThreads) rms_bwd_kernel(const RmsBwd p) {
-  __shared__ float slots[2][32];
-  const int lanes = WARP ? p.lanes : (int)blockDim.x;
-  const int first = WARP ? (int)threadIdx.x & (lanes - 1) : (int)threadIdx.x;
-  const int nvec = p.C / VE;
-  const long long per_cta = WARP ? kWarpThreads / lanes : 1;
-  const long long step = per_cta * gridDim.x;
-  long long row = blockIdx.x * per_cta + (WARP ? (int)threadIdx.x / lanes : 0);
+template <typename Tx, typename Ts, int VE, int V, bool WARP, bool RES>
+__global__ void __launch_bounds__(bwd_threads(VE, V), VE > 1 ? 1 : 0) rms_bwd_kernel(const RmsBwd p) {
+  extern __shared__ __align__(16) char smem[];
+  constexpr bool TEAMS = kTeams<VE, WARP>;
+  __shared__ TeamSlots all_slots[TEAMS ? kMostTeams : 1];
+  Place<VE, WARP, TEAMS> at(p.C, p.lanes, p.stage_bytes, p.stages, smem);
+  TeamSlots& slots = all_slots[TEAMS ? at.group : 0];
+  const int lanes = at.lanes, first = at.first, nvec = at.nvec;
   grid_dep_launch_dependents();
-  const Tx* dy = static_cast<const Tx*>(p.dy);
-  const Tx* add = static_cast<const Tx*>(p.addend);
-  const Ts *ds = static_cast<const Ts*>(p.dsum), *sum = static_cast<const Ts*>(p.sum);
-  Pack<Tx, VE> yv[V], av[V];
-  Pack<Ts, VE> sv[V], dv[V];
-  float rn = 0.f;
-  auto ask = [&](long long at) {
-    fetch<Tx, VE, V>(yv, dy + at * p.dy_stride, first, lanes, nvec);
-    fetch<Ts, VE, V>(sv, sum + at * p.s_stride, first, lanes, nvec);
-    if (add) fetch<Tx, VE, V>(av, add + at * p.a_stride, first, lanes, nvec);
-    if (ds) fetch<Ts, VE, V>(dv, ds + at * p.ds_stride, first, lanes, nvec);
-    rn = p.rstd[at];
+  const Tx *dy = static_cast<const Tx*>(p.dy), *add = RES ? static_cast<const Tx*>(p.addend) : nullptr;
+  const Ts *ds = RES ? static_cast<const Ts*>(p.dsum) : nullptr, *sum = static_cast<const Ts*>(p.sum);
+  // a stage: sum, dy, then the addend and the sum's gradient where there are any
+  const int narrow = segment_bytes(p.C, sizeof(Tx), VE > 1), wide = segment_bytes(p.C, sizeof(Ts), VE > 1);
+  const int dy_at = wide, add_at = dy_at + narrow, ds_at = add_at + (add ? narrow : 0);
+  long long asked = at.row;
+  int ask_stage = 0, stage = 0;
+  auto ask = [&]() {
+    if (asked < p.rows) {
+      char* s = at.stages + ask_stage * p.stage_bytes;
+      ask_row<Ts, VE, V>(s, sum + asked * p.s_stride, p.C, first, lanes);
+      ask_row<Tx, VE, V>(s + dy_at, dy + asked * p.dy_stride, p.C, first, lanes);
+      if (add) ask_row<Tx, VE, V>(s + add_at, add + asked * p.a_stride, p.C, first, lanes);
+      if (ds) ask_row<Ts, VE, V>(s + ds_at, ds + asked * p.ds_stride, p.C, first, lanes);
+    }
+    cp_async_commit();
+    asked += at.step;
+    ask_stage = ask_stage + 1 == p.stages ? 0 : ask_stage + 1;
   };
-  if (row < p.rows) ask(row);
+  // Single elements are free for the next copy only behind the barrier of the row after, so one stage fewer is in flight; a lone
+  // stage gets a barrier of its own.
+  const bool lone = VE == 1 && p.stages == 1;
+  const int ahead = VE > 1 || lone ? p.stages : p.stages - 1;
+  for (int i = 0; i < ahead; ++i) ask();
   float w[V][VE], dw[V][VE];
   fetch_weight<VE, V>(w, p.weight, p.w_dtype, p.offset, first, lanes, nvec);
 #pragma unroll
   for (int v = 0; v < V; ++v)
 #pragma unroll
     for (int e = 0; e < VE; ++e) dw[v][e] = 0.f;
+  if constexpr (!WARP) clear<TEAMS>(slots, at.lanes, at.group, first);
   int turn = 0;
-  for (long long base = blockIdx.x * per_cta; base < p.rows; base += step, row += step) {
-    const bool live = row < p.rows;
+  long long row = at.row;
+  float rn = row < p.rows ? p.rstd[row] : 0.f;
+  for (long long base = at.base; base < p.rows; base += at.step, row += at.step) {
+    const bool live = !WARP || row < p.rows;
     const float rstd = rn;
-    float g[V][VE], n[V][VE], d[V][VE];
-    float dot = 0.f;
+    if (row + at.step < p.rows) rn = p.rstd[row + at.step];
+    cp_async_wait_dyn8(ahead - 1);
+    at.meet();
+    if (VE == 1 && !lone) ask();
+    const char* here = at.stages + stage * p.stage_bytes;
+    stage = stage + 1 == p.stages ? 0 : stage + 1;
+    const Ts* sums = row_in<Ts, VE>(here, sum + row * p.s_stride);
+    const Tx* dys = row_in<Tx, VE>(here + dy_at, dy + row * p.dy_stride);
+    const Tx* adds = row_in<Tx, VE>(here + add_at, add + row * p.a_stride);
+    const Ts* dss = row_in<Ts, VE>(here + ds_at, ds + row * p.ds_stride);
+    // s * rstd and dy of this thread's vector i
+    auto terms = [&](int i, float (&n)[VE], float (&g)[VE]) {
+      unpack<Ts, VE>(load_vec<Ts, VE>(sums + i * VE), n);
+      unpack<Tx, VE>(load_vec<Tx, VE>(dys + i * VE), g);
+      if (add) {
+        float f[VE];
+        unpack<Tx, VE>(load_vec<Tx, VE>(adds + i * VE), f);
+        add_each(n, f);
+      }
+      scale_each(n, rstd);
+    };
+    float dot[2] = {0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-#pragma unroll
-      for (int e = 0; e < VE; ++e) g[v][e] = n[v][e] = d[v][e] = 0.f;
       if (live && first + v * lanes < nvec) {
-        unpack<Tx, VE>(yv[v], g[v]);
-        unpack<Ts, VE>(sv[v], n[v]);
-        if (add) {
-          float f[VE];
-          unpack<Tx, VE>(av[v], f);
-#pragma unroll
-          for (int e = 0; e < VE; ++e) n[v][e] += f[e];
-        }
-        if (ds) unpack<Ts, VE>(dv[v], d[v]);
-#pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          n[v][e] *= rstd;
-          dw[v][e] = fmaf(g[v][e], n[v][e], dw[v][e]);
-          g[v][e] *= w[v][e];
-          dot = fmaf(g[v][e], n[v][e], dot);
-        }
+        float n[VE], g[VE];
+        terms(first + v * lanes, n, g);
+        mul_each(g, n);
+        add_each(dw[v], g);
+        dot_each(dot, g, w[v]);
       }
     }
-    if (row + step < p.rows) ask(row + step);
-    const float c = (WARP ? lanes_sum(dot, lanes) : cta_sum(dot, slots, turn)) * p.inv_c;
+    const float c = -(WARP ? lanes_sum(dot[0] + dot[1], lanes) : team_sum<TEAMS>(dot[0] + dot[1], slots, turn, at.lanes, at.group)) * p.inv_c;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      if (live && first + v * lanes < nvec) {
-        const long long at = row * p.C + (first + v * lanes) * VE;
+      const int i = first + v * lanes;
+      if (live && i < nvec) {
+        float n[VE], g[VE], d[VE];
+        terms(i, n, g);
+        mul_each(g, w[v]);
+        axpy_each(g, n, c);
+        scale_each(g, rstd);
+        if (ds) {
+          unpack<Ts, VE>(load_vec<Ts, VE>(dss + i * VE), d);
+          add_each(d, g);
+        } else {
 #pragma unroll
-        for (int e = 0; e < VE; ++e) d[v][e] = fmaf(rstd, fmaf(-n[v][e], c, g[v][e]), d[v][e]);
-        store_vec<Tx, VE>(static_cast<Tx*>(p.dx) + at, pack<Tx, VE>(d[v]));
+          for (int e = 0; e < VE; ++e) d[e] = g[e];
+        }
+        store_vec<Tx, VE>(static_cast<Tx*>(p.dx) + row * p.C + i * VE, pack<Tx, VE>(d));
         if constexpr (!std::is_same<Tx, Ts>::value)
-          if (p.dsum_out) store_vec<Ts, VE>(static_cast<Ts*>(p.dsum_out) + at, pack<Ts, VE>(d[v]));
+          if (p.dsum_out) store_vec<Ts, VE>(static_cast<Ts*>(p.dsum_out) + row * p.C + i * VE, pack<Ts, VE>(d));
       }
     }
+    if (lone) at.meet();
+    if (VE > 1 || lone) ask();
   }
   if (p.part == nullptr) return;
-  float* part = p.part + (long long)blockIdx.x * p.C;
-  if constexpr (!WARP) {
+  // the groups hold the same channels: their sums are added in order.  They fit the stages, whose rows have two tensors of at least
+  // two bytes an element.
+  cp_async_wait<0>();
+  __syncthreads();
+  float* share = reinterpret_cast<float*>(smem);
+  const int groups = (int)blockDim.x / lanes;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (first + v * lanes < nvec) {
+  for (int v = 0; v < V; ++v) {
+    const int i = first + v * lanes;
+    if (i < nvec) {
 #pragma unroll
-        for (int e = 0; e < VE; ++e) part[(first + v * lanes) * VE + e] = dw[v][e];
-      }
-  } else {
-    // the groups of lanes hold the same channels: added in order, one vector at a time
-    __shared__ float share[kWarpThreads * VE];
-    const int groups = kWarpThreads / lanes;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      __syncthreads();
-#pragma unroll
-      for (int e = 0; e < VE; ++e) share[(threadIdx.x / lanes * VE + e) * lanes + first] = dw[v][e];
-      __syncthreads();
-      for (int i = threadIdx.x; i < lanes * VE; i += kWarpThreads) {
-        const int lane = i / VE, e = i % VE, channel = (lane + v * lanes) * VE + e;
-        float t = 0.f;
-        for (int g = 0; g < groups; ++g) t += share[(g * VE + e) * lanes + lane];
-        if (channel < p.C) part[channel] = t;
-      }
+      for (int e = 0; e < VE; ++e) share[at.group * p.C + i * VE + e] = dw[v][e];
     }
+  }
+  __syncthreads();
+  float* part = p.part + (long long)blockIdx.x * p.C;
+  for (int i = threadIdx.x; i < p.C; i += blockDim.x) {
+    float t = 0.f;
+    for (int g = 0; g < groups; ++g) t += share[g * p.C + i];
+    part[i] = t;
   }
 }
 
 template <typename Tx, typename Ts>
 __global__ void __launch_bounds__(kMostThreads) rms_bwd_any_kernel(const RmsBwd p) {
-  __shared__ float slots[2][32];
+  __shared__ TeamSlots slots;
+  clear<false>(slots, blockDim.x, 0, threadIdx.x);
   int turn = 0;
   grid_dep_launch_dependents();
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
@@ -414,7 +571,7 @@ __global__ void __launch_bounds__(kMostThreads) rms_bwd_any_kernel(const RmsBwd 
     auto n_at = [&](int i) { return (load_param<Ts>(sum, i) + (add ? load_param<Tx>(add, i) : 0.f)) * rstd; };
     float dot = 0.f;
     for (int i = threadIdx.x; i < p.C; i += blockDim.x) dot = fmaf(g_at(i), n_at(i), dot);
-    const float c = cta_sum(dot, slots, turn) * p.inv_c;
+    const float c = team_sum<false>(dot, slots, turn, blockDim.x, 0) * p.inv_c;
     for (int i = threadIdx.x; i < p.C; i += blockDim.x) {
       const float d = fmaf(rstd, fmaf(-n_at(i), c, g_at(i)), ds ? load_param<Ts>(ds, i) : 0.f);
       static_cast<Tx*>(p.dx)[row * p.C + i] = store_param<Tx>(d);
@@ -436,7 +593,7 @@ __global__ void __launch_bounds__(kMostThreads) rms_bwd_any_kernel(const RmsBwd 
 }
 
 // One warp-wide column block of 32 channels per CTA; the rows are dealt out to its warps, whose sums are added in order.
-constexpr int kSumWarps = 16;
+constexpr int kSumWarps = 32;
 __global__ void __launch_bounds__(32 * kSumWarps) column_sums_kernel(const ColumnSums p) {
   __shared__ float share[kSumWarps][32];
   const int per_set = (p.C + 31) / 32, set = (int)blockIdx.x / per_set;
@@ -446,7 +603,7 @@ __global__ void __launch_bounds__(32 * kSumWarps) column_sums_kernel(const Colum
   grid_dep_wait();
   float t = 0.f;
   if (c < p.C) {
-#pragma unroll 4
+#pragma unroll 8
     for (int r = warp; r < rows; r += kSumWarps) t += part[(long long)r * p.C + c];
   }
   share[warp][lane] = t;
@@ -463,38 +620,76 @@ __global__ void __launch_bounds__(32 * kSumWarps) column_sums_kernel(const Colum
 // Host side
 // ---------------------------------------------------------------------------------------------
 struct RmsGeom {
-  int ve, v, lanes, threads;  // lanes: per row, 0 = one CTA per row; ve = 0: the kernels for rows of any length
+  int ve, v, lanes, threads;  // lanes: per row; threads: per CTA; ve = 0: the kernels for rows of any length
+  bool warp;                  // lanes of one warp; otherwise whole warps
 };
 
-RmsGeom rms_geometry(int64_t C, int dtype, bool aligned) {
+RmsGeom rms_geometry(int64_t C, int dtype, bool aligned, bool backward) {
   const int full = dtype == GNB200_F32 ? 4 : 8;
   RmsGeom g = {};
   g.ve = aligned && C % full == 0 ? full : 1;
   const int64_t nvec = C / g.ve;
-  if (g.ve > 1 && nvec <= 32 * 4) {
+  const int in_warp = g.ve > 1 ? 4 : 16;  // vectors a lane that a warp's row may have
+  if (nvec <= 32 * in_warp) {
+    g.warp = true;
     g.lanes = 1;
     while (g.lanes < 32 && g.lanes < nvec) g.lanes *= 2;
-    g.v = nvec <= g.lanes ? 1 : nvec <= 2 * g.lanes ? 2 : 4;
-    g.threads = kWarpThreads;
-    return g;
+    const int64_t each = (nvec + g.lanes - 1) / g.lanes;
+    g.v = g.ve > 1 ? (each <= 1 ? 1 : each <= 2 ? 2 : 4) : (each <= 4 ? 4 : 16);
+  } else {
+    const int most = 32 / g.ve;
+    int v = g.ve == 1 ? 8 : 2;
+    while (v < most && nvec > (int64_t)v * kMostThreads) v = g.ve == 1 ? 32 : 2 * v;
+    if (nvec > (int64_t)v * kMostThreads) return RmsGeom{0, 0, kMostThreads, kMostThreads, false};
+    g.v = v;
+    g.lanes = (int)((nvec + v - 1) / v + 31) / 32 * 32;
   }
-  const int most = 32 / g.ve;  // vectors a thread
-  int v = g.ve == 1 ? 4 : 2;
-  while (v < most && nvec > (int64_t)v * kMostThreads) v = g.ve == 1 ? (v == 4 ? 16 : 32) : 2 * v;
-  if (nvec > (int64_t)v * kMostThreads) return RmsGeom{0, 0, 0, kMostThreads};
-  g.v = v;
-  g.threads = (int)((nvec + v - 1) / v + 31) / 32 * 32;
+  g.threads = g.warp ? kWarpThreads : g.lanes;
+  if (backward) {
+    const int most = bwd_threads(g.ve, g.v);
+    g.threads = g.warp ? most : g.ve == 1 ? g.lanes : std::max(1, std::min(kMostTeams, most / g.lanes)) * g.lanes;
+  }
   return g;
 }
 
-// The CTAs of a call: no more than are resident at once, no more than there are rows
-cudaError_t rms_grid(const void* kernel, const RmsGeom& g, int64_t rows, unsigned* grid) {
-  long long most = 0;
-  const cudaError_t err = resident_ctas(kernel, g.threads, &most);
+constexpr int kMostStages = 4;  // of a row; two do as well where a row is 16 KB, eight are no faster anywhere
+
+struct RmsLaunch {
+  unsigned grid;
+  int threads, smem, stages;
+};
+// CTA size, stages, shared memory and CTAs of a call whose rows take `row_bytes` in a stage (0: no stages): no more CTAs than are resident at
+// once nor than there are rows.  cudaErrorInvalidValue: a row does not fit.
+cudaError_t rms_launch(const void* kernel, const RmsGeom& g, int64_t rows, int64_t row_bytes, RmsLaunch* out) {
+  Residency r = {};
+  out->threads = g.threads;
+  out->stages = out->smem = 0;
+  if (row_bytes > kMostDynamicSmem) return cudaErrorInvalidValue;
+  if (row_bytes) {
+    // fewer teams where two stages for each do not fit, or where there are no rows for them on every SM
+    const auto halve = [&](int teams) { return g.warp ? teams / 2 : teams - 1; };
+    int teams = g.threads / g.lanes;
+    cudaError_t err = residency(kernel, g.threads, 0, &r);
+    if (err != cudaSuccess) return err;
+    const int least = g.warp ? 32 / g.lanes : 1;
+    while (teams > least && (2 * teams * row_bytes > kMostDynamicSmem || (int64_t)teams * r.sms > rows)) teams = std::max(least, halve(teams));
+    out->threads = teams * g.lanes;
+    if ((err = residency(kernel, out->threads, 0, &r)) != cudaSuccess) return err;
+    const int64_t bytes = row_bytes * teams;
+    if (bytes > kMostDynamicSmem) return cudaErrorInvalidValue;
+    int64_t stages = std::max<int64_t>(1, kMostDynamicSmem / r.per_sm / bytes);
+    stages = std::min<int64_t>(kMostStages, std::max<int64_t>(stages, std::min<int64_t>(2, kMostDynamicSmem / bytes)));
+    const int64_t turns = (rows + (int64_t)teams * r.sms - 1) / ((int64_t)teams * r.sms);  // at most, of a team
+    out->stages = (int)std::max<int64_t>(1, std::min(stages, turns));
+    out->smem = (int)(bytes * out->stages);
+  }
+  const int cap = r.per_sm;
+  const cudaError_t err = residency(kernel, out->threads, out->smem, &r);
   if (err != cudaSuccess) return err;
-  const int64_t per_cta = g.lanes ? kWarpThreads / g.lanes : 1;
-  const int64_t need = (rows + per_cta - 1) / per_cta;
-  *grid = (unsigned)(need < most ? need : most);
+  if (row_bytes) r.per_sm = std::min(r.per_sm, cap);
+  const int64_t per_cta = out->threads / g.lanes;
+  const int64_t need = (rows + per_cta - 1) / per_cta, most = (int64_t)r.per_sm * r.sms;
+  out->grid = (unsigned)(need < most ? need : most);
   return cudaSuccess;
 }
 
@@ -511,11 +706,10 @@ using Int = std::integral_constant<int, N>;
 template <int FULL, typename F>
 cudaError_t with_geometry(const RmsGeom& g, F&& f) {
   if (g.ve == 1) {
-    if (g.v == 4) return f(Int<1>(), Int<4>(), std::false_type());
-    if (g.v == 16) return f(Int<1>(), Int<16>(), std::false_type());
-    return f(Int<1>(), Int<32>(), std::false_type());
+    if (g.warp) return g.v == 4 ? f(Int<1>(), Int<4>(), std::true_type()) : f(Int<1>(), Int<16>(), std::true_type());
+    return g.v == 8 ? f(Int<1>(), Int<8>(), std::false_type()) : f(Int<1>(), Int<32>(), std::false_type());
   }
-  if (g.lanes) {
+  if (g.warp) {
     if (g.v == 1) return f(Int<FULL>(), Int<1>(), std::true_type());
     if (g.v == 2) return f(Int<FULL>(), Int<2>(), std::true_type());
     return f(Int<FULL>(), Int<4>(), std::true_type());
@@ -527,47 +721,70 @@ cudaError_t with_geometry(const RmsGeom& g, F&& f) {
   return f(Int<FULL>(), Int<4>(), std::false_type());
 }
 
-template <typename Call>
-cudaError_t launch_rows(void (*kernel)(Call), const RmsGeom& g, unsigned grid, const Call& p, cudaStream_t stream) {
-  kernel<<<grid, g.threads, 0, stream>>>(p);
-  return cudaGetLastError();
-}
-
 template <bool Q>
 cudaError_t launch_rms_fwd(RmsFwd p, int dtype, int sum_dtype, bool aligned, cudaStream_t stream) {
-  const RmsGeom g = rms_geometry(p.C, dtype, aligned);
-  p.lanes = g.lanes;
   return with_types(dtype, sum_dtype, [&](auto tx, auto ts) {
     using Tx = decltype(tx);
     using Ts = decltype(ts);
+    RmsGeom g = rms_geometry(p.C, dtype, aligned, false);
+    bool staged = false;
     auto go = [&](void (*kernel)(const RmsFwd)) {
-      unsigned grid = 0;
-      const cudaError_t err = rms_grid((const void*)kernel, g, p.rows, &grid);
-      return err != cudaSuccess ? err : launch_rows(kernel, g, grid, p, stream);
+      RmsLaunch l = {};
+      const int row_bytes = staged ? segment_bytes(p.C, sizeof(Tx), g.ve > 1) + (p.residual ? segment_bytes(p.C, sizeof(Ts), g.ve > 1) : 0) : 0;
+      const cudaError_t err = rms_launch((const void*)kernel, g, p.rows, row_bytes, &l);
+      if (err != cudaSuccess) return err;
+      p.lanes = g.lanes, p.stages = l.stages, p.stage_bytes = row_bytes;
+      kernel<<<l.grid, l.threads, l.smem, stream>>>(p);
+      return cudaGetLastError();
     };
-    if (g.ve == 0) return go(&rms_fwd_any_kernel<Tx, Ts, Q>);
-    return with_geometry<16 / (int)sizeof(Tx)>(g, [&](auto ve, auto v, auto warp) {
-      return go(&rms_fwd_kernel<Tx, Ts, decltype(ve)::value, decltype(v)::value, decltype(warp)::value, Q>);
-    });
+    if (g.ve) {
+      const cudaError_t err = with_geometry<16 / (int)sizeof(Tx)>(g, [&](auto ve, auto v, auto warp) {
+        constexpr int VE = decltype(ve)::value, V = decltype(v)::value;
+        constexpr bool WARP = decltype(warp)::value;
+        staged = kStaged<Tx, Ts, VE, V, WARP>;
+        if constexpr (std::is_same<Tx, Ts>::value)
+          if (!p.residual) return go(&rms_fwd_kernel<Tx, Ts, VE, V, WARP, Q, false>);
+        return go(&rms_fwd_kernel<Tx, Ts, VE, V, WARP, Q, true>);
+      });
+      if (err != cudaErrorInvalidValue) return err;
+      g = RmsGeom{0, 0, kMostThreads, kMostThreads, false};
+      staged = false;
+    }
+    return go(&rms_fwd_any_kernel<Tx, Ts, Q>);
   });
 }
 
 // `grid_only`: the number of CTAs, that is of rows of partial sums, is all that is wanted
 cudaError_t launch_rms_bwd(RmsBwd p, int dtype, int sum_dtype, bool aligned, cudaStream_t stream, unsigned* grid, bool grid_only) {
-  const RmsGeom g = rms_geometry(p.C, dtype, aligned);
-  p.lanes = g.lanes;
   return with_types(dtype, sum_dtype, [&](auto tx, auto ts) {
     using Tx = decltype(tx);
     using Ts = decltype(ts);
+    RmsGeom g = rms_geometry(p.C, dtype, aligned, true);
     auto go = [&](void (*kernel)(const RmsBwd)) {
-      const cudaError_t err = rms_grid((const void*)kernel, g, p.rows, grid);
-      if (g.ve == 0) *grid = std::min(*grid, (unsigned)std::max(1, (1 << 24) / p.C));  // 64 MB of partial sums at most, or one row
-      return err != cudaSuccess || grid_only ? err : launch_rows(kernel, g, *grid, p, stream);
+      RmsLaunch l = {};
+      int row_bytes = 0;
+      if (g.ve)
+        row_bytes = segment_bytes(p.C, sizeof(Tx), g.ve > 1) * (p.addend ? 2 : 1) + segment_bytes(p.C, sizeof(Ts), g.ve > 1) * (p.dsum ? 2 : 1);
+      const cudaError_t err = rms_launch((const void*)kernel, g, p.rows, row_bytes, &l);
+      if (err != cudaSuccess) return err;
+      *grid = g.ve ? l.grid : std::min(l.grid, (unsigned)std::max(1, (1 << 24) / p.C));  // 64 MB of partial sums at most, or one row
+      if (grid_only) return cudaSuccess;
+      p.lanes = g.lanes, p.stages = l.stages, p.stage_bytes = row_bytes;
+      kernel<<<*grid, l.threads, l.smem, stream>>>(p);
+      return cudaGetLastError();
     };
-    if (g.ve == 0) return go(&rms_bwd_any_kernel<Tx, Ts>);
-    return with_geometry<16 / (int)sizeof(Tx)>(g, [&](auto ve, auto v, auto warp) {
-      return go(&rms_bwd_kernel<Tx, Ts, decltype(ve)::value, decltype(v)::value, decltype(warp)::value>);
-    });
+    if (g.ve) {
+      const cudaError_t err = with_geometry<16 / (int)sizeof(Tx)>(g, [&](auto ve, auto v, auto warp) {
+        constexpr int VE = decltype(ve)::value, V = decltype(v)::value;
+        constexpr bool WARP = decltype(warp)::value;
+        if constexpr (std::is_same<Tx, Ts>::value)
+          if (!p.addend && !p.dsum) return go(&rms_bwd_kernel<Tx, Ts, VE, V, WARP, false>);
+        return go(&rms_bwd_kernel<Tx, Ts, VE, V, WARP, true>);
+      });
+      if (err != cudaErrorInvalidValue) return err;
+      g = RmsGeom{0, 0, kMostThreads, kMostThreads, false};
+    }
+    return go(&rms_bwd_any_kernel<Tx, Ts>);
   });
 }
 
@@ -622,7 +839,7 @@ static int rms_forward(const char* name, const void* x, int64_t x_stride, const 
   p.C = (int)C, p.w_dtype = weight_dtype, p.block = block, p.blocks = block ? (int)((C + block - 1) / block) : 1, p.format = format;
   p.eps = (float)eps, p.offset = (float)offset, p.inv_c = (float)(1.0 / (double)C);
   const int full = dtype == GNB200_F32 ? 4 : 8;
-  const bool aligned = on16(x) && on16(residual) && on16(y) && on16(sum) && x_stride % full == 0 && (!residual || residual_stride % full == 0);
+  const bool aligned = on16(x) && on16(residual) && on16(weight) && on16(y) && on16(sum) && x_stride % full == 0 && (!residual || residual_stride % full == 0);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   return launched(name, codes ? launch_rms_fwd<true>(p, dtype, residual_dtype, aligned, s)
                               : launch_rms_fwd<false>(p, dtype, residual_dtype, aligned, s));
@@ -644,16 +861,23 @@ int gnb200_rms_fwd_8bit(const void* x, int64_t x_stride, const void* residual, i
 
 size_t gnb200_rms_bwd_workspace_bytes(int64_t rows, int64_t C, int dtype, int sum_dtype) {
   if (check_rows("gnb200_rms_bwd_workspace_bytes", rows, C, dtype, sum_dtype, dtype) != GNB200_OK || rows == 0) return 0;
+  static thread_local Remembered<4> known;  // the answer depends on nothing but these and the device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  const Remembered<4>::Key key = {rows, C, dtype * 4 + sum_dtype, dev};
+  if (const size_t* v = known.find(key)) return *v;
   RmsBwd p = {};
   p.rows = rows, p.C = (int)C;
   size_t most = 0;
-  for (int aligned = 0; aligned < 2; ++aligned) {  // whichever kernel the pointers will ask for
+  for (int kind = 0; kind < 8; ++kind) {  // whichever kernel and stages the call's tensors will ask for (none of these is read)
+    p.addend = kind & 1 ? &p : nullptr;
+    p.dsum = kind & 2 ? &p : nullptr;
     unsigned grid = 0;
-    if (launch_rms_bwd(p, dtype, sum_dtype, aligned != 0, nullptr, &grid, true) != cudaSuccess) return 0;
+    if (launch_rms_bwd(p, dtype, sum_dtype, (kind & 4) != 0, nullptr, &grid, true) != cudaSuccess) return 0;
     const size_t need = (size_t)grid * (size_t)C * sizeof(float);
     most = need > most ? need : most;
   }
-  return most;
+  return known.keep(key, most);
 }
 
 int gnb200_rms_bwd(const void* dy, int64_t dy_stride, const void* dsum, int64_t dsum_stride, const void* sum, int64_t sum_stride,
@@ -676,7 +900,7 @@ int gnb200_rms_bwd(const void* dy, int64_t dy_stride, const void* dsum, int64_t 
   p.rows = rows, p.dy_stride = dy_stride, p.ds_stride = dsum_stride, p.s_stride = sum_stride, p.a_stride = addend_stride;
   p.C = (int)C, p.w_dtype = weight_dtype, p.offset = (float)offset, p.inv_c = (float)(1.0 / (double)C);
   const int full = dtype == GNB200_F32 ? 4 : 8;
-  const bool aligned = on16(dy) && on16(dsum) && on16(sum) && on16(addend) && on16(dx) && on16(dsum_out) &&
+  const bool aligned = on16(dy) && on16(dsum) && on16(weight) && on16(sum) && on16(addend) && on16(dx) && on16(dsum_out) &&
                        dy_stride % full == 0 && sum_stride % full == 0 && (!dsum || dsum_stride % full == 0) &&
                        (!addend || addend_stride % full == 0);
   unsigned grid = 0;

@@ -67,14 +67,15 @@ __device__ __forceinline__ void token_angles(const Rotary& p, long long b, long 
   __syncwarp();
 }
 
-// Where a lane's slot of two vectors stands in the head.  Slots 0 .. pairs / VE - 1 are rotated, the others pass.
-template <int VE, bool INTER>
+// Where a lane's slot of two vectors stands in the head.  Slots 0 .. pairs / VE - 1 are turned, the others pass.  WHOLE: the head is
+// turned from end to end and every lane has one slot.
+template <int VE, bool INTER, bool WHOLE>
 struct Slot {
   int a, b;
   bool has_a, has_b, turns;
   __device__ __forceinline__ Slot(int s, int pairs, int D) {
     const int rotated = pairs / VE;
-    turns = s < rotated;
+    turns = WHOLE || s < rotated;
     if (turns) {
       a = INTER ? 2 * s * VE : s * VE;
       b = INTER ? a + VE : pairs + s * VE;
@@ -82,20 +83,31 @@ struct Slot {
       a = 2 * pairs + 2 * (s - rotated) * VE;
       b = a + VE;
     }
-    has_a = a < D;
-    has_b = b < D;
+    has_a = WHOLE || a < D;
+    has_b = WHOLE || b < D;
   }
 };
 
-// f: the slot's two vectors; cs: cos and sin of its VE pairs
+// (a, b) -> (a aa + b ab, b bb + a ba) for the pairs of f, the slot's two vectors
 template <int VE, bool INTER>
-__device__ __forceinline__ void turn(float (&f)[2 * VE], const float (&c)[VE], const float (&s)[VE]) {
+__device__ __forceinline__ void turn(float (&f)[2 * VE], const float (&aa)[VE], const float (&ab)[VE], const float (&bb)[VE], const float (&ba)[VE]) {
+  if constexpr (!INTER && VE % 2 == 0) {
 #pragma unroll
-  for (int e = 0; e < VE; ++e) {
-    const int i = INTER ? 2 * e : e, j = INTER ? 2 * e + 1 : VE + e;
-    const float a = f[i], b = f[j];
-    f[i] = fmaf(a, c[e], -b * s[e]);
-    f[j] = fmaf(b, c[e], a * s[e]);
+    for (int e = 0; e < VE; e += 2) {
+      float u0, u1, v0, v1;
+      mul2(u0, u1, f[VE + e], f[VE + e + 1], ab[e], ab[e + 1]);
+      mul2(v0, v1, f[e], f[e + 1], ba[e], ba[e + 1]);
+      fma2(f[e], f[e + 1], f[e], f[e + 1], aa[e], aa[e + 1], u0, u1);
+      fma2(f[VE + e], f[VE + e + 1], f[VE + e], f[VE + e + 1], bb[e], bb[e + 1], v0, v1);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      const int i = INTER ? 2 * e : e, j = INTER ? 2 * e + 1 : VE + e;
+      const float a = f[i], b = f[j];
+      f[i] = fmaf(a, aa[e], b * ab[e]);
+      f[j] = fmaf(b, bb[e], a * ba[e]);
+    }
   }
 }
 
@@ -111,9 +123,10 @@ __device__ __forceinline__ void unpack_two(const Pack<T, VE>& a, const Pack<T, V
 }
 
 // SLOTS: slots a lane.  BACK: backward of the norm (a backward without one is a forward with the angles' sign changed).
-template <typename T, int VE, int SLOTS, bool INTER, bool NORM, bool BACK>
+template <typename T, int VE, int SLOTS, bool WHOLE, bool INTER, bool NORM, bool BACK>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary p) {
   __shared__ float2 angles[kWarps][kMostHead / 2];
+  using Where = Slot<VE, INTER, WHOLE>;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int l = lane & (p.lanes - 1), group = lane / p.lanes, groups = 32 / p.lanes;
   const int t = blockIdx.x >= p.ctas[0];  // q or k
@@ -123,7 +136,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary p) {
   if constexpr (NORM) {
 #pragma unroll
     for (int j = 0; j < SLOTS; ++j) {
-      const Slot<VE, INTER> slot(l + j * p.lanes, p.pairs, p.D);
+      const Where slot(l + j * p.lanes, p.pairs, p.D);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
         w[j][e] = slot.has_a ? p.offset + param_at(p.weight[t], p.w_dtype[t], slot.a + e, 1.f) : 0.f;
@@ -132,107 +145,114 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary p) {
       }
     }
   }
-  const long long tasks = p.tokens * p.tasks_per_token[t];
+  const T* const tensor = static_cast<const T*>(p.in[t]);
+  const T* const xtensor = static_cast<const T*>(p.x[t]);
+  const long long head_stride = p.in_stride[t][2], xhead_stride = BACK ? p.x_stride[t][2] : 0;
+  const int per_token = p.tasks_per_token[t], per_task = p.per_task[t], heads = p.heads[t];
+  const long long tasks = p.tokens * per_token;
   for (long long task = (long long)cta * kWarps + warp; task < tasks; task += (long long)p.ctas[t] * kWarps) {
-    const long long token = task / p.tasks_per_token[t], b = token / p.S, s = token - b * p.S;
-    const int from = (int)(task - token * p.tasks_per_token[t]) * p.per_task[t], to = min(from + p.per_task[t], p.heads[t]);
+    const long long token = per_token == 1 ? task : task / per_token, b = p.S == p.tokens ? 0 : token / p.S, s = token - b * p.S;
+    const int from = (int)(task - token * per_token) * per_task, to = min(from + per_task, heads);
+    const T* in = tensor + b * p.in_stride[t][0] + s * p.in_stride[t][1];
+    const T* xs = BACK ? xtensor + b * p.x_stride[t][0] + s * p.x_stride[t][1] : nullptr;
+    // the heads of one turn of the warp; a group beyond the last head takes the last one again and stores nothing
+    Pack<T, VE> va[SLOTS], vb[SLOTS], xa[BACK ? SLOTS : 1], xb[BACK ? SLOTS : 1];
+    auto ask = [&](int base) {
+      const int head = min(base + group, to - 1);
+      const T* row = in + head * head_stride;
+      const T* xrow = xs + head * xhead_stride;
+#pragma unroll
+      for (int j = 0; j < SLOTS; ++j) {
+        const Where slot(l + j * p.lanes, p.pairs, p.D);
+        if (slot.has_a) va[j] = load_vec<T, VE>(row + slot.a);
+        if (slot.has_b) vb[j] = load_vec<T, VE>(row + slot.b);
+        if constexpr (BACK) {
+          if (slot.has_a) xa[j] = load_vec<T, VE>(xrow + slot.a);
+          if (slot.has_b) xb[j] = load_vec<T, VE>(xrow + slot.b);
+        }
+      }
+    };
+    ask(from);
     __syncwarp();
     token_angles(p, b, s, angles[warp]);
-    float cs[SLOTS][VE], sn[SLOTS][VE];
+    // The rotation's coefficients; the norm's weights are part of them forward, where nothing needs the rotated values without.
+    float aa[SLOTS][VE], ab[SLOTS][VE], bb[SLOTS][VE], ba[SLOTS][VE];
 #pragma unroll
     for (int j = 0; j < SLOTS; ++j) {
       const int slot = l + j * p.lanes;
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        const float2 v = (slot + 1) * VE <= p.pairs ? angles[warp][slot * VE + e] : make_float2(1.f, 0.f);
-        cs[j][e] = v.x;
-        sn[j][e] = v.y;
+        const float2 v = WHOLE || (slot + 1) * VE <= p.pairs ? angles[warp][slot * VE + e] : make_float2(1.f, 0.f);
+        if constexpr (NORM && !BACK) {
+          const int i = INTER ? 2 * e : e, k = INTER ? 2 * e + 1 : VE + e;
+          aa[j][e] = v.x * w[j][i], ab[j][e] = -v.y * w[j][k], bb[j][e] = v.x * w[j][k], ba[j][e] = v.y * w[j][i];
+        } else {
+          aa[j][e] = bb[j][e] = v.x, ab[j][e] = -v.y, ba[j][e] = v.y;
+        }
       }
     }
-    const T* in = static_cast<const T*>(p.in[t]) + b * p.in_stride[t][0] + s * p.in_stride[t][1];
-    const T* xs = BACK ? static_cast<const T*>(p.x[t]) + b * p.x_stride[t][0] + s * p.x_stride[t][1] : nullptr;
-    T* out = static_cast<T*>(p.out[t]) + token * p.heads[t] * p.D;
+    T* out = static_cast<T*>(p.out[t]) + token * heads * p.D;
     for (int base = from; base < to; base += groups) {
       const int head = base + group;
       const bool live = head < to;
-      Pack<T, VE> va[SLOTS], vb[SLOTS], xa[BACK ? SLOTS : 1], xb[BACK ? SLOTS : 1];
-#pragma unroll
-      for (int j = 0; j < SLOTS; ++j) {
-        const Slot<VE, INTER> slot(l + j * p.lanes, p.pairs, p.D);
-        const T* row = in + head * p.in_stride[t][2];
-        if (live && slot.has_a) va[j] = load_vec<T, VE>(row + slot.a);
-        if (live && slot.has_b) vb[j] = load_vec<T, VE>(row + slot.b);
-        if constexpr (BACK) {
-          const T* xrow = xs + head * p.x_stride[t][2];
-          if (live && slot.has_a) xa[j] = load_vec<T, VE>(xrow + slot.a);
-          if (live && slot.has_b) xb[j] = load_vec<T, VE>(xrow + slot.b);
-        }
-      }
       float f[SLOTS][2 * VE], n[BACK ? SLOTS : 1][2 * VE];
-      float sq = 0.f, dot = 0.f;
+      float sq[2] = {0.f, 0.f}, dot[2] = {0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < SLOTS; ++j) {
-        const Slot<VE, INTER> slot(l + j * p.lanes, p.pairs, p.D);
+        const Where slot(l + j * p.lanes, p.pairs, p.D);
         unpack_two<T, VE>(va[j], vb[j], f[j]);
         if constexpr (BACK) unpack_two<T, VE>(xa[j], xb[j], n[j]);
-#pragma unroll
-        for (int e = 0; e < 2 * VE; ++e) {
-          if (!live || !(e < VE ? slot.has_a : slot.has_b)) {
-            f[j][e] = 0.f;
-            if constexpr (BACK) n[j][e] = 0.f;
-          }
-        }
-        if constexpr (BACK) {
-          if (slot.turns) turn<VE, INTER>(f[j], cs[j], sn[j]);
+        if constexpr (!WHOLE) {
 #pragma unroll
           for (int e = 0; e < 2 * VE; ++e) {
-            sq = fmaf(n[j][e], n[j][e], sq);
-            dot = fmaf(f[j][e] * w[j][e], n[j][e], dot);
-          }
-        } else if constexpr (NORM) {
-#pragma unroll
-          for (int e = 0; e < 2 * VE; ++e) sq = fmaf(f[j][e], f[j][e], sq);
-        }
-      }
-      if constexpr (NORM) {
-        sq = lanes_sum(sq, p.lanes);
-        const float rstd = 1.f / sqrtf(fmaf(sq, p.inv_d, p.eps));
-        if constexpr (BACK) {
-          const float c = lanes_sum(dot, p.lanes) * rstd * p.inv_d;
-#pragma unroll
-          for (int j = 0; j < SLOTS; ++j) {
-#pragma unroll
-            for (int e = 0; e < 2 * VE; ++e) {
-              const float unit = n[j][e] * rstd;
-              if (live) dw[j][e] = fmaf(f[j][e], unit, dw[j][e]);
-              f[j][e] = rstd * fmaf(-unit, c, f[j][e] * w[j][e]);
+            if (!(e < VE ? slot.has_a : slot.has_b)) {
+              f[j][e] = 0.f;
+              if constexpr (BACK) n[j][e] = 0.f;
             }
           }
-        } else {
-#pragma unroll
-          for (int j = 0; j < SLOTS; ++j)
-#pragma unroll
-            for (int e = 0; e < 2 * VE; ++e) f[j][e] *= rstd * w[j][e];
         }
+        if constexpr (NORM && !BACK) dot_each(sq, f[j], f[j]);
+        if (slot.turns) {
+          turn<VE, INTER>(f[j], aa[j], ab[j], bb[j], ba[j]);
+        } else if constexpr (NORM && !BACK) {
+          mul_each(f[j], w[j]);
+        }
+        if constexpr (BACK) dot_each(sq, n[j], n[j]);
       }
-      if (!live) continue;
+      if (base + groups < to) ask(base + groups);
+      if constexpr (NORM) {
+        const float rstd = __frsqrt_rn(fmaf(lanes_sum(sq[0] + sq[1], p.lanes), p.inv_d, p.eps));
+        if constexpr (BACK) {
 #pragma unroll
-      for (int j = 0; j < SLOTS; ++j) {
-        const Slot<VE, INTER> slot(l + j * p.lanes, p.pairs, p.D);
-        if constexpr (!BACK) {
-          if (slot.turns) turn<VE, INTER>(f[j], cs[j], sn[j]);
+          for (int j = 0; j < SLOTS; ++j) {
+            scale_each(n[j], rstd);
+            if (live) fma_each(dw[j], f[j], n[j]);
+            mul_each(f[j], w[j]);
+            dot_each(dot, f[j], n[j]);
+          }
+          const float c = -lanes_sum(dot[0] + dot[1], p.lanes) * p.inv_d;
+#pragma unroll
+          for (int j = 0; j < SLOTS; ++j) axpy_each(f[j], n[j], c);
         }
-        float g[VE];
+#pragma unroll
+        for (int j = 0; j < SLOTS; ++j) scale_each(f[j], rstd);
+      }
+      if (live) {
         T* row = out + (long long)head * p.D;
-        if (slot.has_a) {
 #pragma unroll
-          for (int e = 0; e < VE; ++e) g[e] = f[j][e];
-          store_vec<T, VE>(row + slot.a, pack<T, VE>(g));
-        }
-        if (slot.has_b) {
+        for (int j = 0; j < SLOTS; ++j) {
+          const Where slot(l + j * p.lanes, p.pairs, p.D);
+          float g[VE];
+          if (slot.has_a) {
 #pragma unroll
-          for (int e = 0; e < VE; ++e) g[e] = f[j][VE + e];
-          store_vec<T, VE>(row + slot.b, pack<T, VE>(g));
+            for (int e = 0; e < VE; ++e) g[e] = f[j][e];
+            store_vec<T, VE>(row + slot.a, pack<T, VE>(g));
+          }
+          if (slot.has_b) {
+#pragma unroll
+            for (int e = 0; e < VE; ++e) g[e] = f[j][VE + e];
+            store_vec<T, VE>(row + slot.b, pack<T, VE>(g));
+          }
         }
       }
     }
@@ -243,7 +263,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary p) {
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < SLOTS; ++j) {
-      const Slot<VE, INTER> slot(l + j * p.lanes, p.pairs, p.D);
+      const Where slot(l + j * p.lanes, p.pairs, p.D);
 #pragma unroll
       for (int e = 0; e < 2 * VE; ++e) {
         float v = dw[j][e];
@@ -266,15 +286,17 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary p) {
 // ---------------------------------------------------------------------------------------------
 struct RotaryGeom {
   int ve, slots, lanes;
+  bool whole;
 };
 // ve: the widest vectors that the head, the pairs and (`widest`, by alignment) the tensors allow
-RotaryGeom rotary_geometry(int D, int pairs, int widest) {
-  RotaryGeom g = {widest, 1, 1};
+RotaryGeom rotary_geometry(int D, int pairs, int widest, int widest_full) {
+  RotaryGeom g = {widest, 1, 1, false};
   while (g.ve > 1 && (D % g.ve || pairs % g.ve)) g.ve = g.ve == 8 ? 4 : 1;
   const int count = pairs / g.ve + ((D - 2 * pairs) / g.ve + 1) / 2;
   while (g.lanes < 32 && g.lanes < count) g.lanes *= 2;
   while (g.slots * g.lanes < count) g.slots *= 2;
   if (g.ve == 1) g.slots = g.slots <= 2 ? 2 : 8;
+  g.whole = 2 * pairs == D && g.ve == widest_full && g.slots == 1 && pairs == g.ve * g.lanes;
   return g;
 }
 
@@ -282,18 +304,20 @@ template <int N>
 using Int = std::integral_constant<int, N>;
 template <typename T, typename F>
 cudaError_t with_rotary_geometry(const RotaryGeom& g, F&& f) {
+  if (g.whole) return f(Int<16 / (int)sizeof(T)>(), Int<1>(), std::true_type());
   if constexpr (sizeof(T) == 2) {
-    if (g.ve == 8) return f(Int<8>(), Int<1>());
+    if (g.ve == 8) return f(Int<8>(), Int<1>(), std::false_type());
   }
-  if (g.ve == 4) return g.slots == 1 ? f(Int<4>(), Int<1>()) : f(Int<4>(), Int<2>());
-  return g.slots == 2 ? f(Int<1>(), Int<2>()) : f(Int<1>(), Int<8>());
+  if (g.ve == 4) return g.slots == 1 ? f(Int<4>(), Int<1>(), std::false_type()) : f(Int<4>(), Int<2>(), std::false_type());
+  return g.slots == 2 ? f(Int<1>(), Int<2>(), std::false_type()) : f(Int<1>(), Int<8>(), std::false_type());
 }
 
 // How the tokens' heads are dealt out: warps take whole tokens where there are enough of them, else shares of a token's heads.
 cudaError_t rotary_split(const void* kernel, const RotaryGeom& g, Rotary& p) {
-  long long most = 0;
-  const cudaError_t err = resident_ctas(kernel, kThreads, &most);
+  Residency r;
+  const cudaError_t err = residency(kernel, kThreads, 0, &r);
   if (err != cudaSuccess) return err;
+  const long long most = (long long)r.per_sm * r.sms;
   const int groups = 32 / g.lanes, all = p.heads[0] + p.heads[1];
   long long want[2] = {0, 0};
   for (int t = 0; t < 2; ++t) {
@@ -316,7 +340,7 @@ cudaError_t rotary_split(const void* kernel, const RotaryGeom& g, Rotary& p) {
 
 // plan_only: p.ctas is all that is wanted
 cudaError_t launch_rotary(Rotary& p, int dtype, int widest, bool inter, bool norm, bool back, bool plan_only, cudaStream_t stream) {
-  const RotaryGeom g = rotary_geometry(p.D, p.pairs, widest);
+  const RotaryGeom g = rotary_geometry(p.D, p.pairs, widest, dtype == GNB200_F32 ? 4 : 8);
   p.lanes = g.lanes;
   auto go = [&](void (*kernel)(const Rotary)) {
     const cudaError_t err = rotary_split((const void*)kernel, g, p);
@@ -326,14 +350,15 @@ cudaError_t launch_rotary(Rotary& p, int dtype, int widest, bool inter, bool nor
   };
   auto typed = [&](auto type) {
     using T = decltype(type);
-    return with_rotary_geometry<T>(g, [&](auto ve, auto slots) {
+    return with_rotary_geometry<T>(g, [&](auto ve, auto slots, auto whole) {
       constexpr int VE = decltype(ve)::value, S = decltype(slots)::value;
+      constexpr bool W = decltype(whole)::value;
       if (inter) {
-        if (back) return go(&rotary_kernel<T, VE, S, true, true, true>);
-        return norm ? go(&rotary_kernel<T, VE, S, true, true, false>) : go(&rotary_kernel<T, VE, S, true, false, false>);
+        if (back) return go(&rotary_kernel<T, VE, S, W, true, true, true>);
+        return norm ? go(&rotary_kernel<T, VE, S, W, true, true, false>) : go(&rotary_kernel<T, VE, S, W, true, false, false>);
       }
-      if (back) return go(&rotary_kernel<T, VE, S, false, true, true>);
-      return norm ? go(&rotary_kernel<T, VE, S, false, true, false>) : go(&rotary_kernel<T, VE, S, false, false, false>);
+      if (back) return go(&rotary_kernel<T, VE, S, W, false, true, true>);
+      return norm ? go(&rotary_kernel<T, VE, S, W, false, true, false>) : go(&rotary_kernel<T, VE, S, W, false, false, false>);
     });
   };
   if (dtype == GNB200_F32) return typed(float());

@@ -1,8 +1,9 @@
 // Building blocks of the kernels on token rows (gn_rms.cu, gn_rotary.cu): vectors of any power-of-two width, sums
-// over the lanes or the warps that share a row, parameters of either type, and the number of CTAs that are resident at once.
+// over the lanes or the warps that share a row, parameters of either type, and the CTAs that an SM holds at once.
 #pragma once
 #include <cuda_fp8.h>
 
+#include <array>
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -10,6 +11,8 @@
 #include "gn_common.cuh"
 
 namespace gnb200 {
+
+constexpr int kMostDynamicSmem = 220 << 10;  // of an SM's 227 KB: the kernels have a few KB of static shared memory beside it
 
 // VE consecutive elements; aligned to their size, or to 16 bytes where they are 32 (8 floats beside 8 halves)
 template <typename T, int VE>
@@ -44,6 +47,11 @@ __device__ __forceinline__ void store_vec(T* p, const Pack<T, VE>& v) {
   }
 }
 
+// 16 bytes from global to shared memory, asynchronously; the first `bytes` of them from memory, zeros for the others
+__device__ __forceinline__ void cp_async16_part(uint32_t smem_dst, const void* gmem_src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_dst), "l"(gmem_src), "r"(bytes) : "memory");
+}
+
 // element i of a parameter vector of type `dtype` (0 fp32, 1 fp16, 2 bf16); `none` where there is no vector
 __device__ __forceinline__ float param_at(const void* p, int dtype, long long i, float none) {
   if (p == nullptr) return none;
@@ -60,34 +68,144 @@ __device__ __forceinline__ void store_param_at(void* p, int dtype, long long i, 
     static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
+// VE parameters starting at element i, on the vector path from aligned addresses
+template <int VE>
+__device__ __forceinline__ void params_at(const void* p, int dtype, long long i, float (&f)[VE]) {
+  if constexpr (VE == 1) {
+    f[0] = param_at(p, dtype, i, 1.f);
+  } else if (dtype == 0) {
+    unpack<float, VE>(load_vec<float, VE>(static_cast<const float*>(p) + i), f);
+  } else if (dtype == 1) {
+    unpack<__half, VE>(load_vec<__half, VE>(static_cast<const __half*>(p) + i), f);
+  } else {
+    unpack<__nv_bfloat16, VE>(load_vec<__nv_bfloat16, VE>(static_cast<const __nv_bfloat16*>(p) + i), f);
+  }
+}
+
+// Lane by lane over a vector, two lanes an instruction where there are pairs (the same bits as one by one): a += b, a *= b, a *= s,
+// a += b * c (vectors), a += b * c (c a number).
+template <int N>
+__device__ __forceinline__ void add_each(float (&a)[N], const float (&b)[N]) {
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) add2(a[e], a[e + 1], a[e], a[e + 1], b[e], b[e + 1]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) a[e] += b[e];
+  }
+}
+template <int N>
+__device__ __forceinline__ void mul_each(float (&a)[N], const float (&b)[N]) {
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) mul2(a[e], a[e + 1], a[e], a[e + 1], b[e], b[e + 1]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) a[e] *= b[e];
+  }
+}
+template <int N>
+__device__ __forceinline__ void scale_each(float (&a)[N], float s) {
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) mul2(a[e], a[e + 1], a[e], a[e + 1], s, s);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) a[e] *= s;
+  }
+}
+template <int N>
+__device__ __forceinline__ void fma_each(float (&a)[N], const float (&b)[N], const float (&c)[N]) {
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) fma2(a[e], a[e + 1], b[e], b[e + 1], c[e], c[e + 1], a[e], a[e + 1]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) a[e] = fmaf(b[e], c[e], a[e]);
+  }
+}
+template <int N>
+__device__ __forceinline__ void axpy_each(float (&a)[N], const float (&b)[N], float c) {
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) fma2(a[e], a[e + 1], b[e], b[e + 1], c, c, a[e], a[e + 1]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) a[e] = fmaf(b[e], c, a[e]);
+  }
+}
+// acc += sum of a * b, over even and odd lanes apart
+template <int N>
+__device__ __forceinline__ void dot_each(float (&acc)[2], const float (&a)[N], const float (&b)[N]) {
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) fma2(acc[0], acc[1], a[e], a[e + 1], b[e], b[e + 1], acc[0], acc[1]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e & 1] = fmaf(a[e], b[e], acc[e & 1]);
+  }
+}
+
 // The sum over `lanes` neighbouring lanes (a power of two), the same bits in each: a butterfly adds the same two numbers on both sides.
 __device__ __forceinline__ float lanes_sum(float v, int lanes) {
-  for (int delta = lanes >> 1; delta >= 1; delta >>= 1) v += __shfl_xor_sync(0xffffffffu, v, delta);
+#pragma unroll
+  for (int delta = 16; delta >= 1; delta >>= 1)
+    if (lanes > delta) v += __shfl_xor_sync(0xffffffffu, v, delta);
   return v;
 }
+// (Shuffles for the maximum too: with __reduce_max_sync one of the kernels gave lane 0's value to all lanes.)
 // Magnitudes compare like their bit patterns, with NaN above infinity: an integer maximum keeps a NaN, fmaxf would drop it.
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 __device__ __forceinline__ uint32_t lanes_max(uint32_t v, int lanes) {
-  for (int delta = lanes >> 1; delta >= 1; delta >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, delta));
+#pragma unroll
+  for (int delta = 16; delta >= 1; delta >>= 1)
+    if (lanes > delta) v = max(v, __shfl_xor_sync(0xffffffffu, v, delta));
   return v;
 }
 
-// Sum over the CTA in a fixed order, one barrier.  `slots`: two rows of 32 floats, used in turn: a thread that writes a row
-// again has passed the barrier behind which nobody reads it any more.
-__device__ __forceinline__ float cta_sum(float v, float (*slots)[32], int& turn) {
-  const int warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
+// Teams of whole warps: a barrier of their own (hardware barriers 1 to 15), and the sum over a team in a fixed order behind one of
+// them.  The slots are two rows used in turn: a thread that writes a row again has passed the barrier behind which nobody reads it any
+// more.  The places of warps that are not there hold zeros.
+constexpr int kMostWarps = 16, kMostTeams = 15;
+struct TeamSlots {
+  alignas(16) float row[2][kMostWarps];
+};
+template <bool TEAMS>  // false: the team is the CTA
+__device__ __forceinline__ void team_barrier(int threads, int team) {
+  if constexpr (TEAMS) {
+    __syncwarp();
+    asm volatile("barrier.sync %0, %1;" ::"r"(team + 1), "r"(threads) : "memory");
+  } else {
+    __syncthreads();
+  }
+}
+template <bool TEAMS>
+__device__ __forceinline__ void clear(TeamSlots& slots, int threads, int team, int first) {
+  if (first < 2 * kMostWarps) slots.row[first / kMostWarps][first % kMostWarps] = 0.f;
+  team_barrier<TEAMS>(threads, team);
+}
+template <bool TEAMS>
+__device__ __forceinline__ float team_sum(float v, TeamSlots& slots, int& turn, int threads, int team) {
   v = lanes_sum(v, 32);
-  float* row = slots[turn];
+  float* row = slots.row[turn];
   turn ^= 1;
-  if ((threadIdx.x & 31) == 0) row[warp] = v;
-  __syncthreads();
-  float t = 0.f;
-  for (int w = 0; w < nwarps; ++w) t += row[w];
-  return t;
+  if ((threadIdx.x & 31) == 0) row[(threadIdx.x - (TEAMS ? team * threads : 0)) >> 5] = v;
+  team_barrier<TEAMS>(threads, team);
+  const float4* four = reinterpret_cast<const float4*>(row);
+  float4 t = four[0];
+  if (threads > 128) {
+    const float4 u = four[1];
+    t.x += u.x, t.y += u.y, t.z += u.z, t.w += u.w;
+  }
+  if (threads > 256) {
+    const float4 u = four[2], w = four[3];
+    t.x += u.x + w.x, t.y += u.y + w.y, t.z += u.z + w.z, t.w += u.w + w.w;
+  }
+  return (t.x + t.y) + (t.z + t.w);
 }
 __device__ __forceinline__ uint32_t cta_max(uint32_t v, uint32_t* slots) {  // (a barrier of the caller's lies between two calls)
   const int warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
-  v = __reduce_max_sync(0xffffffffu, v);
+  v = lanes_max(v, 32);
   if ((threadIdx.x & 31) == 0) slots[warp] = v;
   __syncthreads();
   uint32_t t = 0;
@@ -95,29 +213,59 @@ __device__ __forceinline__ uint32_t cta_max(uint32_t v, uint32_t* slots) {  // (
   return t;
 }
 
-// CTAs of `kernel` that the current device holds at once (asked once per kernel, CTA size and device)
-inline cudaError_t resident_ctas(const void* kernel, int threads, long long* out) {
+// CTAs of `kernel` that one SM holds at once with `smem` bytes of dynamic shared memory, and the SMs of the current device (asked once per
+// kernel, CTA size, shared memory and device; the first question raises the kernel's limit of shared memory)
+struct Residency {
+  int per_sm, sms;
+};
+inline cudaError_t residency(const void* kernel, int threads, int smem, Residency* out) {
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
   static std::mutex mu;
-  static std::map<std::tuple<const void*, int, int>, long long> known;
+  static std::map<std::tuple<const void*, int, int, int>, Residency> known;
   std::lock_guard<std::mutex> lock(mu);
-  const auto key = std::make_tuple(kernel, threads, dev);
+  const auto key = std::make_tuple(kernel, threads, smem, dev);
   const auto it = known.find(key);
   if (it != known.end()) {
     *out = it->second;
     return cudaSuccess;
   }
-  int sms = 0, per_sm = 0;
-  err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  Residency r = {};
+  err = cudaDeviceGetAttribute(&r.sms, cudaDevAttrMultiProcessorCount, dev);
   if (err != cudaSuccess) return err;
-  err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0);
+  if (smem > 0) {
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostDynamicSmem);
+    if (err != cudaSuccess) return err;
+  }
+  err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&r.per_sm, kernel, threads, smem);
   if (err != cudaSuccess) return err;
-  if (per_sm < 1) return cudaErrorLaunchOutOfResources;
-  *out = known[key] = (long long)sms * per_sm;
+  if (r.per_sm < 1) return cudaErrorLaunchOutOfResources;
+  *out = known[key] = r;
   return cudaSuccess;
 }
+
+// The last answers to a question that a program asks again and again with the same few arguments
+template <int N>
+struct Remembered {
+  using Key = std::array<int64_t, N>;
+  const size_t* find(const Key& key) const {
+    for (int i = 0; i < used; ++i)
+      if (keys[i] == key) return &values[i];
+    return nullptr;
+  }
+  size_t keep(const Key& key, size_t value) {
+    keys[next] = key;
+    values[next] = value;
+    if (used < kPlaces) ++used;
+    next = (next + 1) % kPlaces;
+    return value;
+  }
+  static constexpr int kPlaces = 16;
+  std::array<Key, kPlaces> keys;
+  size_t values[kPlaces];
+  int used = 0, next = 0;
+};
 
 // Sums over the rows of up to two sets of C columns, in a fixed order, stored as `dtype` (gn_rms.cu); a programmatic dependent of the
 // kernel before it, which writes `part` (`chained`; otherwise in plain stream order)
