@@ -44,28 +44,93 @@ struct Rotary {
   float eps, offset, inv_d, sign;
 };
 
-// cos and sin of this token's angles, into the warp's shared memory
-__device__ __forceinline__ void token_angles(const Rotary& p, long long b, long long s, float2* out) {
-  const long long at = b * p.pos_stride[0] + s * p.pos_stride[1];
-  for (int i = threadIdx.x & 31; i < p.pairs; i += 32) {
+constexpr double kPerTurn = 0.15915494309189535;  // 1 / (2 pi)
+
+// What a CTA knows of its pairs: inv_freq / (2 pi) as the sum of two floats, and the axis.
+struct PairTable {
+  float2 turns[kMostHead / 2];
+  uint8_t axis[kMostHead / 2];
+};
+__device__ __forceinline__ void fill_pairs(const Rotary& p, PairTable& table) {
+  for (int i = threadIdx.x; i < p.pairs; i += kThreads) {
+    const double turns = (double)p.inv_freq[i] * kPerTurn;
+    const float hi = (float)turns;
+    table.turns[i] = make_float2(hi, (float)(turns - (double)hi));
     int axis = 0;
     while (axis + 1 < p.axes && i >= p.last[axis]) ++axis;
-    const long long from = at + axis * p.pos_stride[2];
-    double position;
-    if (p.pos_type == GNB200_POS_I64)
-      position = (double)static_cast<const long long*>(p.positions)[from];
-    else if (p.pos_type == GNB200_POS_I32)
-      position = (double)static_cast<const int*>(p.positions)[from];
-    else
-      position = (double)static_cast<const float*>(p.positions)[from];
-    double turns = position * (double)p.inv_freq[i] * 0.15915494309189535;  // 1 / (2 pi)
-    turns -= rint(turns);
-    float sn, cs;
-    sincospif((float)(2.0 * turns), &sn, &cs);
-    out[i] = make_float2(cs, p.sign * sn);
+    table.axis[i] = (uint8_t)axis;
+  }
+}
+
+// A lane's share of a token's positions: those of pairs lane and lane + 32 (asked for a token ahead; further ones as they are needed).
+struct Positions {
+  long long raw[2];
+};
+__device__ __forceinline__ long long position_at(const Rotary& p, long long at) {
+  if (p.pos_type == GNB200_POS_I64) return static_cast<const long long*>(p.positions)[at];
+  return static_cast<const int*>(p.positions)[at];  // (or the bits of a float)
+}
+__device__ __forceinline__ void ask_positions(const Rotary& p, const PairTable& table, long long b, long long s, Positions& out) {
+  const long long at = b * p.pos_stride[0] + s * p.pos_stride[1];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int i = (int)(threadIdx.x & 31) + 32 * k;
+    if (i < p.pairs) out.raw[k] = position_at(p, at + table.axis[i] * p.pos_stride[2]);
+  }
+}
+
+// cos and sin of pair i's angle.  It is formed in turns, whole ones dropped: position * hi in fp32, what its rounding lost (an fma gives it
+// exactly) and position * lo.  That holds for positions that fp32 holds exactly; larger ones are multiplied in fp64.  FAST: the hardware's
+// sine and cosine, off by 2^-21 on the remaining half turns, for results that are rounded to 16 bits.
+template <bool FAST>
+__device__ __forceinline__ float2 angle_of(const Rotary& p, const PairTable& table, int i, long long raw) {
+  const float2 freq = table.turns[i];
+  const bool is_float = p.pos_type == GNB200_POS_F32;
+  const float position = is_float ? __int_as_float((int)raw) : (float)(int)raw;
+  const bool exact = is_float ? fabsf(position) < 16777216.f : (raw < 16777216 && raw > -16777216);
+  float part;
+  if (exact) {
+    const float turns = position * freq.x;
+    part = (turns - rintf(turns)) + fmaf(position, freq.y, fmaf(position, freq.x, -turns));
+  } else {
+    const double turns = (is_float ? (double)position : (double)raw) * ((double)p.inv_freq[i] * kPerTurn);
+    part = (float)(turns - rint(turns));
+  }
+  float sn, cs;
+  if constexpr (FAST) {
+    part -= rintf(part);  // (the two parts' sum may have passed half a turn)
+    const float radians = part * 6.28318531f;
+    sn = __sinf(radians);
+    cs = __cosf(radians);
+  } else {
+    sincospif(2.f * part, &sn, &cs);
+  }
+  return make_float2(cs, p.sign * sn);
+}
+
+// cos and sin of a token's angles, into the warp's shared memory
+template <bool FAST>
+__device__ __forceinline__ void token_angles(const Rotary& p, const PairTable& table, long long b, long long s, const Positions& known, float2* out) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();  // (nobody reads the token before any more)
+  if (lane < p.pairs) out[lane] = angle_of<FAST>(p, table, lane, known.raw[0]);
+  if (lane + 32 < p.pairs) out[lane + 32] = angle_of<FAST>(p, table, lane + 32, known.raw[1]);
+  if (p.pairs > 64) {
+    const long long at = b * p.pos_stride[0] + s * p.pos_stride[1];
+    for (int i = lane + 64; i < p.pairs; i += 32) out[i] = angle_of<FAST>(p, table, i, position_at(p, at + table.axis[i] * p.pos_stride[2]));
   }
   __syncwarp();
 }
+
+// The heads ahead.  16-byte vectors travel to the warp's ring of stages in shared memory, one stage a turn of the warp, where a lane
+// finds what it copied itself; shorter ones to registers, one turn ahead.
+template <typename T, int VE>
+constexpr bool kRing = sizeof(T) * VE == 16;
+template <bool RING, int STAGES, int VECTORS>  // VECTORS: a lane's, of a turn
+struct Ring {
+  static constexpr int kStages = RING ? STAGES : 1;
+  uint4 at[RING ? kWarps : 1][kStages][RING ? VECTORS : 1][RING ? 32 : 1];
+};
 
 // Where a lane's slot of two vectors stands in the head.  Slots 0 .. pairs / VE - 1 are turned, the others pass.  WHOLE: the head is
 // turned from end to end and every lane has one slot.
@@ -77,8 +142,8 @@ struct Slot {
     const int rotated = pairs / VE;
     turns = WHOLE || s < rotated;
     if (turns) {
-      a = INTER ? 2 * s * VE : s * VE;
-      b = INTER ? a + VE : pairs + s * VE;
+      a = INTER && VE == 1 ? 2 * s : s * VE;
+      b = INTER && VE == 1 ? 2 * s + 1 : pairs + s * VE;
     } else {
       a = 2 * pairs + 2 * (s - rotated) * VE;
       b = a + VE;
@@ -86,7 +151,43 @@ struct Slot {
     has_a = WHOLE || a < D;
     has_b = WHOLE || b < D;
   }
+  // the pair that is turned by the slot's coefficient e; its channels are those of elements first(e) and second(e) of the slot
+  __device__ __forceinline__ int pair(int e) const {
+    if constexpr (!INTER) return a + e;
+    if constexpr (VE == 1) return a / 2;
+    return e < VE / 2 ? a / 2 + e : b / 2 + e - VE / 2;
+  }
+  static __device__ __forceinline__ constexpr int first(int e) { return INTER ? 2 * e : e; }
+  static __device__ __forceinline__ constexpr int second(int e) { return INTER ? 2 * e + 1 : VE + e; }
+  __device__ __forceinline__ int channel(int i) const { return i < VE ? a + i : b + i - VE; }
 };
+
+// cos and sin of the slot's pairs, two pairs a load (they lie together, on 16 bytes)
+template <int VE, typename Slot>
+__device__ __forceinline__ void read_angles(const float2* angles, const Slot& slot, float2 (&v)[VE]) {
+  if constexpr (VE == 1) {
+    v[0] = angles[slot.pair(0)];
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE; e += 2) {
+      const float4 two = *reinterpret_cast<const float4*>(&angles[slot.pair(e)]);
+      v[e] = make_float2(two.x, two.y);
+      v[e + 1] = make_float2(two.z, two.w);
+    }
+  }
+}
+template <int VE>
+__device__ __forceinline__ void read_weights(const float* w, float* out) {
+  if constexpr (VE == 1) {
+    out[0] = w[0];
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE; e += 4) {
+      const float4 four = *reinterpret_cast<const float4*>(w + e);
+      out[e] = four.x, out[e + 1] = four.y, out[e + 2] = four.z, out[e + 3] = four.w;
+    }
+  }
+}
 
 // (a, b) -> (a aa + b ab, b bb + a ba) for the pairs of f, the slot's two vectors
 template <int VE, bool INTER>
@@ -122,162 +223,374 @@ __device__ __forceinline__ void unpack_two(const Pack<T, VE>& a, const Pack<T, V
   for (int e = 0; e < VE; ++e) f[VE + e] = g[e];
 }
 
-// SLOTS: slots a lane.  BACK: backward of the norm (a backward without one is a forward with the angles' sign changed).
-template <typename T, int VE, int SLOTS, bool WHOLE, bool INTER, bool NORM, bool BACK>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary p) {
-  __shared__ float2 angles[kWarps][kMostHead / 2];
+template <typename T, int VE>
+__device__ __forceinline__ void store_two(T* row, int a, int b, bool has_a, bool has_b, const float (&f)[2 * VE]) {
+  float g[VE];
+  if (has_a) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) g[e] = f[e];
+    store_vec<T, VE>(row + a, pack<T, VE>(g));
+  }
+  if (has_b) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) g[e] = f[VE + e];
+    store_vec<T, VE>(row + b, pack<T, VE>(g));
+  }
+}
+
+// SLOTS: slots a lane.  Forward, and backward where there is no norm (the angles' sign changed).  A task is a token's heads of q and then of
+// k, or a share of both, so that the angles serve both; a warp's turn takes the next `groups` of them.
+template <typename T, int VE, int SLOTS, bool WHOLE, bool INTER, bool NORM>
+__global__ void __launch_bounds__(kThreads) rotary_fwd_kernel(const Rotary p) {
+  __shared__ alignas(16) float2 angles[kWarps][kMostHead / 2];
+  __shared__ PairTable table;
+  __shared__ alignas(16) float weights[NORM ? 2 : 1][NORM ? kMostHead : 1];
+  constexpr bool RING = kRing<T, VE>;
+  __shared__ Ring<RING, NORM ? 4 : 2, 2 * SLOTS> ring;
+  constexpr int STAGES = decltype(ring)::kStages;
+  using Where = Slot<VE, INTER, WHOLE>;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int l = lane & (p.lanes - 1), group = lane / p.lanes, groups = 32 / p.lanes;
+  const int per_token = p.tasks_per_token[0];
+  const long long tasks = p.tokens * per_token, step = (long long)gridDim.x * kWarps;
+  const auto token_of = [&](long long task, long long& b, long long& s) {
+    const long long token = per_token == 1 ? task : task / per_token;
+    b = p.S == p.tokens ? 0 : token / p.S;
+    s = token - b * p.S;
+    return token;
+  };
+  // the heads of q (t = 0) or k that are a task's
+  const auto heads_from = [&](long long task, long long token, int t) { return min((int)(task - token * per_token) * p.per_task[t], p.heads[t]); };
+  const auto heads_to = [&](int from, int t) { return min(from + p.per_task[t], p.heads[t]); };
+
+  // What is asked for next: the warp's next turn of a task's heads of q, then of k; row: this lane's head.
+  const long long first_task = (long long)blockIdx.x * kWarps + warp;
+  long long asked = first_task - step, row_step = 0;
+  int ask_t = 1, ask_head = 0, ask_to = 0, ask_stage = 0;
+  const T* row = nullptr;
+  const auto advance = [&]() {  // to the next heads that there are
+    do {
+      if (ask_t == 1) asked += step;
+      ask_t ^= 1;
+      if (asked >= tasks) return;
+      long long b, s;
+      const long long token = token_of(asked, b, s);
+      const int from = heads_from(asked, token, ask_t);
+      ask_to = heads_to(from, ask_t);
+      ask_head = from + group;
+      row = static_cast<const T*>(p.in[ask_t]) + b * p.in_stride[ask_t][0] + s * p.in_stride[ask_t][1] + ask_head * p.in_stride[ask_t][2];
+      row_step = groups * p.in_stride[ask_t][2];
+    } while (ask_head - group >= ask_to);
+  };
+  Pack<T, VE> va[SLOTS], vb[SLOTS];
+  const auto ask = [&]() {
+    if (ask_head < ask_to && asked < tasks) {
+#pragma unroll
+      for (int j = 0; j < SLOTS; ++j) {
+        const Where slot(l + j * p.lanes, p.pairs, p.D);
+        if constexpr (RING) {
+          if (slot.has_a) cp_async16(smem_addr(&ring.at[warp][ask_stage][2 * j][lane]), row + slot.a);
+          if (slot.has_b) cp_async16(smem_addr(&ring.at[warp][ask_stage][2 * j + 1][lane]), row + slot.b);
+        } else {
+          if (slot.has_a) va[j] = load_vec<T, VE>(row + slot.a);
+          if (slot.has_b) vb[j] = load_vec<T, VE>(row + slot.b);
+        }
+      }
+    }
+    if constexpr (RING) {
+      cp_async_commit();
+      ask_stage = (ask_stage + 1) % STAGES;
+    }
+    row += row_step;
+    ask_head += groups;
+    if (ask_head - group >= ask_to && asked < tasks) advance();
+  };
+  advance();
+#pragma unroll
+  for (int i = 0; i < STAGES; ++i) ask();
+  fill_pairs(p, table);
+  if constexpr (NORM) {
+    for (int i = threadIdx.x; i < 2 * p.D; i += kThreads) {
+      const int t = i >= p.D, at = i - t * p.D;
+      if (p.heads[t]) weights[t][at] = p.offset + param_at(p.weight[t], p.w_dtype[t], at, 1.f);
+    }
+  }
+  __syncthreads();
+  Positions positions = {};
+  long long b = 0, s = 0, token = 0;
+  if (first_task < tasks) {
+    token = token_of(first_task, b, s);
+    ask_positions(p, table, b, s, positions);
+  }
+  int stage = 0;
+  for (long long task = first_task; task < tasks; task += step) {
+    token_angles<sizeof(T) == 2>(p, table, b, s, positions, angles[warp]);
+    const long long now = token;
+    if (task + step < tasks) {
+      token = token_of(task + step, b, s);
+      ask_positions(p, table, b, s, positions);
+    }
+    float aa[SLOTS][VE], ab[SLOTS][VE], bb[SLOTS][VE], ba[SLOTS][VE];
+    bool have = false;
+#pragma unroll 1
+    for (int t = 0; t < 2; ++t) {
+      const int from = heads_from(task, now, t), to = heads_to(from, t);
+      if (from >= to) continue;
+      if (NORM || !have) {
+        // The rotation's coefficients, the norm's weights among them.
+        have = true;
+        const float* w = weights[NORM ? t : 0];
+#pragma unroll
+        for (int j = 0; j < SLOTS; ++j) {
+          const Where slot(l + j * p.lanes, p.pairs, p.D);
+          float2 v[VE];
+          if (slot.turns) read_angles<VE>(angles[warp], slot, v);
+          if constexpr (NORM) {
+            float wi[2 * VE] = {};
+            if (slot.has_a) read_weights<VE>(w + slot.a, wi);
+            if (slot.has_b) read_weights<VE>(w + slot.b, wi + VE);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+              if (slot.turns) {
+                const float first = wi[Where::first(e)], second = wi[Where::second(e)];
+                aa[j][e] = v[e].x * first, ab[j][e] = -v[e].y * second, bb[j][e] = v[e].x * second, ba[j][e] = v[e].y * first;
+              } else {  // (the weights alone)
+                aa[j][e] = wi[e], bb[j][e] = wi[VE + e], ab[j][e] = ba[j][e] = 0.f;
+              }
+            }
+          } else if (slot.turns) {
+#pragma unroll
+            for (int e = 0; e < VE; ++e) aa[j][e] = bb[j][e] = v[e].x, ab[j][e] = -v[e].y, ba[j][e] = v[e].y;
+          }
+        }
+      }
+      T* out = static_cast<T*>(p.out[t]) + (now * p.heads[t] + from + group) * p.D;
+      const int out_step = groups * p.D;
+      for (int head = from + group; head - group < to; head += groups, out += out_step) {
+        if constexpr (RING) cp_async_wait<STAGES - 1>();
+        float f[SLOTS][2 * VE];
+        float sq[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < SLOTS; ++j) {
+          const Where slot(l + j * p.lanes, p.pairs, p.D);
+          if constexpr (RING) {
+            va[j] = load_vec<T, VE>(reinterpret_cast<const T*>(&ring.at[warp][stage][2 * j][lane]));
+            vb[j] = load_vec<T, VE>(reinterpret_cast<const T*>(&ring.at[warp][stage][2 * j + 1][lane]));
+          }
+          unpack_two<T, VE>(va[j], vb[j], f[j]);
+          if constexpr (!WHOLE) {
+#pragma unroll
+            for (int e = 0; e < 2 * VE; ++e)
+              if (!(e < VE ? slot.has_a : slot.has_b)) f[j][e] = 0.f;
+          }
+          if constexpr (NORM) dot_each(sq, f[j], f[j]);
+          if (slot.turns) {
+            turn<VE, INTER>(f[j], aa[j], ab[j], bb[j], ba[j]);
+          } else if constexpr (NORM) {
+#pragma unroll
+            for (int e = 0; e < VE; ++e) f[j][e] *= aa[j][e], f[j][VE + e] *= bb[j][e];
+          }
+        }
+        if constexpr (RING) stage = (stage + 1) % STAGES;
+        ask();
+        if constexpr (NORM) {
+          const float rstd = __frsqrt_rn(fmaf(lanes_sum(sq[0] + sq[1], p.lanes), p.inv_d, p.eps));
+#pragma unroll
+          for (int j = 0; j < SLOTS; ++j) scale_each(f[j], rstd);
+        }
+        if (head < to) {  // (a group beyond the last head has nothing to store)
+#pragma unroll
+          for (int j = 0; j < SLOTS; ++j) {
+            const Where slot(l + j * p.lanes, p.pairs, p.D);
+            store_two<T, VE>(out, slot.a, slot.b, slot.has_a, slot.has_b, f[j]);
+          }
+        }
+      }
+    }
+  }
+}
+
+// Backward of the norm.  A CTA takes heads of q or of k alone, since a lane's sums for the weight's gradient stand in registers.
+template <typename T, int VE, int SLOTS, bool WHOLE, bool INTER>
+__global__ void __launch_bounds__(kThreads) rotary_bwd_kernel(const Rotary p) {
+  __shared__ alignas(16) float2 angles[kWarps][kMostHead / 2];
+  __shared__ PairTable table;
+  constexpr bool RING = kRing<T, VE>;
+  __shared__ Ring<RING, 2, 4 * SLOTS> ring;
+  constexpr int STAGES = decltype(ring)::kStages;
   using Where = Slot<VE, INTER, WHOLE>;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int l = lane & (p.lanes - 1), group = lane / p.lanes, groups = 32 / p.lanes;
   const int t = blockIdx.x >= p.ctas[0];  // q or k
   const unsigned cta = blockIdx.x - (t ? p.ctas[0] : 0);
-  if constexpr (BACK) grid_dep_launch_dependents();
-  float w[NORM ? SLOTS : 1][2 * VE], dw[BACK ? SLOTS : 1][2 * VE];
-  if constexpr (NORM) {
-#pragma unroll
-    for (int j = 0; j < SLOTS; ++j) {
-      const Where slot(l + j * p.lanes, p.pairs, p.D);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        w[j][e] = slot.has_a ? p.offset + param_at(p.weight[t], p.w_dtype[t], slot.a + e, 1.f) : 0.f;
-        w[j][VE + e] = slot.has_b ? p.offset + param_at(p.weight[t], p.w_dtype[t], slot.b + e, 1.f) : 0.f;
-        if constexpr (BACK) dw[j][e] = dw[j][VE + e] = 0.f;
-      }
-    }
-  }
-  const T* const tensor = static_cast<const T*>(p.in[t]);
-  const T* const xtensor = static_cast<const T*>(p.x[t]);
-  const long long head_stride = p.in_stride[t][2], xhead_stride = BACK ? p.x_stride[t][2] : 0;
+  grid_dep_launch_dependents();
   const int per_token = p.tasks_per_token[t], per_task = p.per_task[t], heads = p.heads[t];
-  const long long tasks = p.tokens * per_token;
-  for (long long task = (long long)cta * kWarps + warp; task < tasks; task += (long long)p.ctas[t] * kWarps) {
-    const long long token = per_token == 1 ? task : task / per_token, b = p.S == p.tokens ? 0 : token / p.S, s = token - b * p.S;
-    const int from = (int)(task - token * per_token) * per_task, to = min(from + per_task, heads);
-    const T* in = tensor + b * p.in_stride[t][0] + s * p.in_stride[t][1];
-    const T* xs = BACK ? xtensor + b * p.x_stride[t][0] + s * p.x_stride[t][1] : nullptr;
-    // the heads of one turn of the warp; a group beyond the last head takes the last one again and stores nothing
-    Pack<T, VE> va[SLOTS], vb[SLOTS], xa[BACK ? SLOTS : 1], xb[BACK ? SLOTS : 1];
-    auto ask = [&](int base) {
-      const int head = min(base + group, to - 1);
-      const T* row = in + head * head_stride;
-      const T* xrow = xs + head * xhead_stride;
+  const long long tasks = p.tokens * per_token, step = (long long)p.ctas[t] * kWarps;
+  const auto token_of = [&](long long task, long long& b, long long& s) {
+    const long long token = per_token == 1 ? task : task / per_token;
+    b = p.S == p.tokens ? 0 : token / p.S;
+    s = token - b * p.S;
+    return token;
+  };
+  // what is asked for next: the warp's next turn of a task's heads; in, xs: this lane's head of the gradient and of the input
+  const long long first_task = (long long)cta * kWarps + warp;
+  const long long in_step = groups * p.in_stride[t][2], xs_step = groups * p.x_stride[t][2];
+  long long asked = first_task;
+  int ask_head = 0, ask_to = 0, ask_stage = 0;
+  const T *in = nullptr, *xs = nullptr;
+  const auto open = [&]() {
+    long long b, s;
+    const long long token = token_of(asked, b, s);
+    const int from = (int)(asked - token * per_token) * per_task;
+    ask_head = from + group;
+    ask_to = min(from + per_task, heads);
+    in = static_cast<const T*>(p.in[t]) + b * p.in_stride[t][0] + s * p.in_stride[t][1] + ask_head * p.in_stride[t][2];
+    xs = static_cast<const T*>(p.x[t]) + b * p.x_stride[t][0] + s * p.x_stride[t][1] + ask_head * p.x_stride[t][2];
+  };
+  Pack<T, VE> v[SLOTS][4];  // of a slot: the gradient's two vectors, the input's two
+  const auto ask = [&]() {
+    if (ask_head < ask_to && asked < tasks) {
 #pragma unroll
       for (int j = 0; j < SLOTS; ++j) {
         const Where slot(l + j * p.lanes, p.pairs, p.D);
-        if (slot.has_a) va[j] = load_vec<T, VE>(row + slot.a);
-        if (slot.has_b) vb[j] = load_vec<T, VE>(row + slot.b);
-        if constexpr (BACK) {
-          if (slot.has_a) xa[j] = load_vec<T, VE>(xrow + slot.a);
-          if (slot.has_b) xb[j] = load_vec<T, VE>(xrow + slot.b);
-        }
-      }
-    };
-    ask(from);
-    __syncwarp();
-    token_angles(p, b, s, angles[warp]);
-    // The rotation's coefficients; the norm's weights are part of them forward, where nothing needs the rotated values without.
-    float aa[SLOTS][VE], ab[SLOTS][VE], bb[SLOTS][VE], ba[SLOTS][VE];
 #pragma unroll
-    for (int j = 0; j < SLOTS; ++j) {
-      const int slot = l + j * p.lanes;
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const float2 v = WHOLE || (slot + 1) * VE <= p.pairs ? angles[warp][slot * VE + e] : make_float2(1.f, 0.f);
-        if constexpr (NORM && !BACK) {
-          const int i = INTER ? 2 * e : e, k = INTER ? 2 * e + 1 : VE + e;
-          aa[j][e] = v.x * w[j][i], ab[j][e] = -v.y * w[j][k], bb[j][e] = v.x * w[j][k], ba[j][e] = v.y * w[j][i];
-        } else {
-          aa[j][e] = bb[j][e] = v.x, ab[j][e] = -v.y, ba[j][e] = v.y;
+        for (int i = 0; i < 4; ++i) {
+          if (i % 2 ? slot.has_b : slot.has_a) {
+            const T* from = (i / 2 ? xs : in) + (i % 2 ? slot.b : slot.a);
+            if constexpr (RING)
+              cp_async16(smem_addr(&ring.at[warp][ask_stage][4 * j + i][lane]), from);
+            else
+              v[j][i] = load_vec<T, VE>(from);
+          }
         }
       }
     }
-    T* out = static_cast<T*>(p.out[t]) + token * heads * p.D;
-    for (int base = from; base < to; base += groups) {
-      const int head = base + group;
-      const bool live = head < to;
-      float f[SLOTS][2 * VE], n[BACK ? SLOTS : 1][2 * VE];
+    if constexpr (RING) {
+      cp_async_commit();
+      ask_stage = (ask_stage + 1) % STAGES;
+    }
+    in += in_step;
+    xs += xs_step;
+    ask_head += groups;
+    if (ask_head - group >= ask_to && asked < tasks) {
+      asked += step;
+      if (asked < tasks) open();
+    }
+  };
+  if (asked < tasks) open();
+#pragma unroll
+  for (int i = 0; i < STAGES; ++i) ask();
+  fill_pairs(p, table);
+  __syncthreads();
+  float w[SLOTS][2 * VE], dw[SLOTS][2 * VE];
+#pragma unroll
+  for (int j = 0; j < SLOTS; ++j) {
+    const Where slot(l + j * p.lanes, p.pairs, p.D);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      w[j][e] = slot.has_a ? p.offset + param_at(p.weight[t], p.w_dtype[t], slot.a + e, 1.f) : 0.f;
+      w[j][VE + e] = slot.has_b ? p.offset + param_at(p.weight[t], p.w_dtype[t], slot.b + e, 1.f) : 0.f;
+      dw[j][e] = dw[j][VE + e] = 0.f;
+    }
+  }
+  Positions positions = {};
+  long long b = 0, s = 0, token = 0;
+  if (first_task < tasks) {
+    token = token_of(first_task, b, s);
+    ask_positions(p, table, b, s, positions);
+  }
+  int stage = 0;
+  for (long long task = first_task; task < tasks; task += step) {
+    token_angles<sizeof(T) == 2>(p, table, b, s, positions, angles[warp]);
+    const int from = (int)(task - token * per_token) * per_task, to = min(from + per_task, heads);
+    T* out = static_cast<T*>(p.out[t]) + (token * heads + from + group) * p.D;
+    const int out_step = groups * p.D;
+    if (task + step < tasks) {
+      token = token_of(task + step, b, s);
+      ask_positions(p, table, b, s, positions);
+    }
+    float aa[SLOTS][VE], ab[SLOTS][VE], bb[SLOTS][VE], ba[SLOTS][VE];
+#pragma unroll
+    for (int j = 0; j < SLOTS; ++j) {
+      const Where slot(l + j * p.lanes, p.pairs, p.D);
+      if (slot.turns) {
+        float2 c[VE];
+        read_angles<VE>(angles[warp], slot, c);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) aa[j][e] = bb[j][e] = c[e].x, ab[j][e] = -c[e].y, ba[j][e] = c[e].y;
+      }
+    }
+    for (int head = from + group; head - group < to; head += groups, out += out_step) {
+      const bool live = head < to;  // (a group beyond the last head adds and stores nothing)
+      if constexpr (RING) cp_async_wait<STAGES - 1>();
+      float f[SLOTS][2 * VE], n[SLOTS][2 * VE];
       float sq[2] = {0.f, 0.f}, dot[2] = {0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < SLOTS; ++j) {
         const Where slot(l + j * p.lanes, p.pairs, p.D);
-        unpack_two<T, VE>(va[j], vb[j], f[j]);
-        if constexpr (BACK) unpack_two<T, VE>(xa[j], xb[j], n[j]);
+        if constexpr (RING) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[j][i] = load_vec<T, VE>(reinterpret_cast<const T*>(&ring.at[warp][stage][4 * j + i][lane]));
+        }
+        unpack_two<T, VE>(v[j][0], v[j][1], f[j]);
+        unpack_two<T, VE>(v[j][2], v[j][3], n[j]);
         if constexpr (!WHOLE) {
 #pragma unroll
           for (int e = 0; e < 2 * VE; ++e) {
-            if (!(e < VE ? slot.has_a : slot.has_b)) {
-              f[j][e] = 0.f;
-              if constexpr (BACK) n[j][e] = 0.f;
-            }
+            if (!(e < VE ? slot.has_a : slot.has_b)) f[j][e] = n[j][e] = 0.f;
           }
         }
-        if constexpr (NORM && !BACK) dot_each(sq, f[j], f[j]);
-        if (slot.turns) {
-          turn<VE, INTER>(f[j], aa[j], ab[j], bb[j], ba[j]);
-        } else if constexpr (NORM && !BACK) {
-          mul_each(f[j], w[j]);
-        }
-        if constexpr (BACK) dot_each(sq, n[j], n[j]);
+        if (slot.turns) turn<VE, INTER>(f[j], aa[j], ab[j], bb[j], ba[j]);
+        dot_each(sq, n[j], n[j]);
       }
-      if (base + groups < to) ask(base + groups);
-      if constexpr (NORM) {
-        const float rstd = __frsqrt_rn(fmaf(lanes_sum(sq[0] + sq[1], p.lanes), p.inv_d, p.eps));
-        if constexpr (BACK) {
+      if constexpr (RING) stage = (stage + 1) % STAGES;
+      ask();
+      // both sums at once: mean(g w n) = rstd * mean(g w x)
+      float gw[SLOTS][2 * VE];
 #pragma unroll
-          for (int j = 0; j < SLOTS; ++j) {
-            scale_each(n[j], rstd);
-            if (live) fma_each(dw[j], f[j], n[j]);
-            mul_each(f[j], w[j]);
-            dot_each(dot, f[j], n[j]);
-          }
-          const float c = -lanes_sum(dot[0] + dot[1], p.lanes) * p.inv_d;
+      for (int j = 0; j < SLOTS; ++j) {
 #pragma unroll
-          for (int j = 0; j < SLOTS; ++j) axpy_each(f[j], n[j], c);
-        }
+        for (int e = 0; e < 2 * VE; ++e) gw[j][e] = f[j][e];
+        mul_each(gw[j], w[j]);
+        dot_each(dot, gw[j], n[j]);
+      }
+      const float all_sq = lanes_sum(sq[0] + sq[1], p.lanes), all_dot = lanes_sum(dot[0] + dot[1], p.lanes);
+      const float rstd = __frsqrt_rn(fmaf(all_sq, p.inv_d, p.eps)), c = -all_dot * rstd * p.inv_d;
 #pragma unroll
-        for (int j = 0; j < SLOTS; ++j) scale_each(f[j], rstd);
+      for (int j = 0; j < SLOTS; ++j) {
+        scale_each(n[j], rstd);
+        if (live) fma_each(dw[j], f[j], n[j]);
+        axpy_each(gw[j], n[j], c);
+        scale_each(gw[j], rstd);
       }
       if (live) {
-        T* row = out + (long long)head * p.D;
 #pragma unroll
         for (int j = 0; j < SLOTS; ++j) {
           const Where slot(l + j * p.lanes, p.pairs, p.D);
-          float g[VE];
-          if (slot.has_a) {
-#pragma unroll
-            for (int e = 0; e < VE; ++e) g[e] = f[j][e];
-            store_vec<T, VE>(row + slot.a, pack<T, VE>(g));
-          }
-          if (slot.has_b) {
-#pragma unroll
-            for (int e = 0; e < VE; ++e) g[e] = f[j][VE + e];
-            store_vec<T, VE>(row + slot.b, pack<T, VE>(g));
-          }
+          store_two<T, VE>(out, slot.a, slot.b, slot.has_a, slot.has_b, gw[j]);
         }
       }
     }
   }
-  if constexpr (BACK) {
-    // the groups of a warp and the warps of the CTA hold the same channels: added in a fixed order
-    float(*share)[kMostHead] = reinterpret_cast<float(*)[kMostHead]>(&angles[0][0]);  // a warp's angles are as long as a head
-    __syncthreads();
+  // the groups of a warp and the warps of the CTA hold the same channels: added in a fixed order
+  float(*share)[kMostHead] = reinterpret_cast<float(*)[kMostHead]>(&angles[0][0]);  // a warp's angles are as long as a head
+  __syncthreads();
 #pragma unroll
-    for (int j = 0; j < SLOTS; ++j) {
-      const Where slot(l + j * p.lanes, p.pairs, p.D);
+  for (int j = 0; j < SLOTS; ++j) {
+    const Where slot(l + j * p.lanes, p.pairs, p.D);
 #pragma unroll
-      for (int e = 0; e < 2 * VE; ++e) {
-        float v = dw[j][e];
-        for (int delta = 16; delta >= p.lanes; delta >>= 1) v += __shfl_xor_sync(0xffffffffu, v, delta);
-        if (group == 0 && (e < VE ? slot.has_a : slot.has_b)) share[warp][(e < VE ? slot.a + e : slot.b + e - VE)] = v;
-      }
+    for (int e = 0; e < 2 * VE; ++e) {
+      float v = dw[j][e];
+      for (int delta = 16; delta >= p.lanes; delta >>= 1) v += __shfl_xor_sync(0xffffffffu, v, delta);
+      if (group == 0 && (e < VE ? slot.has_a : slot.has_b)) share[warp][(e < VE ? slot.a + e : slot.b + e - VE)] = v;
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < p.D; i += kThreads) {
-      float v = 0.f;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.D; i += kThreads) {
+    float v = 0.f;
 #pragma unroll
-      for (int k = 0; k < kWarps; ++k) v += share[k][i];
-      p.part[t][(long long)cta * p.D + i] = v;
-    }
+    for (int k = 0; k < kWarps; ++k) v += share[k][i];
+    p.part[t][(long long)cta * p.D + i] = v;
   }
 }
 
@@ -312,26 +625,39 @@ cudaError_t with_rotary_geometry(const RotaryGeom& g, F&& f) {
   return g.slots == 2 ? f(Int<1>(), Int<2>(), std::false_type()) : f(Int<1>(), Int<8>(), std::false_type());
 }
 
-// How the tokens' heads are dealt out: warps take whole tokens where there are enough of them, else shares of a token's heads.
-cudaError_t rotary_split(const void* kernel, const RotaryGeom& g, Rotary& p) {
+// How the tokens' heads are dealt out: warps take whole tokens where there are enough of them, else shares of a token's heads.  Forward q and
+// k share the tasks; backward each has CTAs in proportion to a token's turns of the warp, and two more for the angles and all else that a token
+// takes (16384 tokens, 32 and 8 heads of 128: 134 us in proportion to the heads, 98 with them).
+// Without a norm four CTAs an SM are enough: 32 KB of heads ahead, and more of them only disturb one another (16384 tokens, 32 and 32
+// heads of 128, bf16: 3 CTAs 95 us, 4 86, 5 96).
+constexpr int kTokenTurns = 2;
+cudaError_t rotary_split(const void* kernel, const RotaryGeom& g, bool norm, bool back, Rotary& p) {
   Residency r;
   const cudaError_t err = residency(kernel, kThreads, 0, &r);
   if (err != cudaSuccess) return err;
-  const long long most = (long long)r.per_sm * r.sms;
-  const int groups = 32 / g.lanes, all = p.heads[0] + p.heads[1];
-  long long want[2] = {0, 0};
+  const long long most = (long long)(norm ? r.per_sm : std::min(r.per_sm, 4)) * r.sms;
+  const int groups = 32 / g.lanes;
+  long long want[2] = {0, 0}, turns[2] = {0, 0}, weight[2] = {0, 0};
   for (int t = 0; t < 2; ++t) {
     if (!p.heads[t]) continue;
-    const int turns = (p.heads[t] + groups - 1) / groups;  // of a warp, for a token
-    const long long share = std::max(1LL, most * kWarps * p.heads[t] / all / std::max(1LL, p.tokens));
-    const int tasks = (int)std::min<long long>(turns, share);
-    p.per_task[t] = (turns + tasks - 1) / tasks * groups;
+    turns[t] = (p.heads[t] + groups - 1) / groups;  // of a warp, for a token
+    weight[t] = turns[t] + kTokenTurns;
+  }
+  for (int t = 0; t < 2; ++t) {
+    if (!p.heads[t]) continue;
+    const long long warps = back ? most * kWarps * weight[t] / (weight[0] + weight[1]) : most * kWarps;
+    const long long tasks = std::min(turns[t], std::max(1LL, warps / std::max(1LL, p.tokens)));
+    p.per_task[t] = (int)((turns[t] + tasks - 1) / tasks) * groups;
     p.tasks_per_token[t] = (p.heads[t] + p.per_task[t] - 1) / p.per_task[t];
     want[t] = (p.tokens * p.tasks_per_token[t] + kWarps - 1) / kWarps;
   }
-  if (want[0] + want[1] > most) {
+  if (!back) {
+    p.tasks_per_token[0] = std::max(p.tasks_per_token[0], p.tasks_per_token[1]);
+    want[0] = std::min(most, std::max(want[0], want[1]));
+    want[1] = 0;
+  } else if (want[0] + want[1] > most) {
     for (int t = 0; t < 2; ++t)
-      if (p.heads[t]) want[t] = std::max(1LL, std::min(want[t], most * p.heads[t] / all));
+      if (want[t]) want[t] = std::max(1LL, std::min(want[t], most * weight[t] / (weight[0] + weight[1])));
   }
   p.ctas[0] = (unsigned)want[0];
   p.ctas[1] = (unsigned)want[1];
@@ -343,7 +669,7 @@ cudaError_t launch_rotary(Rotary& p, int dtype, int widest, bool inter, bool nor
   const RotaryGeom g = rotary_geometry(p.D, p.pairs, widest, dtype == GNB200_F32 ? 4 : 8);
   p.lanes = g.lanes;
   auto go = [&](void (*kernel)(const Rotary)) {
-    const cudaError_t err = rotary_split((const void*)kernel, g, p);
+    const cudaError_t err = rotary_split((const void*)kernel, g, norm, back, p);
     if (err != cudaSuccess || plan_only) return err;
     kernel<<<p.ctas[0] + p.ctas[1], kThreads, 0, stream>>>(p);
     return cudaGetLastError();
@@ -353,12 +679,9 @@ cudaError_t launch_rotary(Rotary& p, int dtype, int widest, bool inter, bool nor
     return with_rotary_geometry<T>(g, [&](auto ve, auto slots, auto whole) {
       constexpr int VE = decltype(ve)::value, S = decltype(slots)::value;
       constexpr bool W = decltype(whole)::value;
-      if (inter) {
-        if (back) return go(&rotary_kernel<T, VE, S, W, true, true, true>);
-        return norm ? go(&rotary_kernel<T, VE, S, W, true, true, false>) : go(&rotary_kernel<T, VE, S, W, true, false, false>);
-      }
-      if (back) return go(&rotary_kernel<T, VE, S, W, false, true, true>);
-      return norm ? go(&rotary_kernel<T, VE, S, W, false, true, false>) : go(&rotary_kernel<T, VE, S, W, false, false, false>);
+      if (back) return inter ? go(&rotary_bwd_kernel<T, VE, S, W, true>) : go(&rotary_bwd_kernel<T, VE, S, W, false>);
+      if (norm) return inter ? go(&rotary_fwd_kernel<T, VE, S, W, true, true>) : go(&rotary_fwd_kernel<T, VE, S, W, false, true>);
+      return inter ? go(&rotary_fwd_kernel<T, VE, S, W, true, false>) : go(&rotary_fwd_kernel<T, VE, S, W, false, false>);
     });
   };
   if (dtype == GNB200_F32) return typed(float());
@@ -475,6 +798,11 @@ size_t gnb200_rotary_bwd_workspace_bytes(const gnb200_rotary_args* a) {
   if (check_rotary("gnb200_rotary_bwd_workspace_bytes", a) != GNB200_OK || (!a->q_weight && !a->k_weight)) return 0;
   Rotary p = {};
   if (!fill(a, p)) return 0;
+  static thread_local Remembered<8> known;  // the answer depends on nothing but these and the device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  const Remembered<8>::Key key = {p.tokens, p.D, p.pairs, p.heads[0], p.heads[1], a->interleaved != 0, a->dtype, dev};
+  if (const size_t* v = known.find(key)) return *v;
   size_t most = 0;
   for (int which = 1; which < 4; ++which) {  // q, k, both
     for (int widest = 16 / (a->dtype == GNB200_F32 ? 4 : 2); widest >= 1; widest = widest == 8 ? 4 : widest == 4 ? 1 : 0) {
@@ -486,7 +814,7 @@ size_t gnb200_rotary_bwd_workspace_bytes(const gnb200_rotary_args* a) {
       most = std::max(most, ((size_t)call.ctas[0] + call.ctas[1]) * (size_t)p.D * sizeof(float));
     }
   }
-  return most;
+  return known.keep(key, most);
 }
 
 int gnb200_rotary_bwd(const gnb200_rotary_args* a, const void* dq, const int64_t* dq_stride, const void* dk, const int64_t* dk_stride,
