@@ -33,8 +33,8 @@ struct Rotary {
   long long in_stride[2][3], x_stride[2][3];  // batch, token, head; out is contiguous
   int heads[2], per_task[2], tasks_per_token[2];
   unsigned ctas[2];
-  long long tokens;
-  int S, D, pairs, lanes;
+  int tokens, S, D, pairs, lanes;
+  unsigned div_mul, div_shift;  // token / S for token < 2^31: (umulhi(token, mul) + token) >> shift
   const void* positions;
   long long pos_stride[3];  // batch, token, axis
   int pos_type;
@@ -70,8 +70,8 @@ __device__ __forceinline__ long long position_at(const Rotary& p, long long at) 
   if (p.pos_type == GNB200_POS_I64) return static_cast<const long long*>(p.positions)[at];
   return static_cast<const int*>(p.positions)[at];  // (or the bits of a float)
 }
-__device__ __forceinline__ void ask_positions(const Rotary& p, const PairTable& table, long long b, long long s, Positions& out) {
-  const long long at = b * p.pos_stride[0] + s * p.pos_stride[1];
+__device__ __forceinline__ void ask_positions(const Rotary& p, const PairTable& table, int b, int s, Positions& out) {
+  const long long at = p.pos_stride[0] * b + p.pos_stride[1] * s;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int i = (int)(threadIdx.x & 31) + 32 * k;
@@ -110,13 +110,13 @@ __device__ __forceinline__ float2 angle_of(const Rotary& p, const PairTable& tab
 
 // cos and sin of a token's angles, into the warp's shared memory
 template <bool FAST>
-__device__ __forceinline__ void token_angles(const Rotary& p, const PairTable& table, long long b, long long s, const Positions& known, float2* out) {
+__device__ __forceinline__ void token_angles(const Rotary& p, const PairTable& table, int b, int s, const Positions& known, float2* out) {
   const int lane = threadIdx.x & 31;
   __syncwarp();  // (nobody reads the token before any more)
   if (lane < p.pairs) out[lane] = angle_of<FAST>(p, table, lane, known.raw[0]);
   if (lane + 32 < p.pairs) out[lane + 32] = angle_of<FAST>(p, table, lane + 32, known.raw[1]);
   if (p.pairs > 64) {
-    const long long at = b * p.pos_stride[0] + s * p.pos_stride[1];
+    const long long at = p.pos_stride[0] * b + p.pos_stride[1] * s;
     for (int i = lane + 64; i < p.pairs; i += 32) out[i] = angle_of<FAST>(p, table, i, position_at(p, at + table.axis[i] * p.pos_stride[2]));
   }
   __syncwarp();
@@ -161,6 +161,22 @@ struct Slot {
   static __device__ __forceinline__ constexpr int second(int e) { return INTER ? 2 * e + 1 : VE + e; }
   __device__ __forceinline__ int channel(int i) const { return i < VE ? a + i : b + i - VE; }
 };
+
+// a task's token, and its place
+__device__ __forceinline__ int token_of(const Rotary& p, int task, int per_token, int& b, int& s) {
+  const int token = per_token == 1 ? task : task / per_token;
+  b = (int)((__umulhi((unsigned)token, p.div_mul) + (unsigned)token) >> p.div_shift);
+  s = token - b * p.S;
+  return token;
+}
+__device__ __forceinline__ long long place(const long long (&strides)[3], int b, int s, int head) {
+  return strides[0] * b + strides[1] * s + strides[2] * head;
+}
+// Reciprocal root mean square.  The fast one is off by two units of fp32's last place, below what results of 16 bits show.
+template <bool FAST>
+__device__ __forceinline__ float rms_inverse(float mean_square) {
+  return FAST ? rsqrtf(mean_square) : __frsqrt_rn(mean_square);
+}
 
 // cos and sin of the slot's pairs, two pairs a load (they lie together, on 16 bytes)
 template <int VE, typename Slot>
@@ -246,40 +262,38 @@ __global__ void __launch_bounds__(kThreads) rotary_fwd_kernel(const Rotary p) {
   __shared__ PairTable table;
   __shared__ alignas(16) float weights[NORM ? 2 : 1][NORM ? kMostHead : 1];
   constexpr bool RING = kRing<T, VE>;
-  __shared__ Ring<RING, NORM ? 4 : 2, 2 * SLOTS> ring;
+  __shared__ Ring<RING, 2, 2 * SLOTS> ring;
   constexpr int STAGES = decltype(ring)::kStages;
   using Where = Slot<VE, INTER, WHOLE>;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int l = lane & (p.lanes - 1), group = lane / p.lanes, groups = 32 / p.lanes;
   const int per_token = p.tasks_per_token[0];
-  const long long tasks = p.tokens * per_token, step = (long long)gridDim.x * kWarps;
-  const auto token_of = [&](long long task, long long& b, long long& s) {
-    const long long token = per_token == 1 ? task : task / per_token;
-    b = p.S == p.tokens ? 0 : token / p.S;
-    s = token - b * p.S;
-    return token;
-  };
+  const int tasks = p.tokens * per_token, step = (int)gridDim.x * kWarps;
   // the heads of q (t = 0) or k that are a task's
-  const auto heads_from = [&](long long task, long long token, int t) { return min((int)(task - token * per_token) * p.per_task[t], p.heads[t]); };
+  const auto heads_from = [&](int task, int token, int t) { return min((task - token * per_token) * p.per_task[t], p.heads[t]); };
   const auto heads_to = [&](int from, int t) { return min(from + p.per_task[t], p.heads[t]); };
 
   // What is asked for next: the warp's next turn of a task's heads of q, then of k; row: this lane's head.
-  const long long first_task = (long long)blockIdx.x * kWarps + warp;
-  long long asked = first_task - step, row_step = 0;
-  int ask_t = 1, ask_head = 0, ask_to = 0, ask_stage = 0;
+  const int first_task = (int)blockIdx.x * kWarps + warp;
+  int asked = first_task, ask_t = 0, ask_head = 0, ask_to = 0, ask_stage = 0, ask_token = 0, ask_b = 0, ask_s = 0;
   const T* row = nullptr;
+  long long row_step = 0;
+  const auto open = [&]() {
+    const int from = heads_from(asked, ask_token, ask_t);
+    ask_to = heads_to(from, ask_t);
+    ask_head = from + group;
+    row = static_cast<const T*>(p.in[ask_t]) + place(p.in_stride[ask_t], ask_b, ask_s, ask_head);
+    row_step = groups * p.in_stride[ask_t][2];
+  };
   const auto advance = [&]() {  // to the next heads that there are
     do {
-      if (ask_t == 1) asked += step;
       ask_t ^= 1;
-      if (asked >= tasks) return;
-      long long b, s;
-      const long long token = token_of(asked, b, s);
-      const int from = heads_from(asked, token, ask_t);
-      ask_to = heads_to(from, ask_t);
-      ask_head = from + group;
-      row = static_cast<const T*>(p.in[ask_t]) + b * p.in_stride[ask_t][0] + s * p.in_stride[ask_t][1] + ask_head * p.in_stride[ask_t][2];
-      row_step = groups * p.in_stride[ask_t][2];
+      if (ask_t == 0) {
+        asked += step;
+        if (asked >= tasks) return;
+        ask_token = token_of(p, asked, per_token, ask_b, ask_s);
+      }
+      open();
     } while (ask_head - group >= ask_to);
   };
   Pack<T, VE> va[SLOTS], vb[SLOTS];
@@ -305,7 +319,11 @@ __global__ void __launch_bounds__(kThreads) rotary_fwd_kernel(const Rotary p) {
     ask_head += groups;
     if (ask_head - group >= ask_to && asked < tasks) advance();
   };
-  advance();
+  if (asked < tasks) {
+    ask_token = token_of(p, asked, per_token, ask_b, ask_s);
+    open();
+    if (ask_head - group >= ask_to) advance();
+  }
 #pragma unroll
   for (int i = 0; i < STAGES; ++i) ask();
   fill_pairs(p, table);
@@ -317,17 +335,16 @@ __global__ void __launch_bounds__(kThreads) rotary_fwd_kernel(const Rotary p) {
   }
   __syncthreads();
   Positions positions = {};
-  long long b = 0, s = 0, token = 0;
+  int b = 0, s = 0, token = 0, stage = 0;
   if (first_task < tasks) {
-    token = token_of(first_task, b, s);
+    token = token_of(p, first_task, per_token, b, s);
     ask_positions(p, table, b, s, positions);
   }
-  int stage = 0;
-  for (long long task = first_task; task < tasks; task += step) {
+  for (int task = first_task; task < tasks; task += step) {
     token_angles<sizeof(T) == 2>(p, table, b, s, positions, angles[warp]);
-    const long long now = token;
+    const int now = token;
     if (task + step < tasks) {
-      token = token_of(task + step, b, s);
+      token = token_of(p, task + step, per_token, b, s);
       ask_positions(p, table, b, s, positions);
     }
     float aa[SLOTS][VE], ab[SLOTS][VE], bb[SLOTS][VE], ba[SLOTS][VE];
@@ -364,7 +381,7 @@ __global__ void __launch_bounds__(kThreads) rotary_fwd_kernel(const Rotary p) {
           }
         }
       }
-      T* out = static_cast<T*>(p.out[t]) + (now * p.heads[t] + from + group) * p.D;
+      T* out = static_cast<T*>(p.out[t]) + ((long long)now * p.heads[t] + from + group) * p.D;
       const int out_step = groups * p.D;
       for (int head = from + group; head - group < to; head += groups, out += out_step) {
         if constexpr (RING) cp_async_wait<STAGES - 1>();
@@ -394,7 +411,7 @@ __global__ void __launch_bounds__(kThreads) rotary_fwd_kernel(const Rotary p) {
         if constexpr (RING) stage = (stage + 1) % STAGES;
         ask();
         if constexpr (NORM) {
-          const float rstd = __frsqrt_rn(fmaf(lanes_sum(sq[0] + sq[1], p.lanes), p.inv_d, p.eps));
+          const float rstd = rms_inverse<sizeof(T) == 2>(fmaf(lanes_sum(sq[0] + sq[1], p.lanes), p.inv_d, p.eps));
 #pragma unroll
           for (int j = 0; j < SLOTS; ++j) scale_each(f[j], rstd);
         }
@@ -425,27 +442,19 @@ __global__ void __launch_bounds__(kThreads) rotary_bwd_kernel(const Rotary p) {
   const unsigned cta = blockIdx.x - (t ? p.ctas[0] : 0);
   grid_dep_launch_dependents();
   const int per_token = p.tasks_per_token[t], per_task = p.per_task[t], heads = p.heads[t];
-  const long long tasks = p.tokens * per_token, step = (long long)p.ctas[t] * kWarps;
-  const auto token_of = [&](long long task, long long& b, long long& s) {
-    const long long token = per_token == 1 ? task : task / per_token;
-    b = p.S == p.tokens ? 0 : token / p.S;
-    s = token - b * p.S;
-    return token;
-  };
+  const int tasks = p.tokens * per_token, step = (int)p.ctas[t] * kWarps;
   // what is asked for next: the warp's next turn of a task's heads; in, xs: this lane's head of the gradient and of the input
-  const long long first_task = (long long)cta * kWarps + warp;
+  const int first_task = (int)cta * kWarps + warp;
   const long long in_step = groups * p.in_stride[t][2], xs_step = groups * p.x_stride[t][2];
-  long long asked = first_task;
-  int ask_head = 0, ask_to = 0, ask_stage = 0;
+  int asked = first_task, ask_head = 0, ask_to = 0, ask_stage = 0;
   const T *in = nullptr, *xs = nullptr;
   const auto open = [&]() {
-    long long b, s;
-    const long long token = token_of(asked, b, s);
-    const int from = (int)(asked - token * per_token) * per_task;
+    int b, s;
+    const int token = token_of(p, asked, per_token, b, s), from = (asked - token * per_token) * per_task;
     ask_head = from + group;
     ask_to = min(from + per_task, heads);
-    in = static_cast<const T*>(p.in[t]) + b * p.in_stride[t][0] + s * p.in_stride[t][1] + ask_head * p.in_stride[t][2];
-    xs = static_cast<const T*>(p.x[t]) + b * p.x_stride[t][0] + s * p.x_stride[t][1] + ask_head * p.x_stride[t][2];
+    in = static_cast<const T*>(p.in[t]) + place(p.in_stride[t], b, s, ask_head);
+    xs = static_cast<const T*>(p.x[t]) + place(p.x_stride[t], b, s, ask_head);
   };
   Pack<T, VE> v[SLOTS][4];  // of a slot: the gradient's two vectors, the input's two
   const auto ask = [&]() {
@@ -494,19 +503,18 @@ __global__ void __launch_bounds__(kThreads) rotary_bwd_kernel(const Rotary p) {
     }
   }
   Positions positions = {};
-  long long b = 0, s = 0, token = 0;
+  int b = 0, s = 0, token = 0, stage = 0;
   if (first_task < tasks) {
-    token = token_of(first_task, b, s);
+    token = token_of(p, first_task, per_token, b, s);
     ask_positions(p, table, b, s, positions);
   }
-  int stage = 0;
-  for (long long task = first_task; task < tasks; task += step) {
+  for (int task = first_task; task < tasks; task += step) {
     token_angles<sizeof(T) == 2>(p, table, b, s, positions, angles[warp]);
-    const int from = (int)(task - token * per_token) * per_task, to = min(from + per_task, heads);
-    T* out = static_cast<T*>(p.out[t]) + (token * heads + from + group) * p.D;
+    const int from = (task - token * per_token) * per_task, to = min(from + per_task, heads);
+    T* out = static_cast<T*>(p.out[t]) + ((long long)token * heads + from + group) * p.D;
     const int out_step = groups * p.D;
     if (task + step < tasks) {
-      token = token_of(task + step, b, s);
+      token = token_of(p, task + step, per_token, b, s);
       ask_positions(p, table, b, s, positions);
     }
     float aa[SLOTS][VE], ab[SLOTS][VE], bb[SLOTS][VE], ba[SLOTS][VE];
@@ -555,7 +563,7 @@ __global__ void __launch_bounds__(kThreads) rotary_bwd_kernel(const Rotary p) {
         dot_each(dot, gw[j], n[j]);
       }
       const float all_sq = lanes_sum(sq[0] + sq[1], p.lanes), all_dot = lanes_sum(dot[0] + dot[1], p.lanes);
-      const float rstd = __frsqrt_rn(fmaf(all_sq, p.inv_d, p.eps)), c = -all_dot * rstd * p.inv_d;
+      const float rstd = rms_inverse<sizeof(T) == 2>(fmaf(all_sq, p.inv_d, p.eps)), c = -all_dot * rstd * p.inv_d;
 #pragma unroll
       for (int j = 0; j < SLOTS; ++j) {
         scale_each(n[j], rstd);
@@ -628,14 +636,14 @@ cudaError_t with_rotary_geometry(const RotaryGeom& g, F&& f) {
 // How the tokens' heads are dealt out: warps take whole tokens where there are enough of them, else shares of a token's heads.  Forward q and
 // k share the tasks; backward each has CTAs in proportion to a token's turns of the warp, and two more for the angles and all else that a token
 // takes (16384 tokens, 32 and 8 heads of 128: 134 us in proportion to the heads, 98 with them).
-// Without a norm four CTAs an SM are enough: 32 KB of heads ahead, and more of them only disturb one another (16384 tokens, 32 and 32
-// heads of 128, bf16: 3 CTAs 95 us, 4 86, 5 96).
-constexpr int kTokenTurns = 2;
-cudaError_t rotary_split(const void* kernel, const RotaryGeom& g, bool norm, bool back, Rotary& p) {
+// Forward calls with many heads are bound by memory: four CTAs an SM keep 32 KB of heads ahead, and more of them only disturb one another
+// (16384 tokens, 32 and 32 heads of 128, bf16, with norm: 3 CTAs 97.5 us, 4 87.0, 5 97.4).  With few heads a token's angles count for more, and
+// every warp helps (2 x 4096 tokens, 20 and 20 heads of 64: 4 CTAs 18.8, 5 17.7).
+constexpr int kTokenTurns = 2, kManyTurns = 12;
+cudaError_t rotary_split(const void* kernel, const RotaryGeom& g, bool ring, bool back, Rotary& p) {
   Residency r;
   const cudaError_t err = residency(kernel, kThreads, 0, &r);
   if (err != cudaSuccess) return err;
-  const long long most = (long long)(norm ? r.per_sm : std::min(r.per_sm, 4)) * r.sms;
   const int groups = 32 / g.lanes;
   long long want[2] = {0, 0}, turns[2] = {0, 0}, weight[2] = {0, 0};
   for (int t = 0; t < 2; ++t) {
@@ -643,13 +651,15 @@ cudaError_t rotary_split(const void* kernel, const RotaryGeom& g, bool norm, boo
     turns[t] = (p.heads[t] + groups - 1) / groups;  // of a warp, for a token
     weight[t] = turns[t] + kTokenTurns;
   }
+  if (ring && !back && turns[0] + turns[1] >= kManyTurns) r.per_sm = std::min(r.per_sm, 4);
+  const long long most = (long long)r.per_sm * r.sms;
   for (int t = 0; t < 2; ++t) {
     if (!p.heads[t]) continue;
     const long long warps = back ? most * kWarps * weight[t] / (weight[0] + weight[1]) : most * kWarps;
-    const long long tasks = std::min(turns[t], std::max(1LL, warps / std::max(1LL, p.tokens)));
+    const long long tasks = std::min(turns[t], std::max(1LL, warps / std::max(1, p.tokens)));
     p.per_task[t] = (int)((turns[t] + tasks - 1) / tasks) * groups;
     p.tasks_per_token[t] = (p.heads[t] + p.per_task[t] - 1) / p.per_task[t];
-    want[t] = (p.tokens * p.tasks_per_token[t] + kWarps - 1) / kWarps;
+    want[t] = ((long long)p.tokens * p.tasks_per_token[t] + kWarps - 1) / kWarps;
   }
   if (!back) {
     p.tasks_per_token[0] = std::max(p.tasks_per_token[0], p.tasks_per_token[1]);
@@ -669,7 +679,7 @@ cudaError_t launch_rotary(Rotary& p, int dtype, int widest, bool inter, bool nor
   const RotaryGeom g = rotary_geometry(p.D, p.pairs, widest, dtype == GNB200_F32 ? 4 : 8);
   p.lanes = g.lanes;
   auto go = [&](void (*kernel)(const Rotary)) {
-    const cudaError_t err = rotary_split((const void*)kernel, g, norm, back, p);
+    const cudaError_t err = rotary_split((const void*)kernel, g, g.ve == (dtype == GNB200_F32 ? 4 : 8), back, p);
     if (err != cudaSuccess || plan_only) return err;
     kernel<<<p.ctas[0] + p.ctas[1], kThreads, 0, stream>>>(p);
     return cudaGetLastError();
@@ -712,8 +722,9 @@ int check_rotary(const char* name, const gnb200_rotary_args* a) {
   if (a->head_dim > kMostHead)
     return report_error(GNB200_ERR_UNSUPPORTED, "%s: heads of more than %d channels are not supported (got %lld)", name, kMostHead,
                         (long long)a->head_dim);
-  if (a->q_heads > (1 << 20) || a->k_heads > (1 << 20) || a->batch > (1LL << 31) || a->tokens >= (1LL << 31))
-    return report_error(GNB200_ERR_UNSUPPORTED, "%s: more than 2^20 heads or 2^31 tokens", name);
+  if (a->q_heads > (1 << 20) || a->k_heads > (1 << 20) || a->tokens >= (1LL << 30) || a->batch >= (1LL << 30) ||
+      a->batch * a->tokens >= (1LL << 30))
+    return report_error(GNB200_ERR_UNSUPPORTED, "%s: more than 2^20 heads or 2^30 tokens", name);
   if (a->axes < 1 || a->axes > kMostAxes)
     return report_error(GNB200_ERR_INVALID_ARGUMENT, "%s: 1 to %d axes (got %d)", name, kMostAxes, a->axes);
   int64_t pairs = 0;
@@ -731,8 +742,10 @@ int check_rotary(const char* name, const gnb200_rotary_args* a) {
 // The part of the call that forward and backward share; false where there is nothing to do.
 bool fill(const gnb200_rotary_args* a, Rotary& p) {
   if (a->batch == 0 || a->tokens == 0) return false;
-  p.tokens = a->batch * a->tokens;
+  p.tokens = (int)(a->batch * a->tokens);
   p.S = (int)a->tokens;
+  while ((1LL << p.div_shift) < p.S) ++p.div_shift;
+  p.div_mul = (unsigned)(((1ULL << 32) * ((1ULL << p.div_shift) - (unsigned)p.S)) / (unsigned)p.S + 1);
   p.D = (int)a->head_dim;
   p.heads[0] = (int)a->q_heads;
   p.heads[1] = (int)a->k_heads;
