@@ -12,6 +12,7 @@
 // a sum); longer ones still are read twice, element by element (`any`).  The grid holds the CTAs that are resident at once; each keeps its
 // channels' weights in registers, walks over the rows and asks for its next row before it reduces the present one.
 #include <algorithm>
+#include <initializer_list>
 
 #include "../../include/gnb200.h"
 #include "gn_kernels.h"
@@ -44,7 +45,7 @@ __device__ __forceinline__ float scale_of(uint32_t most, int format) {
 }
 __device__ __forceinline__ float inverse_of(float scale) { return __fdividef(1.f, scale); }
 template <int VE>
-__device__ __forceinline__ void store_codes(uint8_t* p, const float (&f)[VE], float inverse, int format) {
+__device__ __forceinline__ Pack<uint8_t, VE> codes_of(const float (&f)[VE], float inverse, int format) {
   Pack<uint8_t, VE> c;
   if (format == GNB200_E4M3) {
     if constexpr (VE % 2 == 0) {
@@ -63,90 +64,176 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float (&f)[VE], fl
 #pragma unroll
     for (int e = 0; e < VE; ++e) c.v[e] = (uint8_t)(int8_t)max(-127, min(127, __float2int_rn(f[e] * inverse)));
   }
-  if constexpr (VE == 8)
-    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(&c);
-  else if constexpr (VE == 4)
-    *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(&c);
-  else
-    *p = c.v[0];
+  return c;
 }
 
 // ---------------------------------------------------------------------------------------------
-// Rows in shared memory
+// Rows as vectors
 // ---------------------------------------------------------------------------------------------
-// Bytes of a tensor's row in a stage: 16-byte chunks, and one more where rows start between chunk boundaries.
-__host__ __device__ constexpr int segment_bytes(int C, int size, bool aligned) { return aligned ? C * size : (C * size + 30) / 16 * 16; }
-
-// Copies a row, 16 bytes a lane, from the chunk boundary at or before its first byte.  That boundary lies in the row's own allocation
-// (which starts on one), and the last copy ends with the row: nothing outside of the tensor's allocation is read.
-template <typename T, int VE, int V>
-__device__ __forceinline__ void ask_row(char* stage, const T* row, int C, int first, int step) {
-  const uint32_t dst = smem_addr(stage);
-  if constexpr (VE > 1) {
-    constexpr int kParts = sizeof(T) * VE / 16;  // 32 bytes where 8 floats stand beside 8 halves
-    const int nvec = C / VE;
+// RAGGED rows start between the boundaries of 16 bytes, or end there.  They are taken in a frame that begins at the boundary before: vector i
+// holds channels i * VE - skew and on, the first and the last one in part.  All tensors of a call have the same frame (checked by the
+// host), and the step from one of a thread's rows to the next is a multiple of VE rows, so that the skew, and with it the channels of a thread, stay:
+// its weights and sums are in registers as they are for aligned rows.  Device us, element by element before and so: 9000 rows of 1111 bf16 with a
+// residual, forward 27.0 and 24.9, backward 42.3 and 43.3; 3000 of 12345, backward 210 and 166; 4000 of 12345 fp16, 8-bit output with
+// blocks, 592 and 245.
+template <int VE, bool RAGGED>
+struct Frame {
+  int skew, nvec, C;
+  __device__ __forceinline__ Frame(uint32_t row_elements, int channels) {
+    C = channels;
+    skew = RAGGED ? (int)(row_elements % VE) : 0;
+    nvec = RAGGED ? (C + skew + VE - 1) / VE : C / VE;
+  }
+  __device__ __forceinline__ bool whole(int i) const { return !RAGGED || (i * VE >= skew && (i + 1) * VE - skew <= C); }
+  __device__ __forceinline__ int channel(int i) const { return i * VE - skew; }  // of the vector's first element; may lie before the row
+  __device__ __forceinline__ bool has(int i, int e) const { return !RAGGED || (unsigned)(channel(i) + e) < (unsigned)C; }
+  // elements outside of the row become zero
+  __device__ __forceinline__ void cut(float (&f)[VE], int i) const {
+    if constexpr (RAGGED) {
+      if (!whole(i)) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int at = first + v * step;
-      if (at < nvec) {
-#pragma unroll
-        for (int i = 0; i < kParts; ++i) cp_async16(dst + (at * kParts + i) * 16, reinterpret_cast<const char*>(row + (long long)at * VE) + i * 16);
+        for (int e = 0; e < VE; ++e)
+          if (!has(i, e)) f[e] = 0.f;
       }
     }
-  } else {
-    const int skew = (int)(reinterpret_cast<uintptr_t>(row) & 15), bytes = skew + C * (int)sizeof(T);
-    const char* src = reinterpret_cast<const char*>(row) - skew;
-    for (int at = first * 16; at < bytes; at += step * 16) cp_async16_part(dst + at, src + at, min(16, bytes - at));
   }
-}
-// where the row begins in the stage
-template <typename T, int VE>
-__device__ __forceinline__ const T* row_in(const char* stage, const T* row) {
-  return reinterpret_cast<const T*>(stage + (VE > 1 ? 0 : (reinterpret_cast<uintptr_t>(row) & 15)));
+  // Whether vector i may be read as a whole, with elements of the rows beside it: in the tensor's first and last row (not `inner`) only
+  // where it lies in the row.  What may not is fetched where it is used.
+  __device__ __forceinline__ bool readable(int i, bool inner) const { return !RAGGED || inner || whole(i); }
+  template <typename T>
+  __device__ __forceinline__ Pack<T, VE> fetch(const T* row, int i) const {
+    Pack<T, VE> v;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      v.v[e] = store_param<T>(0.f);
+      if (has(i, e)) v.v[e] = row[i * VE + e];
+    }
+    return v;
+  }
+  // Sums over a ragged row go through shared memory, so that they are taken in the row's own order: the same bits wherever the row
+  // stands.  Channel j is word j / VE of plane j % VE, which is free of bank conflicts for frames of any skew.
+  __device__ __forceinline__ int words() const { return (C + VE - 1) / VE; }  // of a plane
+  __device__ __forceinline__ void lay_out(float* planes, int i, const float (&f)[VE]) const {
+    const bool all = whole(i);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      // plane and word of element e of vector 0, which are those of vector i but for i words
+      const int at = ((e - skew) & (VE - 1)) * words() - (e < skew ? 1 : 0);
+      if (all || has(i, e)) planes[at + i] = f[e];
+    }
+  }
+  __device__ __forceinline__ void take(const float* planes, int i, float (&f)[VE]) const {
+    if ((i + 1) * VE <= C) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) f[e] = planes[e * words() + i];
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) f[e] = i * VE + e < C ? planes[e * words() + i] : 0.f;
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(T* row, int i, const float (&f)[VE]) const {
+    if (whole(i)) {
+      store_vec<T, VE>(row + i * VE, pack<T, VE>(f));
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+        if (has(i, e)) row[i * VE + e] = store_param<T>(f[e]);
+    }
+  }
+};
+
+// Bytes of a tensor's row in a stage
+__host__ __device__ constexpr int segment_bytes(int C, int ve, int size, bool ragged) { return ragged ? (C + 2 * ve - 2) / ve * ve * size : C * size; }
+
+// ... and of the planes of its sum
+__host__ __device__ constexpr int plane_bytes(int C, int ve, bool ragged) { return ragged ? ((C + ve - 1) / ve * ve * 4 + 15) / 16 * 16 : 0; }
+
+// Copies a row to its stage, 16 bytes a lane; of the tensor's first and last row (not `inner`) no chunk that begins before it and no byte behind
+// it, so that nothing outside of the tensor is read.
+template <typename T, int VE, int V, bool RAGGED>
+__device__ __forceinline__ void ask_row(char* stage, const T* row, const Frame<VE, RAGGED>& frame, int first, int step, bool inner) {
+  const uint32_t dst = smem_addr(stage);
+  constexpr int kParts = sizeof(T) * VE / 16;  // 32 bytes where 8 floats stand beside 8 halves
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int i = first + v * step;
+    if (i < frame.nvec) {
+      if (frame.readable(i, inner)) {
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) cp_async16(dst + (i * kParts + k) * 16, reinterpret_cast<const char*>(row) + (i * kParts + k) * 16);
+      } else {
+        for (int e = 0; e < VE; ++e)
+          if (frame.has(i, e)) reinterpret_cast<T*>(stage)[i * VE + e] = row[i * VE + e];
+      }
+    }
+  }
 }
 
 // (offset + w) of this thread's channels
-template <int VE, int V>
-__device__ __forceinline__ void fetch_weight(float (&w)[V][VE], const void* p, int dtype, float offset, int first, int step, int nvec) {
+template <int VE, int V, bool RAGGED>
+__device__ __forceinline__ void fetch_weight(float (&w)[V][VE], const void* p, int dtype, float offset, const Frame<VE, RAGGED>& frame, int first,
+                                             int step) {
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int at = first + v * step;
+    const int i = first + v * step;
 #pragma unroll
     for (int e = 0; e < VE; ++e) w[v][e] = 1.f;
-    if (p != nullptr && at < nvec) {
-      params_at<VE>(p, dtype, (long long)at * VE, w[v]);
+    if (p != nullptr && i < frame.nvec) {
+      if constexpr (RAGGED) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+          if (frame.has(i, e)) w[v][e] = param_at(p, dtype, frame.channel(i) + e, 1.f);
+      } else {
+        params_at<VE>(p, dtype, i * VE, w[v]);
+      }
 #pragma unroll
       for (int e = 0; e < VE; ++e) w[v][e] += offset;
     }
   }
 }
 
-// How the rows are dealt out: this thread's place in its row's group, the group's rows and its stages.  A group is a power-of-two number
-// of lanes of one warp (WARP), a team of whole warps (TEAMS) or the CTA.
-template <int VE, bool WARP, bool TEAMS>
+// the codes of vector i of the row whose frame begins at `row`
+template <int VE, bool RAGGED>
+__device__ __forceinline__ void store_codes(uint8_t* row, const Frame<VE, RAGGED>& frame, int i, const float (&f)[VE], float inverse, int format) {
+  const Pack<uint8_t, VE> c = codes_of<VE>(f, inverse, format);
+  if (frame.whole(i)) {
+    if constexpr (VE == 8)
+      *reinterpret_cast<uint2*>(row + i * VE) = *reinterpret_cast<const uint2*>(&c);
+    else
+      *reinterpret_cast<uint32_t*>(row + i * VE) = *reinterpret_cast<const uint32_t*>(&c);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE; ++e)
+      if (frame.has(i, e)) row[i * VE + e] = c.v[e];
+  }
+}
+
+// How the rows are dealt out: this thread's place in its row's group, the group's rows and its stages.
+// A group is a power-of-two number of lanes of one warp (WARP), a team of whole warps (TEAMS) or the CTA.
+template <bool WARP, bool TEAMS>
 struct Place {
-  int lanes, first, nvec, group;
+  int lanes, first, group;
   long long per_cta, base, row, step;
   char* stages;
-  __device__ __forceinline__ Place(int C, int row_lanes, int stage_bytes, int nstages, char* smem) {
+  float* planes;
+  __device__ __forceinline__ Place(int row_lanes, int stage_bytes, int nstages, int plane_bytes, char* smem) {
     lanes = WARP || TEAMS ? row_lanes : (int)blockDim.x;
     group = WARP || TEAMS ? (int)threadIdx.x / lanes : 0;
     first = (int)threadIdx.x - group * lanes;
-    nvec = C / VE;
     per_cta = WARP || TEAMS ? (int)blockDim.x / lanes : 1;
     base = blockIdx.x * per_cta + (WARP ? 0 : group);  // (a warp's groups take their turns together, teams each for themselves)
     row = blockIdx.x * per_cta + group;
     step = per_cta * gridDim.x;
-    stages = smem + (long long)group * stage_bytes * nstages;
+    stages = smem + (long long)group * (stage_bytes * nstages + plane_bytes);
+    planes = reinterpret_cast<float*>(stages + stage_bytes * nstages);
   }
-  // copies that other lanes waited for become visible
+  // what the group's other lanes wrote becomes visible
   __device__ __forceinline__ void meet() const {
-    if constexpr (VE == 1) {
-      if constexpr (WARP)
-        __syncwarp();
-      else
-        team_barrier<TEAMS>(lanes, group);
-    }
+    if constexpr (WARP)
+      __syncwarp();
+    else
+      team_barrier<TEAMS>(lanes, group);
   }
 };
 
@@ -155,19 +242,24 @@ struct Place {
 // ---------------------------------------------------------------------------------------------
 // What a thread holds of the row that comes next: registers where a few vectors do, otherwise the stages.
 template <typename Tx, typename Ts, int VE, int V, bool WARP>
-constexpr bool kStaged = VE == 1 || (!WARP && V * VE * (sizeof(Tx) + sizeof(Ts)) > 64);
+constexpr bool kStaged = !WARP && V * VE * (sizeof(Tx) + sizeof(Ts)) > 64;
+constexpr int kMostBlocks = 512;  // of the rows that these kernels take
 
-template <typename Tx, typename Ts, int VE, int V, bool WARP, bool Q, bool RES>
+template <typename Tx, typename Ts, int VE, int V, bool WARP, bool Q, bool RES, bool RAGGED>
 __global__ void __launch_bounds__(WARP ? kWarpThreads : kMostThreads) rms_fwd_kernel(const RmsFwd p) {
   constexpr bool STAGED = kStaged<Tx, Ts, VE, V, WARP>;
   extern __shared__ __align__(16) char smem[];
   __shared__ TeamSlots slots;
-  __shared__ uint32_t most[VE == 1 && Q ? V * (kMostThreads / 32) : 32];
-  Place<VE, WARP, false> at(p.C, p.lanes, p.stage_bytes, p.stages, smem);
-  const int lanes = at.lanes, first = at.first, nvec = at.nvec;
-  const int r_at = segment_bytes(p.C, sizeof(Tx), VE > 1);
+  __shared__ uint32_t most[32];
+  __shared__ uint32_t blocks[Q && RAGGED ? 2 : 1][Q && RAGGED ? kMostBlocks : 1];
+  const Place<WARP, false> at(p.lanes, p.stage_bytes, p.stages, plane_bytes(p.C, VE, RAGGED), smem);
+  const int lanes = at.lanes, first = at.first;
   const Tx* next_x = static_cast<const Tx*>(p.x) + at.row * p.x_stride;  // the next row to be asked for
   const Ts* next_r = RES ? static_cast<const Ts*>(p.residual) + at.row * p.r_stride : nullptr;
+  const Frame<VE, RAGGED> frame((uint32_t)(reinterpret_cast<uintptr_t>(next_x) / sizeof(Tx)), p.C);
+  const int nvec = frame.nvec, r_at = segment_bytes(p.C, VE, sizeof(Tx), RAGGED);
+  next_x -= frame.skew;
+  if (RES) next_r -= frame.skew;
   const long long x_step = at.step * p.x_stride, r_step = RES ? at.step * p.r_stride : 0;
   long long asked = at.row;
   int ask_stage = 0, stage = 0;
@@ -175,15 +267,16 @@ __global__ void __launch_bounds__(WARP ? kWarpThreads : kMostThreads) rms_fwd_ke
   Pack<Ts, VE> rv[STAGED || !RES ? 1 : V];
   auto ask = [&]() {
     if (asked < p.rows) {
+      const bool inner = asked > 0 && asked < p.rows - 1;
       if constexpr (STAGED) {
         char* s = at.stages + ask_stage * p.stage_bytes;
-        ask_row<Tx, VE, V>(s, next_x, p.C, first, lanes);
-        if constexpr (RES) ask_row<Ts, VE, V>(s + r_at, next_r, p.C, first, lanes);
+        ask_row<Tx, VE, V, RAGGED>(s, next_x, frame, first, lanes, inner);
+        if constexpr (RES) ask_row<Ts, VE, V, RAGGED>(s + r_at, next_r, frame, first, lanes, inner);
       } else {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const int i = first + v * lanes;
-          if (i < nvec) {
+          if (i < nvec && frame.readable(i, inner)) {
             xv[v] = load_vec<Tx, VE>(next_x + i * VE);
             if constexpr (RES) rv[v] = load_vec<Ts, VE>(next_r + i * VE);
           }
@@ -202,27 +295,25 @@ __global__ void __launch_bounds__(WARP ? kWarpThreads : kMostThreads) rms_fwd_ke
   if constexpr (STAGED)
     for (int i = 1; i < p.stages; ++i) ask();
   float w[V][VE];
-  fetch_weight<VE, V>(w, p.weight, p.w_dtype, p.offset, first, lanes, nvec);
-  if constexpr (!WARP) clear<false>(slots, lanes, 0, first);
-  int turn = 0;
+  fetch_weight<VE, V, RAGGED>(w, p.weight, p.w_dtype, p.offset, frame, first, lanes);
+  if constexpr (Q && RAGGED)
+    for (int i = threadIdx.x; i < 2 * kMostBlocks; i += blockDim.x) blocks[i / kMostBlocks][i % kMostBlocks] = 0;
+  if constexpr (!WARP)
+    clear<false>(slots, lanes, 0, first);
+  else if constexpr (Q && RAGGED)
+    __syncthreads();
+  int turn = 0, block_turn = 0;
   long long row = at.row;
-  uintptr_t x_skew = reinterpret_cast<uintptr_t>(static_cast<const Tx*>(p.x) + row * p.x_stride), r_skew = 0;
-  if constexpr (RES) r_skew = reinterpret_cast<uintptr_t>(static_cast<const Ts*>(p.residual) + row * p.r_stride);
   // (every thread of a warp takes the same number of turns: the shuffles want all lanes)
   for (long long base = at.base; base < p.rows; base += at.step, row += at.step) {
     const bool live = !WARP || row < p.rows;
     const char* here = nullptr;
     if constexpr (STAGED) {
       cp_async_wait_dyn8(p.stages - 1);
-      at.meet();
       here = at.stages + stage * p.stage_bytes;
       stage = stage + 1 == p.stages ? 0 : stage + 1;
     }
-    const Tx* xs = reinterpret_cast<const Tx*>(here + (VE > 1 ? 0 : (x_skew & 15)));
-    const Ts* rs = reinterpret_cast<const Ts*>(here + r_at + (VE > 1 ? 0 : (r_skew & 15)));
-    x_skew += x_step * sizeof(Tx);
-    r_skew += r_step * sizeof(Ts);
-    Ts* sum = static_cast<Ts*>(p.sum) + row * p.C;
+    const long long out_at = row * p.C - frame.skew;  // where the row's frame begins in the outputs
     float s[V][VE];
     float sq[2] = {0.f, 0.f};
 #pragma unroll
@@ -231,25 +322,42 @@ __global__ void __launch_bounds__(WARP ? kWarpThreads : kMostThreads) rms_fwd_ke
 #pragma unroll
       for (int e = 0; e < VE; ++e) s[v][e] = 0.f;
       if (live && i < nvec) {
+        if (RAGGED && !STAGED && !frame.readable(i, row > 0 && row < p.rows - 1)) {
+          xv[STAGED ? 0 : v] = frame.fetch(static_cast<const Tx*>(p.x) + row * p.x_stride - frame.skew, i);
+          if constexpr (RES) rv[STAGED ? 0 : v] = frame.fetch(static_cast<const Ts*>(p.residual) + row * p.r_stride - frame.skew, i);
+        }
         if constexpr (STAGED)
-          unpack<Tx, VE>(load_vec<Tx, VE>(xs + i * VE), s[v]);
+          unpack<Tx, VE>(load_vec<Tx, VE>(reinterpret_cast<const Tx*>(here) + i * VE), s[v]);
         else
           unpack<Tx, VE>(xv[v], s[v]);
         if constexpr (RES) {
           float f[VE];
           if constexpr (STAGED)
-            unpack<Ts, VE>(load_vec<Ts, VE>(rs + i * VE), f);
+            unpack<Ts, VE>(load_vec<Ts, VE>(reinterpret_cast<const Ts*>(here + r_at) + i * VE), f);
           else
             unpack<Ts, VE>(rv[v], f);
           add_each(s[v], f);
-          store_vec<Ts, VE>(sum + i * VE, pack<Ts, VE>(s[v]));
+          frame.store(static_cast<Ts*>(p.sum) + out_at, i, s[v]);
+        }
+        frame.cut(s[v], i);
+        if constexpr (RAGGED) frame.lay_out(at.planes, i, s[v]);
+      }
+      if constexpr (!RAGGED) dot_each(sq, s[v], s[v]);
+    }
+    if constexpr (RAGGED) {
+      at.meet();
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int i = first + v * lanes;
+        if (live && i < frame.words()) {
+          float f[VE];
+          frame.take(at.planes, i, f);
+          dot_each(sq, f, f);
         }
       }
-      dot_each(sq, s[v], s[v]);
     }
-    if constexpr (VE > 1) ask();  // (a lane's own chunks: read, so free)
+    ask();  // (a lane's own vectors: read, so free)
     const float all_sq = WARP ? lanes_sum(sq[0] + sq[1], lanes) : team_sum<false>(sq[0] + sq[1], slots, turn, lanes, 0);
-    if constexpr (VE == 1) ask();  // (behind the sum's barrier, or its shuffles, every lane has read the row)
     const float rstd = __frsqrt_rn(fmaf(all_sq, p.inv_c, p.eps));
     if (p.rstd && live && first == 0) p.rstd[row] = rstd;
 #pragma unroll
@@ -258,89 +366,88 @@ __global__ void __launch_bounds__(WARP ? kWarpThreads : kMostThreads) rms_fwd_ke
       mul_each(s[v], w[v]);
     }
     if constexpr (!Q) {
-      if (live) {
-        Tx* out = static_cast<Tx*>(p.y) + row * p.C;
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          if (first + v * lanes < nvec) store_vec<Tx, VE>(out + (first + v * lanes) * VE, pack<Tx, VE>(s[v]));
-      }
-    } else {
-      uint8_t* out = static_cast<uint8_t*>(p.y) + row * p.C;
-      uint32_t m[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        m[v] = 0;
-        if (first + v * lanes < nvec) {  // (beyond the row a NaN rstd would leave NaN in the zeros)
-#pragma unroll
-          for (int e = 0; e < VE; ++e) m[v] = max(m[v], magnitude(s[v][e]));
-        }
+        const int i = first + v * lanes;
+        if (live && i < nvec) frame.store(static_cast<Tx*>(p.y) + out_at, i, s[v]);
       }
-      if (p.block == 0) {
-        uint32_t all = 0;
-#pragma unroll
-        for (int v = 0; v < V; ++v) all = max(all, m[v]);
-        all = WARP ? lanes_max(all, lanes) : cta_max(all, most);
-        const float scale = scale_of(all, p.format), inverse = inverse_of(scale);
-        if (live && first == 0) p.scale[row] = scale;
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          if (live && first + v * lanes < nvec) store_codes<VE>(out + (first + v * lanes) * VE, s[v], inverse, p.format);
-      } else if constexpr (VE > 1) {
-        // a block's vectors lie in neighbouring lanes: block / VE of them, at most a warp's
-        const int share = p.block / VE, among = min(share, WARP ? lanes : 32);
+    } else {
+      uint8_t* const out = static_cast<uint8_t*>(p.y) + out_at;
+      if (RAGGED && p.block != 0) {
+        // a vector may hold the end of one block and the beginning of the next: the blocks' maxima meet in shared memory
+        const int shift = 31 - __clz(p.block), mine = WARP ? (int)threadIdx.x / lanes * lanes : 0;
+        uint32_t* const now = blocks[block_turn];
+        uint32_t* const then = blocks[block_turn ^ 1];
+        block_turn ^= 1;
+        for (int i = first; i < (WARP ? lanes : kMostBlocks); i += lanes) then[mine + i] = 0;  // (last read before this row's sum)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const int i = first + v * lanes;
-          const float scale = scale_of(lanes_max(m[v], among), p.format), inverse = inverse_of(scale);
+          const int i = first + v * lanes, from = max(frame.channel(i), 0), to = min(frame.channel(i) + VE, p.C) - 1;
           if (live && i < nvec) {
-            if (i % share == 0) p.scale[row * p.blocks + i / share] = scale;
-            store_codes<VE>(out + i * VE, s[v], inverse, p.format);
+            uint32_t low = 0, high = 0;
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+              const uint32_t m = frame.has(i, e) ? magnitude(s[v][e]) : 0;
+              if ((frame.channel(i) + e) >> shift == to >> shift)
+                high = max(high, m);
+              else
+                low = max(low, m);
+            }
+            atomicMax(&now[mine + (to >> shift)], high);
+            if (from >> shift != to >> shift) atomicMax(&now[mine + (from >> shift)], low);
           }
         }
-      } else if constexpr (WARP) {
-        // single elements in one warp: turn v holds channels v * lanes and on; a block is one, two or four turns of a whole warp (a row
-        // of fewer lanes has one turn's worth of channels a lane and one block)
-        const int share = max(1, p.block / lanes);
-        uint32_t all = 0;
+        if constexpr (WARP)
+          __syncwarp();
+        else
+          __syncthreads();
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const int in = v % share;
-          all = in == 0 ? m[v] : max(all, m[v]);
-          m[v] = all;  // over the block so far
-        }
-#pragma unroll
-        for (int v = V - 1; v >= 0; --v) {
-          const int last = min(v / share * share + share, V) - 1;  // the block's last turn has seen all of it
-          if (v != last) m[v] = m[v + 1];
-        }
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const int i = first + v * lanes;
-          const float scale = scale_of(lanes_max(m[v], lanes), p.format);
+          const int i = first + v * lanes, from = max(frame.channel(i), 0), to = min(frame.channel(i) + VE, p.C) - 1;
           if (live && i < nvec) {
-            if (i % p.block == 0) p.scale[row * p.blocks + i / p.block] = scale;
-            store_codes<1>(out + i, s[v], inverse_of(scale), p.format);
+            const float low = scale_of(now[mine + (from >> shift)], p.format), high = scale_of(now[mine + (to >> shift)], p.format);
+            if ((to & (p.block - 1)) <= to - from) p.scale[row * p.blocks + (to >> shift)] = high;  // (the block's first channel is here)
+            const float inverse_low = inverse_of(low), inverse_high = inverse_of(high);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) s[v][e] *= (frame.channel(i) + e) >> shift == to >> shift ? inverse_high : inverse_low;
+            store_codes<VE, RAGGED>(out, frame, i, s[v], 1.f, p.format);
           }
         }
       } else {
-        // single elements: a block is one, two or four warps' worth; entry i of `most` is that of channels 32 i to 32 i + 31
-        const int nwarps = lanes >> 5, warp = first >> 5, share = p.block / 32;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const uint32_t mv = lanes_max(m[v], 32);
-          if ((first & 31) == 0) most[v * nwarps + warp] = mv;
-        }
-        __syncthreads();
+        uint32_t m[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const int i = first + v * lanes;
-          if (i < nvec) {
-            const int from = i / p.block * share, to = min(from + share, V * nwarps);
-            uint32_t all = 0;
-            for (int k = from; k < to; ++k) all = max(all, most[k]);
-            const float scale = scale_of(all, p.format);
-            if (i % p.block == 0) p.scale[row * p.blocks + i / p.block] = scale;
-            store_codes<1>(out + i, s[v], inverse_of(scale), p.format);
+          m[v] = 0;
+          if (i < nvec) {  // (beyond the row a NaN rstd would leave NaN in the zeros)
+#pragma unroll
+            for (int e = 0; e < VE; ++e)
+              if (frame.has(i, e)) m[v] = max(m[v], magnitude(s[v][e]));
+          }
+        }
+        if (p.block == 0) {
+          uint32_t all = 0;
+#pragma unroll
+          for (int v = 0; v < V; ++v) all = max(all, m[v]);
+          all = WARP ? lanes_max(all, lanes) : cta_max(all, most);
+          const float scale = scale_of(all, p.format), inverse = inverse_of(scale);
+          if (live && first == 0) p.scale[row] = scale;
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            const int i = first + v * lanes;
+            if (live && i < nvec) store_codes<VE, RAGGED>(out, frame, i, s[v], inverse, p.format);
+          }
+        } else {
+          // a block's vectors lie in neighbouring lanes: block / VE of them, at most a warp's
+          const int share = p.block / VE, among = min(share, WARP ? lanes : 32);
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            const int i = first + v * lanes;
+            const float scale = scale_of(lanes_max(m[v], among), p.format), inverse = inverse_of(scale);
+            if (live && i < nvec) {
+              if (i % share == 0) p.scale[row * p.blocks + i / share] = scale;
+              store_codes<VE, RAGGED>(out, frame, i, s[v], inverse, p.format);
+            }
           }
         }
       }
@@ -384,7 +491,7 @@ __global__ void __launch_bounds__(kMostThreads) rms_fwd_any_kernel(const RmsFwd 
         if (threadIdx.x == 0) p.scale[row] = scale;
         for (int i = threadIdx.x; i < p.C; i += blockDim.x) {
           const float f[1] = {y_at(i)};
-          store_codes<1>(out + i, f, inverse, p.format);
+          out[i] = codes_of<1>(f, inverse, p.format).v[0];
         }
       } else {  // one warp per block of at most 128 channels
         const int lane = threadIdx.x & 31, nwarps = blockDim.x >> 5;
@@ -402,7 +509,7 @@ __global__ void __launch_bounds__(kMostThreads) rms_fwd_any_kernel(const RmsFwd 
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             const int in = lane + 32 * v, i = b * p.block + in;
-            if (in < p.block && i < p.C) store_codes<1>(out + i, f[v], inverse, p.format);
+            if (in < p.block && i < p.C) out[i] = codes_of<1>(f[v], inverse, p.format).v[0];
           }
         }
       }
@@ -414,9 +521,7 @@ __global__ void __launch_bounds__(kMostThreads) rms_fwd_any_kernel(const RmsFwd 
 // Backward
 // ---------------------------------------------------------------------------------------------
 // CTA sizes: the more rows a CTA takes at once, the fewer rows of partial sums there are to add up afterwards
-template <int VE, bool WARP>
-constexpr bool kTeams = VE > 1 && !WARP;
-constexpr int bwd_threads(int ve, int v) { return ve > 1 && ve * v <= 8 ? 1024 : 512; }
+constexpr int bwd_threads(int ve, int v) { return ve * v <= 8 ? 1024 : 512; }
 
 struct RmsBwd {
   const void *dy, *dsum, *sum, *addend, *weight;  // s = sum, or sum + addend (dy's type) where the stored sum was rounded to 16 bits
@@ -428,41 +533,40 @@ struct RmsBwd {
   float offset, inv_c;
 };
 
-template <typename Tx, typename Ts, int VE, int V, bool WARP, bool RES>
-__global__ void __launch_bounds__(bwd_threads(VE, V), VE > 1 ? 1 : 0) rms_bwd_kernel(const RmsBwd p) {
+template <typename Tx, typename Ts, int VE, int V, bool WARP, bool RES, bool RAGGED>
+__global__ void __launch_bounds__(bwd_threads(VE, V), 1) rms_bwd_kernel(const RmsBwd p) {
+  constexpr bool TEAMS = !WARP;
   extern __shared__ __align__(16) char smem[];
-  constexpr bool TEAMS = kTeams<VE, WARP>;
   __shared__ TeamSlots all_slots[TEAMS ? kMostTeams : 1];
-  Place<VE, WARP, TEAMS> at(p.C, p.lanes, p.stage_bytes, p.stages, smem);
+  const Place<WARP, TEAMS> at(p.lanes, p.stage_bytes, p.stages, plane_bytes(p.C, VE, RAGGED), smem);
   TeamSlots& slots = all_slots[TEAMS ? at.group : 0];
-  const int lanes = at.lanes, first = at.first, nvec = at.nvec;
+  const int lanes = at.lanes, first = at.first;
   grid_dep_launch_dependents();
-  const Tx *dy = static_cast<const Tx*>(p.dy), *add = RES ? static_cast<const Tx*>(p.addend) : nullptr;
-  const Ts *ds = RES ? static_cast<const Ts*>(p.dsum) : nullptr, *sum = static_cast<const Ts*>(p.sum);
+  const Frame<VE, RAGGED> frame((uint32_t)(reinterpret_cast<uintptr_t>(static_cast<const Tx*>(p.dy) + at.row * p.dy_stride) / sizeof(Tx)), p.C);
+  const int nvec = frame.nvec;
+  const Tx *dy = static_cast<const Tx*>(p.dy) - frame.skew, *add = RES && p.addend ? static_cast<const Tx*>(p.addend) - frame.skew : nullptr;
+  const Ts *ds = RES && p.dsum ? static_cast<const Ts*>(p.dsum) - frame.skew : nullptr, *sum = static_cast<const Ts*>(p.sum) - frame.skew;
   // a stage: sum, dy, then the addend and the sum's gradient where there are any
-  const int narrow = segment_bytes(p.C, sizeof(Tx), VE > 1), wide = segment_bytes(p.C, sizeof(Ts), VE > 1);
+  const int narrow = segment_bytes(p.C, VE, sizeof(Tx), RAGGED), wide = segment_bytes(p.C, VE, sizeof(Ts), RAGGED);
   const int dy_at = wide, add_at = dy_at + narrow, ds_at = add_at + (add ? narrow : 0);
   long long asked = at.row;
   int ask_stage = 0, stage = 0;
   auto ask = [&]() {
     if (asked < p.rows) {
+      const bool inner = asked > 0 && asked < p.rows - 1;
       char* s = at.stages + ask_stage * p.stage_bytes;
-      ask_row<Ts, VE, V>(s, sum + asked * p.s_stride, p.C, first, lanes);
-      ask_row<Tx, VE, V>(s + dy_at, dy + asked * p.dy_stride, p.C, first, lanes);
-      if (add) ask_row<Tx, VE, V>(s + add_at, add + asked * p.a_stride, p.C, first, lanes);
-      if (ds) ask_row<Ts, VE, V>(s + ds_at, ds + asked * p.ds_stride, p.C, first, lanes);
+      ask_row<Ts, VE, V, RAGGED>(s, sum + asked * p.s_stride, frame, first, lanes, inner);
+      ask_row<Tx, VE, V, RAGGED>(s + dy_at, dy + asked * p.dy_stride, frame, first, lanes, inner);
+      if (add) ask_row<Tx, VE, V, RAGGED>(s + add_at, add + asked * p.a_stride, frame, first, lanes, inner);
+      if (ds) ask_row<Ts, VE, V, RAGGED>(s + ds_at, ds + asked * p.ds_stride, frame, first, lanes, inner);
     }
     cp_async_commit();
     asked += at.step;
     ask_stage = ask_stage + 1 == p.stages ? 0 : ask_stage + 1;
   };
-  // Single elements are free for the next copy only behind the barrier of the row after, so one stage fewer is in flight; a lone
-  // stage gets a barrier of its own.
-  const bool lone = VE == 1 && p.stages == 1;
-  const int ahead = VE > 1 || lone ? p.stages : p.stages - 1;
-  for (int i = 0; i < ahead; ++i) ask();
+  for (int i = 0; i < p.stages; ++i) ask();
   float w[V][VE], dw[V][VE];
-  fetch_weight<VE, V>(w, p.weight, p.w_dtype, p.offset, first, lanes, nvec);
+  fetch_weight<VE, V, RAGGED>(w, p.weight, p.w_dtype, p.offset, frame, first, lanes);
 #pragma unroll
   for (int v = 0; v < V; ++v)
 #pragma unroll
@@ -475,25 +579,21 @@ __global__ void __launch_bounds__(bwd_threads(VE, V), VE > 1 ? 1 : 0) rms_bwd_ke
     const bool live = !WARP || row < p.rows;
     const float rstd = rn;
     if (row + at.step < p.rows) rn = p.rstd[row + at.step];
-    cp_async_wait_dyn8(ahead - 1);
-    at.meet();
-    if (VE == 1 && !lone) ask();
+    cp_async_wait_dyn8(p.stages - 1);
     const char* here = at.stages + stage * p.stage_bytes;
     stage = stage + 1 == p.stages ? 0 : stage + 1;
-    const Ts* sums = row_in<Ts, VE>(here, sum + row * p.s_stride);
-    const Tx* dys = row_in<Tx, VE>(here + dy_at, dy + row * p.dy_stride);
-    const Tx* adds = row_in<Tx, VE>(here + add_at, add + row * p.a_stride);
-    const Ts* dss = row_in<Ts, VE>(here + ds_at, ds + row * p.ds_stride);
     // s * rstd and dy of this thread's vector i
     auto terms = [&](int i, float (&n)[VE], float (&g)[VE]) {
-      unpack<Ts, VE>(load_vec<Ts, VE>(sums + i * VE), n);
-      unpack<Tx, VE>(load_vec<Tx, VE>(dys + i * VE), g);
+      unpack<Ts, VE>(load_vec<Ts, VE>(reinterpret_cast<const Ts*>(here) + i * VE), n);
+      unpack<Tx, VE>(load_vec<Tx, VE>(reinterpret_cast<const Tx*>(here + dy_at) + i * VE), g);
       if (add) {
         float f[VE];
-        unpack<Tx, VE>(load_vec<Tx, VE>(adds + i * VE), f);
+        unpack<Tx, VE>(load_vec<Tx, VE>(reinterpret_cast<const Tx*>(here + add_at) + i * VE), f);
         add_each(n, f);
       }
       scale_each(n, rstd);
+      frame.cut(n, i);
+      frame.cut(g, i);
     };
     float dot[2] = {0.f, 0.f};
 #pragma unroll
@@ -503,10 +603,29 @@ __global__ void __launch_bounds__(bwd_threads(VE, V), VE > 1 ? 1 : 0) rms_bwd_ke
         terms(first + v * lanes, n, g);
         mul_each(g, n);
         add_each(dw[v], g);
-        dot_each(dot, g, w[v]);
+        if constexpr (RAGGED) {
+          mul_each(g, w[v]);
+          frame.lay_out(at.planes, first + v * lanes, g);
+        } else {
+          dot_each(dot, g, w[v]);
+        }
+      }
+    }
+    if constexpr (RAGGED) {
+      at.meet();
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int i = first + v * lanes;
+        if (live && i < frame.words()) {
+          float f[VE];
+          frame.take(at.planes, i, f);
+#pragma unroll
+          for (int e = 0; e < VE; ++e) dot[e & 1] += f[e];
+        }
       }
     }
     const float c = -(WARP ? lanes_sum(dot[0] + dot[1], lanes) : team_sum<TEAMS>(dot[0] + dot[1], slots, turn, at.lanes, at.group)) * p.inv_c;
+    const long long out_at = row * p.C - frame.skew;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int i = first + v * lanes;
@@ -517,19 +636,18 @@ __global__ void __launch_bounds__(bwd_threads(VE, V), VE > 1 ? 1 : 0) rms_bwd_ke
         axpy_each(g, n, c);
         scale_each(g, rstd);
         if (ds) {
-          unpack<Ts, VE>(load_vec<Ts, VE>(dss + i * VE), d);
+          unpack<Ts, VE>(load_vec<Ts, VE>(reinterpret_cast<const Ts*>(here + ds_at) + i * VE), d);
           add_each(d, g);
         } else {
 #pragma unroll
           for (int e = 0; e < VE; ++e) d[e] = g[e];
         }
-        store_vec<Tx, VE>(static_cast<Tx*>(p.dx) + row * p.C + i * VE, pack<Tx, VE>(d));
+        frame.store(static_cast<Tx*>(p.dx) + out_at, i, d);
         if constexpr (!std::is_same<Tx, Ts>::value)
-          if (p.dsum_out) store_vec<Ts, VE>(static_cast<Ts*>(p.dsum_out) + row * p.C + i * VE, pack<Ts, VE>(d));
+          if (p.dsum_out) frame.store(static_cast<Ts*>(p.dsum_out) + out_at, i, d);
       }
     }
-    if (lone) at.meet();
-    if (VE > 1 || lone) ask();
+    ask();  // (a lane's own vectors: read, so free)
   }
   if (p.part == nullptr) return;
   // the groups hold the same channels: their sums are added in order.  They fit the stages, whose rows have two tensors of at least
@@ -543,7 +661,8 @@ __global__ void __launch_bounds__(bwd_threads(VE, V), VE > 1 ? 1 : 0) rms_bwd_ke
     const int i = first + v * lanes;
     if (i < nvec) {
 #pragma unroll
-      for (int e = 0; e < VE; ++e) share[at.group * p.C + i * VE + e] = dw[v][e];
+      for (int e = 0; e < VE; ++e)
+        if (frame.has(i, e)) share[at.group * p.C + frame.channel(i) + e] = dw[v][e];
     }
   }
   __syncthreads();
@@ -620,34 +739,36 @@ __global__ void __launch_bounds__(32 * kSumWarps) column_sums_kernel(const Colum
 // Host side
 // ---------------------------------------------------------------------------------------------
 struct RmsGeom {
-  int ve, v, lanes, threads;  // lanes: per row; threads: per CTA; ve = 0: the kernels for rows of any length
-  bool warp;                  // lanes of one warp; otherwise whole warps
+  int ve, v, lanes, threads;  // lanes: per row; threads: per CTA; v = 0: the kernels for rows of any length
+  bool warp, ragged;          // warp: lanes of one warp; otherwise whole warps
 };
 
-RmsGeom rms_geometry(int64_t C, int dtype, bool aligned, bool backward) {
-  const int full = dtype == GNB200_F32 ? 4 : 8;
+// How a call's rows lie: on vector boundaries, all in the same frame, or neither
+enum Rows { kAligned, kRagged, kAny };
+
+RmsGeom rms_geometry(int64_t C, int dtype, Rows rows, bool backward) {
   RmsGeom g = {};
-  g.ve = aligned && C % full == 0 ? full : 1;
-  const int64_t nvec = C / g.ve;
-  const int in_warp = g.ve > 1 ? 4 : 16;  // vectors a lane that a warp's row may have
-  if (nvec <= 32 * in_warp) {
+  g.ve = dtype == GNB200_F32 ? 4 : 8;
+  if (rows == kAny) return RmsGeom{1, 0, kMostThreads, kMostThreads, false, false};
+  g.ragged = rows == kRagged;
+  const int64_t nvec = g.ragged ? (C + 2 * g.ve - 2) / g.ve : C / g.ve;  // (ragged: one more for rows that begin late in their frame)
+  if (nvec <= 32 * 4) {  // four vectors a lane
     g.warp = true;
     g.lanes = 1;
     while (g.lanes < 32 && g.lanes < nvec) g.lanes *= 2;
     const int64_t each = (nvec + g.lanes - 1) / g.lanes;
-    g.v = g.ve > 1 ? (each <= 1 ? 1 : each <= 2 ? 2 : 4) : (each <= 4 ? 4 : 16);
+    g.v = each <= 1 ? 1 : each <= 2 ? 2 : 4;
   } else {
     const int most = 32 / g.ve;
-    int v = g.ve == 1 ? 8 : 2;
-    while (v < most && nvec > (int64_t)v * kMostThreads) v = g.ve == 1 ? 32 : 2 * v;
-    if (nvec > (int64_t)v * kMostThreads) return RmsGeom{0, 0, kMostThreads, kMostThreads, false};
-    g.v = v;
-    g.lanes = (int)((nvec + v - 1) / v + 31) / 32 * 32;
+    g.v = 2;  // (one a thread and more teams: the backward of 16384 x 4096 bf16 takes 131 us instead of 106)
+    while (g.v < most && nvec > (int64_t)g.v * kMostThreads) g.v *= 2;
+    if (nvec > (int64_t)g.v * kMostThreads) return RmsGeom{1, 0, kMostThreads, kMostThreads, false, false};
+    g.lanes = (int)((nvec + g.v - 1) / g.v + 31) / 32 * 32;
   }
   g.threads = g.warp ? kWarpThreads : g.lanes;
   if (backward) {
     const int most = bwd_threads(g.ve, g.v);
-    g.threads = g.warp ? most : g.ve == 1 ? g.lanes : std::max(1, std::min(kMostTeams, most / g.lanes)) * g.lanes;
+    g.threads = g.warp ? most : std::max(1, std::min(kMostTeams, most / g.lanes)) * g.lanes;
   }
   return g;
 }
@@ -658,13 +779,15 @@ struct RmsLaunch {
   unsigned grid;
   int threads, smem, stages;
 };
-// CTA size, stages, shared memory and CTAs of a call whose rows take `row_bytes` in a stage (0: no stages): no more CTAs than are resident at
-// once nor than there are rows.  cudaErrorInvalidValue: a row does not fit.
-cudaError_t rms_launch(const void* kernel, const RmsGeom& g, int64_t rows, int64_t row_bytes, RmsLaunch* out) {
+// CTA size, stages, shared memory and CTAs of a call whose rows take `row_bytes` in a stage (0: no stages) and `planes` for their sums: no more CTAs than are resident at
+// once nor than there are rows; where ragged rows take several turns, a number that
+// keeps their frames.  cudaErrorInvalidValue: a row does not fit.
+cudaError_t rms_launch(const void* kernel, const RmsGeom& g, int64_t rows, int64_t row_bytes, int64_t planes, RmsLaunch* out) {
   Residency r = {};
   out->threads = g.threads;
-  out->stages = out->smem = 0;
-  if (row_bytes > kMostDynamicSmem) return cudaErrorInvalidValue;
+  out->stages = 0;
+  if (row_bytes + planes > kMostDynamicSmem) return cudaErrorInvalidValue;
+  out->smem = (int)(g.threads / g.lanes * planes);
   if (row_bytes) {
     // fewer teams where two stages for each do not fit, or where there are no rows for them on every SM
     const auto halve = [&](int teams) { return g.warp ? teams / 2 : teams - 1; };
@@ -672,16 +795,16 @@ cudaError_t rms_launch(const void* kernel, const RmsGeom& g, int64_t rows, int64
     cudaError_t err = residency(kernel, g.threads, 0, &r);
     if (err != cudaSuccess) return err;
     const int least = g.warp ? 32 / g.lanes : 1;
-    while (teams > least && (2 * teams * row_bytes > kMostDynamicSmem || (int64_t)teams * r.sms > rows)) teams = std::max(least, halve(teams));
+    while (teams > least && (teams * (2 * row_bytes + planes) > kMostDynamicSmem || (int64_t)teams * r.sms > rows)) teams = std::max(least, halve(teams));
     out->threads = teams * g.lanes;
     if ((err = residency(kernel, out->threads, 0, &r)) != cudaSuccess) return err;
-    const int64_t bytes = row_bytes * teams;
-    if (bytes > kMostDynamicSmem) return cudaErrorInvalidValue;
-    int64_t stages = std::max<int64_t>(1, kMostDynamicSmem / r.per_sm / bytes);
-    stages = std::min<int64_t>(kMostStages, std::max<int64_t>(stages, std::min<int64_t>(2, kMostDynamicSmem / bytes)));
+    const int64_t bytes = row_bytes * teams, fixed = planes * teams;
+    if (bytes + fixed > kMostDynamicSmem) return cudaErrorInvalidValue;
+    int64_t stages = std::max<int64_t>(1, (kMostDynamicSmem / r.per_sm - fixed) / bytes);
+    stages = std::min<int64_t>(kMostStages, std::max<int64_t>(stages, std::min<int64_t>(2, (kMostDynamicSmem - fixed) / bytes)));
     const int64_t turns = (rows + (int64_t)teams * r.sms - 1) / ((int64_t)teams * r.sms);  // at most, of a team
     out->stages = (int)std::max<int64_t>(1, std::min(stages, turns));
-    out->smem = (int)(bytes * out->stages);
+    out->smem = (int)(bytes * out->stages + fixed);
   }
   const int cap = r.per_sm;
   const cudaError_t err = residency(kernel, out->threads, out->smem, &r);
@@ -690,6 +813,12 @@ cudaError_t rms_launch(const void* kernel, const RmsGeom& g, int64_t rows, int64
   const int64_t per_cta = out->threads / g.lanes;
   const int64_t need = (rows + per_cta - 1) / per_cta, most = (int64_t)r.per_sm * r.sms;
   out->grid = (unsigned)(need < most ? need : most);
+  if (g.ragged && need > most) {  // the step, per_cta * grid rows, becomes a multiple of VE
+    int64_t grid = out->grid;
+    while (grid > 1 && per_cta * grid % g.ve != 0) --grid;
+    if (per_cta * grid % g.ve != 0) return cudaErrorInvalidValue;
+    out->grid = (unsigned)grid;
+  }
   return cudaSuccess;
 }
 
@@ -702,52 +831,50 @@ cudaError_t with_types(int dtype, int sum_dtype, F&& f) {
 }
 template <int N>
 using Int = std::integral_constant<int, N>;
-// ... and with the geometry's numbers: elements a vector, vectors a thread, one group of lanes per row?
-template <int FULL, typename F>
+// ... and with the geometry's numbers: elements a vector, vectors a thread, one group of lanes per row?, ragged?
+template <int VE, typename F>
 cudaError_t with_geometry(const RmsGeom& g, F&& f) {
-  if (g.ve == 1) {
-    if (g.warp) return g.v == 4 ? f(Int<1>(), Int<4>(), std::true_type()) : f(Int<1>(), Int<16>(), std::true_type());
-    return g.v == 8 ? f(Int<1>(), Int<8>(), std::false_type()) : f(Int<1>(), Int<32>(), std::false_type());
-  }
+  const auto ragged = [&](auto v, auto warp) { return g.ragged ? f(Int<VE>(), v, warp, std::true_type()) : f(Int<VE>(), v, warp, std::false_type()); };
   if (g.warp) {
-    if (g.v == 1) return f(Int<FULL>(), Int<1>(), std::true_type());
-    if (g.v == 2) return f(Int<FULL>(), Int<2>(), std::true_type());
-    return f(Int<FULL>(), Int<4>(), std::true_type());
+    if (g.v == 1) return ragged(Int<1>(), std::true_type());
+    if (g.v == 2) return ragged(Int<2>(), std::true_type());
+    return ragged(Int<4>(), std::true_type());
   }
-  if (g.v == 2) return f(Int<FULL>(), Int<2>(), std::false_type());
-  if constexpr (FULL == 4) {
-    if (g.v == 8) return f(Int<FULL>(), Int<8>(), std::false_type());
+  if (g.v == 2) return ragged(Int<2>(), std::false_type());
+  if constexpr (VE == 4) {
+    if (g.v == 8) return ragged(Int<8>(), std::false_type());
   }
-  return f(Int<FULL>(), Int<4>(), std::false_type());
+  return ragged(Int<4>(), std::false_type());
 }
 
 template <bool Q>
-cudaError_t launch_rms_fwd(RmsFwd p, int dtype, int sum_dtype, bool aligned, cudaStream_t stream) {
+cudaError_t launch_rms_fwd(RmsFwd p, int dtype, int sum_dtype, Rows rows, cudaStream_t stream) {
   return with_types(dtype, sum_dtype, [&](auto tx, auto ts) {
     using Tx = decltype(tx);
     using Ts = decltype(ts);
-    RmsGeom g = rms_geometry(p.C, dtype, aligned, false);
+    RmsGeom g = rms_geometry(p.C, dtype, rows, false);
     bool staged = false;
     auto go = [&](void (*kernel)(const RmsFwd)) {
       RmsLaunch l = {};
-      const int row_bytes = staged ? segment_bytes(p.C, sizeof(Tx), g.ve > 1) + (p.residual ? segment_bytes(p.C, sizeof(Ts), g.ve > 1) : 0) : 0;
-      const cudaError_t err = rms_launch((const void*)kernel, g, p.rows, row_bytes, &l);
+      int row_bytes = 0;
+      if (staged) row_bytes = segment_bytes(p.C, g.ve, sizeof(Tx), g.ragged) + (p.residual ? segment_bytes(p.C, g.ve, sizeof(Ts), g.ragged) : 0);
+      const cudaError_t err = rms_launch((const void*)kernel, g, p.rows, row_bytes, g.v ? plane_bytes(p.C, g.ve, g.ragged) : 0, &l);
       if (err != cudaSuccess) return err;
       p.lanes = g.lanes, p.stages = l.stages, p.stage_bytes = row_bytes;
       kernel<<<l.grid, l.threads, l.smem, stream>>>(p);
       return cudaGetLastError();
     };
-    if (g.ve) {
-      const cudaError_t err = with_geometry<16 / (int)sizeof(Tx)>(g, [&](auto ve, auto v, auto warp) {
+    if (g.v) {
+      const cudaError_t err = with_geometry<16 / (int)sizeof(Tx)>(g, [&](auto ve, auto v, auto warp, auto ragged) {
         constexpr int VE = decltype(ve)::value, V = decltype(v)::value;
-        constexpr bool WARP = decltype(warp)::value;
+        constexpr bool WARP = decltype(warp)::value, RAGGED = decltype(ragged)::value;
         staged = kStaged<Tx, Ts, VE, V, WARP>;
         if constexpr (std::is_same<Tx, Ts>::value)
-          if (!p.residual) return go(&rms_fwd_kernel<Tx, Ts, VE, V, WARP, Q, false>);
-        return go(&rms_fwd_kernel<Tx, Ts, VE, V, WARP, Q, true>);
+          if (!p.residual) return go(&rms_fwd_kernel<Tx, Ts, VE, V, WARP, Q, false, RAGGED>);
+        return go(&rms_fwd_kernel<Tx, Ts, VE, V, WARP, Q, true, RAGGED>);
       });
       if (err != cudaErrorInvalidValue) return err;
-      g = RmsGeom{0, 0, kMostThreads, kMostThreads, false};
+      g = RmsGeom{1, 0, kMostThreads, kMostThreads, false, false};
       staged = false;
     }
     return go(&rms_fwd_any_kernel<Tx, Ts, Q>);
@@ -755,40 +882,60 @@ cudaError_t launch_rms_fwd(RmsFwd p, int dtype, int sum_dtype, bool aligned, cud
 }
 
 // `grid_only`: the number of CTAs, that is of rows of partial sums, is all that is wanted
-cudaError_t launch_rms_bwd(RmsBwd p, int dtype, int sum_dtype, bool aligned, cudaStream_t stream, unsigned* grid, bool grid_only) {
+cudaError_t launch_rms_bwd(RmsBwd p, int dtype, int sum_dtype, Rows rows, cudaStream_t stream, unsigned* grid, bool grid_only) {
   return with_types(dtype, sum_dtype, [&](auto tx, auto ts) {
     using Tx = decltype(tx);
     using Ts = decltype(ts);
-    RmsGeom g = rms_geometry(p.C, dtype, aligned, true);
+    RmsGeom g = rms_geometry(p.C, dtype, rows, true);
     auto go = [&](void (*kernel)(const RmsBwd)) {
       RmsLaunch l = {};
       int row_bytes = 0;
-      if (g.ve)
-        row_bytes = segment_bytes(p.C, sizeof(Tx), g.ve > 1) * (p.addend ? 2 : 1) + segment_bytes(p.C, sizeof(Ts), g.ve > 1) * (p.dsum ? 2 : 1);
-      const cudaError_t err = rms_launch((const void*)kernel, g, p.rows, row_bytes, &l);
+      if (g.v)
+        row_bytes = segment_bytes(p.C, g.ve, sizeof(Tx), g.ragged) * (p.addend ? 2 : 1) + segment_bytes(p.C, g.ve, sizeof(Ts), g.ragged) * (p.dsum ? 2 : 1);
+      const cudaError_t err = rms_launch((const void*)kernel, g, p.rows, row_bytes, g.v ? plane_bytes(p.C, g.ve, g.ragged) : 0, &l);
       if (err != cudaSuccess) return err;
-      *grid = g.ve ? l.grid : std::min(l.grid, (unsigned)std::max(1, (1 << 24) / p.C));  // 64 MB of partial sums at most, or one row
+      *grid = g.v ? l.grid : std::min(l.grid, (unsigned)std::max(1, (1 << 24) / p.C));  // 64 MB of partial sums at most, or one row
       if (grid_only) return cudaSuccess;
       p.lanes = g.lanes, p.stages = l.stages, p.stage_bytes = row_bytes;
       kernel<<<*grid, l.threads, l.smem, stream>>>(p);
       return cudaGetLastError();
     };
-    if (g.ve) {
-      const cudaError_t err = with_geometry<16 / (int)sizeof(Tx)>(g, [&](auto ve, auto v, auto warp) {
+    if (g.v) {
+      const cudaError_t err = with_geometry<16 / (int)sizeof(Tx)>(g, [&](auto ve, auto v, auto warp, auto ragged) {
         constexpr int VE = decltype(ve)::value, V = decltype(v)::value;
-        constexpr bool WARP = decltype(warp)::value;
+        constexpr bool WARP = decltype(warp)::value, RAGGED = decltype(ragged)::value;
         if constexpr (std::is_same<Tx, Ts>::value)
-          if (!p.addend && !p.dsum) return go(&rms_bwd_kernel<Tx, Ts, VE, V, WARP, false>);
-        return go(&rms_bwd_kernel<Tx, Ts, VE, V, WARP, true>);
+          if (!p.addend && !p.dsum) return go(&rms_bwd_kernel<Tx, Ts, VE, V, WARP, false, RAGGED>);
+        return go(&rms_bwd_kernel<Tx, Ts, VE, V, WARP, true, RAGGED>);
       });
       if (err != cudaErrorInvalidValue) return err;
-      g = RmsGeom{0, 0, kMostThreads, kMostThreads, false};
+      g = RmsGeom{1, 0, kMostThreads, kMostThreads, false, false};
     }
     return go(&rms_bwd_any_kernel<Tx, Ts>);
   });
 }
 
-bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// How the rows of a call's tensors lie together.  `width`: elements a vector.  Aligned: addresses and strides on vector boundaries, whole
+// vectors a row.  In one frame: every tensor's first row begins as many elements behind a vector boundary, and its rows keep the distance of
+// contiguous ones from such boundaries.
+struct TensorRows {
+  const void* p;  // NULL: not there
+  int64_t stride;
+  int size;
+};
+Rows rows_of(int width, int64_t C, int64_t rows, const void* weight, std::initializer_list<TensorRows> tensors) {
+  bool aligned = C % width == 0 && reinterpret_cast<uintptr_t>(weight) % 16 == 0, framed = true;
+  int64_t skew = -1;
+  for (const TensorRows& t : tensors) {
+    if (!t.p) continue;
+    const int64_t bytes = (int64_t)width * t.size, behind = (int64_t)(reinterpret_cast<uintptr_t>(t.p) % (uintptr_t)bytes);
+    aligned = aligned && behind % std::min<int64_t>(bytes, 16) == 0 && (rows == 1 || t.stride % width == 0);
+    framed = framed && behind % t.size == 0 && (skew < 0 || behind / t.size == skew) && (rows == 1 || (t.stride - C) % width == 0);
+    if (skew < 0) skew = behind / t.size;
+  }
+  return aligned ? kAligned : framed ? kRagged : kAny;
+}
+int size_of(int dtype) { return dtype == GNB200_F32 ? 4 : 2; }
 bool dtype_ok(int d) { return d == GNB200_F32 || d == GNB200_F16 || d == GNB200_BF16; }
 
 int check_rows(const char* name, int64_t rows, int64_t C, int dtype, int sum_dtype, int w_dtype) {
@@ -838,11 +985,12 @@ static int rms_forward(const char* name, const void* x, int64_t x_stride, const 
   p.rows = rows, p.x_stride = x_stride, p.r_stride = residual_stride;
   p.C = (int)C, p.w_dtype = weight_dtype, p.block = block, p.blocks = block ? (int)((C + block - 1) / block) : 1, p.format = format;
   p.eps = (float)eps, p.offset = (float)offset, p.inv_c = (float)(1.0 / (double)C);
-  const int full = dtype == GNB200_F32 ? 4 : 8;
-  const bool aligned = on16(x) && on16(residual) && on16(weight) && on16(y) && on16(sum) && x_stride % full == 0 && (!residual || residual_stride % full == 0);
+  const int size = size_of(dtype), wide = size_of(residual_dtype);
+  const Rows how = rows_of(dtype == GNB200_F32 ? 4 : 8, C, rows, weight,
+                           {{x, x_stride, size}, {residual, residual_stride, wide}, {y, C, codes ? 1 : size}, {sum, C, wide}});
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return launched(name, codes ? launch_rms_fwd<true>(p, dtype, residual_dtype, aligned, s)
-                              : launch_rms_fwd<false>(p, dtype, residual_dtype, aligned, s));
+  return launched(name, codes ? launch_rms_fwd<true>(p, dtype, residual_dtype, how, s)
+                              : launch_rms_fwd<false>(p, dtype, residual_dtype, how, s));
 }
 
 int gnb200_rms_fwd(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight, int64_t rows,
@@ -869,11 +1017,14 @@ size_t gnb200_rms_bwd_workspace_bytes(int64_t rows, int64_t C, int dtype, int su
   RmsBwd p = {};
   p.rows = rows, p.C = (int)C;
   size_t most = 0;
-  for (int kind = 0; kind < 8; ++kind) {  // whichever kernel and stages the call's tensors will ask for (none of these is read)
+  const int width = dtype == GNB200_F32 ? 4 : 8;
+  for (int kind = 0; kind < 12; ++kind) {  // whichever kernel and stages the call's tensors will ask for (none of these is read)
     p.addend = kind & 1 ? &p : nullptr;
     p.dsum = kind & 2 ? &p : nullptr;
+    const Rows how = kind < 4 ? kAligned : kind < 8 ? kRagged : kAny;
+    if (how == kAligned && C % width != 0) continue;
     unsigned grid = 0;
-    if (launch_rms_bwd(p, dtype, sum_dtype, (kind & 4) != 0, nullptr, &grid, true) != cudaSuccess) return 0;
+    if (launch_rms_bwd(p, dtype, sum_dtype, how, nullptr, &grid, true) != cudaSuccess) return 0;
     const size_t need = (size_t)grid * (size_t)C * sizeof(float);
     most = need > most ? need : most;
   }
@@ -899,20 +1050,20 @@ int gnb200_rms_bwd(const void* dy, int64_t dy_stride, const void* dsum, int64_t 
   p.dy = dy, p.dsum = dsum, p.sum = sum, p.addend = addend, p.weight = weight, p.rstd = rstd, p.dx = dx, p.dsum_out = dsum_out;
   p.rows = rows, p.dy_stride = dy_stride, p.ds_stride = dsum_stride, p.s_stride = sum_stride, p.a_stride = addend_stride;
   p.C = (int)C, p.w_dtype = weight_dtype, p.offset = (float)offset, p.inv_c = (float)(1.0 / (double)C);
-  const int full = dtype == GNB200_F32 ? 4 : 8;
-  const bool aligned = on16(dy) && on16(dsum) && on16(weight) && on16(sum) && on16(addend) && on16(dx) && on16(dsum_out) &&
-                       dy_stride % full == 0 && sum_stride % full == 0 && (!dsum || dsum_stride % full == 0) &&
-                       (!addend || addend_stride % full == 0);
+  const int size = size_of(dtype), wide = size_of(sum_dtype);
+  const Rows how = rows_of(dtype == GNB200_F32 ? 4 : 8, C, rows, weight,
+                           {{dy, dy_stride, size}, {dsum, dsum_stride, wide}, {sum, sum_stride, wide}, {addend, addend_stride, size},
+                            {dx, C, size}, {dsum_out, C, wide}});
   unsigned grid = 0;
   if (dweight) {
-    cudaError_t err = launch_rms_bwd(p, dtype, sum_dtype, aligned, s, &grid, true);
+    cudaError_t err = launch_rms_bwd(p, dtype, sum_dtype, how, s, &grid, true);
     if (err != cudaSuccess) return launched(name, err);
     const size_t need = (size_t)grid * (size_t)C * sizeof(float);
     if (!workspace || workspace_bytes < need)
       return report_error(GNB200_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu are needed", name, workspace ? workspace_bytes : (size_t)0, need);
     p.part = static_cast<float*>(workspace);
   }
-  cudaError_t err = launch_rms_bwd(p, dtype, sum_dtype, aligned, s, &grid, false);
+  cudaError_t err = launch_rms_bwd(p, dtype, sum_dtype, how, s, &grid, false);
   if (err == cudaSuccess && dweight) err = launch_column_sums(ColumnSums{{p.part}, {dweight}, {(int)grid}, (int)C, weight_dtype}, 1, s, true);
   return launched(name, err);
 }

@@ -56,10 +56,19 @@ bool uniform_rows(const Tensor& t, int64_t* stride) {
   *stride = rows == 1 ? sizes[last] : step;
   return true;
 }
-Tensor as_rows(const Tensor& t, int64_t* stride) {
-  if (!t.defined() || t.numel() == 0 || uniform_rows(t, stride)) return t;
-  Tensor c = t.contiguous();
-  uniform_rows(c, stride);
+// The rows as the vector kernels take them: in place where they lie on vector boundaries, or are contiguous from one on (as results are:
+// the same frame); copied first otherwise.  x_type: of the call's x, whose vectors the others' follow.
+Tensor as_rows(const Tensor& t, at::ScalarType x_type, int64_t* stride) {
+  if (!t.defined() || t.numel() == 0) return t;
+  const int64_t width = x_type == at::kFloat ? 4 : 8, C = t.size(-1), frame = width * (int64_t)t.element_size();
+  const auto at = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+  if (uniform_rows(t, stride)) {
+    if (C % width == 0 && *stride % width == 0 && at % 16 == 0) return t;
+    if ((*stride == C || t.numel() == C) && at % frame == 0) return t;
+  }
+  Tensor c = empty_like_sizes(t.sizes(), t.scalar_type(), t);
+  c.copy_(t);
+  *stride = C;
   return c;
 }
 
@@ -96,7 +105,8 @@ RmsOut rms_forward(const Tensor& x, const Tensor& weight, const Tensor& residual
   c10::cuda::CUDAGuard guard(x.device());
   const int64_t C = x.size(-1), rows = x.numel() / C;
   int64_t x_stride = C, r_stride = C;
-  const Tensor xr = as_rows(x, &x_stride), rr = as_rows(residual, &r_stride);
+  const auto st = x.scalar_type();
+  const Tensor xr = as_rows(x, st, &x_stride), rr = as_rows(residual, st, &r_stride);
   RmsOut out;
   if (residual.defined()) out.sum = empty_like_sizes(x.sizes(), residual.scalar_type(), x);
   const auto stream = c10::cuda::getCurrentCUDAStream().stream();
@@ -142,7 +152,9 @@ RmsGrads rms_backward(const Tensor& dy, const Tensor& dsum, const Tensor& sum, c
               "gnb200: weight must be a contiguous vector of one element per channel in the dtype of dy or float32");
   c10::cuda::CUDAGuard guard(dy.device());
   int64_t dy_stride = C, ds_stride = C, s_stride = C, a_stride = C;
-  const Tensor dyr = as_rows(dy, &dy_stride), dsr = as_rows(dsum, &ds_stride), sr = as_rows(sum, &s_stride), ar = as_rows(addend, &a_stride);
+  const auto st = dy.scalar_type();
+  const Tensor dyr = as_rows(dy, st, &dy_stride), dsr = as_rows(dsum, st, &ds_stride), sr = as_rows(sum, st, &s_stride),
+               ar = as_rows(addend, st, &a_stride);
   const int dtype = code_of(dy), sum_dtype = code_of(sum);
   RmsGrads out;
   out.dx = empty_like_sizes(dy.sizes(), dy.scalar_type(), dy);
