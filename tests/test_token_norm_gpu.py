@@ -293,3 +293,61 @@ def test_refusals():
         with pytest.raises(ValueError):
             bad()
     assert torch.isfinite(pkg.rms_norm(x, w, r)[0]).all()  # nothing was left broken
+
+
+def test_rows_without_a_common_frame_through_the_c_abi():
+    # the Python functions copy such tensors; the C entry points take them as they are
+    import ctypes
+
+    from channels_last_groupnorm_b200 import _native as nt
+
+    rows, c = 9, 150
+    base = torch.randn(rows, 157, device="cuda").to(BF16)
+    x, r = base[:, 3:153], torch.randn(rows, 160, device="cuda").to(BF16)[:, 1:151]
+    w = torch.rand(c, device="cuda").to(BF16)
+    y, s = torch.full((rows * c + 5,), 7.0, device="cuda", dtype=BF16), torch.full((rows * c + 5,), 7.0, device="cuda", dtype=BF16)
+    rstd = torch.empty(rows, device="cuda")
+    at = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    out = lambda t: ctypes.c_void_p(t.data_ptr() + 4)  # noqa: E731
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    nt.check(nt.lib.gnb200_rms_fwd(at(x), 157, at(r), 160, at(w), rows, c, 1e-6, 0.0, 2, 2, 2, out(y), out(s), at(rstd), stream))
+    want, sums, root = ref.rms(x, w, r, 1e-6, 0.0)
+    ref.within(y[2:-3].view(rows, c), want, ref.rounded(want, BF16) + FORWARD * want.abs())
+    ref.within(rstd, root.squeeze(-1), FORWARD * root.squeeze(-1))
+    for t in (y, s):
+        assert (t[:2] == 7).all() and (t[-3:] == 7).all()
+    dy = torch.randn(rows, 151, device="cuda").to(BF16)[:, :c]
+    dx = torch.full((rows * c + 5,), 7.0, device="cuda", dtype=BF16)
+    dw = torch.empty(c, device="cuda", dtype=BF16)
+    need = nt.lib.gnb200_rms_bwd_workspace_bytes(rows, c, 2, 2)
+    ws = torch.empty(need, device="cuda", dtype=torch.uint8)
+    nt.check(nt.lib.gnb200_rms_bwd(at(dy), 151, None, 0, at(r), 160, at(x), 157, at(w), at(rstd), rows, c, 0.0, 2, 2, 2, out(dx), None, at(dw), at(ws),
+                                   need, stream))
+    d, dweight, size, wsize = ref.rms_grads(dy, None, x.double() + r.double(), root, w, 0.0)
+    ref.within(dx[2:-3].view(rows, c), d, ref.rounded(d, BF16) + 2 * FORWARD * size)
+    ref.within(dw, dweight, ref.rounded(dweight, BF16) + (FORWARD + (rows + 64) * ref.U32) * wsize)
+    assert (dx[:2] == 7).all() and (dx[-3:] == 7).all()
+    # a workspace that is too small is refused before anything is launched
+    assert nt.lib.gnb200_rms_bwd(at(dy), 151, None, 0, at(r), 160, at(x), 157, at(w), at(rstd), rows, c, 0.0, 2, 2, 2, out(dx), None, at(dw), at(ws),
+                                 16, stream) == -2
+
+
+@pytest.mark.parametrize("c", [31, 150, 1111, 2050, 12345])
+@pytest.mark.parametrize("rows", [1, 2, 17, 3000])
+def test_odd_rows_write_nothing_beside_them(c, rows):
+    # outputs in the middle of larger buffers, rows of every skew; all parts of a row beside rows of other values
+    if rows * c > 2e7:
+        rows = 301
+    x, w, r, dy, ds = _inputs(rows, c, BF16, BF16, BF16, seed=3, grads=True)
+    for t in (x, r, w):
+        t.requires_grad_(True)
+    y, s = pkg.rms_norm(x, w, r)
+    grads = torch.autograd.grad((y, s), (x, r, w), (dy, ds))
+    pick = sorted({0, 1, rows // 2, rows - 1} & set(range(rows)))
+    one, two = pkg.rms_norm(x.detach()[pick], w.detach(), r.detach()[pick])
+    assert torch.equal(y[pick], one) and torch.equal(s[pick], two)
+    _, _, rstd = ref.rms(x.detach(), None, r.detach(), 1e-6, 0.0)
+    d, dw, size, wsize = ref.rms_grads(dy, ds, x.detach().double() + r.detach().double(), rstd, w.detach(), 0.0)
+    ref.within(grads[0], d, ref.rounded(d, BF16) + 2 * FORWARD * size)
+    ref.within(grads[2], dw, ref.rounded(dw, BF16) + (FORWARD + (rows + 64) * ref.U32) * wsize)
+    _check_quant(x.detach(), w.detach(), r.detach(), 64, torch.float8_e4m3fn)
