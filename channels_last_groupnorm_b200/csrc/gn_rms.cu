@@ -44,27 +44,31 @@ __device__ __forceinline__ float scale_of(uint32_t most, int format) {
   return s < kSmallestScale ? kSmallestScale : s;  // (a NaN stays)
 }
 __device__ __forceinline__ float inverse_of(float scale) { return __fdividef(1.f, scale); }
+__device__ __forceinline__ uint32_t code_of(float v, int format) {
+  if (format == GNB200_E4M3) return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+  return (uint32_t)max(-127, min(127, __float2int_rn(v))) & 0xffu;
+}
+// VE codes, four a word
 template <int VE>
-__device__ __forceinline__ Pack<uint8_t, VE> codes_of(const float (&f)[VE], float inverse, int format) {
-  Pack<uint8_t, VE> c;
-  if (format == GNB200_E4M3) {
-    if constexpr (VE % 2 == 0) {
+__device__ __forceinline__ void codes_of(const float (&f)[VE], float inverse, int format, uint32_t (&w)[VE / 4]) {
+  float v[VE];
 #pragma unroll
-      for (int e = 0; e < VE; e += 2) {
-        const __nv_fp8x2_storage_t two =
-            __nv_cvt_float2_to_fp8x2(make_float2(f[e] * inverse, f[e + 1] * inverse), __NV_SATFINITE, __NV_E4M3);
-        c.v[e] = (uint8_t)(two & 0xff);
-        c.v[e + 1] = (uint8_t)(two >> 8);
-      }
+  for (int e = 0; e < VE; ++e) v[e] = f[e];
+  scale_each(v, inverse);
+#pragma unroll
+  for (int k = 0; k < VE / 4; ++k) {
+    const float* g = v + 4 * k;
+    if (format == GNB200_E4M3) {
+      const uint32_t low = __nv_cvt_float2_to_fp8x2(make_float2(g[0], g[1]), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t high = __nv_cvt_float2_to_fp8x2(make_float2(g[2], g[3]), __NV_SATFINITE, __NV_E4M3);
+      w[k] = __byte_perm(low, high, 0x5410);
     } else {
+      int n[4];
 #pragma unroll
-      for (int e = 0; e < VE; ++e) c.v[e] = (uint8_t)__nv_cvt_float_to_fp8(f[e] * inverse, __NV_SATFINITE, __NV_E4M3);
+      for (int e = 0; e < 4; ++e) n[e] = max(-127, min(127, __float2int_rn(g[e])));
+      w[k] = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < VE; ++e) c.v[e] = (uint8_t)(int8_t)max(-127, min(127, __float2int_rn(f[e] * inverse)));
   }
-  return c;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -196,16 +200,17 @@ __device__ __forceinline__ void fetch_weight(float (&w)[V][VE], const void* p, i
 // the codes of vector i of the row whose frame begins at `row`
 template <int VE, bool RAGGED>
 __device__ __forceinline__ void store_codes(uint8_t* row, const Frame<VE, RAGGED>& frame, int i, const float (&f)[VE], float inverse, int format) {
-  const Pack<uint8_t, VE> c = codes_of<VE>(f, inverse, format);
+  uint32_t w[VE / 4];
+  codes_of<VE>(f, inverse, format, w);
   if (frame.whole(i)) {
     if constexpr (VE == 8)
-      *reinterpret_cast<uint2*>(row + i * VE) = *reinterpret_cast<const uint2*>(&c);
+      *reinterpret_cast<uint2*>(row + i * VE) = make_uint2(w[0], w[1]);
     else
-      *reinterpret_cast<uint32_t*>(row + i * VE) = *reinterpret_cast<const uint32_t*>(&c);
+      *reinterpret_cast<uint32_t*>(row + i * VE) = w[0];
   } else {
 #pragma unroll
     for (int e = 0; e < VE; ++e)
-      if (frame.has(i, e)) row[i * VE + e] = c.v[e];
+      if (frame.has(i, e)) row[i * VE + e] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
   }
 }
 
@@ -420,9 +425,11 @@ __global__ void __launch_bounds__(WARP ? kWarpThreads : kMostThreads) rms_fwd_ke
           const int i = first + v * lanes;
           m[v] = 0;
           if (i < nvec) {  // (beyond the row a NaN rstd would leave NaN in the zeros)
+            float most_of = 0.f;
 #pragma unroll
             for (int e = 0; e < VE; ++e)
-              if (frame.has(i, e)) m[v] = max(m[v], magnitude(s[v][e]));
+              if (frame.has(i, e)) most_of = larger(most_of, fabsf(s[v][e]));
+            m[v] = magnitude(most_of);
           }
         }
         if (p.block == 0) {
@@ -491,7 +498,7 @@ __global__ void __launch_bounds__(kMostThreads) rms_fwd_any_kernel(const RmsFwd 
         if (threadIdx.x == 0) p.scale[row] = scale;
         for (int i = threadIdx.x; i < p.C; i += blockDim.x) {
           const float f[1] = {y_at(i)};
-          out[i] = codes_of<1>(f, inverse, p.format).v[0];
+          out[i] = (uint8_t)code_of(f[0] * inverse, p.format);
         }
       } else {  // one warp per block of at most 128 channels
         const int lane = threadIdx.x & 31, nwarps = blockDim.x >> 5;
@@ -509,7 +516,7 @@ __global__ void __launch_bounds__(kMostThreads) rms_fwd_any_kernel(const RmsFwd 
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             const int in = lane + 32 * v, i = b * p.block + in;
-            if (in < p.block && i < p.C) out[i] = codes_of<1>(f[v], inverse, p.format).v[0];
+            if (in < p.block && i < p.C) out[i] = (uint8_t)code_of(f[v][0] * inverse, p.format);
           }
         }
       }
@@ -881,8 +888,10 @@ cudaError_t launch_rms_fwd(RmsFwd p, int dtype, int sum_dtype, Rows rows, cudaSt
   });
 }
 
-// `grid_only`: the number of CTAs, that is of rows of partial sums, is all that is wanted
-cudaError_t launch_rms_bwd(RmsBwd p, int dtype, int sum_dtype, Rows rows, cudaStream_t stream, unsigned* grid, bool grid_only) {
+// `grid`: the number of CTAs, that is of rows of partial sums.  With `room` (bytes of workspace) nothing is launched where they do not fit;
+// kGridOnly: nothing at all.
+constexpr size_t kGridOnly = ~(size_t)0;
+cudaError_t launch_rms_bwd(RmsBwd p, int dtype, int sum_dtype, Rows rows, cudaStream_t stream, unsigned* grid, size_t room) {
   return with_types(dtype, sum_dtype, [&](auto tx, auto ts) {
     using Tx = decltype(tx);
     using Ts = decltype(ts);
@@ -895,7 +904,7 @@ cudaError_t launch_rms_bwd(RmsBwd p, int dtype, int sum_dtype, Rows rows, cudaSt
       const cudaError_t err = rms_launch((const void*)kernel, g, p.rows, row_bytes, g.v ? plane_bytes(p.C, g.ve, g.ragged) : 0, &l);
       if (err != cudaSuccess) return err;
       *grid = g.v ? l.grid : std::min(l.grid, (unsigned)std::max(1, (1 << 24) / p.C));  // 64 MB of partial sums at most, or one row
-      if (grid_only) return cudaSuccess;
+      if (room == kGridOnly || (p.part && (size_t)*grid * (size_t)p.C * sizeof(float) > room)) return cudaSuccess;
       p.lanes = g.lanes, p.stages = l.stages, p.stage_bytes = row_bytes;
       kernel<<<*grid, l.threads, l.smem, stream>>>(p);
       return cudaGetLastError();
@@ -1024,7 +1033,7 @@ size_t gnb200_rms_bwd_workspace_bytes(int64_t rows, int64_t C, int dtype, int su
     const Rows how = kind < 4 ? kAligned : kind < 8 ? kRagged : kAny;
     if (how == kAligned && C % width != 0) continue;
     unsigned grid = 0;
-    if (launch_rms_bwd(p, dtype, sum_dtype, how, nullptr, &grid, true) != cudaSuccess) return 0;
+    if (launch_rms_bwd(p, dtype, sum_dtype, how, nullptr, &grid, kGridOnly) != cudaSuccess) return 0;
     const size_t need = (size_t)grid * (size_t)C * sizeof(float);
     most = need > most ? need : most;
   }
@@ -1056,14 +1065,13 @@ int gnb200_rms_bwd(const void* dy, int64_t dy_stride, const void* dsum, int64_t 
                             {dx, C, size}, {dsum_out, C, wide}});
   unsigned grid = 0;
   if (dweight) {
-    cudaError_t err = launch_rms_bwd(p, dtype, sum_dtype, how, s, &grid, true);
-    if (err != cudaSuccess) return launched(name, err);
-    const size_t need = (size_t)grid * (size_t)C * sizeof(float);
-    if (!workspace || workspace_bytes < need)
-      return report_error(GNB200_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu are needed", name, workspace ? workspace_bytes : (size_t)0, need);
+    if (!workspace) return report_error(GNB200_ERR_WORKSPACE, "%s: a gradient of the weight without a workspace", name);
     p.part = static_cast<float*>(workspace);
   }
-  cudaError_t err = launch_rms_bwd(p, dtype, sum_dtype, how, s, &grid, false);
+  cudaError_t err = launch_rms_bwd(p, dtype, sum_dtype, how, s, &grid, workspace_bytes);
+  const size_t need = (size_t)grid * (size_t)C * sizeof(float);
+  if (err == cudaSuccess && dweight && need > workspace_bytes)
+    return report_error(GNB200_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu are needed", name, workspace_bytes, need);
   if (err == cudaSuccess && dweight) err = launch_column_sums(ColumnSums{{p.part}, {dweight}, {(int)grid}, (int)C, weight_dtype}, 1, s, true);
   return launched(name, err);
 }

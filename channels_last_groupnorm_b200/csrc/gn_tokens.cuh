@@ -4,9 +4,6 @@
 #include <cuda_fp8.h>
 
 #include <array>
-#include <map>
-#include <mutex>
-#include <tuple>
 
 #include "gn_common.cuh"
 
@@ -156,6 +153,12 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {
 // (Shuffles for the maximum too: with __reduce_max_sync one of the kernels gave lane 0's value to all lanes.)
 // Magnitudes compare like their bit patterns, with NaN above infinity: an integer maximum keeps a NaN, fmaxf would drop it.
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// the larger of two magnitudes, or NaN where one is
+__device__ __forceinline__ float larger(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
 __device__ __forceinline__ uint32_t lanes_max(uint32_t v, int lanes) {
 #pragma unroll
   for (int delta = 16; delta >= 1; delta >>= 1)
@@ -213,24 +216,15 @@ __device__ __forceinline__ uint32_t cta_max(uint32_t v, uint32_t* slots) {  // (
   return t;
 }
 
-// CTAs of `kernel` that one SM holds at once with `smem` bytes of dynamic shared memory, and the SMs of the current device (asked once per
-// kernel, CTA size, shared memory and device; the first question raises the kernel's limit of shared memory)
+// CTAs of `kernel` that one SM holds at once with `smem` bytes of dynamic shared memory, and the SMs of the current device (the question
+// also raises the kernel's limit of shared memory)
 struct Residency {
   int per_sm, sms;
 };
-inline cudaError_t residency(const void* kernel, int threads, int smem, Residency* out) {
+inline cudaError_t ask_residency(const void* kernel, int threads, int smem, Residency* out) {
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
-  static std::mutex mu;
-  static std::map<std::tuple<const void*, int, int, int>, Residency> known;
-  std::lock_guard<std::mutex> lock(mu);
-  const auto key = std::make_tuple(kernel, threads, smem, dev);
-  const auto it = known.find(key);
-  if (it != known.end()) {
-    *out = it->second;
-    return cudaSuccess;
-  }
   Residency r = {};
   err = cudaDeviceGetAttribute(&r.sms, cudaDevAttrMultiProcessorCount, dev);
   if (err != cudaSuccess) return err;
@@ -241,7 +235,30 @@ inline cudaError_t residency(const void* kernel, int threads, int smem, Residenc
   err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&r.per_sm, kernel, threads, smem);
   if (err != cudaSuccess) return err;
   if (r.per_sm < 1) return cudaErrorLaunchOutOfResources;
-  *out = known[key] = r;
+  *out = r;
+  return cudaSuccess;
+}
+inline cudaError_t residency(const void* kernel, int threads, int smem, Residency* out) {
+  // a thread's last answers, one per place of a small table
+  struct Known {
+    const void* kernel;
+    int threads, smem, dev;
+    Residency r;
+  };
+  constexpr int kPlaces = 64;
+  static thread_local Known known[kPlaces] = {};
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  const size_t mix = (reinterpret_cast<uintptr_t>(kernel) >> 4) * 31 + (size_t)threads * 7 + (size_t)(smem >> 4) * 13 + (size_t)dev;
+  Known& k = known[mix % kPlaces];
+  if (k.kernel != kernel || k.threads != threads || k.smem != smem || k.dev != dev) {
+    Residency r;
+    err = ask_residency(kernel, threads, smem, &r);
+    if (err != cudaSuccess) return err;
+    k = Known{kernel, threads, smem, dev, r};
+  }
+  *out = k.r;
   return cudaSuccess;
 }
 

@@ -98,8 +98,9 @@ struct RmsOut {
 };
 // format < 0: y in x's type; else codes
 RmsOut rms_forward(const Tensor& x, const Tensor& weight, const Tensor& residual, double eps, double offset, bool want_rstd, int64_t block,
-                   int format) {
-  if (const char* why = refusal_of_rows(x, weight, residual)) TORCH_CHECK(false, "gnb200: ", why);
+                   int format, bool checked = false) {
+  if (!checked)
+    if (const char* why = refusal_of_rows(x, weight, residual)) TORCH_CHECK(false, "gnb200: ", why);
   TORCH_CHECK(format < 0 || block == 0 || block == 32 || block == 64 || block == 128,
               "gnb200: block is 0 (one scale per row), 32, 64 or 128 channels, got ", block);
   c10::cuda::CUDAGuard guard(x.device());
@@ -203,7 +204,7 @@ struct RmsFunction : torch::autograd::Function<RmsFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual_arg, const OptTensor& weight_arg, double eps,
                                double offset) {
     const Tensor residual = value(residual_arg), weight = value(weight_arg);
-    RmsOut o = rms_forward(x, weight, residual, eps, offset, true, 0, -1);
+    RmsOut o = rms_forward(x, weight, residual, eps, offset, true, 0, -1, true);
     ctx->set_materialize_grads(false);
     // The stored sum of a 16-bit stream is rounded: good enough for the gradient of x, whose terms are rounded alike, but it would cost
     // the weight's gradient, a sum in fp32 over all rows, what its 16 bits lack.  There the backward adds x and the residual again.
@@ -484,7 +485,7 @@ std::tuple<Tensor, Tensor> gnb200_ops::rms_norm_direct(const Tensor& x, const Te
     return {out[0], out.size() > 1 ? out[1] : Tensor()};
   }
   at::AutoDispatchBelowADInplaceOrView guard;
-  RmsOut o = rms_forward(x, weight, residual, eps, offset, false, 0, -1);
+  RmsOut o = rms_forward(x, weight, residual, eps, offset, false, 0, -1, true);
   return {o.y, o.sum};
 }
 
@@ -494,7 +495,7 @@ std::tuple<Tensor, Tensor, Tensor> gnb200_ops::rms_quant_direct(const Tensor& x,
         (block == 0 || block == 32 || block == 64 || block == 128) && (format == GNB200_E4M3 || format == GNB200_INT8);
   if (!*ok) return {};
   at::AutoDispatchBelowADInplaceOrView guard;
-  RmsOut o = rms_forward(x, weight, residual, eps, offset, false, block, (int)format);
+  RmsOut o = rms_forward(x, weight, residual, eps, offset, false, block, (int)format, true);
   return {o.y, o.scale, o.sum};
 }
 
