@@ -7,10 +7,18 @@
 //   d = ds + rstd * (g - n * mean(g * n))   with n = s * rstd, g = dy * (offset + w): the gradient of x and of r
 //   dw = sum over rows of dy * n
 //
-// Every element is read and written once: a row's elements stay in registers between the sum over the row and the
-// output.  Rows of up to four vectors a lane belong to a group of lanes of one warp (shuffles only), longer ones to a CTA (one barrier
-// a sum); longer ones still are read twice, element by element (`any`).  The grid holds the CTAs that are resident at once; each keeps its
-// channels' weights in registers, walks over the rows and asks for its next row before it reduces the present one.
+// Every element is read and written once: a row's elements stay in registers (backward: in shared memory) between the sum over the row and
+// the output, and the only traffic beside them is a row of partial sums per CTA in the backward.  Bound by HBM where there are rows enough:
+// 16384 x 4096 bf16 with the residual, forward 88 us = 6.1 TB/s, backward (four tensors read, one written) 106 us = 6.3 TB/s, 93 and
+// 96 % of a copy's rate; 8192 x 8192 bf16 over an fp32 stream to 8 bits 118 us = 6.3 TB/s.  A call of one row takes 2.2 us, of 8 rows in
+// 8 bits 3: launch, first load and one reduction.
+//
+// Rows of up to four vectors a lane belong to a group of lanes of one warp (shuffles only), longer ones to a CTA, or in the backward to a team of
+// warps, of which a CTA has several so that fewer partial rows are left to add up; rows longer than those are read twice, element by
+// element (`any`).  The grid holds the CTAs that are resident at once; each keeps its channels' weights in registers, walks over the rows and
+// asks for the next ones early: into registers while these are few (one row, 64 bytes a thread), otherwise by cp.async into a ring of rows
+// in shared memory, which costs two more instructions a vector but no registers (8192 x 8192 to 8 bits 136 -> 121 us; the backward of
+// 16384 x 4096 125 -> 106, whose spills it ended; the forward of 16384 x 4096 stays in registers: 88 against 93).
 #include <algorithm>
 #include <initializer_list>
 
@@ -22,7 +30,7 @@ namespace gnb200 {
 namespace {
 
 constexpr int kWarpThreads = 128;  // CTA size of the kernels with one group of lanes per row
-constexpr int kMostThreads = 512;  // CTA size limit of the kernels with one CTA per row
+constexpr int kMostThreads = 512;  // CTA size of the kernels for rows of any length
 constexpr float kSmallestScale = 1.17549435e-38f;  // 2^-126: its reciprocal is finite, a block of zeros gets codes of zero
 
 struct RmsFwd {
@@ -78,8 +86,8 @@ __device__ __forceinline__ void codes_of(const float (&f)[VE], float inverse, in
 // holds channels i * VE - skew and on, the first and the last one in part.  All tensors of a call have the same frame (checked by the
 // host), and the step from one of a thread's rows to the next is a multiple of VE rows, so that the skew, and with it the channels of a thread, stay:
 // its weights and sums are in registers as they are for aligned rows.  Device us, element by element before and so: 9000 rows of 1111 bf16 with a
-// residual, forward 27.0 and 24.9, backward 42.3 and 43.3; 3000 of 12345, backward 210 and 166; 4000 of 12345 fp16, 8-bit output with
-// blocks, 592 and 245.
+// residual, forward 27.0 and 25.0, backward 42.3 and 47.1; 3000 of 12345, backward 210 and 167; 4000 of 12345 fp16, 8-bit output with
+// blocks, 592 and 219.  Twice the instructions of aligned rows bound them: the sums' way through shared memory, and the edges.
 template <int VE, bool RAGGED>
 struct Frame {
   int skew, nvec, C;
@@ -117,13 +125,16 @@ struct Frame {
   // Sums over a ragged row go through shared memory, so that they are taken in the row's own order: the same bits wherever the row
   // stands.  Channel j is word j / VE of plane j % VE, which is free of bank conflicts for frames of any skew.
   __device__ __forceinline__ int words() const { return (C + VE - 1) / VE; }  // of a plane
+  // plane and word of element e of vector 0; those of vector i lie i words on
+  __device__ __forceinline__ int place(int e) const { return ((e - skew) & (VE - 1)) * words() - (e < skew ? 1 : 0); }
   __device__ __forceinline__ void lay_out(float* planes, int i, const float (&f)[VE]) const {
-    const bool all = whole(i);
+    if (whole(i)) {
 #pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      // plane and word of element e of vector 0, which are those of vector i but for i words
-      const int at = ((e - skew) & (VE - 1)) * words() - (e < skew ? 1 : 0);
-      if (all || has(i, e)) planes[at + i] = f[e];
+      for (int e = 0; e < VE; ++e) planes[place(e) + i] = f[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+        if (has(i, e)) planes[place(e) + i] = f[e];
     }
   }
   __device__ __forceinline__ void take(const float* planes, int i, float (&f)[VE]) const {
@@ -246,13 +257,14 @@ struct Place {
 // Forward
 // ---------------------------------------------------------------------------------------------
 // What a thread holds of the row that comes next: registers where a few vectors do, otherwise the stages.
-template <typename Tx, typename Ts, int VE, int V, bool WARP>
-constexpr bool kStaged = !WARP && V * VE * (sizeof(Tx) + sizeof(Ts)) > 64;
+template <typename Tx, typename Ts, int VE, int V, int THREADS>
+constexpr bool kStaged = THREADS > kWarpThreads && (THREADS > 512 || V * VE * (sizeof(Tx) + sizeof(Ts)) > 64);
 constexpr int kMostBlocks = 512;  // of the rows that these kernels take
 
-template <typename Tx, typename Ts, int VE, int V, bool WARP, bool Q, bool RES, bool RAGGED>
-__global__ void __launch_bounds__(WARP ? kWarpThreads : kMostThreads) rms_fwd_kernel(const RmsFwd p) {
-  constexpr bool STAGED = kStaged<Tx, Ts, VE, V, WARP>;
+// THREADS: the CTA's at most; kWarpThreads where a row has a group of lanes, otherwise a row has the CTA
+template <typename Tx, typename Ts, int VE, int V, int THREADS, bool Q, bool RES, bool RAGGED>
+__global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
+  constexpr bool WARP = THREADS == kWarpThreads, STAGED = kStaged<Tx, Ts, VE, V, THREADS>;
   extern __shared__ __align__(16) char smem[];
   __shared__ TeamSlots slots;
   __shared__ uint32_t most[32];
@@ -528,7 +540,7 @@ __global__ void __launch_bounds__(kMostThreads) rms_fwd_any_kernel(const RmsFwd 
 // Backward
 // ---------------------------------------------------------------------------------------------
 // CTA sizes: the more rows a CTA takes at once, the fewer rows of partial sums there are to add up afterwards
-constexpr int bwd_threads(int ve, int v) { return ve * v <= 8 ? 1024 : 512; }
+constexpr int bwd_threads(int ve, int v) { return ve * v <= 8 ? 1024 : ve * v <= 16 ? 640 : 512; }
 
 struct RmsBwd {
   const void *dy, *dsum, *sum, *addend, *weight;  // s = sum, or sum + addend (dy's type) where the stored sum was rounded to 16 bits
@@ -540,9 +552,9 @@ struct RmsBwd {
   float offset, inv_c;
 };
 
-template <typename Tx, typename Ts, int VE, int V, bool WARP, bool RES, bool RAGGED>
+template <typename Tx, typename Ts, int VE, int V, int THREADS, bool RES, bool RAGGED>
 __global__ void __launch_bounds__(bwd_threads(VE, V), 1) rms_bwd_kernel(const RmsBwd p) {
-  constexpr bool TEAMS = !WARP;
+  constexpr bool WARP = THREADS == kWarpThreads, TEAMS = !WARP;
   extern __shared__ __align__(16) char smem[];
   __shared__ TeamSlots all_slots[TEAMS ? kMostTeams : 1];
   const Place<WARP, TEAMS> at(p.lanes, p.stage_bytes, p.stages, plane_bytes(p.C, VE, RAGGED), smem);
@@ -748,6 +760,7 @@ __global__ void __launch_bounds__(32 * kSumWarps) column_sums_kernel(const Colum
 struct RmsGeom {
   int ve, v, lanes, threads;  // lanes: per row; threads: per CTA; v = 0: the kernels for rows of any length
   bool warp, ragged;          // warp: lanes of one warp; otherwise whole warps
+  int most;                   // the kernel's limit of lanes
 };
 
 // How a call's rows lie: on vector boundaries, all in the same frame, or neither
@@ -756,7 +769,7 @@ enum Rows { kAligned, kRagged, kAny };
 RmsGeom rms_geometry(int64_t C, int dtype, Rows rows, bool backward) {
   RmsGeom g = {};
   g.ve = dtype == GNB200_F32 ? 4 : 8;
-  if (rows == kAny) return RmsGeom{1, 0, kMostThreads, kMostThreads, false, false};
+  if (rows == kAny) return RmsGeom{1, 0, kMostThreads, kMostThreads, false, false, 0};
   g.ragged = rows == kRagged;
   const int64_t nvec = g.ragged ? (C + 2 * g.ve - 2) / g.ve : C / g.ve;  // (ragged: one more for rows that begin late in their frame)
   if (nvec <= 32 * 4) {  // four vectors a lane
@@ -765,11 +778,20 @@ RmsGeom rms_geometry(int64_t C, int dtype, Rows rows, bool backward) {
     while (g.lanes < 32 && g.lanes < nvec) g.lanes *= 2;
     const int64_t each = (nvec + g.lanes - 1) / g.lanes;
     g.v = each <= 1 ? 1 : each <= 2 ? 2 : 4;
+    g.most = kWarpThreads;
   } else {
-    const int most = 32 / g.ve;
-    g.v = 2;  // (one a thread and more teams: the backward of 16384 x 4096 bf16 takes 131 us instead of 106)
-    while (g.v < most && nvec > (int64_t)g.v * kMostThreads) g.v *= 2;
-    if (nvec > (int64_t)g.v * kMostThreads) return RmsGeom{1, 0, kMostThreads, kMostThreads, false, false};
+    // two vectors a thread, and four of fp32 above 512 threads; the backward, with twice the registers, up to 640 threads, above them four
+    // (eight of fp32) and 512.  (One vector a thread and more teams: the backward of 16384 x 4096 bf16 takes 131 us instead of 106.)
+    const auto fits = [&](int v, int most) {
+      if (nvec > (int64_t)v * most) return false;
+      g.v = v;
+      g.most = most;
+      return true;
+    };
+    const int twice = g.ve == 4 ? 2 : 1;
+    const bool any = backward ? fits(2, 512) || (g.ve == 4 && fits(4, 512)) || fits(2 * twice, 640) || fits(4 * twice, 512)
+                              : fits(2, 512) || (g.ve == 4 && fits(4, 512)) || fits(2 * twice, 1024);
+    if (!any) return rms_geometry(C, dtype, kAny, backward);
     g.lanes = (int)((nvec + g.v - 1) / g.v + 31) / 32 * 32;
   }
   g.threads = g.warp ? kWarpThreads : g.lanes;
@@ -838,20 +860,29 @@ cudaError_t with_types(int dtype, int sum_dtype, F&& f) {
 }
 template <int N>
 using Int = std::integral_constant<int, N>;
-// ... and with the geometry's numbers: elements a vector, vectors a thread, one group of lanes per row?, ragged?
-template <int VE, typename F>
+// ... and with the geometry's numbers: elements a vector, vectors a thread, the limit of threads, ragged?
+template <int VE, bool BACK, typename F>
 cudaError_t with_geometry(const RmsGeom& g, F&& f) {
-  const auto ragged = [&](auto v, auto warp) { return g.ragged ? f(Int<VE>(), v, warp, std::true_type()) : f(Int<VE>(), v, warp, std::false_type()); };
+  const auto ragged = [&](auto v, auto most) { return g.ragged ? f(Int<VE>(), v, most, std::true_type()) : f(Int<VE>(), v, most, std::false_type()); };
   if (g.warp) {
-    if (g.v == 1) return ragged(Int<1>(), std::true_type());
-    if (g.v == 2) return ragged(Int<2>(), std::true_type());
-    return ragged(Int<4>(), std::true_type());
+    if (g.v == 1) return ragged(Int<1>(), Int<kWarpThreads>());
+    if (g.v == 2) return ragged(Int<2>(), Int<kWarpThreads>());
+    return ragged(Int<4>(), Int<kWarpThreads>());
   }
-  if (g.v == 2) return ragged(Int<2>(), std::false_type());
-  if constexpr (VE == 4) {
-    if (g.v == 8) return ragged(Int<8>(), std::false_type());
+  // (the backward's limit goes by its vectors)
+  if constexpr (BACK) {
+    if (g.v == 2) return ragged(Int<2>(), Int<512>());
+    if (g.v == 4) return ragged(Int<4>(), Int<512>());
+    if constexpr (VE == 4) return ragged(Int<8>(), Int<512>());
+    return cudaErrorInvalidValue;
+  } else {
+    if constexpr (VE == 8) {
+      return g.most == 512 ? ragged(Int<2>(), Int<512>()) : ragged(Int<2>(), Int<1024>());
+    } else {
+      if (g.v == 2) return ragged(Int<2>(), Int<512>());
+      return g.most == 512 ? ragged(Int<4>(), Int<512>()) : ragged(Int<4>(), Int<1024>());
+    }
   }
-  return ragged(Int<4>(), std::false_type());
 }
 
 template <bool Q>
@@ -872,16 +903,16 @@ cudaError_t launch_rms_fwd(RmsFwd p, int dtype, int sum_dtype, Rows rows, cudaSt
       return cudaGetLastError();
     };
     if (g.v) {
-      const cudaError_t err = with_geometry<16 / (int)sizeof(Tx)>(g, [&](auto ve, auto v, auto warp, auto ragged) {
-        constexpr int VE = decltype(ve)::value, V = decltype(v)::value;
-        constexpr bool WARP = decltype(warp)::value, RAGGED = decltype(ragged)::value;
-        staged = kStaged<Tx, Ts, VE, V, WARP>;
+      const cudaError_t err = with_geometry<16 / (int)sizeof(Tx), false>(g, [&](auto ve, auto v, auto most, auto ragged) {
+        constexpr int VE = decltype(ve)::value, V = decltype(v)::value, THREADS = decltype(most)::value;
+        constexpr bool RAGGED = decltype(ragged)::value;
+        staged = kStaged<Tx, Ts, VE, V, THREADS>;
         if constexpr (std::is_same<Tx, Ts>::value)
-          if (!p.residual) return go(&rms_fwd_kernel<Tx, Ts, VE, V, WARP, Q, false, RAGGED>);
-        return go(&rms_fwd_kernel<Tx, Ts, VE, V, WARP, Q, true, RAGGED>);
+          if (!p.residual) return go(&rms_fwd_kernel<Tx, Ts, VE, V, THREADS, Q, false, RAGGED>);
+        return go(&rms_fwd_kernel<Tx, Ts, VE, V, THREADS, Q, true, RAGGED>);
       });
       if (err != cudaErrorInvalidValue) return err;
-      g = RmsGeom{1, 0, kMostThreads, kMostThreads, false, false};
+      g = RmsGeom{1, 0, kMostThreads, kMostThreads, false, false, 0};
       staged = false;
     }
     return go(&rms_fwd_any_kernel<Tx, Ts, Q>);
@@ -910,15 +941,15 @@ cudaError_t launch_rms_bwd(RmsBwd p, int dtype, int sum_dtype, Rows rows, cudaSt
       return cudaGetLastError();
     };
     if (g.v) {
-      const cudaError_t err = with_geometry<16 / (int)sizeof(Tx)>(g, [&](auto ve, auto v, auto warp, auto ragged) {
-        constexpr int VE = decltype(ve)::value, V = decltype(v)::value;
-        constexpr bool WARP = decltype(warp)::value, RAGGED = decltype(ragged)::value;
+      const cudaError_t err = with_geometry<16 / (int)sizeof(Tx), true>(g, [&](auto ve, auto v, auto most, auto ragged) {
+        constexpr int VE = decltype(ve)::value, V = decltype(v)::value, THREADS = decltype(most)::value;
+        constexpr bool RAGGED = decltype(ragged)::value;
         if constexpr (std::is_same<Tx, Ts>::value)
-          if (!p.addend && !p.dsum) return go(&rms_bwd_kernel<Tx, Ts, VE, V, WARP, false, RAGGED>);
-        return go(&rms_bwd_kernel<Tx, Ts, VE, V, WARP, true, RAGGED>);
+          if (!p.addend && !p.dsum) return go(&rms_bwd_kernel<Tx, Ts, VE, V, THREADS, false, RAGGED>);
+        return go(&rms_bwd_kernel<Tx, Ts, VE, V, THREADS, true, RAGGED>);
       });
       if (err != cudaErrorInvalidValue) return err;
-      g = RmsGeom{1, 0, kMostThreads, kMostThreads, false, false};
+      g = RmsGeom{1, 0, kMostThreads, kMostThreads, false, false, 0};
     }
     return go(&rms_bwd_any_kernel<Tx, Ts>);
   });

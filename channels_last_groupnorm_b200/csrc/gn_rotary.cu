@@ -9,9 +9,13 @@
 //
 // Both tensors are read and written once.  A warp takes a token's heads, or a share of them: it computes the token's
 // angles once, in its own piece of shared memory, and 32 / lanes heads at a time pass through registers, each in `lanes` lanes.  A
-// lane holds both channels of its pairs (two vectors), so the rotation exchanges nothing and the norm one butterfly.  The
-// product of position and frequency is formed and reduced to a fraction of a turn in fp64, so that the angle of a position of a
-// million is as exact as that of the first; per token that is a few instructions beside hundreds of channels.
+// lane holds both channels of its pairs (two vectors), so the rotation exchanges nothing and the norm one butterfly (two in the backward, at
+// once).  Angles are formed in turns from two floats, so that the angle of a position of ten million is as exact as that of the first.
+//
+// Bound by HBM with many heads: 16384 tokens of 32 + 32 heads of 128, bf16, with norm 87 us = 6.2 TB/s (94 % of a copy's rate), without 87 us,
+// backward with norm (four tensors read, two written) 130 us = 6.2 TB/s.  With few heads by instructions: a token's angles, coefficients and
+// addresses cost as much as four turns of the warp (2 x 4096 tokens of 20 + 20 heads of 64 with norm 17.7 us, 16384 of 4 + 4 of 128
+// 24 us, 1.4 and 2.4 times their bytes' time).  A single token takes 3.2 us: launch, first load, one turn.
 #include <algorithm>
 
 #include "../../include/gnb200.h"

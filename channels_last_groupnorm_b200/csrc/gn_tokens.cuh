@@ -44,11 +44,6 @@ __device__ __forceinline__ void store_vec(T* p, const Pack<T, VE>& v) {
   }
 }
 
-// 16 bytes from global to shared memory, asynchronously; the first `bytes` of them from memory, zeros for the others
-__device__ __forceinline__ void cp_async16_part(uint32_t smem_dst, const void* gmem_src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_dst), "l"(gmem_src), "r"(bytes) : "memory");
-}
-
 // element i of a parameter vector of type `dtype` (0 fp32, 1 fp16, 2 bf16); `none` where there is no vector
 __device__ __forceinline__ float param_at(const void* p, int dtype, long long i, float none) {
   if (p == nullptr) return none;
@@ -169,7 +164,7 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t v, int lanes) {
 // Teams of whole warps: a barrier of their own (hardware barriers 1 to 15), and the sum over a team in a fixed order behind one of
 // them.  The slots are two rows used in turn: a thread that writes a row again has passed the barrier behind which nobody reads it any
 // more.  The places of warps that are not there hold zeros.
-constexpr int kMostWarps = 16, kMostTeams = 15;
+constexpr int kMostWarps = 32, kMostTeams = 15;
 struct TeamSlots {
   alignas(16) float row[2][kMostWarps];
 };
@@ -184,7 +179,7 @@ __device__ __forceinline__ void team_barrier(int threads, int team) {
 }
 template <bool TEAMS>
 __device__ __forceinline__ void clear(TeamSlots& slots, int threads, int team, int first) {
-  if (first < 2 * kMostWarps) slots.row[first / kMostWarps][first % kMostWarps] = 0.f;
+  for (int i = first; i < 2 * kMostWarps; i += threads) slots.row[i / kMostWarps][i % kMostWarps] = 0.f;
   team_barrier<TEAMS>(threads, team);
 }
 template <bool TEAMS>
@@ -203,6 +198,12 @@ __device__ __forceinline__ float team_sum(float v, TeamSlots& slots, int& turn, 
   if (threads > 256) {
     const float4 u = four[2], w = four[3];
     t.x += u.x + w.x, t.y += u.y + w.y, t.z += u.z + w.z, t.w += u.w + w.w;
+  }
+  if (threads > 512) {
+    float4 s = four[4];
+#pragma unroll
+    for (int k = 5; k < kMostWarps / 4; ++k) s.x += four[k].x, s.y += four[k].y, s.z += four[k].z, s.w += four[k].w;
+    t.x += s.x, t.y += s.y, t.z += s.z, t.w += s.w;
   }
   return (t.x + t.y) + (t.z + t.w);
 }
