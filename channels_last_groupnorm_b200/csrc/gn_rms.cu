@@ -458,13 +458,13 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
           }
         } else {
           // a block's vectors lie in neighbouring lanes: block / VE of them, at most a warp's
-          const int share = p.block / VE, among = min(share, WARP ? lanes : 32);
+          const int share = p.block / VE, among = min(share, WARP ? lanes : 32), shift = 31 - __clz(share);
 #pragma unroll
           for (int v = 0; v < V; ++v) {
             const int i = first + v * lanes;
             const float scale = scale_of(lanes_max(m[v], among), p.format), inverse = inverse_of(scale);
             if (live && i < nvec) {
-              if (i % share == 0) p.scale[row * p.blocks + i / share] = scale;
+              if ((i & (share - 1)) == 0) p.scale[row * p.blocks + (i >> shift)] = scale;
               store_codes<VE, RAGGED>(out, frame, i, s[v], inverse, p.format);
             }
           }

@@ -351,3 +351,13 @@ def test_odd_rows_write_nothing_beside_them(c, rows):
     ref.within(grads[0], d, ref.rounded(d, BF16) + 2 * FORWARD * size)
     ref.within(grads[2], dw, ref.rounded(dw, BF16) + (FORWARD + (rows + 64) * ref.U32) * wsize)
     _check_quant(x.detach(), w.detach(), r.detach(), 64, torch.float8_e4m3fn)
+
+
+def test_gradients_with_a_graph_of_their_own():
+    x, w, r, dy, ds = _inputs(5, 72, BF16, BF16, F32, grads=True)
+    for t in (x, w, r):
+        t.requires_grad_(True)
+    plain = torch.autograd.grad(pkg.rms_norm(x, w, r), (x, r, w), (dy, ds))
+    graphed = torch.autograd.grad(pkg.rms_norm(x, w, r), (x, r, w), (dy, ds), create_graph=True)
+    for a, b in zip(plain, graphed):
+        assert torch.equal(a, b)

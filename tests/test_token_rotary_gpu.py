@@ -265,3 +265,42 @@ def test_refusals():
         with pytest.raises(ValueError):
             bad()
     assert torch.isfinite(call(q, k, positions, inv_freq, sections, qw, kw)[0]).all()
+
+
+def test_gradients_with_a_graph_of_their_own():
+    q, k, positions, inv_freq, sections, qw, kw = _inputs((2, 7), 4, 2, 64, (16, 16), BF16, BF16)
+    for t in (q, k, qw, kw):
+        t.requires_grad_(True)
+    out = pkg.rotary(q, k, positions, inv_freq, sections, qw, kw)
+    cots = [torch.randn_like(o) for o in out]
+    plain = torch.autograd.grad(out, (q, k, qw, kw), cots)
+    graphed = torch.autograd.grad(pkg.rotary(q, k, positions, inv_freq, sections, qw, kw), (q, k, qw, kw), cots, create_graph=True)
+    for a, b in zip(plain, graphed):
+        assert torch.equal(a, b)
+
+
+def test_captured_in_a_graph():
+    q, k, positions, inv_freq, sections, qw, kw = _inputs((3, 50), 4, 2, 128, (20, 22, 22), F16, F16)
+    pkg.rotary(q, k, positions, inv_freq, sections, qw, kw)
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        out = pkg.rotary(q, k, positions, inv_freq, sections, qw, kw)
+    q.copy_(torch.randn_like(q))
+    positions.add_(3)
+    graph.replay()
+    again = pkg.rotary(q, k, positions, inv_freq, sections, qw, kw)
+    assert torch.equal(out[0], again[0]) and torch.equal(out[1], again[1])
+
+
+def test_integer_and_list_arguments_take_the_other_path():
+    q, k, positions, inv_freq, sections, qw, kw = _inputs((2, 5), 4, 2, 64, (16, 16), F32, F32)
+    want = pkg.rotary(q, k, positions, inv_freq, sections, qw, kw, 1.0)
+    got = pkg.rotary(q, k, positions, inv_freq, list(sections), qw, kw, 1, 0, 0)
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+    for t in (q, k, qw, kw):
+        t.requires_grad_(True)
+    cots = [torch.randn_like(o) for o in want]
+    a = torch.autograd.grad(pkg.rotary(q, k, positions, inv_freq, sections, qw, kw, 1.0), (q, k, qw, kw), cots)
+    b = torch.autograd.grad(pkg.rotary(q, k, positions, inv_freq, list(sections), qw, kw, 1, 0, 0), (q, k, qw, kw), cots)
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
