@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
   extern __shared__ __align__(16) char smem[];
   __shared__ TeamSlots slots;
   __shared__ uint32_t most[32];
-  __shared__ uint32_t blocks[Q && RAGGED ? 2 : 1][Q && RAGGED ? kMostBlocks : 1];
+  __shared__ uint2 blocks[Q && RAGGED ? kMostBlocks : 1];  // maxima of a block's own vectors, of the channels before them
   const Place<WARP, false> at(p.lanes, p.stage_bytes, p.stages, plane_bytes(p.C, VE, RAGGED), smem);
   const int lanes = at.lanes, first = at.first;
   const Tx* next_x = static_cast<const Tx*>(p.x) + at.row * p.x_stride;  // the next row to be asked for
@@ -313,13 +313,8 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
     for (int i = 1; i < p.stages; ++i) ask();
   float w[V][VE];
   fetch_weight<VE, V, RAGGED>(w, p.weight, p.w_dtype, p.offset, frame, first, lanes);
-  if constexpr (Q && RAGGED)
-    for (int i = threadIdx.x; i < 2 * kMostBlocks; i += blockDim.x) blocks[i / kMostBlocks][i % kMostBlocks] = 0;
-  if constexpr (!WARP)
-    clear<false>(slots, lanes, 0, first);
-  else if constexpr (Q && RAGGED)
-    __syncthreads();
-  int turn = 0, block_turn = 0;
+  if constexpr (!WARP) clear<false>(slots, lanes, 0, first);
+  int turn = 0;
   long long row = at.row;
   // (every thread of a warp takes the same number of turns: the shuffles want all lanes)
   for (long long base = at.base; base < p.rows; base += at.step, row += at.step) {
@@ -390,83 +385,67 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
       }
     } else {
       uint8_t* const out = static_cast<uint8_t*>(p.y) + out_at;
-      if (RAGGED && p.block != 0) {
-        // a vector may hold the end of one block and the beginning of the next: the blocks' maxima meet in shared memory
-        const int shift = 31 - __clz(p.block), mine = WARP ? (int)threadIdx.x / lanes * lanes : 0;
-        uint32_t* const now = blocks[block_turn];
-        uint32_t* const then = blocks[block_turn ^ 1];
-        block_turn ^= 1;
-        for (int i = first; i < (WARP ? lanes : kMostBlocks); i += lanes) then[mine + i] = 0;  // (last read before this row's sum)
+      uint32_t m[V], before[RAGGED ? V : 1];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const int i = first + v * lanes, from = max(frame.channel(i), 0), to = min(frame.channel(i) + VE, p.C) - 1;
-          if (live && i < nvec) {
-            uint32_t low = 0, high = 0;
+      for (int v = 0; v < V; ++v) {
+        const int i = first + v * lanes;
+        m[v] = 0;
+        if constexpr (RAGGED) before[v] = 0;
+        if (i < nvec) {  // (beyond the row a NaN rstd would leave NaN in the zeros)
+          frame.cut(s[v], i);
+          float most_of = 0.f, most_before = 0.f;
 #pragma unroll
-            for (int e = 0; e < VE; ++e) {
-              const uint32_t m = frame.has(i, e) ? magnitude(s[v][e]) : 0;
-              if ((frame.channel(i) + e) >> shift == to >> shift)
-                high = max(high, m);
-              else
-                low = max(low, m);
-            }
-            atomicMax(&now[mine + (to >> shift)], high);
-            if (from >> shift != to >> shift) atomicMax(&now[mine + (from >> shift)], low);
+          for (int e = 0; e < VE; ++e) {
+            const float a = fabsf(s[v][e]);
+            const bool early = RAGGED && e < frame.skew;
+            most_of = larger(most_of, early ? 0.f : a);
+            if constexpr (RAGGED) most_before = larger(most_before, early ? a : 0.f);
           }
+          m[v] = magnitude(most_of);
+          if constexpr (RAGGED) before[v] = magnitude(most_before);
         }
-        if constexpr (WARP)
-          __syncwarp();
-        else
-          __syncthreads();
+      }
+      if (p.block == 0) {
+        uint32_t all = 0;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const int i = first + v * lanes, from = max(frame.channel(i), 0), to = min(frame.channel(i) + VE, p.C) - 1;
-          if (live && i < nvec) {
-            const float low = scale_of(now[mine + (from >> shift)], p.format), high = scale_of(now[mine + (to >> shift)], p.format);
-            if ((to & (p.block - 1)) <= to - from) p.scale[row * p.blocks + (to >> shift)] = high;  // (the block's first channel is here)
-            const float inverse_low = inverse_of(low), inverse_high = inverse_of(high);
-#pragma unroll
-            for (int e = 0; e < VE; ++e) s[v][e] *= (frame.channel(i) + e) >> shift == to >> shift ? inverse_high : inverse_low;
-            store_codes<VE, RAGGED>(out, frame, i, s[v], 1.f, p.format);
-          }
-        }
-      } else {
-        uint32_t m[V];
+        for (int v = 0; v < V; ++v) all = RAGGED ? max(all, max(m[v], before[v])) : max(all, m[v]);
+        all = WARP ? lanes_max(all, lanes) : cta_max(all, most);
+        const float scale = scale_of(all, p.format), inverse = inverse_of(scale);
+        if (live && first == 0) p.scale[row] = scale;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const int i = first + v * lanes;
-          m[v] = 0;
-          if (i < nvec) {  // (beyond the row a NaN rstd would leave NaN in the zeros)
-            float most_of = 0.f;
-#pragma unroll
-            for (int e = 0; e < VE; ++e)
-              if (frame.has(i, e)) most_of = larger(most_of, fabsf(s[v][e]));
-            m[v] = magnitude(most_of);
-          }
+          if (live && i < nvec) store_codes<VE, RAGGED>(out, frame, i, s[v], inverse, p.format);
         }
-        if (p.block == 0) {
-          uint32_t all = 0;
+      } else {
+        // A block's vectors lie in neighbouring lanes: block / VE of them, at most a warp's.  In a frame the first of them begins with the
+        // `skew` last channels of the block before: both parts of a block's maximum meet in shared memory, each written by one lane (the
+        // row's sum has a barrier between two rows' use of it).  (Maxima by shared atomics: 4000 x 12345 in blocks of 128 219 us.)
+        const int share = p.block / VE, among = min(share, WARP ? lanes : 32), shift = 31 - __clz(share);
+        uint2* const parts = blocks + (WARP ? (int)threadIdx.x / lanes * lanes : 0);
 #pragma unroll
-          for (int v = 0; v < V; ++v) all = max(all, m[v]);
-          all = WARP ? lanes_max(all, lanes) : cta_max(all, most);
-          const float scale = scale_of(all, p.format), inverse = inverse_of(scale);
-          if (live && first == 0) p.scale[row] = scale;
+        for (int v = 0; v < V; ++v) {
+          const int i = first + v * lanes;
+          const bool leads = (i & (share - 1)) == 0;
+          m[v] = lanes_max(RAGGED && !leads ? max(m[v], before[v]) : m[v], among);
+          if (RAGGED && leads && i < nvec) parts[i >> shift] = make_uint2(m[v], before[v]);
+        }
+        if constexpr (RAGGED) at.meet();
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            const int i = first + v * lanes;
-            if (live && i < nvec) store_codes<VE, RAGGED>(out, frame, i, s[v], inverse, p.format);
-          }
-        } else {
-          // a block's vectors lie in neighbouring lanes: block / VE of them, at most a warp's
-          const int share = p.block / VE, among = min(share, WARP ? lanes : 32), shift = 31 - __clz(share);
+        for (int v = 0; v < V; ++v) {
+          const int i = first + v * lanes, block = i >> shift;
+          if (live && i < nvec) {
+            const bool leads = (i & (share - 1)) == 0;
+            if (RAGGED && (block + 1) * share < nvec) m[v] = max(m[v], parts[block + 1].y);
+            const float scale = scale_of(m[v], p.format), inverse = inverse_of(scale);
+            if (leads && (!RAGGED || block < p.blocks)) p.scale[row * p.blocks + block] = scale;  // (the last vector may hold the last block's end alone)
+            if constexpr (RAGGED) {
+              float early = inverse;
+              if (leads && block > 0) early = inverse_of(scale_of(max(parts[block - 1].x, before[v]), p.format));
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            const int i = first + v * lanes;
-            const float scale = scale_of(lanes_max(m[v], among), p.format), inverse = inverse_of(scale);
-            if (live && i < nvec) {
-              if ((i & (share - 1)) == 0) p.scale[row * p.blocks + (i >> shift)] = scale;
-              store_codes<VE, RAGGED>(out, frame, i, s[v], inverse, p.format);
+              for (int e = 0; e < VE; ++e) s[v][e] *= e < frame.skew ? early : inverse;
             }
+            store_codes<VE, RAGGED>(out, frame, i, s[v], RAGGED ? 1.f : inverse, p.format);
           }
         }
       }
