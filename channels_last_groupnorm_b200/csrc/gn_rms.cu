@@ -122,29 +122,18 @@ struct Frame {
     }
     return v;
   }
-  // Sums over a ragged row go through shared memory, so that they are taken in the row's own order: the same bits wherever the row
-  // stands.  Channel j is word j / VE of plane j % VE, which is free of bank conflicts for frames of any skew.
-  __device__ __forceinline__ int words() const { return (C + VE - 1) / VE; }  // of a plane
-  // plane and word of element e of vector 0; those of vector i lie i words on
-  __device__ __forceinline__ int place(int e) const { return ((e - skew) & (VE - 1)) * words() - (e < skew ? 1 : 0); }
-  __device__ __forceinline__ void lay_out(float* planes, int i, const float (&f)[VE]) const {
-    if (whole(i)) {
+  // Sums over a ragged row go through shared memory, so that each lane adds the same channels in the same order wherever the row stands:
+  // written as vectors of the frame, read a channel a lane, each lane a vector or
+  // a channel.  (In planes of channel mod VE: 27002 x 1111 bf16 69 us instead of 58, its backward 116 instead of 95.)
+  __device__ __forceinline__ void lay_out(float* line, int i, const float (&f)[VE]) const {
 #pragma unroll
-      for (int e = 0; e < VE; ++e) planes[place(e) + i] = f[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < VE; ++e)
-        if (has(i, e)) planes[place(e) + i] = f[e];
-    }
+    for (int e = 0; e < VE; e += 4) *reinterpret_cast<float4*>(line + i * VE + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
   }
-  __device__ __forceinline__ void take(const float* planes, int i, float (&f)[VE]) const {
-    if ((i + 1) * VE <= C) {
+  // channels first + step * (v VE + 0, 1, ...); zeros behind the row
+  __device__ __forceinline__ void take(const float* line, int v, int first, int step, float (&f)[VE]) const {
+    const int from = first + v * VE * step;
 #pragma unroll
-      for (int e = 0; e < VE; ++e) f[e] = planes[e * words() + i];
-    } else {
-#pragma unroll
-      for (int e = 0; e < VE; ++e) f[e] = i * VE + e < C ? planes[e * words() + i] : 0.f;
-    }
+    for (int e = 0; e < VE; ++e) f[e] = from + e * step < C ? line[skew + from + e * step] : 0.f;
   }
   template <typename T>
   __device__ __forceinline__ void store(T* row, int i, const float (&f)[VE]) const {
@@ -161,8 +150,8 @@ struct Frame {
 // Bytes of a tensor's row in a stage
 __host__ __device__ constexpr int segment_bytes(int C, int ve, int size, bool ragged) { return ragged ? (C + 2 * ve - 2) / ve * ve * size : C * size; }
 
-// ... and of the planes of its sum
-__host__ __device__ constexpr int plane_bytes(int C, int ve, bool ragged) { return ragged ? ((C + ve - 1) / ve * ve * 4 + 15) / 16 * 16 : 0; }
+// ... and of the line of its sum
+__host__ __device__ constexpr int line_bytes(int C, int ve, bool ragged) { return segment_bytes(C, ve, ragged ? 4 : 0, ragged); }
 
 // Copies a row to its stage, 16 bytes a lane; of the tensor's first and last row (not `inner`) no chunk that begins before it and no byte behind
 // it, so that nothing outside of the tensor is read.
@@ -232,8 +221,8 @@ struct Place {
   int lanes, first, group;
   long long per_cta, base, row, step;
   char* stages;
-  float* planes;
-  __device__ __forceinline__ Place(int row_lanes, int stage_bytes, int nstages, int plane_bytes, char* smem) {
+  float* line;
+  __device__ __forceinline__ Place(int row_lanes, int stage_bytes, int nstages, int line_bytes, char* smem) {
     lanes = WARP || TEAMS ? row_lanes : (int)blockDim.x;
     group = WARP || TEAMS ? (int)threadIdx.x / lanes : 0;
     first = (int)threadIdx.x - group * lanes;
@@ -241,8 +230,8 @@ struct Place {
     base = blockIdx.x * per_cta + (WARP ? 0 : group);  // (a warp's groups take their turns together, teams each for themselves)
     row = blockIdx.x * per_cta + group;
     step = per_cta * gridDim.x;
-    stages = smem + (long long)group * (stage_bytes * nstages + plane_bytes);
-    planes = reinterpret_cast<float*>(stages + stage_bytes * nstages);
+    stages = smem + (long long)group * (stage_bytes * nstages + line_bytes);
+    line = reinterpret_cast<float*>(stages + stage_bytes * nstages);
   }
   // what the group's other lanes wrote becomes visible
   __device__ __forceinline__ void meet() const {
@@ -269,7 +258,7 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
   __shared__ TeamSlots slots;
   __shared__ uint32_t most[32];
   __shared__ uint2 blocks[Q && RAGGED ? kMostBlocks : 1];  // maxima of a block's own vectors, of the channels before them
-  const Place<WARP, false> at(p.lanes, p.stage_bytes, p.stages, plane_bytes(p.C, VE, RAGGED), smem);
+  const Place<WARP, false> at(p.lanes, p.stage_bytes, p.stages, line_bytes(p.C, VE, RAGGED), smem);
   const int lanes = at.lanes, first = at.first;
   const Tx* next_x = static_cast<const Tx*>(p.x) + at.row * p.x_stride;  // the next row to be asked for
   const Ts* next_r = RES ? static_cast<const Ts*>(p.residual) + at.row * p.r_stride : nullptr;
@@ -352,7 +341,7 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
           frame.store(static_cast<Ts*>(p.sum) + out_at, i, s[v]);
         }
         frame.cut(s[v], i);
-        if constexpr (RAGGED) frame.lay_out(at.planes, i, s[v]);
+        if constexpr (RAGGED) frame.lay_out(at.line, i, s[v]);
       }
       if constexpr (!RAGGED) dot_each(sq, s[v], s[v]);
     }
@@ -360,10 +349,9 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
       at.meet();
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const int i = first + v * lanes;
-        if (live && i < frame.words()) {
+        if (live) {
           float f[VE];
-          frame.take(at.planes, i, f);
+          frame.take(at.line, v, first, lanes, f);
           dot_each(sq, f, f);
         }
       }
@@ -420,7 +408,8 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
       } else {
         // A block's vectors lie in neighbouring lanes: block / VE of them, at most a warp's.  In a frame the first of them begins with the
         // `skew` last channels of the block before: both parts of a block's maximum meet in shared memory, each written by one lane (the
-        // row's sum has a barrier between two rows' use of it).  (Maxima by shared atomics: 4000 x 12345 in blocks of 128 219 us.)
+        // row's sum has a barrier between two rows' use of it).  (4000 x 12345 fp16 over fp32 in blocks
+        // of 128 takes 216 us, 80 instructions an element, with maxima by shared atomics as much.)
         const int share = p.block / VE, among = min(share, WARP ? lanes : 32), shift = 31 - __clz(share);
         uint2* const parts = blocks + (WARP ? (int)threadIdx.x / lanes * lanes : 0);
 #pragma unroll
@@ -536,7 +525,7 @@ __global__ void __launch_bounds__(bwd_threads(VE, V), 1) rms_bwd_kernel(const Rm
   constexpr bool WARP = THREADS == kWarpThreads, TEAMS = !WARP;
   extern __shared__ __align__(16) char smem[];
   __shared__ TeamSlots all_slots[TEAMS ? kMostTeams : 1];
-  const Place<WARP, TEAMS> at(p.lanes, p.stage_bytes, p.stages, plane_bytes(p.C, VE, RAGGED), smem);
+  const Place<WARP, TEAMS> at(p.lanes, p.stage_bytes, p.stages, line_bytes(p.C, VE, RAGGED), smem);
   TeamSlots& slots = all_slots[TEAMS ? at.group : 0];
   const int lanes = at.lanes, first = at.first;
   grid_dep_launch_dependents();
@@ -603,7 +592,7 @@ __global__ void __launch_bounds__(bwd_threads(VE, V), 1) rms_bwd_kernel(const Rm
         add_each(dw[v], g);
         if constexpr (RAGGED) {
           mul_each(g, w[v]);
-          frame.lay_out(at.planes, first + v * lanes, g);
+          frame.lay_out(at.line, first + v * lanes, g);
         } else {
           dot_each(dot, g, w[v]);
         }
@@ -613,10 +602,9 @@ __global__ void __launch_bounds__(bwd_threads(VE, V), 1) rms_bwd_kernel(const Rm
       at.meet();
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const int i = first + v * lanes;
-        if (live && i < frame.words()) {
+        if (live) {
           float f[VE];
-          frame.take(at.planes, i, f);
+          frame.take(at.line, v, first, lanes, f);
 #pragma unroll
           for (int e = 0; e < VE; ++e) dot[e & 1] += f[e];
         }
@@ -787,15 +775,15 @@ struct RmsLaunch {
   unsigned grid;
   int threads, smem, stages;
 };
-// CTA size, stages, shared memory and CTAs of a call whose rows take `row_bytes` in a stage (0: no stages) and `planes` for their sums: no more CTAs than are resident at
+// CTA size, stages, shared memory and CTAs of a call whose rows take `row_bytes` in a stage (0: no stages) and `line` for their sums: no more CTAs than are resident at
 // once nor than there are rows; where ragged rows take several turns, a number that
 // keeps their frames.  cudaErrorInvalidValue: a row does not fit.
-cudaError_t rms_launch(const void* kernel, const RmsGeom& g, int64_t rows, int64_t row_bytes, int64_t planes, RmsLaunch* out) {
+cudaError_t rms_launch(const void* kernel, const RmsGeom& g, int64_t rows, int64_t row_bytes, int64_t line, RmsLaunch* out) {
   Residency r = {};
   out->threads = g.threads;
   out->stages = 0;
-  if (row_bytes + planes > kMostDynamicSmem) return cudaErrorInvalidValue;
-  out->smem = (int)(g.threads / g.lanes * planes);
+  if (row_bytes + line > kMostDynamicSmem) return cudaErrorInvalidValue;
+  out->smem = (int)(g.threads / g.lanes * line);
   if (row_bytes) {
     // fewer teams where two stages for each do not fit, or where there are no rows for them on every SM
     const auto halve = [&](int teams) { return g.warp ? teams / 2 : teams - 1; };
@@ -803,10 +791,10 @@ cudaError_t rms_launch(const void* kernel, const RmsGeom& g, int64_t rows, int64
     cudaError_t err = residency(kernel, g.threads, 0, &r);
     if (err != cudaSuccess) return err;
     const int least = g.warp ? 32 / g.lanes : 1;
-    while (teams > least && (teams * (2 * row_bytes + planes) > kMostDynamicSmem || (int64_t)teams * r.sms > rows)) teams = std::max(least, halve(teams));
+    while (teams > least && (teams * (2 * row_bytes + line) > kMostDynamicSmem || (int64_t)teams * r.sms > rows)) teams = std::max(least, halve(teams));
     out->threads = teams * g.lanes;
     if ((err = residency(kernel, out->threads, 0, &r)) != cudaSuccess) return err;
-    const int64_t bytes = row_bytes * teams, fixed = planes * teams;
+    const int64_t bytes = row_bytes * teams, fixed = line * teams;
     if (bytes + fixed > kMostDynamicSmem) return cudaErrorInvalidValue;
     int64_t stages = std::max<int64_t>(1, (kMostDynamicSmem / r.per_sm - fixed) / bytes);
     stages = std::min<int64_t>(kMostStages, std::max<int64_t>(stages, std::min<int64_t>(2, (kMostDynamicSmem - fixed) / bytes)));
@@ -875,7 +863,7 @@ cudaError_t launch_rms_fwd(RmsFwd p, int dtype, int sum_dtype, Rows rows, cudaSt
       RmsLaunch l = {};
       int row_bytes = 0;
       if (staged) row_bytes = segment_bytes(p.C, g.ve, sizeof(Tx), g.ragged) + (p.residual ? segment_bytes(p.C, g.ve, sizeof(Ts), g.ragged) : 0);
-      const cudaError_t err = rms_launch((const void*)kernel, g, p.rows, row_bytes, g.v ? plane_bytes(p.C, g.ve, g.ragged) : 0, &l);
+      const cudaError_t err = rms_launch((const void*)kernel, g, p.rows, row_bytes, g.v ? line_bytes(p.C, g.ve, g.ragged) : 0, &l);
       if (err != cudaSuccess) return err;
       p.lanes = g.lanes, p.stages = l.stages, p.stage_bytes = row_bytes;
       kernel<<<l.grid, l.threads, l.smem, stream>>>(p);
@@ -911,7 +899,7 @@ cudaError_t launch_rms_bwd(RmsBwd p, int dtype, int sum_dtype, Rows rows, cudaSt
       int row_bytes = 0;
       if (g.v)
         row_bytes = segment_bytes(p.C, g.ve, sizeof(Tx), g.ragged) * (p.addend ? 2 : 1) + segment_bytes(p.C, g.ve, sizeof(Ts), g.ragged) * (p.dsum ? 2 : 1);
-      const cudaError_t err = rms_launch((const void*)kernel, g, p.rows, row_bytes, g.v ? plane_bytes(p.C, g.ve, g.ragged) : 0, &l);
+      const cudaError_t err = rms_launch((const void*)kernel, g, p.rows, row_bytes, g.v ? line_bytes(p.C, g.ve, g.ragged) : 0, &l);
       if (err != cudaSuccess) return err;
       *grid = g.v ? l.grid : std::min(l.grid, (unsigned)std::max(1, (1 << 24) / p.C));  // 64 MB of partial sums at most, or one row
       if (room == kGridOnly || (p.part && (size_t)*grid * (size_t)p.C * sizeof(float) > room)) return cudaSuccess;
