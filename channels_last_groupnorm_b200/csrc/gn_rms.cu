@@ -123,8 +123,7 @@ struct Frame {
     return v;
   }
   // Sums over a ragged row go through shared memory, so that each lane adds the same channels in the same order wherever the row stands:
-  // written as vectors of the frame, read a channel a lane, each lane a vector or
-  // a channel.  (In planes of channel mod VE: 27002 x 1111 bf16 69 us instead of 58, its backward 116 instead of 95.)
+  // written as vectors of the frame, read a channel a lane.  (In planes of channel mod VE: 27002 x 1111 bf16 69 us instead of 58, its backward 116 instead of 95.)
   __device__ __forceinline__ void lay_out(float* line, int i, const float (&f)[VE]) const {
 #pragma unroll
     for (int e = 0; e < VE; e += 4) *reinterpret_cast<float4*>(line + i * VE + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
@@ -409,7 +408,7 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
         // A block's vectors lie in neighbouring lanes: block / VE of them, at most a warp's.  In a frame the first of them begins with the
         // `skew` last channels of the block before: both parts of a block's maximum meet in shared memory, each written by one lane (the
         // row's sum has a barrier between two rows' use of it).  (4000 x 12345 fp16 over fp32 in blocks
-        // of 128 takes 216 us, 80 instructions an element, with maxima by shared atomics as much.)
+        // of 128 takes 216 us, 80 instructions an element.)
         const int share = p.block / VE, among = min(share, WARP ? lanes : 32), shift = 31 - __clz(share);
         uint2* const parts = blocks + (WARP ? (int)threadIdx.x / lanes * lanes : 0);
 #pragma unroll
