@@ -45,24 +45,49 @@ struct RmsFwd {
 // ---------------------------------------------------------------------------------------------
 // 8-bit codes
 // ---------------------------------------------------------------------------------------------
-// (the product and the reciprocal are an ulp or two off the quotients, some 2^-22 of a code's rounding step of 2^-4; the division's
-// slow path would be most of the instructions of a small block)
-__device__ __forceinline__ float scale_of(uint32_t most, int format) {
+// A code is that of y / scale rounded as a division rounds it, so that codes and y / scale agree wherever they are formed: the product
+// q = y * inverse with the correctly rounded reciprocal is at most one unit of its last place off, and q - inverse * (q * scale - y), the
+// remainder taken exactly by an fma, is the rounded quotient (Markstein's theorem; y below 2^-126 aside).  The reciprocal: one Newton
+// step from the hardware's, which is a unit off at most (the same bits as __frcp_rn for every mantissa, without its branch for other ranges).  Two
+// fma an element; the product alone gave one code in 100 000 of the neighbouring value, where bf16 inputs put y / scale midway between
+// two codes.  2048 x 4096 bf16 in blocks of 128: product alone 10.7 us, so 11.2, with __frcp_rn 11.7; 8192 x 8192 over fp32 118.5 and 115.
+struct Scale {
+  float value, inverse;
+  float back;  // value; 0 where it is infinite: what is finite over infinity is zero, not the remainder's NaN
+};
+__device__ __forceinline__ Scale scale_of(uint32_t most, int format) {
   const float s = __uint_as_float(most) * (format == GNB200_E4M3 ? 1.f / 448.f : 1.f / 127.f);
-  return s < kSmallestScale ? kSmallestScale : s;  // (a NaN stays)
+  Scale scale;
+  scale.value = s < kSmallestScale ? kSmallestScale : s;  // (a NaN stays)
+  float near;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(near) : "f"(scale.value));
+  const bool infinite = near == 0.f;
+  scale.inverse = infinite ? 0.f : fmaf(fmaf(-scale.value, near, 1.f), near, near);
+  scale.back = infinite ? 0.f : scale.value;
+  return scale;
 }
-__device__ __forceinline__ float inverse_of(float scale) { return __fdividef(1.f, scale); }
+__device__ __forceinline__ float over(float y, float inverse, float back) {
+  const float q = y * inverse;
+  return fmaf(-inverse, fmaf(q, back, -y), q);
+}
+template <int VE>
+__device__ __forceinline__ void over_each(float (&f)[VE], const Scale& scale) {
+  const float inverse = scale.inverse, back = scale.back, less = -inverse;
+#pragma unroll
+  for (int e = 0; e < VE; e += 2) {
+    float q0, q1, r0, r1;
+    mul2(q0, q1, f[e], f[e + 1], inverse, inverse);
+    fma2(r0, r1, q0, q1, back, back, -f[e], -f[e + 1]);
+    fma2(f[e], f[e + 1], r0, r1, less, less, q0, q1);
+  }
+}
 __device__ __forceinline__ uint32_t code_of(float v, int format) {
   if (format == GNB200_E4M3) return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
   return (uint32_t)max(-127, min(127, __float2int_rn(v))) & 0xffu;
 }
-// VE codes, four a word
+// VE codes of quotients, four a word
 template <int VE>
-__device__ __forceinline__ void codes_of(const float (&f)[VE], float inverse, int format, uint32_t (&w)[VE / 4]) {
-  float v[VE];
-#pragma unroll
-  for (int e = 0; e < VE; ++e) v[e] = f[e];
-  scale_each(v, inverse);
+__device__ __forceinline__ void codes_of(const float (&v)[VE], int format, uint32_t (&w)[VE / 4]) {
 #pragma unroll
   for (int k = 0; k < VE / 4; ++k) {
     const float* g = v + 4 * k;
@@ -198,9 +223,9 @@ __device__ __forceinline__ void fetch_weight(float (&w)[V][VE], const void* p, i
 
 // the codes of vector i of the row whose frame begins at `row`
 template <int VE, bool RAGGED>
-__device__ __forceinline__ void store_codes(uint8_t* row, const Frame<VE, RAGGED>& frame, int i, const float (&f)[VE], float inverse, int format) {
+__device__ __forceinline__ void store_codes(uint8_t* row, const Frame<VE, RAGGED>& frame, int i, const float (&quotients)[VE], int format) {
   uint32_t w[VE / 4];
-  codes_of<VE>(f, inverse, format, w);
+  codes_of<VE>(quotients, format, w);
   if (frame.whole(i)) {
     if constexpr (VE == 8)
       *reinterpret_cast<uint2*>(row + i * VE) = make_uint2(w[0], w[1]);
@@ -397,18 +422,21 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
 #pragma unroll
         for (int v = 0; v < V; ++v) all = RAGGED ? max(all, max(m[v], before[v])) : max(all, m[v]);
         all = WARP ? lanes_max(all, lanes) : cta_max(all, most);
-        const float scale = scale_of(all, p.format), inverse = inverse_of(scale);
-        if (live && first == 0) p.scale[row] = scale;
+        const Scale scale = scale_of(all, p.format);
+        if (live && first == 0) p.scale[row] = scale.value;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const int i = first + v * lanes;
-          if (live && i < nvec) store_codes<VE, RAGGED>(out, frame, i, s[v], inverse, p.format);
+          if (live && i < nvec) {
+            over_each<VE>(s[v], scale);
+            store_codes<VE, RAGGED>(out, frame, i, s[v], p.format);
+          }
         }
       } else {
         // A block's vectors lie in neighbouring lanes: block / VE of them, at most a warp's.  In a frame the first of them begins with the
         // `skew` last channels of the block before: both parts of a block's maximum meet in shared memory, each written by one lane (the
         // row's sum has a barrier between two rows' use of it).  (4000 x 12345 fp16 over fp32 in blocks
-        // of 128 takes 216 us, 80 instructions an element.)
+        // of 128 takes 223 us.)
         const int share = p.block / VE, among = min(share, WARP ? lanes : 32), shift = 31 - __clz(share);
         uint2* const parts = blocks + (WARP ? (int)threadIdx.x / lanes * lanes : 0);
 #pragma unroll
@@ -425,15 +453,17 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
           if (live && i < nvec) {
             const bool leads = (i & (share - 1)) == 0;
             if (RAGGED && (block + 1) * share < nvec) m[v] = max(m[v], parts[block + 1].y);
-            const float scale = scale_of(m[v], p.format), inverse = inverse_of(scale);
-            if (leads && (!RAGGED || block < p.blocks)) p.scale[row * p.blocks + block] = scale;  // (the last vector may hold the last block's end alone)
+            const Scale scale = scale_of(m[v], p.format);
+            if (leads && (!RAGGED || block < p.blocks)) p.scale[row * p.blocks + block] = scale.value;  // (the last vector may hold the last block's end alone)
             if constexpr (RAGGED) {
-              float early = inverse;
-              if (leads && block > 0) early = inverse_of(scale_of(max(parts[block - 1].x, before[v]), p.format));
+              Scale early = scale;
+              if (leads && block > 0) early = scale_of(max(parts[block - 1].x, before[v]), p.format);
 #pragma unroll
-              for (int e = 0; e < VE; ++e) s[v][e] *= e < frame.skew ? early : inverse;
+              for (int e = 0; e < VE; ++e) s[v][e] = e < frame.skew ? over(s[v][e], early.inverse, early.back) : over(s[v][e], scale.inverse, scale.back);
+            } else {
+              over_each<VE>(s[v], scale);
             }
-            store_codes<VE, RAGGED>(out, frame, i, s[v], RAGGED ? 1.f : inverse, p.format);
+            store_codes<VE, RAGGED>(out, frame, i, s[v], p.format);
           }
         }
       }
@@ -473,29 +503,26 @@ __global__ void __launch_bounds__(kMostThreads) rms_fwd_any_kernel(const RmsFwd 
       if (p.block == 0) {
         uint32_t m = 0;
         for (int i = threadIdx.x; i < p.C; i += blockDim.x) m = max(m, magnitude(y_at(i)));
-        const float scale = scale_of(cta_max(m, most), p.format), inverse = inverse_of(scale);
-        if (threadIdx.x == 0) p.scale[row] = scale;
-        for (int i = threadIdx.x; i < p.C; i += blockDim.x) {
-          const float f[1] = {y_at(i)};
-          out[i] = (uint8_t)code_of(f[0] * inverse, p.format);
-        }
+        const Scale scale = scale_of(cta_max(m, most), p.format);
+        if (threadIdx.x == 0) p.scale[row] = scale.value;
+        for (int i = threadIdx.x; i < p.C; i += blockDim.x) out[i] = (uint8_t)code_of(over(y_at(i), scale.inverse, scale.back), p.format);
       } else {  // one warp per block of at most 128 channels
         const int lane = threadIdx.x & 31, nwarps = blockDim.x >> 5;
         for (int b = threadIdx.x >> 5; b < p.blocks; b += nwarps) {
-          float f[4][1];
+          float f[4];
           uint32_t m = 0;
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             const int in = lane + 32 * v, i = b * p.block + in;
-            f[v][0] = in < p.block && i < p.C ? y_at(i) : 0.f;
-            m = max(m, magnitude(f[v][0]));
+            f[v] = in < p.block && i < p.C ? y_at(i) : 0.f;
+            m = max(m, magnitude(f[v]));
           }
-          const float scale = scale_of(lanes_max(m, 32), p.format), inverse = inverse_of(scale);
-          if (lane == 0) p.scale[row * p.blocks + b] = scale;
+          const Scale scale = scale_of(lanes_max(m, 32), p.format);
+          if (lane == 0) p.scale[row * p.blocks + b] = scale.value;
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             const int in = lane + 32 * v, i = b * p.block + in;
-            if (in < p.block && i < p.C) out[i] = (uint8_t)code_of(f[v][0] * inverse, p.format);
+            if (in < p.block && i < p.C) out[i] = (uint8_t)code_of(over(f[v], scale.inverse, scale.back), p.format);
           }
         }
       }

@@ -63,7 +63,8 @@ def rms_norm_quant(x, weight=None, residual=None, eps=1e-6, offset=0.0, block=0,
 
     dtype: torch.float8_e4m3fn or torch.int8.  block: 0 for one scale per row (scales of shape (*, 1)), or 32, 64 or 128 channels
     that share one (shape (*, ceil(channels / block))).  A scale is the largest magnitude of its channels over the largest code (448
-    or 127), at least 2^-126; a NaN among them makes it NaN.  y is not rounded in between.  Inference only: it refuses to run where
+    or 127), at least 2^-126; a NaN among them makes it NaN.  A code is that of y / scale, rounded as a division rounds it, with y in 32
+    bits.  Inference only: it refuses to run where
     a gradient would be recorded.
     """
     if dtype not in QUANT_FORMATS:
