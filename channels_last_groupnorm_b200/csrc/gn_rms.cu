@@ -24,6 +24,7 @@
 
 #include "../../include/gnb200.h"
 #include "gn_kernels.h"
+#include "gn_rows.h"
 #include "gn_tokens.cuh"
 
 namespace gnb200 {
@@ -37,7 +38,7 @@ struct RmsFwd {
   const void *x, *residual, *weight;
   void *y, *sum;  // y: or the codes
   float *rstd, *scale;
-  long long rows, x_stride, r_stride;
+  long long rows, x_stride, r_stride, edge;  // edge: rows at either end that Frame::readable looks at
   int C, lanes, stages, stage_bytes, w_dtype, block, blocks, format;
   float eps, offset, inv_c;
 };
@@ -134,8 +135,8 @@ struct Frame {
       }
     }
   }
-  // Whether vector i may be read as a whole, with elements of the rows beside it: in the tensor's first and last row (not `inner`) only
-  // where it lies in the row.  What may not is fetched where it is used.
+  // Whether vector i may be read as a whole, with elements of the rows beside it: in the tensor's first and last rows (not `inner`, by
+  // edge_rows()) only where it lies in the row.  What may not is fetched where it is used.
   __device__ __forceinline__ bool readable(int i, bool inner) const { return !RAGGED || inner || whole(i); }
   template <typename T>
   __device__ __forceinline__ Pack<T, VE> fetch(const T* row, int i) const {
@@ -177,8 +178,8 @@ __host__ __device__ constexpr int segment_bytes(int C, int ve, int size, bool ra
 // ... and of the line of its sum
 __host__ __device__ constexpr int line_bytes(int C, int ve, bool ragged) { return segment_bytes(C, ve, ragged ? 4 : 0, ragged); }
 
-// Copies a row to its stage, 16 bytes a lane; of the tensor's first and last row (not `inner`) no chunk that begins before it and no byte behind
-// it, so that nothing outside of the tensor is read.
+// Copies a row to its stage, 16 bytes a lane; of the tensor's first and last rows (not `inner`) its own elements alone, so that nothing
+// outside of the tensor is read.
 template <typename T, int VE, int V, bool RAGGED>
 __device__ __forceinline__ void ask_row(char* stage, const T* row, const Frame<VE, RAGGED>& frame, int first, int step, bool inner) {
   const uint32_t dst = smem_addr(stage);
@@ -297,7 +298,7 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
   Pack<Ts, VE> rv[STAGED || !RES ? 1 : V];
   auto ask = [&]() {
     if (asked < p.rows) {
-      const bool inner = asked > 0 && asked < p.rows - 1;
+      const bool inner = asked >= p.edge && asked < p.rows - p.edge;
       if constexpr (STAGED) {
         char* s = at.stages + ask_stage * p.stage_bytes;
         ask_row<Tx, VE, V, RAGGED>(s, next_x, frame, first, lanes, inner);
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
 #pragma unroll
       for (int e = 0; e < VE; ++e) s[v][e] = 0.f;
       if (live && i < nvec) {
-        if (RAGGED && !STAGED && !frame.readable(i, row > 0 && row < p.rows - 1)) {
+        if (RAGGED && !STAGED && !frame.readable(i, row >= p.edge && row < p.rows - p.edge)) {
           xv[STAGED ? 0 : v] = frame.fetch(static_cast<const Tx*>(p.x) + row * p.x_stride - frame.skew, i);
           if constexpr (RES) rv[STAGED ? 0 : v] = frame.fetch(static_cast<const Ts*>(p.residual) + row * p.r_stride - frame.skew, i);
         }
@@ -541,7 +542,7 @@ struct RmsBwd {
   const float* rstd;
   void *dx, *dsum_out;  // the same gradient in dy's type and, where sum has another type, in sum's
   float* part;          // one row of C floats per CTA, or NULL
-  long long rows, dy_stride, ds_stride, s_stride, a_stride;
+  long long rows, dy_stride, ds_stride, s_stride, a_stride, edge;
   int C, lanes, stages, stage_bytes, w_dtype;
   float offset, inv_c;
 };
@@ -566,7 +567,7 @@ __global__ void __launch_bounds__(bwd_threads(VE, V), 1) rms_bwd_kernel(const Rm
   int ask_stage = 0, stage = 0;
   auto ask = [&]() {
     if (asked < p.rows) {
-      const bool inner = asked > 0 && asked < p.rows - 1;
+      const bool inner = asked >= p.edge && asked < p.rows - p.edge;
       char* s = at.stages + ask_stage * p.stage_bytes;
       ask_row<Ts, VE, V, RAGGED>(s, sum + asked * p.s_stride, frame, first, lanes, inner);
       ask_row<Tx, VE, V, RAGGED>(s + dy_at, dy + asked * p.dy_stride, frame, first, lanes, inner);
@@ -968,6 +969,12 @@ Rows rows_of(int width, int64_t C, int64_t rows, const void* weight, std::initia
   }
   return aligned ? kAligned : framed ? kRagged : kAny;
 }
+int64_t edge_of(int width, int64_t rows, std::initializer_list<TensorRows> tensors) {
+  int64_t edge = 1;
+  for (const TensorRows& t : tensors)
+    if (t.p) edge = std::max(edge, edge_rows(width, rows, t.stride));
+  return edge;
+}
 int size_of(int dtype) { return dtype == GNB200_F32 ? 4 : 2; }
 bool dtype_ok(int d) { return d == GNB200_F32 || d == GNB200_F16 || d == GNB200_BF16; }
 
@@ -1019,8 +1026,10 @@ static int rms_forward(const char* name, const void* x, int64_t x_stride, const 
   p.C = (int)C, p.w_dtype = weight_dtype, p.block = block, p.blocks = block ? (int)((C + block - 1) / block) : 1, p.format = format;
   p.eps = (float)eps, p.offset = (float)offset, p.inv_c = (float)(1.0 / (double)C);
   const int size = size_of(dtype), wide = size_of(residual_dtype);
-  const Rows how = rows_of(dtype == GNB200_F32 ? 4 : 8, C, rows, weight,
+  const int width = dtype == GNB200_F32 ? 4 : 8;
+  const Rows how = rows_of(width, C, rows, weight,
                            {{x, x_stride, size}, {residual, residual_stride, wide}, {y, C, codes ? 1 : size}, {sum, C, wide}});
+  p.edge = edge_of(width, rows, {{x, x_stride, size}, {residual, residual_stride, wide}});
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   return launched(name, codes ? launch_rms_fwd<true>(p, dtype, residual_dtype, how, s)
                               : launch_rms_fwd<false>(p, dtype, residual_dtype, how, s));
@@ -1084,7 +1093,9 @@ int gnb200_rms_bwd(const void* dy, int64_t dy_stride, const void* dsum, int64_t 
   p.rows = rows, p.dy_stride = dy_stride, p.ds_stride = dsum_stride, p.s_stride = sum_stride, p.a_stride = addend_stride;
   p.C = (int)C, p.w_dtype = weight_dtype, p.offset = (float)offset, p.inv_c = (float)(1.0 / (double)C);
   const int size = size_of(dtype), wide = size_of(sum_dtype);
-  const Rows how = rows_of(dtype == GNB200_F32 ? 4 : 8, C, rows, weight,
+  const int width = dtype == GNB200_F32 ? 4 : 8;
+  p.edge = edge_of(width, rows, {{dy, dy_stride, size}, {dsum, dsum_stride, wide}, {sum, sum_stride, wide}, {addend, addend_stride, size}});
+  const Rows how = rows_of(width, C, rows, weight,
                            {{dy, dy_stride, size}, {dsum, dsum_stride, wide}, {sum, sum_stride, wide}, {addend, addend_stride, size},
                             {dx, C, size}, {dsum_out, C, wide}});
   unsigned grid = 0;
