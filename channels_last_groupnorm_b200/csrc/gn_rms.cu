@@ -265,6 +265,11 @@ struct Place {
     else
       team_barrier<TEAMS>(lanes, group);
   }
+  // what the group's other lanes read may be written again behind the row's sum: a team has that sum's barrier, lanes of a warp only shuffles,
+  // which order no memory
+  __device__ __forceinline__ void part() const {
+    if constexpr (WARP) __syncwarp();
+  }
 };
 
 // ---------------------------------------------------------------------------------------------
@@ -380,6 +385,7 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
           dot_each(sq, f, f);
         }
       }
+      at.part();
     }
     ask();  // (a lane's own vectors: read, so free)
     const float all_sq = WARP ? lanes_sum(sq[0] + sq[1], lanes) : team_sum<false>(sq[0] + sq[1], slots, turn, lanes, 0);
@@ -636,6 +642,7 @@ __global__ void __launch_bounds__(bwd_threads(VE, V), 1) rms_bwd_kernel(const Rm
           for (int e = 0; e < VE; ++e) dot[e & 1] += f[e];
         }
       }
+      at.part();
     }
     const float c = -(WARP ? lanes_sum(dot[0] + dot[1], lanes) : team_sum<TEAMS>(dot[0] + dot[1], slots, turn, at.lanes, at.group)) * p.inv_c;
     const long long out_at = row * p.C - frame.skew;
