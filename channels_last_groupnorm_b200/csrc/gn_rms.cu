@@ -478,7 +478,8 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
   }
 }
 
-// Rows of any length: one CTA per row, element by element, read once for the sum and once more for each thing that needs it.
+// Rows of any length: one CTA per row, element by element, read once for the sum and once more for each thing that needs it.  Outputs are
+// stored in the last of these passes, by the thread that has just read the element: y and sum may be the inputs' own buffers.
 template <typename Tx, typename Ts, bool Q>
 __global__ void __launch_bounds__(kMostThreads) rms_fwd_any_kernel(const RmsFwd p) {
   __shared__ TeamSlots slots;
@@ -497,22 +498,26 @@ __global__ void __launch_bounds__(kMostThreads) rms_fwd_any_kernel(const RmsFwd 
     for (int i = threadIdx.x; i < p.C; i += blockDim.x) {
       const float s = sum_at(i);
       sq = fmaf(s, s, sq);
-      if (r) static_cast<Ts*>(p.sum)[row * p.C + i] = store_param<Ts>(s);
     }
     sq = team_sum<false>(sq, slots, turn, blockDim.x, 0);
     const float rstd = __frsqrt_rn(fmaf(sq, p.inv_c, p.eps));
     if (p.rstd && threadIdx.x == 0) p.rstd[row] = rstd;
-    auto y_at = [&](int i) { return sum_at(i) * rstd * (p.weight ? p.offset + param_at(p.weight, p.w_dtype, i, 1.f) : 1.f); };
+    auto y_of = [&](int i, float s) { return s * rstd * (p.weight ? p.offset + param_at(p.weight, p.w_dtype, i, 1.f) : 1.f); };
+    auto y_and_store_sum = [&](int i) {  // the last look at element i
+      const float s = sum_at(i);
+      if (r) static_cast<Ts*>(p.sum)[row * p.C + i] = store_param<Ts>(s);
+      return y_of(i, s);
+    };
     if constexpr (!Q) {
-      for (int i = threadIdx.x; i < p.C; i += blockDim.x) static_cast<Tx*>(p.y)[row * p.C + i] = store_param<Tx>(y_at(i));
+      for (int i = threadIdx.x; i < p.C; i += blockDim.x) static_cast<Tx*>(p.y)[row * p.C + i] = store_param<Tx>(y_and_store_sum(i));
     } else {
       uint8_t* out = static_cast<uint8_t*>(p.y) + row * p.C;
       if (p.block == 0) {
         uint32_t m = 0;
-        for (int i = threadIdx.x; i < p.C; i += blockDim.x) m = max(m, magnitude(y_at(i)));
+        for (int i = threadIdx.x; i < p.C; i += blockDim.x) m = max(m, magnitude(y_of(i, sum_at(i))));
         const Scale scale = scale_of(cta_max(m, most), p.format);
         if (threadIdx.x == 0) p.scale[row] = scale.value;
-        for (int i = threadIdx.x; i < p.C; i += blockDim.x) out[i] = (uint8_t)code_of(over(y_at(i), scale.inverse, scale.back), p.format);
+        for (int i = threadIdx.x; i < p.C; i += blockDim.x) out[i] = (uint8_t)code_of(over(y_and_store_sum(i), scale.inverse, scale.back), p.format);
       } else {  // one warp per block of at most 128 channels
         const int lane = threadIdx.x & 31, nwarps = blockDim.x >> 5;
         for (int b = threadIdx.x >> 5; b < p.blocks; b += nwarps) {
@@ -521,7 +526,7 @@ __global__ void __launch_bounds__(kMostThreads) rms_fwd_any_kernel(const RmsFwd 
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             const int in = lane + 32 * v, i = b * p.block + in;
-            f[v] = in < p.block && i < p.C ? y_at(i) : 0.f;
+            f[v] = in < p.block && i < p.C ? y_and_store_sum(i) : 0.f;
             m = max(m, magnitude(f[v]));
           }
           const Scale scale = scale_of(lanes_max(m, 32), p.format);
@@ -700,6 +705,17 @@ __global__ void __launch_bounds__(kMostThreads) rms_bwd_any_kernel(const RmsBwd 
   clear<false>(slots, blockDim.x, 0, threadIdx.x);
   int turn = 0;
   grid_dep_launch_dependents();
+  // The weight's gradient: a look at the CTA's own rows, one channel per thread, before the same thread overwrites that channel where dx or
+  // dsum_out is an input's own buffer.
+  for (int i = threadIdx.x; p.part != nullptr && i < p.C; i += blockDim.x) {
+    float t = 0.f;
+    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+      float s = load_param<Ts>(static_cast<const Ts*>(p.sum) + row * p.s_stride, i);
+      if (p.addend) s += load_param<Tx>(static_cast<const Tx*>(p.addend) + row * p.a_stride, i);
+      t = fmaf(load_param<Tx>(static_cast<const Tx*>(p.dy) + row * p.dy_stride, i), s * p.rstd[row], t);
+    }
+    p.part[(long long)blockIdx.x * p.C + i] = t;
+  }
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const Tx* dy = static_cast<const Tx*>(p.dy) + row * p.dy_stride;
     const Ts* sum = static_cast<const Ts*>(p.sum) + row * p.s_stride;
@@ -717,17 +733,6 @@ __global__ void __launch_bounds__(kMostThreads) rms_bwd_any_kernel(const RmsBwd 
       if constexpr (!std::is_same<Tx, Ts>::value)
         if (p.dsum_out) static_cast<Ts*>(p.dsum_out)[row * p.C + i] = store_param<Ts>(d);
     }
-  }
-  if (p.part == nullptr) return;
-  // (a second look at the CTA's own rows, one channel per thread)
-  for (int i = threadIdx.x; i < p.C; i += blockDim.x) {
-    float t = 0.f;
-    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
-      float s = load_param<Ts>(static_cast<const Ts*>(p.sum) + row * p.s_stride, i);
-      if (p.addend) s += load_param<Tx>(static_cast<const Tx*>(p.addend) + row * p.a_stride, i);
-      t = fmaf(load_param<Tx>(static_cast<const Tx*>(p.dy) + row * p.dy_stride, i), s * p.rstd[row], t);
-    }
-    p.part[(long long)blockIdx.x * p.C + i] = t;
   }
 }
 

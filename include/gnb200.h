@@ -242,6 +242,8 @@ int gnb200_allreduce_param_grads(float* dgamma_dbeta_f32, void* dgamma, void* db
  *   d = dsum + rstd * (g - n * mean(g * n)), the gradient of x and of the residual, to dx in dy's type and, where the sum has
  *   another type, to dsum_out in the sum's (NULL otherwise); and dweight = sum over rows of dy * n (NULL: not wanted) in the
  *   weight's type, added in a fixed order.  The workspace is needed only for dweight.
+ * In place: y, sum, dx and dsum_out may each be the buffer of an input of their type whose rows are contiguous (y that of x, sum that of the
+ *   residual, dx that of dy, dsum_out that of dsum, and so on), one output to a buffer.  Outputs must not overlap inputs in another way.
  */
 enum { GNB200_E4M3 = 0, GNB200_INT8 = 1 };
 int gnb200_rms_fwd(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight,
