@@ -98,9 +98,14 @@ class RMSNorm(nn.Module):
         self.offset = float(offset)
         self.affine = affine
         if affine:
-            self.weight = nn.Parameter(torch.full((num_channels,), 1.0 - self.offset, device=device, dtype=dtype))
+            self.weight = nn.Parameter(torch.empty((num_channels,), device=device, dtype=dtype))
         else:
             self.register_parameter("weight", None)
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        if self.affine:
+            nn.init.constant_(self.weight, 1.0 - self.offset)
 
     def _expect(self, x):
         if x.ndim < 1 or x.shape[-1] != self.num_channels:

@@ -77,7 +77,8 @@ class AxialRotary(nn.Module):
 
     `forward(q, k, positions)` is `rotary` with frequencies of base^(-j / n): with shared=False every axis has the whole range (n its
     own pairs), with shared=True the axes divide one range among them (n = all pairs), in the order of `sections`.  qk_norm
-    adds the heads' norms with learned weights `q_weight` and `k_weight`.
+    adds the heads' norms with learned weights `q_weight` and `k_weight`.  The frequencies are no part of a checkpoint: a module that was
+    built on the meta device has them again as soon as it leaves it (`to_empty`, then `load_state_dict` or `reset_parameters`).
     """
 
     def __init__(self, head_dim: int, sections, base=10000.0, shared=False, interleaved=False, qk_norm=False, eps=1e-6, device=None, dtype=None):
@@ -88,18 +89,32 @@ class AxialRotary(nn.Module):
         self.eps = float(eps)
         if not 1 <= len(self.sections) <= MAX_AXES or min(self.sections) < 0 or not 2 <= 2 * sum(self.sections) <= head_dim <= MAX_HEAD_DIM:
             raise ValueError("AxialRotary: %s pairs do not fit heads of %d channels" % (self.sections, head_dim))
-        n = sum(self.sections)
-        exponents = [i / n for i in range(n)] if shared else [i / s for s in self.sections for i in range(s)]
-        self.register_buffer("inv_freq", torch.tensor([float(base) ** -e for e in exponents], dtype=torch.float32, device=device), persistent=False)
+        self.base = float(base)
+        self.shared = bool(shared)
+        self.register_buffer("inv_freq", self._frequencies(device), persistent=False)
         for name in ("q_weight", "k_weight"):
             self.register_parameter(name, nn.Parameter(torch.ones(head_dim, device=device, dtype=dtype)) if qk_norm else None)
 
+    def _frequencies(self, device):
+        n = sum(self.sections)
+        exponents = [i / n for i in range(n)] if self.shared else [i / s for s in self.sections for i in range(s)]
+        return torch.tensor([self.base ** -e for e in exponents], dtype=torch.float32, device=device)
+
+    def reset_parameters(self):
+        """Weights of one and the frequencies of the module's base, as the constructor makes them."""
+        self.inv_freq = self._frequencies(self.inv_freq.device)
+        with torch.no_grad():
+            for w in (self.q_weight, self.k_weight):
+                if w is not None:
+                    w.fill_(1.0)
+
     def _apply(self, fn, recurse=True):
-        # moved, but never rounded: frequencies stay in 32 bits where the module goes to 16, an angle of many turns needs them
+        # Moved, but neither rounded nor emptied: frequencies stay in 32 bits where the module goes to 16, an angle of many turns needs
+        # them, and to_empty() leaves them as they are, since no checkpoint brings them back.
         kept = self.inv_freq
         super()._apply(fn, recurse)
-        if self.inv_freq.dtype != torch.float32:
-            self.inv_freq = kept.to(self.inv_freq.device)
+        device = self.inv_freq.device
+        self.inv_freq = self._frequencies(device) if kept.is_meta and device.type != "meta" else kept.to(device)
         return self
 
     def forward(self, q, k, positions):
