@@ -233,7 +233,7 @@ struct RmsFunction : torch::autograd::Function<RmsFunction> {
       }
       return out;
     }
-    if (c10::GradMode::is_enabled()) {  // a graph of the backward is asked for: through the dispatcher, as any op without a second derivative
+    if (c10::GradMode::is_enabled()) {  // a graph of the backward is asked for: through the dispatcher, whose formula refuses a second derivative
       static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("gnb200::rms_bwd", "").typed<decltype(rms_bwd_op)>();
       auto [dx, ds, dw] = op.call(dy, opt(dsum), sum, opt(addend), opt(weight), rstd, offset);
       out[0] = dx;
@@ -455,8 +455,15 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
     if (!dq.defined() && !dk.defined()) return out;
     const double eps = ctx->saved_data["eps"].toDouble(), offset = ctx->saved_data["offset"].toDouble();
     const bool interleaved = ctx->saved_data["interleaved"].toBool();
-    if (c10::GradMode::is_enabled() && dq.defined()) {  // through the dispatcher, as any op without a second derivative
+    if (c10::GradMode::is_enabled()) {  // through the dispatcher, whose formula refuses a second derivative
       static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("gnb200::rotary_bwd", "").typed<decltype(rotary_bwd_op)>();
+      if (!dq.defined()) {  // (the keys alone, in the queries' place)
+        auto [gk, none, gkw, no_weight] = op.call(dk, OptTensor(), saved[1].defined() ? saved[1] : dk, OptTensor(), saved[4], saved[5], sections,
+                                                  opt(saved[3]), OptTensor(), eps, offset, interleaved);
+        out[1] = gk;
+        if (saved[3].defined()) out[3] = gkw;
+        return out;
+      }
       auto [gq, gk, gqw, gkw] = op.call(dq, opt(dk), saved[0].defined() ? saved[0] : dq, opt(saved[1]), saved[4], saved[5], sections,
                                         opt(saved[2]), dk.defined() ? opt(saved[3]) : OptTensor(), eps, offset, interleaved);
       out[0] = gq;

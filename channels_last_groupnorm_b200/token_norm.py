@@ -45,7 +45,8 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6, offset=0.0):
     adds to; the norm itself takes the sum before that rounding.  x: (*, channels) in float32, float16 or bfloat16; rows at any
     one distance are read in place (slices of a wider tensor), other layouts are copied first.  residual: x's sizes, x's dtype
     or float32.  weight: (channels,) in x's dtype or float32, or None for no weight; offset=1 is for weights stored as
-    differences from one.  Differentiable once in x, weight and residual; the weight's gradient is summed in a fixed order.
+    differences from one.  Differentiable once in x, weight and residual (a gradient of the gradients is an error); the weight's
+    gradient is summed in a fixed order.
     """
     if not torch.compiler.is_compiling():
         out = _rms_norm(x, weight, residual, eps, offset)

@@ -59,7 +59,8 @@ def rotary(q, k, positions, inv_freq, sections, q_weight=None, k_weight=None, ep
     may be None.  positions: (*tokens, axes), int32, int64 or float32.  sections: pairs of each axis; inv_freq: float32, one
     frequency per pair, the first sections[0] of axis 0 and so on.  Pair i is channels (i, i + pairs), or (2 i, 2 i + 1) with
     interleaved=True; channels beyond the 2 * sum(sections) first ones pass.  q_weight, k_weight: weights of a root-mean-square
-    norm of each head in front of the rotation, (offset + weight); None for no norm.  Differentiable once in q, k and the weights.
+    norm of each head in front of the rotation, (offset + weight); None for no norm.  Differentiable once in q, k and the weights (a gradient of
+    the gradients is an error).
     """
     if not torch.compiler.is_compiling() and not inv_freq.requires_grad and not positions.requires_grad:
         out = _rotary(q, k, positions, inv_freq, sections, q_weight, k_weight, eps, offset, interleaved)
