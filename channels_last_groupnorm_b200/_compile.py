@@ -144,15 +144,16 @@ torch.library.register_autograd("gnb200::rotary_bwd", _once("rotary"))
 def _rotary_setup_context(ctx, inputs, output):
     q, k, positions, inv_freq, ctx.sections, q_weight, k_weight, ctx.eps, ctx.offset, ctx.interleaved = inputs
     ctx.has_k = k is not None
-    ctx.save_for_backward(q, k, positions, inv_freq, q_weight, k_weight)
+    # (as the native node: a rotation alone needs nothing of its input)
+    ctx.save_for_backward(None if q_weight is None else q, None if k_weight is None else k, positions, inv_freq, q_weight, k_weight)
     if not ctx.has_k:
         ctx.mark_non_differentiable(output[1])
 
 
 def _rotary_backward(ctx, dq, dk):
     q, k, positions, inv_freq, q_weight, k_weight = ctx.saved_tensors
-    gq, gk, gqw, gkw = torch.ops.gnb200.rotary_bwd(dq, dk if ctx.has_k else None, q, k, positions, inv_freq, ctx.sections, q_weight, k_weight,
-                                                   ctx.eps, ctx.offset, ctx.interleaved)
+    gq, gk, gqw, gkw = torch.ops.gnb200.rotary_bwd(dq, dk if ctx.has_k else None, dq if q is None else q, k, positions, inv_freq, ctx.sections,
+                                                   q_weight, k_weight, ctx.eps, ctx.offset, ctx.interleaved)
     return (gq, gk if ctx.has_k else None, None, None, None, None if q_weight is None else gqw, None if k_weight is None else gkw,
             None, None, None)
 
