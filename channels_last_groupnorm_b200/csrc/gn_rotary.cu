@@ -84,10 +84,9 @@ __device__ __forceinline__ void ask_positions(const Rotary& p, const PairTable& 
 }
 
 // cos and sin of pair i's angle.  It is formed in turns, whole ones dropped: position * hi in fp32, what its rounding lost (an fma gives it
-// exactly) and position * lo.  That holds for positions that fp32 holds exactly; larger ones are multiplied in fp64.  FAST: the hardware's
-// sine and cosine, off by 2^-21 on the remaining half turns, for results that are rounded to 16 bits.
-template <bool FAST>
-__device__ __forceinline__ float2 angle_of(const Rotary& p, const PairTable& table, int i, long long raw) {
+// exactly) and position * lo.  That holds for positions that fp32 holds exactly; larger ones are multiplied in fp64.  fast: the hardware's
+// sine and cosine, off by 2^-21 on the remaining half turns, where all results are rounded to 16 bits.
+__device__ __forceinline__ float2 angle_of(const Rotary& p, const PairTable& table, int i, long long raw, bool fast) {
   const float2 freq = table.turns[i];
   const bool is_float = p.pos_type == GNB200_POS_F32;
   const float position = is_float ? __int_as_float((int)raw) : (float)(int)raw;
@@ -101,7 +100,7 @@ __device__ __forceinline__ float2 angle_of(const Rotary& p, const PairTable& tab
     part = (float)(turns - rint(turns));
   }
   float sn, cs;
-  if constexpr (FAST) {
+  if (fast) {
     part -= rintf(part);  // (the two parts' sum may have passed half a turn)
     const float radians = part * 6.28318531f;
     sn = __sinf(radians);
@@ -113,15 +112,14 @@ __device__ __forceinline__ float2 angle_of(const Rotary& p, const PairTable& tab
 }
 
 // cos and sin of a token's angles, into the warp's shared memory
-template <bool FAST>
-__device__ __forceinline__ void token_angles(const Rotary& p, const PairTable& table, int b, int s, const Positions& known, float2* out) {
+__device__ __forceinline__ void token_angles(const Rotary& p, const PairTable& table, int b, int s, const Positions& known, bool fast, float2* out) {
   const int lane = threadIdx.x & 31;
   __syncwarp();  // (nobody reads the token before any more)
-  if (lane < p.pairs) out[lane] = angle_of<FAST>(p, table, lane, known.raw[0]);
-  if (lane + 32 < p.pairs) out[lane + 32] = angle_of<FAST>(p, table, lane + 32, known.raw[1]);
+  if (lane < p.pairs) out[lane] = angle_of(p, table, lane, known.raw[0], fast);
+  if (lane + 32 < p.pairs) out[lane + 32] = angle_of(p, table, lane + 32, known.raw[1], fast);
   if (p.pairs > 64) {
     const long long at = p.pos_stride[0] * b + p.pos_stride[1] * s;
-    for (int i = lane + 64; i < p.pairs; i += 32) out[i] = angle_of<FAST>(p, table, i, position_at(p, at + table.axis[i] * p.pos_stride[2]));
+    for (int i = lane + 64; i < p.pairs; i += 32) out[i] = angle_of(p, table, i, position_at(p, at + table.axis[i] * p.pos_stride[2]), fast);
   }
   __syncwarp();
 }
@@ -177,9 +175,8 @@ __device__ __forceinline__ long long place(const long long (&strides)[3], int b,
   return strides[0] * b + strides[1] * s + strides[2] * head;
 }
 // Reciprocal root mean square.  The fast one is off by two units of fp32's last place, below what results of 16 bits show.
-template <bool FAST>
-__device__ __forceinline__ float rms_inverse(float mean_square) {
-  return FAST ? rsqrtf(mean_square) : __frsqrt_rn(mean_square);
+__device__ __forceinline__ float rms_inverse(float mean_square, bool fast) {
+  return fast ? rsqrtf(mean_square) : __frsqrt_rn(mean_square);
 }
 
 // cos and sin of the slot's pairs, two pairs a load (they lie together, on 16 bytes)
@@ -345,7 +342,7 @@ __global__ void __launch_bounds__(kThreads) rotary_fwd_kernel(const Rotary p) {
     ask_positions(p, table, b, s, positions);
   }
   for (int task = first_task; task < tasks; task += step) {
-    token_angles<sizeof(T) == 2>(p, table, b, s, positions, angles[warp]);
+    token_angles(p, table, b, s, positions, sizeof(T) == 2, angles[warp]);
     const int now = token;
     if (task + step < tasks) {
       token = token_of(p, task + step, per_token, b, s);
@@ -415,7 +412,7 @@ __global__ void __launch_bounds__(kThreads) rotary_fwd_kernel(const Rotary p) {
         if constexpr (RING) stage = (stage + 1) % STAGES;
         ask();
         if constexpr (NORM) {
-          const float rstd = rms_inverse<sizeof(T) == 2>(fmaf(lanes_sum(sq[0] + sq[1], p.lanes), p.inv_d, p.eps));
+          const float rstd = rms_inverse(fmaf(lanes_sum(sq[0] + sq[1], p.lanes), p.inv_d, p.eps), sizeof(T) == 2);
 #pragma unroll
           for (int j = 0; j < SLOTS; ++j) scale_each(f[j], rstd);
         }
@@ -446,6 +443,8 @@ __global__ void __launch_bounds__(kThreads) rotary_bwd_kernel(const Rotary p) {
   const unsigned cta = blockIdx.x - (t ? p.ctas[0] : 0);
   grid_dep_launch_dependents();
   const int per_token = p.tasks_per_token[t], per_task = p.per_task[t], heads = p.heads[t];
+  // (the gradient of an fp32 weight is a sum of the same terms that stays in 32 bits: 16384 tokens of 32 + 32 heads 134 us, fast 130)
+  const bool fast = sizeof(T) == 2 && p.w_dtype[t] != GNB200_F32;
   const int tasks = p.tokens * per_token, step = (int)p.ctas[t] * kWarps;
   // what is asked for next: the warp's next turn of a task's heads; in, xs: this lane's head of the gradient and of the input
   const int first_task = (int)cta * kWarps + warp;
@@ -513,7 +512,7 @@ __global__ void __launch_bounds__(kThreads) rotary_bwd_kernel(const Rotary p) {
     ask_positions(p, table, b, s, positions);
   }
   for (int task = first_task; task < tasks; task += step) {
-    token_angles<sizeof(T) == 2>(p, table, b, s, positions, angles[warp]);
+    token_angles(p, table, b, s, positions, fast, angles[warp]);
     const int from = (task - token * per_token) * per_task, to = min(from + per_task, heads);
     T* out = static_cast<T*>(p.out[t]) + ((long long)token * heads + from + group) * p.D;
     const int out_step = groups * p.D;
@@ -567,7 +566,7 @@ __global__ void __launch_bounds__(kThreads) rotary_bwd_kernel(const Rotary p) {
         dot_each(dot, gw[j], n[j]);
       }
       const float all_sq = lanes_sum(sq[0] + sq[1], p.lanes), all_dot = lanes_sum(dot[0] + dot[1], p.lanes);
-      const float rstd = rms_inverse<sizeof(T) == 2>(fmaf(all_sq, p.inv_d, p.eps)), c = -all_dot * rstd * p.inv_d;
+      const float rstd = rms_inverse(fmaf(all_sq, p.inv_d, p.eps), fast), c = -all_dot * rstd * p.inv_d;
 #pragma unroll
       for (int j = 0; j < SLOTS; ++j) {
         scale_each(n[j], rstd);
