@@ -639,11 +639,15 @@ cudaError_t with_rotary_geometry(const RotaryGeom& g, F&& f) {
 // How the tokens' heads are dealt out: warps take whole tokens where there are enough of them, else shares of a token's heads.  Forward q and
 // k share the tasks; backward each has CTAs in proportion to a token's turns of the warp, and two more for the angles and all else that a token
 // takes (16384 tokens, 32 and 8 heads of 128: 134 us in proportion to the heads, 98 with them).
-// Forward calls with many heads are bound by memory: four CTAs an SM keep 32 KB of heads ahead, and more of them only disturb one another
-// (16384 tokens, 32 and 32 heads of 128, bf16, with norm: 3 CTAs 97.5 us, 4 87.0, 5 97.4).  With few heads a token's angles count for more, and
-// every warp helps (2 x 4096 tokens, 20 and 20 heads of 64: 4 CTAs 18.8, 5 17.7).
-constexpr int kTokenTurns = 2, kManyTurns = 12;
-cudaError_t rotary_split(const void* kernel, const RotaryGeom& g, bool ring, bool back, Rotary& p) {
+// Forward calls with many heads are bound by memory: four CTAs an SM keep 32 KB of heads ahead, and more of them only disturb one another.
+// With few heads a token's angles count for more, with a norm its coefficients too, and every warp helps.  16384 tokens, bf16, us with four CTAs and
+// with five, by a token's turns of the warp:
+//   heads of 128, norm    6: 41.3, 38.9    8: 49.5, 47.4    9: 54.2, 53.3    10: 58.6, 58.5 and 59.9    12: 67.6, 73.9    16: 87.9, 98.9
+//   without               6: 36.1, 36.5    7: 40.7, 42.3    8: 45.2, 48.8    10: 55.5, 60.7    12: 65.3, 71.8    16: 88.0, 94.0
+//   heads of 64, norm     6: 36.1, 35.7    8: 45.8, 48.0    10: 55.4, 61.4;   of 256    8: 54.0, 50.8    10: 63.0, 61.1    12: 71.4, 71.2    16: 90.8, 99.8
+//   without               6: 34.7, 36.1    8: 44.6, 49.0;                      of 256    6: 37.4, 36.9    8: 46.9, 49.1
+constexpr int kTokenTurns = 2, kManyTurns = 7, kManyTurnsWithNorm = 10;
+cudaError_t rotary_split(const void* kernel, const RotaryGeom& g, bool ring, bool norm, bool back, Rotary& p) {
   Residency r;
   const cudaError_t err = residency(kernel, kThreads, 0, &r);
   if (err != cudaSuccess) return err;
@@ -654,7 +658,7 @@ cudaError_t rotary_split(const void* kernel, const RotaryGeom& g, bool ring, boo
     turns[t] = (p.heads[t] + groups - 1) / groups;  // of a warp, for a token
     weight[t] = turns[t] + kTokenTurns;
   }
-  if (ring && !back && turns[0] + turns[1] >= kManyTurns) r.per_sm = std::min(r.per_sm, 4);
+  if (ring && !back && turns[0] + turns[1] >= (norm ? kManyTurnsWithNorm : kManyTurns)) r.per_sm = std::min(r.per_sm, 4);
   const long long most = (long long)r.per_sm * r.sms;
   for (int t = 0; t < 2; ++t) {
     if (!p.heads[t]) continue;
@@ -682,7 +686,7 @@ cudaError_t launch_rotary(Rotary& p, int dtype, int widest, bool inter, bool nor
   const RotaryGeom g = rotary_geometry(p.D, p.pairs, widest, dtype == GNB200_F32 ? 4 : 8);
   p.lanes = g.lanes;
   auto go = [&](void (*kernel)(const Rotary)) {
-    const cudaError_t err = rotary_split((const void*)kernel, g, g.ve == (dtype == GNB200_F32 ? 4 : 8), back, p);
+    const cudaError_t err = rotary_split((const void*)kernel, g, g.ve == (dtype == GNB200_F32 ? 4 : 8), norm, back, p);
     if (err != cudaSuccess || plan_only) return err;
     kernel<<<p.ctas[0] + p.ctas[1], kThreads, 0, stream>>>(p);
     return cudaGetLastError();
