@@ -6,10 +6,10 @@ namespace gnb200 {
 
 // Rows at either end of a tensor whose edge vectors may reach out of it.  Vectors of `width` elements begin up to width - 1 elements before a
 // row or end as many behind it; a row with as much of the tensor on both sides may be read in whole vectors.  One row at either end where rows are no
-// shorter than that, several where they are (or where they overlap, as rows at a distance of 0 do).  stride: from row to row.
-inline int64_t edge_rows(int width, int64_t rows, int64_t stride) {
+// shorter than that, several where they are, or where they overlap.  stride: from row to row, not 0.
+inline int edge_rows(int width, int64_t stride) {
   const int64_t step = stride < 0 ? -stride : stride;
-  return step == 0 ? rows : (width - 1 + step - 1) / step;
+  return step < width - 1 ? (int)((width - 1 + step - 1) / (step > 0 ? step : 1)) : 1;
 }
 
 }  // namespace gnb200

@@ -13,10 +13,10 @@ from channels_last_groupnorm_b200 import build
 def edge_rows(tmp_path_factory):
     folder = tmp_path_factory.mktemp("rows")
     source, lib = folder / "rows.cpp", folder / "rows.so"
-    source.write_text('#include "gn_rows.h"\nextern "C" int64_t edge_rows(int w, int64_t r, int64_t s) { return gnb200::edge_rows(w, r, s); }\n')
+    source.write_text('#include "gn_rows.h"\nextern "C" int edge_rows(int w, int64_t s) { return gnb200::edge_rows(w, s); }\n')
     subprocess.check_call(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-I", build.CSRC, str(source), "-o", str(lib)])
     fn = ctypes.CDLL(os.fspath(lib)).edge_rows
-    fn.restype, fn.argtypes = ctypes.c_int64, [ctypes.c_int, ctypes.c_int64, ctypes.c_int64]
+    fn.restype, fn.argtypes = ctypes.c_int, [ctypes.c_int, ctypes.c_int64]
     return fn
 
 
@@ -39,9 +39,9 @@ def reads_outside(width, c, rows, stride, skew, edge):
 def test_no_vector_reaches_out_of_the_tensor(edge_rows, width):
     some = 0
     for c in range(1, 2 * width + 2):
-        for stride in {c + k * width for k in range(-3, 3)} | {0}:
+        for stride in {c + k * width for k in range(-3, 3)} - {0}:  # (rows at a distance of 0 go element by element)
             for rows in (1, 2, 3, 4, 9, 20):
-                edge = max(1, edge_rows(width, rows, stride))
+                edge = edge_rows(width, stride)
                 for skew in range(width):
                     assert not reads_outside(width, c, rows, stride, skew, edge), (c, stride, rows, skew)
                     some += bool(reads_outside(width, c, rows, stride, skew, 1))
@@ -51,4 +51,4 @@ def test_no_vector_reaches_out_of_the_tensor(edge_rows, width):
 @pytest.mark.parametrize("width", [4, 8])
 def test_longer_rows_have_one_edge_row(edge_rows, width):
     for stride in (width - 1, width, 999, 1 << 40, -999):
-        assert edge_rows(width, 1 << 30, stride) == 1
+        assert edge_rows(width, stride) == 1
