@@ -9,16 +9,18 @@
 //
 // Every element is read and written once: a row's elements stay in registers (backward: in shared memory) between the sum over the row and
 // the output, and the only traffic beside them is a row of partial sums per CTA in the backward.  Bound by HBM where there are rows enough:
-// 16384 x 4096 bf16 with the residual, forward 88 us = 6.1 TB/s, backward (four tensors read, one written) 106 us = 6.3 TB/s, 93 and
-// 96 % of a copy's rate; 8192 x 8192 bf16 over an fp32 stream to 8 bits 118 us = 6.3 TB/s.  A call of one row takes 2.2 us, of 8 rows in
+// 16384 x 4096 bf16 with the residual, forward 89 us = 6.0 TB/s, backward (four tensors read, one written) 107 us = 6.3 TB/s, 92 and
+// 96 % of a copy's rate; 8192 x 8192 bf16 over an fp32 stream to 8 bits 115 us = 6.4 TB/s.  A call of one row takes 2.2 us, of 8 rows in
 // 8 bits 3: launch, first load and one reduction.
 //
-// Rows of up to four vectors a lane belong to a group of lanes of one warp (shuffles only), longer ones to a CTA, or in the backward to a team of
-// warps, of which a CTA has several so that fewer partial rows are left to add up; rows longer than those are read twice, element by
-// element (`any`).  The grid holds the CTAs that are resident at once; each keeps its channels' weights in registers, walks over the rows and
-// asks for the next ones early: into registers while these are few (one row, 64 bytes a thread), otherwise by cp.async into a ring of rows
-// in shared memory, which costs two more instructions a vector but no registers (8192 x 8192 to 8 bits 136 -> 121 us; the backward of
-// 16384 x 4096 125 -> 106, whose spills it ended; the forward of 16384 x 4096 stays in registers: 88 against 93).
+// Rows of up to four vectors a lane belong to a group of lanes of one warp (shuffles only), longer ones to a CTA, or in the backward to a
+// team of warps, of which a CTA has several so that fewer partial rows are left to add up; rows longer than those (more than 16384
+// channels, odd ones a little fewer) are read two or three times, element by element (`any`).  The backward of short and odd widths is
+// bound by instructions and by idle lanes, not by HBM: 30000 x 320 bf16 27 us for 14.6 of traffic, 9000 x 1112 28 for 15.3, 4000 x 1280
+// fp32 19.5 for 12.5.  The grid holds the CTAs that are resident at once; each keeps its channels' weights in registers, walks over the
+// rows and asks for the next ones early: into registers while these are few (one row, 64 bytes a thread), otherwise by cp.async into a ring
+// of rows in shared memory, which costs two more instructions a vector but no registers (8192 x 8192 to 8 bits 136 -> 121 us; the backward
+// of 16384 x 4096 125 -> 106, whose spills it ended; the forward of 16384 x 4096 stays in registers: 88 against 93).
 #include <algorithm>
 #include <initializer_list>
 
@@ -113,9 +115,9 @@ __device__ __forceinline__ void codes_of(const float (&v)[VE], int format, uint3
 // RAGGED rows start between the boundaries of 16 bytes, or end there.  They are taken in a frame that begins at the boundary before: vector i
 // holds channels i * VE - skew and on, the first and the last one in part.  All tensors of a call have the same frame (checked by the
 // host), and the step from one of a thread's rows to the next is a multiple of VE rows, so that the skew, and with it the channels of a thread, stay:
-// its weights and sums are in registers as they are for aligned rows.  Device us, element by element before and so: 9000 rows of 1111 bf16 with a
-// residual, forward 27.0 and 25.0, backward 42.3 and 47.1; 3000 of 12345, backward 210 and 167; 4000 of 12345 fp16, 8-bit output with
-// blocks, 592 and 219.  Twice the instructions of aligned rows bound them: the sums' way through shared memory, and the edges.
+// its weights and sums are in registers as they are for aligned rows.  Device us, element by element and so: 9000 rows of 1111 bf16 with a
+// residual, forward 27.0 and 21.1, backward 42.3 and 40.2; 3000 of 12345, backward 210 and 154; 4000 of 12345 fp16 over fp32, 8-bit output with
+// blocks, 592 and 224.  Twice the instructions of aligned rows bound them: the sums' way through shared memory, and the edges.
 template <int VE, bool RAGGED>
 struct Frame {
   int skew, nvec, C;

@@ -145,7 +145,7 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {
     if (lanes > delta) v += __shfl_xor_sync(0xffffffffu, v, delta);
   return v;
 }
-// (Shuffles for the maximum too: with __reduce_max_sync one of the kernels gave lane 0's value to all lanes.)
+// (Maxima by shuffles as well: they serve groups of a few lanes, which a reduction over the warp does not.)
 // Magnitudes compare like their bit patterns, with NaN above infinity: an integer maximum keeps a NaN, fmaxf would drop it.
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 // the larger of two magnitudes, or NaN where one is

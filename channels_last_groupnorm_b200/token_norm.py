@@ -1,8 +1,8 @@
 """Root-mean-square norm of token rows with the residual's addition, and the same with an 8-bit output and scales.
 
 What the blocks around attention and feed-forward layers start with: `rms_norm` in training and inference, `rms_norm_quant`
-in front of 8-bit products in inference.  Both run as one kernel that reads and writes every element once (csrc/gn_rms.cu).
-The reference has no counterpart.
+in front of 8-bit products in inference.  Both run as one kernel that reads and writes every element once, but for rows of more than
+some 16384 channels, which it reads two or three times (csrc/gn_rms.cu).  The reference has no counterpart.
 """
 import torch
 import torch.nn as nn
@@ -42,8 +42,8 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6, offset=0.0):
     """y = s * rsqrt(mean(s^2) + eps) * (offset + weight) over the last dimension, with s = x + residual.
 
     Returns y without a residual, else (y, s): s, rounded once to the residual's dtype, is the residual stream that the next block
-    adds to; the norm itself takes the sum before that rounding.  x: (*, channels) in float32, float16 or bfloat16; rows at any
-    one distance are read in place (slices of a wider tensor), other layouts are copied first.  residual: x's sizes, x's dtype
+    adds to; the norm itself takes the sum before that rounding.  x: (*, channels) in float32, float16 or bfloat16; contiguous rows
+    and slices of a wider tensor whose channels, start and distance are whole 16-byte vectors are read in place, other layouts are copied first.  residual: x's sizes, x's dtype
     or float32.  weight: (channels,) in x's dtype or float32, or None for no weight; offset=1 is for weights stored as
     differences from one.  Differentiable once in x, weight and residual (a gradient of the gradients is an error); the weight's
     gradient is summed in a fixed order.

@@ -225,8 +225,15 @@ int gnb200_allreduce_param_grads(float* dgamma_dbeta_f32, void* dgamma, void* db
 
 /*
  * Token rows: what stands around the attention and feed-forward blocks of transformers.  No counterparts in the reference.
- * Rows are C contiguous elements; a row stride (in elements) may be larger, as for slices of a wider tensor.  Pointers that are
- * 16-byte aligned, with strides and C that are multiples of a 16-byte vector, take the vector kernels, all others single elements.
+ * Rows are C contiguous elements; a row stride (in elements) may be larger, as for slices of a wider tensor.  The norms take one of three routes,
+ * by where the rows lie among vectors (of 4 elements where x is fp32, else 8):
+ *   aligned: every pointer (the weight's too) 16-byte aligned, strides and C whole vectors: the fastest;
+ *   common frame: every tensor's first row begins the same number of elements behind a vector boundary (a boundary of the whole vector: 32 bytes for an
+ *     fp32 stream beside 16-bit x), and strides differ from C by whole vectors, as those of contiguous rows of any C do: vector kernels too, at
+ *     up to twice the time;
+ *   otherwise, and for rows of more than some 16384 channels: element by element, inputs read two or three times.
+ * So a weight at an odd place of a larger buffer takes aligned rows off the first route (16384 x 4096 bf16: 157 us instead of 89).  Rotary positions go by the widest
+ * vectors that addresses, strides, the head and its pairs allow (16 bytes, 8 or 16 for 4 elements, or single elements).
  * Types are those of x: GNB200_F32 / F16 / BF16; the residual (and `sum`) and the weight may be fp32 beside 16-bit x.
  *
  * gnb200_rms_fwd: root-mean-square norm with the residual's addition.
@@ -235,13 +242,14 @@ int gnb200_allreduce_param_grads(float* dgamma_dbeta_f32, void* dgamma, void* db
  *   with a residual) and rstd (rows floats, may be NULL).  s is not rounded before the norm.
  * gnb200_rms_fwd_8bit: the same with y as 8-bit codes q and fp32 scales, y = q * scale: scale = max |y| / 448 (e4m3) or / 127
  *   (int8), at least 2^-126, one per row (block 0: `rows` floats) or per block of 32, 64 or 128 channels (rows x ceil(C / block)
- *   floats).  A NaN makes the scale of its block NaN.
+ *   floats).  A NaN makes the scale of its block NaN.  q is y / scale as a division rounds it, then rounded to the code.
  * gnb200_rms_bwd: dy and, where the sum was used, dsum (may be NULL) are the gradients of y and sum; s is `sum`, what the forward
  *   stored, or x where there was no residual; or, with an addend in dy's type (otherwise NULL), sum + addend: the residual and x, for
  *   a gradient of the weight that is as exact as the forward where the stored sum is rounded to 16 bits.  With n = s * rstd and g = dy * (offset + weight) it writes
  *   d = dsum + rstd * (g - n * mean(g * n)), the gradient of x and of the residual, to dx in dy's type and, where the sum has
  *   another type, to dsum_out in the sum's (NULL otherwise); and dweight = sum over rows of dy * n (NULL: not wanted) in the
- *   weight's type, added in a fixed order.  The workspace is needed only for dweight.
+ *   weight's type, added in a fixed order.  The workspace is needed only for dweight; the bytes asked for are
+ *   those of whichever route the call's tensors may take.
  * In place: y, sum, dx and dsum_out may each be the buffer of an input of their type whose rows are contiguous (y that of x, sum that of the
  *   residual, dx that of dy, dsum_out that of dsum, and so on), one output to a buffer.  Outputs must not overlap inputs in another way.
  */
