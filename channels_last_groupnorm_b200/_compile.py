@@ -129,18 +129,6 @@ def _rms_backward(ctx, dy, ds, drstd):
 torch.library.register_autograd("gnb200::rms_fwd", _rms_backward, setup_context=_rms_setup_context)
 
 
-def _once(name):
-    """A gradient's own gradient: an error, where an op without a formula would leave its term out."""
-    def backward(ctx, *grads):
-        raise RuntimeError("gnb200: %s is differentiable once; a gradient of its gradient was asked for" % name)
-
-    return backward
-
-
-torch.library.register_autograd("gnb200::rms_bwd", _once("rms_norm"))
-torch.library.register_autograd("gnb200::rotary_bwd", _once("rotary"))
-
-
 def _rotary_setup_context(ctx, inputs, output):
     q, k, positions, inv_freq, ctx.sections, q_weight, k_weight, ctx.eps, ctx.offset, ctx.interleaved = inputs
     ctx.has_k = k is not None

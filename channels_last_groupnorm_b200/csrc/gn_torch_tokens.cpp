@@ -6,7 +6,7 @@
 //   rms_quant(x, residual?, weight?, eps, offset, block, format) -> (codes, scales, sum)
 //   rotary(q, k?, positions, inv_freq, sections, q_weight?, k_weight?, eps, offset, interleaved) -> (q, k)
 //   rotary_bwd(dq, dk?, q, k?, positions, ...) -> (dq, dk, dq_weight, dk_weight)
-// The functional ops serve tracing (torch.compile, functorch) and libtorch programs; eager calls of the package take the plain calls,
+// The functional ops serve tracing (torch.compile) and libtorch programs; eager calls of the package take the plain calls,
 // which run the same code without the dispatcher and with a native autograd node.
 #include <ATen/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
@@ -194,6 +194,11 @@ std::tuple<Tensor, Tensor, Tensor> rms_quant_op(const Tensor& x, const OptTensor
   return {o.y, o.scale, o.sum.defined() ? o.sum : none_of(x)};
 }
 
+const auto& rms_bwd_handle() {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("gnb200::rms_bwd", "").typed<decltype(rms_bwd_op)>();
+  return op;
+}
+
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
@@ -234,8 +239,7 @@ struct RmsFunction : torch::autograd::Function<RmsFunction> {
       return out;
     }
     if (c10::GradMode::is_enabled()) {  // a graph of the backward is asked for: through the dispatcher, whose formula refuses a second derivative
-      static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("gnb200::rms_bwd", "").typed<decltype(rms_bwd_op)>();
-      auto [dx, ds, dw] = op.call(dy, opt(dsum), sum, opt(addend), opt(weight), rstd, offset);
+      auto [dx, ds, dw] = rms_bwd_handle().call(dy, opt(dsum), sum, opt(addend), opt(weight), rstd, offset);
       out[0] = dx;
       if (want_dsum) out[1] = sum.scalar_type() == x_type ? dx : ds;
       if (want_dweight) out[2] = dw;
@@ -249,17 +253,43 @@ struct RmsFunction : torch::autograd::Function<RmsFunction> {
   }
 };
 
-bool plain(std::initializer_list<const Tensor*> tensors) {
-  if (!gnb200_ops::only_cuda_sees(tensors)) return false;
-  for (const Tensor* t : tensors)
-    if (t->defined() && t->_fw_grad(0).defined()) return false;  // dual tensors
-  return true;
-}
 bool wants_graph(std::initializer_list<const Tensor*> tensors) {
   if (!c10::GradMode::is_enabled()) return false;
   for (const Tensor* t : tensors)
     if (t->defined() && t->requires_grad()) return true;
   return false;
+}
+// The gradients' own gradients: an error, where an op without a formula would leave its term out.
+void refuse_second(const char* name) { TORCH_CHECK(false, "gnb200: ", name, " is differentiable once; a gradient of its gradient was asked for"); }
+
+struct RmsBackwardOnce : torch::autograd::Function<RmsBackwardOnce> {
+  static variable_list forward(AutogradContext*, const Tensor& dy, const OptTensor& dsum, const Tensor& sum, const OptTensor& addend,
+                               const OptTensor& weight, const Tensor& rstd, double offset) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [dx, ds, dw] = rms_bwd_handle().call(dy, dsum, sum, addend, weight, rstd, offset);
+    return {dx, ds, dw};
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    refuse_second("rms_norm");
+    return {};
+  }
+};
+std::tuple<Tensor, Tensor, Tensor> rms_bwd_autograd(const Tensor& dy, const OptTensor& dsum, const Tensor& sum, const OptTensor& addend,
+                                                    const OptTensor& weight, const Tensor& rstd, double offset) {
+  const Tensor ds = value(dsum), a = value(addend), w = value(weight);
+  if (wants_graph({&dy, &ds, &sum, &a, &w, &rstd})) {
+    variable_list out = RmsBackwardOnce::apply(dy, dsum, sum, addend, weight, rstd, offset);
+    return {out[0], out[1], out[2]};
+  }
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return rms_bwd_handle().call(dy, dsum, sum, addend, weight, rstd, offset);
+}
+
+bool plain(std::initializer_list<const Tensor*> tensors) {
+  if (!gnb200_ops::only_cuda_sees(tensors)) return false;
+  for (const Tensor* t : tensors)
+    if (t->defined() && t->_fw_grad(0).defined()) return false;  // dual tensors
+  return true;
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -431,6 +461,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rotary_bwd_op(const Tensor& dq, const
   return {filled(g.dq), filled(g.dk), filled(g.dq_weight), filled(g.dk_weight)};
 }
 
+const auto& rotary_bwd_handle() {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("gnb200::rotary_bwd", "").typed<decltype(rotary_bwd_op)>();
+  return op;
+}
+
 struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const OptTensor& k_arg, const OptTensor& q_weight_arg,
                                const OptTensor& k_weight_arg, const Tensor& positions, const Tensor& inv_freq,
@@ -456,7 +491,7 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
     const double eps = ctx->saved_data["eps"].toDouble(), offset = ctx->saved_data["offset"].toDouble();
     const bool interleaved = ctx->saved_data["interleaved"].toBool();
     if (c10::GradMode::is_enabled()) {  // through the dispatcher, whose formula refuses a second derivative
-      static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("gnb200::rotary_bwd", "").typed<decltype(rotary_bwd_op)>();
+      const auto& op = rotary_bwd_handle();
       if (!dq.defined()) {  // (the keys alone, in the queries' place)
         auto [gk, none, gkw, no_weight] = op.call(dk, OptTensor(), saved[1].defined() ? saved[1] : dk, OptTensor(), saved[4], saved[5], sections,
                                                   opt(saved[3]), OptTensor(), eps, offset, interleaved);
@@ -480,6 +515,33 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
     return out;
   }
 };
+
+struct RotaryBackwardOnce : torch::autograd::Function<RotaryBackwardOnce> {
+  static variable_list forward(AutogradContext*, const Tensor& dq, const OptTensor& dk, const Tensor& q, const OptTensor& k,
+                               const OptTensor& q_weight, const OptTensor& k_weight, const Tensor& positions, const Tensor& inv_freq,
+                               const std::vector<int64_t>& sections, double eps, double offset, bool interleaved) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [gq, gk, gqw, gkw] = rotary_bwd_handle().call(dq, dk, q, k, positions, inv_freq, sections, q_weight, k_weight, eps, offset, interleaved);
+    return {gq, gk, gqw, gkw};
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    refuse_second("rotary");
+    return {};
+  }
+};
+std::tuple<Tensor, Tensor, Tensor, Tensor> rotary_bwd_autograd(const Tensor& dq, const OptTensor& dk, const Tensor& q, const OptTensor& k,
+                                                               const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections,
+                                                               const OptTensor& q_weight, const OptTensor& k_weight, double eps, double offset,
+                                                               bool interleaved) {
+  const Tensor dk_ = value(dk), k_ = value(k), qw = value(q_weight), kw = value(k_weight);
+  if (wants_graph({&dq, &dk_, &q, &k_, &qw, &kw})) {
+    variable_list out =
+        RotaryBackwardOnce::apply(dq, dk, q, k, q_weight, k_weight, positions, inv_freq, sections.vec(), eps, offset, interleaved);
+    return {out[0], out[1], out[2], out[3]};
+  }
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return rotary_bwd_handle().call(dq, dk, q, k, positions, inv_freq, sections, q_weight, k_weight, eps, offset, interleaved);
+}
 
 }  // namespace
 
@@ -536,6 +598,11 @@ TORCH_LIBRARY_IMPL(gnb200, CUDA, m) {
   m.impl("rms_quant", &rms_quant_op);
   m.impl("rotary", &rotary_op);
   m.impl("rotary_bwd", &rotary_bwd_op);
+}
+
+TORCH_LIBRARY_IMPL(gnb200, Autograd, m) {
+  m.impl("rms_bwd", &rms_bwd_autograd);
+  m.impl("rotary_bwd", &rotary_bwd_autograd);
 }
 
 // (registered to refuse with a message of this library)
