@@ -147,3 +147,75 @@ def _rotary_backward(ctx, dq, dk):
 
 
 torch.library.register_autograd("gnb200::rotary", _rotary_backward, setup_context=_rotary_setup_context)
+
+
+# ---------------------------------------------------------------------------------------------- rows in four bits, dropout
+
+
+def _up(n, to):
+    return (n + to - 1) // to * to
+
+
+def _four_like(x, block):
+    c = x.shape[-1]
+    wide, rows = _up(c, 32), x.numel() // c
+    return (x.new_empty(x.shape[:-1] + (wide // 2,), dtype=torch.float4_e2m1fn_x2),
+            x.new_empty((_up(rows, 128), _up(wide // block, 4)), dtype=torch.float8_e4m3fn if block == 16 else torch.float8_e8m0fnu))
+
+
+@torch.library.register_fake("gnb200::quantize_4bit")
+def _quantize_4bit_fake(x, block, scale):
+    return _four_like(x, block)
+
+
+@torch.library.register_fake("gnb200::rms_quant_4bit")
+def _rms_quant_4bit_fake(x, residual, weight, eps, offset, block, scale):
+    s = _none_of(x) if residual is None else torch.empty_like(residual, memory_format=torch.contiguous_format)
+    return _four_like(x, block) + (s,)
+
+
+@torch.library.register_fake("gnb200::dequantize_4bit")
+def _dequantize_4bit_fake(codes, scales, channels, scale, dtype):
+    return codes.new_empty(codes.shape[:-1] + (channels,), dtype=dtype)
+
+
+@torch.library.register_fake("gnb200::linear_4bit")
+def _linear_4bit_fake(codes, scales, weight_codes, weight_scales, scale, weight_scale, bias, dtype):
+    return codes.new_empty(codes.shape[:-1] + (weight_codes.shape[0],), dtype=dtype)
+
+
+@torch.library.register_fake("gnb200::dropout_add")
+def _dropout_add_fake(x, residual, p, seed_at, seed, layer):
+    return torch.empty_like(x, memory_format=torch.contiguous_format, dtype=x.dtype if residual is None else residual.dtype)
+
+
+@torch.library.register_fake("gnb200::dropout_mask")
+def _dropout_mask_fake(t, p, seed_at, seed, layer, dtype):
+    return torch.empty_like(t, memory_format=torch.contiguous_format, dtype=dtype)
+
+
+def _dropout_setup_context(ctx, inputs, output):
+    x, residual, ctx.p, seed_at, ctx.seed, ctx.layer = inputs
+    ctx.x_type, ctx.has_residual = x.dtype, residual is not None
+    ctx.save_for_backward(seed_at)
+
+
+def _dropout_backward(ctx, ds):
+    dx = torch.ops.gnb200.dropout_mask(ds, ctx.p, ctx.saved_tensors[0], ctx.seed, ctx.layer, ctx.x_type) if ctx.needs_input_grad[0] else None
+    return dx, ds if ctx.has_residual else None, None, None, None, None
+
+
+torch.library.register_autograd("gnb200::dropout_add", _dropout_backward, setup_context=_dropout_setup_context)
+
+
+def _mask_setup_context(ctx, inputs, output):
+    t, ctx.p, seed_at, ctx.seed, ctx.layer, _ = inputs
+    ctx.t_type = t.dtype
+    ctx.save_for_backward(seed_at)
+
+
+def _mask_backward(ctx, d):
+    return torch.ops.gnb200.dropout_mask(d, ctx.p, ctx.saved_tensors[0], ctx.seed, ctx.layer, ctx.t_type), None, None, None, None, None
+
+
+torch.library.register_autograd("gnb200::dropout_mask", _mask_backward, setup_context=_mask_setup_context)

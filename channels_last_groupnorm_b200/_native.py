@@ -125,6 +125,21 @@ lib.gnb200_rotary_bwd_workspace_bytes.argtypes = [ctypes.POINTER(RotaryArgs)]
 lib.gnb200_rotary_bwd.restype = _c_int
 lib.gnb200_rotary_bwd.argtypes = [ctypes.POINTER(RotaryArgs)] + [_c_void_p, _c_strides] * 4 + [_c_void_p] * 5 + [ctypes.c_size_t, _c_void_p]
 
+lib.gnb200_4bit_code_bytes.restype = ctypes.c_size_t
+lib.gnb200_4bit_code_bytes.argtypes = [_c_int64, _c_int64]
+lib.gnb200_4bit_scale_bytes.restype = ctypes.c_size_t
+lib.gnb200_4bit_scale_bytes.argtypes = [_c_int64, _c_int64, _c_int]
+lib.gnb200_quantize_4bit.restype = _c_int
+lib.gnb200_quantize_4bit.argtypes = [_c_void_p, _c_int64, _c_int64, _c_int64, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p]
+lib.gnb200_dequantize_4bit.restype = _c_int
+lib.gnb200_dequantize_4bit.argtypes = [_c_void_p, _c_void_p, _c_int64, _c_int64, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p]
+lib.gnb200_rms_fwd_4bit.restype = _c_int
+lib.gnb200_rms_fwd_4bit.argtypes = lib.gnb200_rms_fwd.argtypes[:12] + [_c_int] + [_c_void_p] * 5
+lib.gnb200_linear_4bit.restype = _c_int
+lib.gnb200_linear_4bit.argtypes = [_c_void_p] * 7 + [_c_int64] * 3 + [_c_int] * 3 + [_c_void_p] * 2
+lib.gnb200_dropout_add.restype = _c_int
+lib.gnb200_dropout_add.argtypes = [_c_void_p, _c_void_p, _c_int64, _c_double, _c_void_p, ctypes.c_uint64, ctypes.c_uint64, _c_int, _c_int, _c_void_p, _c_void_p]
+
 
 class Gnb200Error(RuntimeError):
     """A C-ABI call returned a non-zero status."""

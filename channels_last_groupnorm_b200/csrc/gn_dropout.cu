@@ -1,0 +1,157 @@
+// Dropout with the residual's addition, its mask made from a counter wherever it is needed and never stored:
+//
+//   s_i = r_i + (k_i ? x_i / (1 - p) : 0)       in fp32, rounded once;   backward  dx_i = k_i ? ds_i / (1 - p) : 0,  dr = ds
+//   k_i: word i % 4 of Philox 4x32 with ten rounds (Salmon, Moraes, Dror and Shaw, 2011) is at least p 2^32; counter (i / 4, layer), 64 bits each, key the seed
+//
+// i counts the elements in order, so that the mask depends neither on layout nor on the grid.  A dropped element is zero whatever it was.
+#include <algorithm>
+
+#include "../../include/gnb200.h"
+#include "gn_kernels.h"
+#include "gn_tokens.cuh"
+
+namespace gnb200 {
+namespace {
+
+constexpr int VE = 8, kThreads = 256;
+
+struct DropoutArgs {
+  const void *in, *residual;
+  void* out;
+  const unsigned long long* seed_at;  // on the device, or NULL: `seed`
+  unsigned long long seed, layer;
+  long long n;
+  uint32_t least;  // kept from this word on
+  float scale;
+};
+
+// Four words of Philox 4x32-10
+struct Philox {
+  uint32_t k0, k1, l0, l1;
+  __device__ __forceinline__ void words(unsigned long long at, uint32_t (&w)[4]) const {
+    uint32_t a = (uint32_t)at, b = (uint32_t)(at >> 32), c = l0, d = l1, x = k0, y = k1;
+#pragma unroll
+    for (int round = 0; round < 10; ++round) {
+      const unsigned long long left = (unsigned long long)a * 0xD2511F53u, right = (unsigned long long)c * 0xCD9E8D57u;
+      a = (uint32_t)(right >> 32) ^ b ^ x, b = (uint32_t)right;
+      c = (uint32_t)(left >> 32) ^ d ^ y, d = (uint32_t)left;
+      x += 0x9E3779B9u, y += 0xBB67AE85u;
+    }
+    w[0] = a, w[1] = b, w[2] = c, w[3] = d;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&f)[VE]) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+  } else {
+    unpack<T, VE>(load_vec<T, VE>(p), f);
+  }
+}
+
+// VEC: tensors begin on 16 bytes and are taken 8 elements a thread, but for their end; otherwise element by element.
+template <typename Ti, typename Tr, typename To, bool RES, bool VEC>
+__global__ void __launch_bounds__(kThreads) dropout_kernel(const DropoutArgs p) {
+  const Ti* in = static_cast<const Ti*>(p.in);
+  const Tr* res = static_cast<const Tr*>(p.residual);
+  To* out = static_cast<To*>(p.out);
+  const unsigned long long seed = p.seed_at ? *p.seed_at : p.seed;
+  const Philox philox = {(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)p.layer, (uint32_t)(p.layer >> 32)};
+  const long long step = (long long)gridDim.x * kThreads, vectors = (p.n + VE - 1) / VE;
+  for (long long v = (long long)blockIdx.x * kThreads + threadIdx.x; v < vectors; v += step) {
+    const long long first = v * VE;
+    const bool whole = VEC && first + VE <= p.n;
+    float f[VE], r[VE];
+    if (whole) {
+      load8<Ti>(in + first, f);
+      if constexpr (RES) load8<Tr>(res + first, r);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        f[e] = first + e < p.n ? load_param<Ti>(in + first, e) : 0.f;
+        if constexpr (RES) r[e] = first + e < p.n ? load_param<Tr>(res + first, e) : 0.f;
+      }
+    }
+    uint32_t w[2][4];
+    philox.words(2 * v, w[0]);
+    philox.words(2 * v + 1, w[1]);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      const bool kept = w[e / 4][e % 4] >= p.least;
+      if constexpr (RES)
+        f[e] = kept ? fmaf(f[e], p.scale, r[e]) : r[e];
+      else
+        f[e] = kept ? f[e] * p.scale : 0.f;
+    }
+    if (whole) {
+      store_vec<To, VE>(out + first, pack<To, VE>(f));
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+        if (first + e < p.n) out[first + e] = store_param<To>(f[e]);
+    }
+  }
+}
+
+template <typename F>
+cudaError_t with_type(int dtype, F&& f) {
+  if (dtype == GNB200_F32) return f(float());
+  if (dtype == GNB200_F16) return f(__half());
+  return f(__nv_bfloat16());
+}
+bool dtype_ok(int d) { return d == GNB200_F32 || d == GNB200_F16 || d == GNB200_BF16; }
+bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+template <typename Ti, typename To, bool RES>
+cudaError_t launch_dropout(const DropoutArgs& p, cudaStream_t stream) {
+  const auto go = [&](void (*kernel)(const DropoutArgs)) {
+    Residency r = {};
+    const cudaError_t err = residency((const void*)kernel, kThreads, 0, &r);
+    if (err != cudaSuccess) return err;
+    const long long need = ((p.n + VE - 1) / VE + kThreads - 1) / kThreads;
+    kernel<<<(unsigned)std::min<long long>(need, (long long)r.per_sm * r.sms), kThreads, 0, stream>>>(p);
+    return cudaGetLastError();
+  };
+  return on16(p.in) && on16(p.residual) && on16(p.out) ? go(&dropout_kernel<Ti, To, To, RES, true>) : go(&dropout_kernel<Ti, To, To, RES, false>);
+}
+
+}  // namespace
+}  // namespace gnb200
+
+using namespace gnb200;
+
+extern "C" int gnb200_dropout_add(const void* x, const void* residual, int64_t n, double p, const int64_t* seed_at, uint64_t seed, uint64_t layer, int dtype,
+                                  int out_dtype, void* out, void* stream) {
+  const char* name = "gnb200_dropout_add";
+  if (!dtype_ok(dtype) || !dtype_ok(out_dtype)) return report_error(GNB200_ERR_INVALID_ARGUMENT, "%s: unknown dtype code (0=f32, 1=f16, 2=bf16)", name);
+  if (dtype != out_dtype && dtype != GNB200_F32 && out_dtype != GNB200_F32)
+    return report_error(GNB200_ERR_INVALID_ARGUMENT, "%s: the types of the input and the output are the same, or one is float32", name);
+  if (residual && dtype == GNB200_F32 && out_dtype != GNB200_F32)
+    return report_error(GNB200_ERR_INVALID_ARGUMENT, "%s: a residual has the type of x or float32", name);
+  if (n < 0) return report_error(GNB200_ERR_INVALID_ARGUMENT, "%s: the number of elements must not be negative (got %lld)", name, (long long)n);
+  const double word = p * 4294967296.0;
+  if (!(p >= 0.0) || !(word < 4294967295.5)) return report_error(GNB200_ERR_INVALID_ARGUMENT, "%s: p is at least 0 and less than 1 (got %g)", name, p);
+  if (n == 0) return GNB200_OK;
+  if (!x || !out) return report_error(GNB200_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
+  DropoutArgs a = {};
+  a.in = x, a.residual = residual, a.out = out, a.seed_at = reinterpret_cast<const unsigned long long*>(seed_at), a.seed = seed, a.layer = layer, a.n = n;
+  a.least = (uint32_t)(word + 0.5), a.scale = (float)(1.0 / (1.0 - p));
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t err = with_type(dtype, [&](auto ti) {
+    return with_type(out_dtype, [&](auto to) {
+      using Ti = decltype(ti);
+      using To = decltype(to);
+      if constexpr (std::is_same<Ti, To>::value || std::is_same<To, float>::value) {
+        return residual ? launch_dropout<Ti, To, true>(a, s) : launch_dropout<Ti, To, false>(a, s);
+      } else if constexpr (std::is_same<Ti, float>::value) {
+        return launch_dropout<Ti, To, false>(a, s);
+      } else {
+        return cudaErrorInvalidValue;
+      }
+    });
+  });
+  if (err != cudaSuccess) return report_error(GNB200_ERR_CUDA, "%s: CUDA error: %s", name, cudaGetErrorString(err));
+  return GNB200_OK;
+}

@@ -6,10 +6,14 @@
 //
 // rms_norm(x, weight, residual, eps, offset) -> y or (y, sum), rms_quant(x, weight, residual, eps, offset, block, format) ->
 // (codes, scales[, sum]), rotary(q, k, positions, inv_freq, sections, q_weight, k_weight, eps, offset, interleaved) -> (q, k): the same for the
-// operators on token rows; None, for an absent tensor, is an argument like any other there.
+// operators on token rows; None, for an absent tensor, is an argument like any other there.  So are quantize_4bit(x, block, scale),
+// dequantize_4bit(codes, scales, channels, scale, dtype), rms_quant_4bit(x, weight, residual, eps, offset, block, scale),
+// linear_4bit(codes, scales, weight_codes, weight_scales, scale, weight_scale, bias, dtype) and dropout_add(x, residual, p, seed, layer), whose seed
+// is a tensor or a number.
 #include <Python.h>
 
 #include <ATen/PythonTorchFunctionTLS.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -122,10 +126,123 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+bool dtype_of(PyObject* o, at::ScalarType* out) {
+  if (!THPDtype_Check(o)) return false;
+  *out = reinterpret_cast<THPDtype*>(o)->scalar_type;
+  return true;
+}
+
+PyObject* quantize_4bit(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  at::Tensor x, scale, codes, scales;
+  if (nargs != 3 || !exact_tensor(args[0]) || !tensor_or_none(args[0], &x) || !PyLong_CheckExact(args[1]) || !tensor_or_none(args[2], &scale) ||
+      at::impl::torch_function_mode_enabled())
+    Py_RETURN_NONE;
+  const long long block = PyLong_AsLongLong(args[1]);
+  if (PyErr_Occurred()) return nullptr;
+  bool ok = false;
+  {
+    pybind11::gil_scoped_release no_gil;
+    std::tie(codes, scales) = gnb200_ops::quantize_4bit_direct(x, block, scale, &ok);
+  }
+  if (!ok) Py_RETURN_NONE;
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(codes)), THPVariable_Wrap(std::move(scales)));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* dequantize_4bit(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  at::Tensor codes, scales, scale, out;
+  at::ScalarType dtype;
+  if (nargs != 5 || !exact_tensor(args[0]) || !tensor_or_none(args[0], &codes) || !exact_tensor(args[1]) || !tensor_or_none(args[1], &scales) ||
+      !PyLong_CheckExact(args[2]) || !tensor_or_none(args[3], &scale) || !dtype_of(args[4], &dtype) || at::impl::torch_function_mode_enabled())
+    Py_RETURN_NONE;
+  const long long channels = PyLong_AsLongLong(args[2]);
+  if (PyErr_Occurred()) return nullptr;
+  bool ok = false;
+  {
+    pybind11::gil_scoped_release no_gil;
+    out = gnb200_ops::dequantize_4bit_direct(codes, scales, channels, scale, dtype, &ok);
+  }
+  if (!ok) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* rms_quant_4bit(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  at::Tensor x, weight, residual, scale, codes, scales, sum;
+  if (nargs != 7 || !exact_tensor(args[0]) || !tensor_or_none(args[0], &x) || !tensor_or_none(args[1], &weight) ||
+      !tensor_or_none(args[2], &residual) || !PyFloat_CheckExact(args[3]) || !PyFloat_CheckExact(args[4]) || !PyLong_CheckExact(args[5]) ||
+      !tensor_or_none(args[6], &scale) || at::impl::torch_function_mode_enabled())
+    Py_RETURN_NONE;
+  const double eps = PyFloat_AS_DOUBLE(args[3]), offset = PyFloat_AS_DOUBLE(args[4]);
+  const long long block = PyLong_AsLongLong(args[5]);
+  if (PyErr_Occurred()) return nullptr;
+  bool ok = false;
+  {
+    pybind11::gil_scoped_release no_gil;
+    std::tie(codes, scales, sum) = gnb200_ops::rms_quant_4bit_direct(x, weight, residual, eps, offset, block, scale, &ok);
+  }
+  if (!ok) Py_RETURN_NONE;
+  if (!sum.defined()) return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(codes)), THPVariable_Wrap(std::move(scales)));
+  return Py_BuildValue("(NNN)", THPVariable_Wrap(std::move(codes)), THPVariable_Wrap(std::move(scales)), THPVariable_Wrap(std::move(sum)));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* linear_4bit(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  at::Tensor t[7], out;
+  at::ScalarType dtype;
+  if (nargs != 8 || !dtype_of(args[7], &dtype) || at::impl::torch_function_mode_enabled()) Py_RETURN_NONE;
+  for (int i = 0; i < 7; ++i)
+    if ((i < 4 && !exact_tensor(args[i])) || !tensor_or_none(args[i], &t[i])) Py_RETURN_NONE;
+  bool ok = false;
+  {
+    pybind11::gil_scoped_release no_gil;
+    out = gnb200_ops::linear_4bit_direct(t[0], t[1], t[2], t[3], t[4], t[5], t[6], dtype, &ok);
+  }
+  if (!ok) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* dropout_add(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  at::Tensor x, residual, seed_at, out;
+  if (nargs != 5 || !exact_tensor(args[0]) || !tensor_or_none(args[0], &x) || !tensor_or_none(args[1], &residual) || !PyFloat_CheckExact(args[2]) ||
+      !PyLong_CheckExact(args[4]) || at::impl::torch_function_mode_enabled())
+    Py_RETURN_NONE;
+  long long seed = 0;
+  if (PyLong_CheckExact(args[3]))
+    seed = PyLong_AsLongLong(args[3]);
+  else if (args[3] == Py_None || !tensor_or_none(args[3], &seed_at))
+    Py_RETURN_NONE;
+  const long long layer = PyLong_AsLongLong(args[4]);
+  if (PyErr_Occurred()) {  // beyond 64 bits: Python looks at it
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  const double p = PyFloat_AS_DOUBLE(args[2]);
+  bool ok = false;
+  {
+    pybind11::gil_scoped_release no_gil;
+    out = gnb200_ops::dropout_add_direct(x, residual, p, seed_at, seed, layer, &ok);
+  }
+  if (!ok) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef kMethods[] = {{"plain_call", (PyCFunction)(void (*)())plain_call, METH_FASTCALL, nullptr},
                           {"rms_norm", (PyCFunction)(void (*)())rms_norm, METH_FASTCALL, nullptr},
                           {"rms_quant", (PyCFunction)(void (*)())rms_quant, METH_FASTCALL, nullptr},
                           {"rotary", (PyCFunction)(void (*)())rotary, METH_FASTCALL, nullptr},
+                          {"quantize_4bit", (PyCFunction)(void (*)())quantize_4bit, METH_FASTCALL, nullptr},
+                          {"dequantize_4bit", (PyCFunction)(void (*)())dequantize_4bit, METH_FASTCALL, nullptr},
+                          {"rms_quant_4bit", (PyCFunction)(void (*)())rms_quant_4bit, METH_FASTCALL, nullptr},
+                          {"linear_4bit", (PyCFunction)(void (*)())linear_4bit, METH_FASTCALL, nullptr},
+                          {"dropout_add", (PyCFunction)(void (*)())dropout_add, METH_FASTCALL, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "gnb200_python", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

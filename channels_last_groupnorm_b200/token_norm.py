@@ -8,34 +8,14 @@ import torch
 import torch.nn as nn
 
 from . import _native
+from .token_four import rms_norm_quant_4bit
+from .token_rows import check_rows
 
 _rms_norm = _native.python_module.rms_norm
 _rms_quant = _native.python_module.rms_quant
 
 #: 8-bit types of `rms_norm_quant` and their codes in the C ABI
 QUANT_FORMATS = {torch.float8_e4m3fn: 0, torch.int8: 1}
-_TYPES = (torch.float32, torch.float16, torch.bfloat16)
-
-
-def _check(name, x, weight, residual):
-    if not x.is_cuda:
-        raise ValueError("%s: x must be a CUDA tensor; this package has no CPU path" % name)
-    if x.ndim < 1 or x.shape[-1] < 1:
-        raise ValueError("%s: x must have shape (*, channels), got %s" % (name, tuple(x.shape)))
-    if x.dtype not in _TYPES:
-        raise ValueError("%s: x must be float32, float16 or bfloat16, got %s" % (name, x.dtype))
-    if residual is not None:
-        if residual.shape != x.shape or residual.device != x.device:
-            raise ValueError("%s: residual must match x in sizes and device, got %s on %s for %s on %s"
-                             % (name, tuple(residual.shape), residual.device, tuple(x.shape), x.device))
-        if residual.dtype not in (x.dtype, torch.float32):
-            raise ValueError("%s: residual must have the dtype of x or float32, got %s for %s" % (name, residual.dtype, x.dtype))
-    if weight is not None:
-        if weight.shape != x.shape[-1:] or weight.device != x.device:
-            raise ValueError("%s: weight must be a vector of %d elements on the device of x, got %s on %s"
-                             % (name, x.shape[-1], tuple(weight.shape), weight.device))
-        if weight.dtype not in (x.dtype, torch.float32):
-            raise ValueError("%s: weight must have the dtype of x or float32, got %s for %s" % (name, weight.dtype, x.dtype))
 
 
 def rms_norm(x, weight=None, residual=None, eps=1e-6, offset=0.0):
@@ -52,7 +32,7 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6, offset=0.0):
         out = _rms_norm(x, weight, residual, eps, offset)
         if out is not None:
             return out
-    _check("rms_norm", x, weight, residual)
+    check_rows("rms_norm", x, weight, residual)
     if weight is not None:
         weight = weight.contiguous()
     y, s, _ = torch.ops.gnb200.rms_fwd(x, residual, weight, float(eps), float(offset))
@@ -74,7 +54,7 @@ def rms_norm_quant(x, weight=None, residual=None, eps=1e-6, offset=0.0, block=0,
         out = _rms_quant(x, weight, residual, eps, offset, block, QUANT_FORMATS[dtype])
         if out is not None:
             return out
-    _check("rms_norm_quant", x, weight, residual)
+    check_rows("rms_norm_quant", x, weight, residual)
     if block not in (0, 32, 64, 128):
         raise ValueError("rms_norm_quant: block must be 0 (one scale per row), 32, 64 or 128, got %s" % (block,))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
@@ -89,7 +69,7 @@ class RMSNorm(nn.Module):
     """RMSNorm(num_channels, eps=1e-6, offset=0.0, affine=True, device=None, dtype=None)
 
     `forward(x, residual=None)` is `rms_norm`, `quantize(x, residual=None, block=0, dtype=torch.float8_e4m3fn)` is
-    `rms_norm_quant`.  The weight starts so that offset + weight is one.
+    `rms_norm_quant`, `quantize_4bit(x, residual=None, block=16, scale=None)` is `rms_norm_quant_4bit`.  The weight starts so that offset + weight is one.
     """
 
     def __init__(self, num_channels: int, eps=1e-6, offset=0.0, affine=True, device=None, dtype=None):
@@ -119,6 +99,10 @@ class RMSNorm(nn.Module):
     def quantize(self, x, residual=None, block=0, dtype=torch.float8_e4m3fn):
         self._expect(x)
         return rms_norm_quant(x, self.weight, residual, self.eps, self.offset, block, dtype)
+
+    def quantize_4bit(self, x, residual=None, block=16, scale=None):
+        self._expect(x)
+        return rms_norm_quant_4bit(x, self.weight, residual, self.eps, self.offset, block, scale)
 
     def extra_repr(self):
         return "{num_channels}, eps={eps}, offset={offset}, affine={affine}".format(**self.__dict__)

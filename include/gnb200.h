@@ -301,6 +301,43 @@ int gnb200_rotary_bwd(const gnb200_rotary_args* args, const void* dq, const int6
                       void* stream);
 
 /*
+ * Rows in four bits: e2m1 codes, two a byte (the first channel in the low half), with a scale for each block of 16 or 32 channels.
+ *   block 16: a scale s in e4m3 beside a scale g of the whole tensor, one float on the device (NULL: 1; s * g must not be subnormal).  s = max |x| /
+ *     (6 g), at least 2^-9, at most 448, rounded to e4m3; codes are those of x / (s g), product and quotient in fp32 as IEEE rounds them.
+ *   block 32: the scale is the power of two 2^(floor(log2 max |x|) - 2), in e8m0, at least 2^-127; no scale of the tensor (NULL).
+ *   Codes go to the nearest value, ties to the even code, and saturate at 6.  A NaN or an infinity makes the scale of its block NaN.
+ * Codes lie in rows of ceil(C / 32) * 16 bytes (gnb200_4bit_code_bytes for all rows), zeros behind the channels.  Scales lie in tiles of 512 bytes
+ * for 128 rows and 4 blocks, byte (r % 32) * 16 + r % 128 / 32 * 4 + b % 4 of a tile; a row's tiles lie behind one another, then come those of the
+ * next 128 rows; zeros for rows and blocks that are not there (gnb200_4bit_scale_bytes for all of them).  Codes and scales begin on 16 bytes.
+ * gnb200_quantize_4bit: rows of x, x_stride elements apart.  gnb200_dequantize_4bit: contiguous rows of C values code * s * g, rounded once.
+ * gnb200_rms_fwd_4bit: gnb200_rms_fwd (in place as there) with its y, not rounded before, as codes and scales.
+ * gnb200_linear_4bit: out[tokens][features] = sum over channels of x * w, + bias (NULL: none; any of the three types): both operands codes and scales of
+ *   the same block, sums in fp32, one rounding to dtype.  It waits inside the kernel as the group norm does (bounded; see below).
+ */
+size_t gnb200_4bit_code_bytes(int64_t rows, int64_t C);
+size_t gnb200_4bit_scale_bytes(int64_t rows, int64_t C, int block);
+int gnb200_quantize_4bit(const void* x, int64_t x_stride, int64_t rows, int64_t C, int dtype, int block, const float* tensor_scale,
+                         void* codes, void* scales, void* stream);
+int gnb200_dequantize_4bit(const void* codes, const void* scales, int64_t rows, int64_t C, int block, const float* tensor_scale,
+                           int dtype, void* out, void* stream);
+int gnb200_rms_fwd_4bit(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight,
+                        int64_t rows, int64_t C, double eps, double offset, int dtype, int residual_dtype, int weight_dtype,
+                        int block, const float* tensor_scale, void* codes, void* scales, void* sum, void* stream);
+int gnb200_linear_4bit(const void* x_codes, const void* x_scales, const float* x_scale, const void* w_codes, const void* w_scales,
+                       const float* w_scale, const void* bias, int64_t tokens, int64_t features, int64_t channels, int block,
+                       int bias_dtype, int dtype, void* out, void* stream);
+
+/*
+ * Dropout with the residual's addition, over n contiguous elements: out = residual + (kept ? x / (1 - p) : 0) in fp32, rounded once to out's
+ * type, which is the residual's (NULL: none) and that of x or fp32.  Its backward is the same call on the gradient, without a residual (there the
+ * input may be fp32 and the output 16 bits).  Element i is kept where word i % 4 of Philox 4x32 with ten rounds is at least p 2^32: counter
+ * (i / 4, layer), 64 bits each, key the seed, which is *seed_at where that is not NULL (read by the kernel: a captured graph follows it).
+ * 0 <= p < 1.  out may be the buffer of x or of the residual where it has its type.
+ */
+int gnb200_dropout_add(const void* x, const void* residual, int64_t n, double p, const int64_t* seed_at, uint64_t seed,
+                       uint64_t layer, int dtype, int out_dtype, void* out, void* stream);
+
+/*
  * Describes the launch plan chosen for a problem ("fwd fused k=4 cw=64 ..."; the plans are fused,
  * twopass, wave and resident, the last with the plan that takes over where its grid cannot be
  * resident: "fallback=twopass"), for logs, tests and benchmarks.  Writes at most buf_len bytes including the terminating NUL; returns the
