@@ -14,6 +14,7 @@ namespace gnb200 {
 namespace {
 
 constexpr int VE = 8, kThreads = 256;
+constexpr long long kNear = 1ll << 33;  // elements up to which 32 bits count the vectors and the counters, the grid's last steps included
 
 struct DropoutArgs {
   const void *in, *residual;
@@ -25,17 +26,22 @@ struct DropoutArgs {
   float scale;
 };
 
-// Four words of Philox 4x32-10
+// Four words of Philox 4x32-10.  The keys of the rounds are in registers: what is left of a round is two products of 64 bits and two xors.
 struct Philox {
-  uint32_t k0, k1, l0, l1;
-  __device__ __forceinline__ void words(unsigned long long at, uint32_t (&w)[4]) const {
-    uint32_t a = (uint32_t)at, b = (uint32_t)(at >> 32), c = l0, d = l1, x = k0, y = k1;
+  uint32_t k0[10], k1[10], l0, l1;
+  __device__ __forceinline__ Philox(unsigned long long seed, unsigned long long layer) {
+    l0 = (uint32_t)layer, l1 = (uint32_t)(layer >> 32);
+#pragma unroll
+    for (int round = 0; round < 10; ++round) k0[round] = (uint32_t)seed + round * 0x9E3779B9u, k1[round] = (uint32_t)(seed >> 32) + round * 0xBB67AE85u;
+  }
+  template <typename I>  // (of 32 bits: the counter's high word is zero, and with it the first two rounds have half their products from the layer alone)
+  __device__ __forceinline__ void words(I at, uint32_t (&w)[4]) const {
+    uint32_t a = (uint32_t)at, b = sizeof(I) == 8 ? (uint32_t)((unsigned long long)at >> 32) : 0u, c = l0, d = l1;
 #pragma unroll
     for (int round = 0; round < 10; ++round) {
       const unsigned long long left = (unsigned long long)a * 0xD2511F53u, right = (unsigned long long)c * 0xCD9E8D57u;
-      a = (uint32_t)(right >> 32) ^ b ^ x, b = (uint32_t)right;
-      c = (uint32_t)(left >> 32) ^ d ^ y, d = (uint32_t)left;
-      x += 0x9E3779B9u, y += 0xBB67AE85u;
+      a = (uint32_t)(right >> 32) ^ b ^ k0[round], b = (uint32_t)right;
+      c = (uint32_t)(left >> 32) ^ d ^ k1[round], d = (uint32_t)left;
     }
     w[0] = a, w[1] = b, w[2] = c, w[3] = d;
   }
@@ -51,46 +57,60 @@ __device__ __forceinline__ void load8(const T* p, float (&f)[VE]) {
   }
 }
 
-// VEC: tensors begin on 16 bytes and are taken 8 elements a thread, but for their end; otherwise element by element.
-template <typename Ti, typename Tr, typename To, bool RES, bool VEC>
+// acc + x * scale where the word is large enough, else acc; x * scale or zero
+__device__ __forceinline__ float add_kept(float acc, float x, float scale, uint32_t word, uint32_t least) {
+  asm("{\n\t.reg .pred p;\n\tsetp.hs.u32 p, %3, %4;\n\t@p fma.rn.f32 %0, %1, %2, %0;\n\t}" : "+f"(acc) : "f"(x), "f"(scale), "r"(word), "r"(least));
+  return acc;
+}
+
+// VEC: tensors begin on 16 bytes and are taken 8 elements a thread, but for their end; otherwise element by element.  I: an index of vectors and
+// of counters, two a vector.
+template <typename Ti, typename To, bool RES, bool VEC, typename I>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropoutArgs p) {
+  constexpr int AT_ONCE = VEC ? 2 : 1;  // vectors that a thread has under way: four chains of products hide their latency, two did not (bf16 without a residual 78 us)
   const Ti* in = static_cast<const Ti*>(p.in);
-  const Tr* res = static_cast<const Tr*>(p.residual);
+  const To* res = static_cast<const To*>(p.residual);
   To* out = static_cast<To*>(p.out);
-  const unsigned long long seed = p.seed_at ? *p.seed_at : p.seed;
-  const Philox philox = {(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)p.layer, (uint32_t)(p.layer >> 32)};
-  const long long step = (long long)gridDim.x * kThreads, vectors = (p.n + VE - 1) / VE;
-  for (long long v = (long long)blockIdx.x * kThreads + threadIdx.x; v < vectors; v += step) {
-    const long long first = v * VE;
-    const bool whole = VEC && first + VE <= p.n;
-    float f[VE], r[VE];
-    if (whole) {
-      load8<Ti>(in + first, f);
-      if constexpr (RES) load8<Tr>(res + first, r);
-    } else {
+  const Philox philox(p.seed_at ? *p.seed_at : p.seed, p.layer);
+  const I vectors = (I)((p.n + VE - 1) / VE), step = gridDim.x * kThreads;
+  const float scale = p.scale;
+  const uint32_t least = p.least;
+  for (I v = blockIdx.x * kThreads + threadIdx.x; v < vectors; v += AT_ONCE * step) {
+    float f[AT_ONCE][VE], r[AT_ONCE][VE];
+    bool whole[AT_ONCE];
 #pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        f[e] = first + e < p.n ? load_param<Ti>(in + first, e) : 0.f;
-        if constexpr (RES) r[e] = first + e < p.n ? load_param<Tr>(res + first, e) : 0.f;
+    for (int k = 0; k < AT_ONCE; ++k) {
+      const long long first = (long long)(v + k * step) * VE;
+      whole[k] = VEC && first + VE <= p.n;
+      if (whole[k]) {
+        load8<Ti>(in + first, f[k]);
+        if constexpr (RES) load8<To>(res + first, r[k]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          f[k][e] = first + e < p.n ? load_param<Ti>(in + first, e) : 0.f;
+          if constexpr (RES) r[k][e] = first + e < p.n ? load_param<To>(res + first, e) : 0.f;
+        }
       }
     }
-    uint32_t w[2][4];
-    philox.words(2 * v, w[0]);
-    philox.words(2 * v + 1, w[1]);
+    uint32_t w[AT_ONCE][2][4];
 #pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      const bool kept = w[e / 4][e % 4] >= p.least;
-      if constexpr (RES)
-        f[e] = kept ? fmaf(f[e], p.scale, r[e]) : r[e];
-      else
-        f[e] = kept ? f[e] * p.scale : 0.f;
+    for (int k = 0; k < AT_ONCE; ++k) {
+      philox.words<I>(2 * (v + k * step), w[k][0]);
+      philox.words<I>(2 * (v + k * step) + 1, w[k][1]);
     }
-    if (whole) {
-      store_vec<To, VE>(out + first, pack<To, VE>(f));
-    } else {
 #pragma unroll
-      for (int e = 0; e < VE; ++e)
-        if (first + e < p.n) out[first + e] = store_param<To>(f[e]);
+    for (int k = 0; k < AT_ONCE; ++k) {
+      const long long first = (long long)(v + k * step) * VE;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) f[k][e] = add_kept(RES ? r[k][e] : 0.f, f[k][e], scale, w[k][e / 4][e % 4], least);
+      if (whole[k]) {
+        store_vec<To, VE>(out + first, pack<To, VE>(f[k]));
+      } else {
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+          if (first + e < p.n) out[first + e] = store_param<To>(f[k][e]);
+      }
     }
   }
 }
@@ -114,7 +134,9 @@ cudaError_t launch_dropout(const DropoutArgs& p, cudaStream_t stream) {
     kernel<<<(unsigned)std::min<long long>(need, (long long)r.per_sm * r.sms), kThreads, 0, stream>>>(p);
     return cudaGetLastError();
   };
-  return on16(p.in) && on16(p.residual) && on16(p.out) ? go(&dropout_kernel<Ti, To, To, RES, true>) : go(&dropout_kernel<Ti, To, To, RES, false>);
+  const bool vec = on16(p.in) && on16(p.residual) && on16(p.out);
+  if (p.n < kNear) return vec ? go(&dropout_kernel<Ti, To, RES, true, uint32_t>) : go(&dropout_kernel<Ti, To, RES, false, uint32_t>);
+  return vec ? go(&dropout_kernel<Ti, To, RES, true, unsigned long long>) : go(&dropout_kernel<Ti, To, RES, false, unsigned long long>);
 }
 
 }  // namespace

@@ -1,8 +1,8 @@
 // Rows to four bits and back, and the root-mean-square norm with the residual's addition straight into four bits (formulas and layout:
 // gn_four.cuh; the norm is that of gn_rms.cu: s = x + r in fp32, y = s * rsqrt(mean(s^2) + eps) * (offset + w), y not rounded before its codes).
 //
-// A lane holds 8 channels, neighbouring lanes a block: its largest magnitude by shuffles, one scale, 4 bytes of codes a lane; the scales of
-// four blocks become one word.
+// A lane holds 16 channels: a block of 16, or half of one of 32, whose largest magnitude a shuffle completes; 8 bytes of codes a lane; the scales
+// of four blocks become one word.
 #include <algorithm>
 
 #include "../../include/gnb200.h"
@@ -12,7 +12,9 @@
 namespace gnb200 {
 namespace {
 
-constexpr int VE = 8;  // channels of a lane
+constexpr int VE = 16;  // channels of a lane
+template <int BLOCK>
+constexpr int kLanes = BLOCK / VE;  // lanes of a block
 
 struct FourRows {
   uint8_t *codes, *scales;
@@ -24,94 +26,178 @@ struct FourRows {
 // ---------------------------------------------------------------------------------------------
 // Codes and scales
 // ---------------------------------------------------------------------------------------------
-// A code is that of the fp32 quotient y / d, as a division rounds it: with 16-bit inputs y / d lies midway between two codes often enough that
-// a quotient one unit off shows.  The reciprocal is the correctly rounded one (a Newton step from the hardware's), the quotient is corrected by
-// its remainder (Markstein's theorem).
+// Quotients are those of a division: with 16-bit inputs y / d lies midway between two codes often enough that a quotient one unit off shows.  The
+// reciprocal is the correctly rounded one (a Newton step from the hardware's), a quotient is corrected by its remainder (Markstein's theorem).
+__device__ __forceinline__ float reciprocal(float d) {
+  float near;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(near) : "f"(d));
+  return fmaf(fmaf(-d, near, 1.f), near, near);
+}
+__device__ __forceinline__ float scale_value(uint32_t byte, int block) {
+  if (block == 16) return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
+  return byte == 0xff ? __uint_as_float(0x7fc00000u) : byte == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);  // (2^-127 is subnormal)
+}
+// The tensor's scale and what is made of it once
+struct TensorScale {
+  float g, six, inverse;  // 6 g and its reciprocal
+  __device__ __forceinline__ TensorScale(const float* at) {
+    g = at ? *at : 1.f;
+    six = 6.f * g;
+    inverse = reciprocal(six);
+  }
+};
 struct Step {
   float value, inverse;
   uint32_t byte;
 };
 template <int BLOCK>
-__device__ __forceinline__ Step step_of(uint32_t most, float g, float six_g) {
+__device__ __forceinline__ Step step_of(float most, const TensorScale& t) {
   Step step;
-  const bool finite = most < 0x7f800000u;
+  const bool finite = most < __uint_as_float(0x7f800000u);  // (no NaN either)
   if constexpr (BLOCK == 16) {
-    const float s = fmaxf(__fdiv_rn(__uint_as_float(most), six_g), 0.001953125f);
+    const float q = most * t.inverse;
+    const float s = q >= 448.f ? 448.f : fmaxf(fmaf(-t.inverse, fmaf(q, t.six, -most), q), 0.001953125f);
     step.byte = finite ? __nv_cvt_float_to_fp8(s, __NV_SATFINITE, __NV_E4M3) : 0x7fu;
-    step.value = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)step.byte, __NV_E4M3))) * g;
-    float near;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(near) : "f"(step.value));
-    step.inverse = fmaf(fmaf(-step.value, near, 1.f), near, near);
+    step.value = scale_value(step.byte, 16) * t.g;
+    step.inverse = reciprocal(step.value);
   } else {
-    const int e = max((int)(most >> 23) - 2, 0);
+    const int e = max((int)(__float_as_uint(most) >> 23) - 2, 0);
     step.byte = finite ? (uint32_t)e : 0xffu;
     step.value = 0.f;  // (a product with the inverse, a power of two, is the quotient)
     step.inverse = __uint_as_float((uint32_t)(254 - min(e, 252)) << 23);
   }
   return step;
 }
+// 8 codes
 template <int BLOCK>
-__device__ __forceinline__ uint32_t codes_of(const float (&y)[VE], const Step& step) {
-  uint32_t word = 0;
+__device__ __forceinline__ uint32_t codes_of(const float* y, const Step& step) {
+  float q[8];
 #pragma unroll
-  for (int e = 0; e < VE; e += 2) {
-    float q0, q1;
-    mul2(q0, q1, y[e], y[e + 1], step.inverse, step.inverse);
+  for (int e = 0; e < 8; e += 2) {
+    mul2(q[e], q[e + 1], y[e], y[e + 1], step.inverse, step.inverse);
     if constexpr (BLOCK == 16) {
       float r0, r1;
-      fma2(r0, r1, q0, q1, step.value, step.value, -y[e], -y[e + 1]);
-      fma2(q0, q1, r0, r1, -step.inverse, -step.inverse, q0, q1);
+      fma2(r0, r1, q[e], q[e + 1], step.value, step.value, -y[e], -y[e + 1]);
+      fma2(q[e], q[e + 1], r0, r1, -step.inverse, -step.inverse, q[e], q[e + 1]);
     }
-    word |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(q0, q1), __NV_E2M1, cudaRoundNearest) << (4 * e);
   }
+  uint32_t word;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(word)
+      : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
   return word;
 }
-// Codes of the 8 channels y of vector v of a row (zeros where it has none) and the scales that its lanes share; by whole warps.
+// Codes of the 16 channels y of vector v of a row (zeros where it has none) and the scales that its lanes share; by whole warps.
 template <int BLOCK>
-__device__ __forceinline__ void put(const FourRows& p, long long row, int v, bool live, const float (&y)[VE], float g, float six_g) {
-  constexpr int LANES = BLOCK / VE;
+__device__ __forceinline__ void put(const FourRows& p, long long row, int v, bool live, const float (&y)[VE], const TensorScale& t) {
+  constexpr int LANES = kLanes<BLOCK>;
   float most = 0.f;
 #pragma unroll
   for (int e = 0; e < VE; ++e) most = larger(most, fabsf(y[e]));
-  const Step step = step_of<BLOCK>(lanes_max(magnitude(most), LANES), g, six_g);
-  const uint32_t word = codes_of<BLOCK>(y, step);
+  if constexpr (LANES > 1) most = larger(most, __shfl_xor_sync(0xffffffffu, most, 1));
+  const Step step = step_of<BLOCK>(most, t);
+  const uint2 words = make_uint2(codes_of<BLOCK>(y, step), codes_of<BLOCK>(y + 8, step));
   const bool inside = v * VE < p.wide;
-  if (live && inside) *reinterpret_cast<uint32_t*>(p.codes + (row * (p.wide / VE) + v) * 4) = word;
+  if (live && inside) *reinterpret_cast<uint2*>(p.codes + (row * (p.wide / VE) + v) * 8) = words;
   const int block = v / LANES;
   uint32_t scales = inside ? step.byte << (8 * (block & 3)) : 0;
   scales |= __shfl_xor_sync(0xffffffffu, scales, LANES);
   scales |= __shfl_xor_sync(0xffffffffu, scales, 2 * LANES);
-  if (live && v % (4 * LANES) == 0) *reinterpret_cast<uint32_t*>(p.scales + four_scale_at(row, block >> 2, p.tiles)) = scales;
+  if (live && v % (4 * LANES) == 0) {
+    uint32_t* const at = reinterpret_cast<uint32_t*>(p.scales + four_scale_at(row, block >> 2, p.tiles));
+    at[0] = scales;
+    // zeros for the rows of this lane's 16 bytes that are not there
+    if (row + 32 >= p.rows)
+      for (int k = 1; k < 4 - (int)(row >> 5 & 3); ++k) at[k] = 0;
+  }
 }
-// The scales of rows that fill up the last tile, by all threads of the grid.
-__device__ __forceinline__ void clear_behind(const FourRows& p, long long thread, long long threads) {
-  const int behind = (int)(-p.rows & 127);
-  for (long long i = thread; i < (long long)behind * p.tiles; i += threads)
-    *reinterpret_cast<uint32_t*>(p.scales + four_scale_at(p.rows + i % behind, i / behind, p.tiles)) = 0;
+// The scales of the lanes of the last tile that have no row at all, by all threads of the grid.
+__device__ __forceinline__ void clear_behind(const FourRows& p, unsigned thread, unsigned threads) {
+  const unsigned rows = (unsigned)(p.rows & 127);
+  if (rows == 0 || rows >= 32) return;
+  uint8_t* const last = p.scales + (p.rows >> 7) * p.tiles * kScaleTile;
+  const unsigned lanes = 32 - rows, all = lanes * (unsigned)p.tiles;
+  for (unsigned i = thread; i < all; i += threads) *reinterpret_cast<uint4*>(last + (size_t)(i / lanes) * kScaleTile + (rows + i % lanes) * 16) = make_uint4(0, 0, 0, 0);
 }
 
+// ---------------------------------------------------------------------------------------------
+// 16 channels of a row
+// ---------------------------------------------------------------------------------------------
+// A tensor's bytes: vectors that reach beyond a row may be read as long as they stay in these.
+struct Bounds {
+  const char *begin, *end;
+};
+// Aligned (VEC, rows of whole 8 channels), or from any address: then the 16-byte vectors that the channels lie in are read whole and shifted into place,
+// three of them for 16 bits where element by element it were 16 loads (9001 x 1111 bf16 to four bits 66 us so); element by element at the ends of a
+// row and where a vector would reach out of the tensor.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* row, int v, int C, float (&f)[VE]) {
+__device__ __forceinline__ void load16(const T* row, int v, int C, const Bounds& bounds, float (&f)[VE]) {
+  constexpr int N = VE * (int)sizeof(T) / 16;  // vectors
+  const T* at = row + v * VE;
   if constexpr (VEC) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = reinterpret_cast<const float4*>(row)[2 * v], b = reinterpret_cast<const float4*>(row)[2 * v + 1];
-      f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-    } else {
-      unpack<T, VE>(load_vec<T, VE>(row + v * VE), f);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      float part[16 / sizeof(T)];
+      if (v * VE + k * (int)(16 / sizeof(T)) < C) {
+        unpack16<T, 16 / sizeof(T)>(reinterpret_cast<const uint4*>(at)[k], part);
+      } else {
+#pragma unroll
+        for (int e = 0; e < (int)(16 / sizeof(T)); ++e) part[e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < (int)(16 / sizeof(T)); ++e) f[k * (16 / sizeof(T)) + e] = part[e];
     }
   } else {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(at);
+    const char* const from = reinterpret_cast<const char*>(a & ~(uintptr_t)15);
+    if (v * VE + VE <= C && from >= bounds.begin && from + 16 * (N + 1) <= bounds.end) {
+      uint32_t w[4 * (N + 1)];
 #pragma unroll
-    for (int e = 0; e < VE; ++e) f[e] = v * VE + e < C ? load_param<T>(row, v * VE + e) : 0.f;
+      for (int k = 0; k <= N; ++k) {
+        const uint4 q = reinterpret_cast<const uint4*>(from)[k];
+        w[4 * k] = q.x, w[4 * k + 1] = q.y, w[4 * k + 2] = q.z, w[4 * k + 3] = q.w;
+      }
+      const bool two = a & 8, one = a & 4, half = a & 2;
+#pragma unroll
+      for (int k = 0; k < 4 * N + 2; ++k) w[k] = two ? w[k + 2] : w[k];
+#pragma unroll
+      for (int k = 0; k < 4 * N + 1; ++k) w[k] = one ? w[k + 1] : w[k];
+#pragma unroll
+      for (int k = 0; k < 4 * N; ++k) {
+        if constexpr (sizeof(T) == 4) {
+          f[k] = __uint_as_float(w[k]);
+        } else {
+          const uint32_t pair = __funnelshift_r(w[k], w[k + 1], half ? 16 : 0);
+          float part[2];
+          unpack<T, 2>(*reinterpret_cast<const Pack<T, 2>*>(&pair), part);
+          f[2 * k] = part[0], f[2 * k + 1] = part[1];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) f[e] = v * VE + e < C ? load_param<T>(at, e) : 0.f;
+    }
   }
 }
 template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* row, int v, int C, const float (&f)[VE]) {
-  if constexpr (VEC) {
-    store_vec<T, VE>(row + v * VE, pack<T, VE>(f));
-  } else {
+__device__ __forceinline__ void store16(T* row, int v, int C, const float (&f)[VE]) {
+  constexpr int W = 16 / sizeof(T);
+  T* at = row + v * VE;
 #pragma unroll
-    for (int e = 0; e < VE; ++e)
-      if (v * VE + e < C) row[v * VE + e] = store_param<T>(f[e]);
+  for (int k = 0; k < VE / W; ++k) {
+    float part[W];
+#pragma unroll
+    for (int e = 0; e < W; ++e) part[e] = f[k * W + e];
+    if constexpr (VEC) {
+      if (v * VE + k * W < C) store_vec<T, W>(at + k * W, pack<T, W>(part));
+    } else {
+#pragma unroll
+      for (int e = 0; e < W; ++e)
+        if (v * VE + k * W + e < C) at[k * W + e] = store_param<T>(part[e]);
+    }
   }
 }
 __device__ __forceinline__ void zero(float (&f)[VE]) {
@@ -124,55 +210,91 @@ __device__ __forceinline__ void zero(float (&f)[VE]) {
 // ---------------------------------------------------------------------------------------------
 constexpr int kThreads = 256;
 
-// `lanes` (a power of two) threads share a row's piece; the grid's second axis shares a row out.
+// 2^shift threads share a row's piece; the grid's second axis shares a row out.
 template <typename T, int BLOCK, bool VEC>
-__global__ void __launch_bounds__(kThreads) quantize_kernel(const T* x, long long x_stride, const FourRows p, int lanes) {
+__global__ void __launch_bounds__(kThreads) quantize_kernel(const T* x, long long x_stride, const Bounds bounds, const FourRows p, int shift) {
+  constexpr int AT_ONCE = sizeof(T) == 2 ? 2 : 1;  // vectors that a thread has under way
   grid_dep_launch_dependents();
-  const int per_cta = kThreads / lanes, lane = threadIdx.x % lanes, vectors = p.tiles * 4 * (BLOCK / VE), step = gridDim.y * lanes;
-  const float g = BLOCK == 16 && p.tensor_scale ? *p.tensor_scale : 1.f, six_g = 6.f * g;
+  const int lanes = 1 << shift, per_cta = kThreads >> shift, lane = threadIdx.x & (lanes - 1), vectors = p.tiles * 4 * kLanes<BLOCK>, step = gridDim.y << shift;
+  const TensorScale t(BLOCK == 16 ? p.tensor_scale : nullptr);
   for (long long base = (long long)blockIdx.x * per_cta; base < p.rows; base += (long long)gridDim.x * per_cta) {
-    const long long row = base + threadIdx.x / lanes;
+    const long long row = base + (threadIdx.x >> shift);
     const bool live = row < p.rows;
     const T* from = x + row * x_stride;
-    for (int first = blockIdx.y * lanes; first < vectors; first += 2 * step) {
-      float y[2][VE];
+    for (int first = blockIdx.y << shift; first < vectors; first += AT_ONCE * step) {
+      float y[AT_ONCE][VE];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+      for (int k = 0; k < AT_ONCE; ++k) {
         zero(y[k]);
         const int v = first + k * step + lane;
-        if (live && v * VE < p.C) load8<T, VEC>(from, v, p.C, y[k]);
+        if (live && v * VE < p.C) load16<T, VEC>(from, v, p.C, bounds, y[k]);
       }
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+      for (int k = 0; k < AT_ONCE; ++k) {
         const int v = first + k * step + lane;
-        put<BLOCK>(p, row, v, live && v < vectors, y[k], g, six_g);
+        put<BLOCK>(p, row, v, live && v < vectors, y[k], t);
       }
     }
   }
-  clear_behind(p, ((long long)blockIdx.y * gridDim.x + blockIdx.x) * kThreads + threadIdx.x, (long long)gridDim.x * gridDim.y * kThreads);
+  clear_behind(p, (blockIdx.y * gridDim.x + blockIdx.x) * kThreads + threadIdx.x, gridDim.x * gridDim.y * kThreads);
 }
 
-__device__ __forceinline__ float scale_value(uint32_t byte, int block) {
-  if (block == 16) return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
-  return byte == 0xff ? __uint_as_float(0x7fc00000u) : byte == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);  // (2^-127 is subnormal)
-}
-template <typename T, int BLOCK, bool VEC>
-__global__ void __launch_bounds__(kThreads) dequantize_kernel(const FourRows p, T* out, int lanes) {
-  const int per_cta = kThreads / lanes, lane = threadIdx.x % lanes, step = gridDim.y * lanes;
-  const float g = BLOCK == 16 && p.tensor_scale ? *p.tensor_scale : 1.f;
-  for (long long row = (long long)blockIdx.x * per_cta + threadIdx.x / lanes; row < p.rows; row += (long long)gridDim.x * per_cta) {
-    for (int v = blockIdx.y * lanes + lane; v * VE < p.C; v += step) {
-      const uint32_t word = *reinterpret_cast<const uint32_t*>(p.codes + (row * (p.wide / VE) + v) * 4);
-      const int block = v / (BLOCK / VE);
-      const float scale = scale_value(p.scales[four_scale_at(row, block >> 2, p.tiles) + (block & 3)], BLOCK);
-      float f[VE];
+__device__ __forceinline__ void values_of(uint32_t word, float (&f)[8]) {
 #pragma unroll
-      for (int e = 0; e < VE; e += 2) {
-        const float2 two = __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)(word >> (4 * e)), __NV_E2M1)));
-        f[e] = two.x * scale * g;
-        f[e + 1] = two.y * scale * g;
+  for (int e = 0; e < 8; e += 2) {
+    const float2 two = __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)(word >> (4 * e)), __NV_E2M1)));
+    f[e] = two.x, f[e + 1] = two.y;
+  }
+}
+// VEC: output rows of whole 16-byte vectors on their boundaries.
+template <typename T, int BLOCK, bool VEC>
+__global__ void __launch_bounds__(kThreads) dequantize_kernel(const FourRows p, T* out, int shift) {
+  const int lanes = 1 << shift, per_cta = kThreads >> shift, lane = threadIdx.x & (lanes - 1), step = gridDim.y << shift;
+  const float g = BLOCK == 16 && p.tensor_scale ? *p.tensor_scale : 1.f;
+  const auto scale_at = [&](long long row, int channel) {
+    const int block = channel / BLOCK;
+    return scale_value(p.scales[four_scale_at(row, block >> 2, p.tiles) + (block & 3)], BLOCK);
+  };
+  for (long long row = (long long)blockIdx.x * per_cta + (threadIdx.x >> shift); row < p.rows; row += (long long)gridDim.x * per_cta) {
+    const uint8_t* const codes = p.codes + row * (p.wide / 2);
+    T* const to = out + row * p.C;
+    if constexpr (VEC) {
+      for (int v = (blockIdx.y << shift) + lane; v * VE < p.C; v += step) {
+        const uint2 words = *reinterpret_cast<const uint2*>(codes + v * 8);
+        const float scale = scale_at(row, v * VE);
+        float f[VE], low[8], high[8];
+        values_of(words.x, low);
+        values_of(words.y, high);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = low[e], f[8 + e] = high[e];
+        scale_each(f, scale);
+        if constexpr (BLOCK == 16) scale_each(f, g);
+        store16<T, true>(to, v, p.C, f);
       }
-      store8<T, VEC>(out + row * p.C, v, p.C, f);
+    } else {
+      // in the frame of the output's 16-byte vectors, whose first and last have elements of the rows beside this one; 8 codes from any one on
+      constexpr int W = 16 / sizeof(T);
+      const int skew = (int)(reinterpret_cast<uintptr_t>(to) / sizeof(T) % W), count = (p.C + skew + W - 1) / W, words = p.wide / 8;
+      for (int v = (blockIdx.y << shift) + lane; v < count; v += step) {
+        const int c = v * W - skew, at = c < 0 ? -1 : c / 8;
+        const uint32_t* const w = reinterpret_cast<const uint32_t*>(codes);
+        const uint32_t below = at >= 0 ? w[at] : 0, above = at + 1 < words ? w[at + 1] : 0;
+        float f[8];
+        values_of(__funnelshift_r(below, above, 4 * (c & 7)), f);
+        const int border = ((c + W - 1) / BLOCK) * BLOCK;  // channels from here on have the last one's scale
+        const float last = scale_at(row, min(c + W - 1, p.C - 1)), first = c >= 0 && c < border ? scale_at(row, c) : last;
+        const bool whole = c >= 0 && c + W <= p.C;
+        float o[W];
+#pragma unroll
+        for (int e = 0; e < W; ++e) o[e] = f[e] * (c + e < border ? first : last) * g;
+        if (whole) {
+          store_vec<T, W>(to + c, pack<T, W>(o));
+        } else {
+#pragma unroll
+          for (int e = 0; e < W; ++e)
+            if ((unsigned)(c + e) < (unsigned)p.C) to[c + e] = store_param<T>(o[e]);
+        }
+      }
     }
   }
 }
@@ -184,19 +306,22 @@ struct NormArgs {
   const void *x, *residual, *weight;
   void* sum;
   long long x_stride, r_stride;
+  Bounds x_bounds, r_bounds;
   int w_dtype;
   float eps, offset, inv_c;
 };
 
-// (offset + w) of 8 channels, from addresses on 16 bytes (VEC) or any
+// (offset + w) of 16 channels, from addresses on 16 bytes (VEC) or any
 template <bool VEC>
-__device__ __forceinline__ void weight8(const NormArgs& a, int v, int C, float (&w)[VE]) {
+__device__ __forceinline__ void weight16(const NormArgs& a, int v, int C, float (&w)[VE]) {
   if constexpr (VEC) {
-    if (a.w_dtype == 0) {
-      load8<float, true>(static_cast<const float*>(a.weight), v, C, w);
-    } else {
-      params_at<VE>(a.weight, a.w_dtype, (long long)v * VE, w);
-    }
+    const Bounds none = {};
+    if (a.w_dtype == 0)
+      load16<float, true>(static_cast<const float*>(a.weight), v, C, none, w);
+    else if (a.w_dtype == 1)
+      load16<__half, true>(static_cast<const __half*>(a.weight), v, C, none, w);
+    else
+      load16<__nv_bfloat16, true>(static_cast<const __nv_bfloat16*>(a.weight), v, C, none, w);
   } else {
 #pragma unroll
     for (int e = 0; e < VE; ++e) w[e] = v * VE + e < C ? param_at(a.weight, a.w_dtype, v * VE + e, 1.f) : 0.f;
@@ -207,25 +332,24 @@ __device__ __forceinline__ void weight8(const NormArgs& a, int v, int C, float (
 
 // A row to a warp (WARP) or a CTA, V vectors a thread in registers; V = 0: rows of any length, read twice.
 template <typename Tx, typename Ts, int BLOCK, int V, bool WARP, bool VEC>
-__global__ void __launch_bounds__(WARP ? 128 : 1024) norm_kernel(const NormArgs a, const FourRows p) {
+__global__ void __launch_bounds__(WARP ? 128 : V == 1 ? 512 : 1024) norm_kernel(const NormArgs a, const FourRows p) {
   constexpr int HELD = V > 0 ? V : 1;
   __shared__ TeamSlots slots;
   grid_dep_launch_dependents();
   const int threads = WARP ? 32 : (int)blockDim.x, at = WARP ? (int)threadIdx.x & 31 : (int)threadIdx.x;
   const long long row = WARP ? (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
   const bool live = row < p.rows;
-  const int vectors = p.tiles * 4 * (BLOCK / VE);
-  const float g = BLOCK == 16 && p.tensor_scale ? *p.tensor_scale : 1.f, six_g = 6.f * g;
+  const int vectors = p.tiles * 4 * kLanes<BLOCK>;
   const Tx* x = static_cast<const Tx*>(a.x) + row * a.x_stride;
   const Ts* r = a.residual ? static_cast<const Ts*>(a.residual) + row * a.r_stride : nullptr;
   if constexpr (!WARP) clear<false>(slots, threads, 0, at);
   auto sum_of = [&](int v, float (&s)[VE]) {
     zero(s);
     if (live && v * VE < p.C) {
-      load8<Tx, VEC>(x, v, p.C, s);
+      load16<Tx, VEC>(x, v, p.C, a.x_bounds, s);
       if (r) {
         float f[VE];
-        load8<Ts, VEC>(r, v, p.C, f);
+        load16<Ts, VEC>(r, v, p.C, a.r_bounds, f);
         add_each(s, f);
       }
     }
@@ -237,7 +361,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_kernel(const NormArgs 
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       const int v = at + k * threads;
-      if (r && live && v * VE < p.C) store8<Ts, VEC>(static_cast<Ts*>(a.sum) + row * p.C, v, p.C, s[k]);
+      if (r && live && v * VE < p.C) store16<Ts, VEC>(static_cast<Ts*>(a.sum) + row * p.C, v, p.C, s[k]);
       dot_each(sq, s[k], s[k]);
     }
   } else {
@@ -246,6 +370,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_kernel(const NormArgs 
       dot_each(sq, s[0], s[0]);
     }
   }
+  const TensorScale t(BLOCK == 16 ? p.tensor_scale : nullptr);
   int turn = 0;
   const float all = WARP ? lanes_sum(sq[0] + sq[1], 32) : team_sum<false>(sq[0] + sq[1], slots, turn, threads, 0);
   const float rstd = __frsqrt_rn(fmaf(all, a.inv_c, a.eps));
@@ -254,16 +379,16 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_kernel(const NormArgs 
       scale_each(y, rstd);
       if (a.weight) {
         float w[VE];
-        weight8<VEC>(a, v, p.C, w);
+        weight16<VEC>(a, v, p.C, w);
         mul_each(y, w);
       }
-    }
-    if constexpr (!VEC) {  // (behind the row a NaN rstd would leave NaN in the zeros)
+      if (v * VE + VE > p.C) {  // (behind the row a NaN rstd would leave NaN in the zeros)
 #pragma unroll
-      for (int e = 0; e < VE; ++e)
-        if (v * VE + e >= p.C) y[e] = 0.f;
+        for (int e = 0; e < VE; ++e)
+          if (v * VE + e >= p.C) y[e] = 0.f;
+      }
     }
-    put<BLOCK>(p, row, v, live && v < vectors, y, g, six_g);
+    put<BLOCK>(p, row, v, live && v < vectors, y, t);
   };
   if constexpr (V > 0) {
 #pragma unroll
@@ -271,11 +396,11 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_kernel(const NormArgs 
   } else {
     for (int first = 0; first < vectors; first += threads) {
       sum_of(first + at, s[0]);  // (the last look at these: the sum may be the residual's own buffer)
-      if (r && (first + at) * VE < p.C) store8<Ts, VEC>(static_cast<Ts*>(a.sum) + row * p.C, first + at, p.C, s[0]);
+      if (r && (first + at) * VE < p.C) store16<Ts, VEC>(static_cast<Ts*>(a.sum) + row * p.C, first + at, p.C, s[0]);
       finish(first + at, s[0]);
     }
   }
-  clear_behind(p, (long long)blockIdx.x * blockDim.x + threadIdx.x, (long long)gridDim.x * blockDim.x);
+  clear_behind(p, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -298,9 +423,13 @@ cudaError_t with_block(int block, F&& f) {
 bool dtype_ok(int d) { return d == GNB200_F32 || d == GNB200_F16 || d == GNB200_BF16; }
 int size_of(int dtype) { return dtype == GNB200_F32 ? 4 : 2; }
 bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+Bounds bounds_of(const void* p, int64_t rows, int64_t stride, int64_t C, int size) {
+  const char* const begin = static_cast<const char*>(p);
+  return p && stride >= 0 ? Bounds{begin, begin + ((rows - 1) * stride + C) * size} : Bounds{};
+}
 
 struct Shares {
-  int lanes;
+  int shift;
   dim3 grid;
 };
 // Lanes of a row's piece: a row's vectors where they are few, a warp's where there are rows enough to fill the GPU with warps, otherwise the
@@ -310,11 +439,11 @@ cudaError_t share_out(int64_t rows, int64_t vectors, int least, const void* kern
   const cudaError_t err = residency(kernel, kThreads, 0, &r);
   if (err != cudaSuccess) return err;
   const int64_t resident = (int64_t)r.per_sm * r.sms;
-  int lanes = least;
-  const int most = rows * 32 >= resident * kThreads ? 32 : kThreads;
-  while (lanes < most && lanes < vectors) lanes *= 2;
-  const int64_t need = (rows + kThreads / lanes - 1) / (kThreads / lanes), pieces = (vectors + lanes - 1) / lanes;
-  out->lanes = lanes;
+  const int most = rows * 32 >= resident * kThreads ? 5 : 8;
+  int shift = 0;
+  while (1 << shift < least || (shift < most && 1 << shift < vectors)) ++shift;
+  const int64_t need = (rows + (kThreads >> shift) - 1) / (kThreads >> shift), pieces = (vectors + (1 << shift) - 1) >> shift;
+  out->shift = shift;
   out->grid = dim3((unsigned)std::min(need, resident), (unsigned)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(pieces, 65535), resident / need)));
   return cudaSuccess;
 }
@@ -362,7 +491,8 @@ int gnb200_quantize_4bit(const void* x, int64_t x_stride, int64_t rows, int64_t 
   if (!x || !codes || !scales) return report_error(GNB200_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
   if (!on16(codes) || !on16(scales)) return report_error(GNB200_ERR_INVALID_ARGUMENT, "%s: codes and scales begin on 16 bytes", name);
   const FourRows p = four_rows(rows, C, block, tensor_scale, codes, scales);
-  const bool vec = on16(x) && C % VE == 0 && (rows == 1 || x_stride * size_of(dtype) % 16 == 0);
+  const int width = 16 / size_of(dtype);
+  const bool vec = on16(x) && C % width == 0 && (rows == 1 || x_stride % width == 0);
   return launched(name, with_type(dtype, [&](auto t) {
     using T = decltype(t);
     return with_block(block, [&](auto b) {
@@ -370,9 +500,9 @@ int gnb200_quantize_4bit(const void* x, int64_t x_stride, int64_t rows, int64_t 
         constexpr int BLOCK = decltype(b)::value;
         auto kernel = &quantize_kernel<T, BLOCK, decltype(v)::value>;
         Shares s;
-        const cudaError_t err = share_out(rows, (int64_t)p.tiles * 4 * (BLOCK / VE), 4 * (BLOCK / VE), (const void*)kernel, &s);
+        const cudaError_t err = share_out(rows, (int64_t)p.tiles * 4 * kLanes<BLOCK>, 4 * kLanes<BLOCK>, (const void*)kernel, &s);
         if (err != cudaSuccess) return err;
-        kernel<<<s.grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const T*>(x), x_stride, p, s.lanes);
+        kernel<<<s.grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const T*>(x), x_stride, bounds_of(x, rows, x_stride, C, sizeof(T)), p, s.shift);
         return cudaGetLastError();
       });
     });
@@ -388,16 +518,17 @@ int gnb200_dequantize_4bit(const void* codes, const void* scales, int64_t rows, 
   if (!out || !codes || !scales) return report_error(GNB200_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
   if (!on16(codes) || !on16(scales)) return report_error(GNB200_ERR_INVALID_ARGUMENT, "%s: codes and scales begin on 16 bytes", name);
   const FourRows p = four_rows(rows, C, block, tensor_scale, codes, scales);
-  const bool vec = on16(out) && C % VE == 0;
+  const int width = 16 / size_of(dtype);
+  const bool vec = on16(out) && C % width == 0;
   return launched(name, with_type(dtype, [&](auto t) {
     using T = decltype(t);
     return with_block(block, [&](auto b) {
       return with_flag(vec, [&](auto v) {
         auto kernel = &dequantize_kernel<T, decltype(b)::value, decltype(v)::value>;
         Shares s;
-        const cudaError_t err = share_out(rows, (C + VE - 1) / VE, 8, (const void*)kernel, &s);
+        const cudaError_t err = share_out(rows, vec ? (C + VE - 1) / VE : C / width + 1, 4, (const void*)kernel, &s);
         if (err != cudaSuccess) return err;
-        kernel<<<s.grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p, static_cast<T*>(out), s.lanes);
+        kernel<<<s.grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p, static_cast<T*>(out), s.shift);
         return cudaGetLastError();
       });
     });
@@ -422,18 +553,19 @@ int gnb200_rms_fwd_4bit(const void* x, int64_t x_stride, const void* residual, i
   NormArgs a = {};
   a.x = x, a.residual = residual, a.weight = weight, a.sum = sum, a.x_stride = x_stride, a.r_stride = residual_stride, a.w_dtype = weight_dtype;
   a.eps = (float)eps, a.offset = (float)offset, a.inv_c = (float)(1.0 / (double)C);
-  const bool vec = C % VE == 0 && on16(x) && on16(residual) && on16(weight) && on16(sum) &&
+  a.x_bounds = bounds_of(x, rows, x_stride, C, size_of(dtype)), a.r_bounds = bounds_of(residual, rows, residual_stride, C, size_of(residual_dtype));
+  const bool vec = C % 8 == 0 && on16(x) && on16(residual) && on16(weight) && on16(sum) &&
                    (rows == 1 || (x_stride * size_of(dtype) % 16 == 0 && (!residual || residual_stride * size_of(residual_dtype) % 16 == 0)));
   const int64_t vectors = (int64_t)p.tiles * 4 * (block / VE);
-  // a warp to a row of four vectors a lane at most, where there are rows for the SMs' warps; else a CTA with one or two vectors a thread, four
-  // above 16384 channels; longer rows are read twice
+  // a warp to a row of four vectors a lane at most, where there are rows for the SMs' warps; else a CTA with one vector a thread, two above 8192
+  // channels; longer rows are read twice
   const bool warp = vectors <= 128 && rows >= 148 * 8;
   int V, threads;
   if (warp) {
     V = vectors <= 32 ? 1 : vectors <= 64 ? 2 : 4;
     threads = 128;
   } else {
-    V = vectors <= 256 ? 1 : vectors <= 2048 ? 2 : vectors <= 4096 ? 4 : 0;
+    V = vectors <= 512 ? 1 : vectors <= 2048 ? 2 : 0;
     threads = V == 0 ? 1024 : (int)((vectors + V - 1) / V + 31) / 32 * 32;
   }
   const int64_t grid = warp ? (rows + 3) / 4 : rows;
@@ -456,7 +588,6 @@ int gnb200_rms_fwd_4bit(const void* x, int64_t x_stride, const void* residual, i
           }
           if (V == 1) return go(&norm_kernel<Tx, Ts, BLOCK, 1, false, VEC>);
           if (V == 2) return go(&norm_kernel<Tx, Ts, BLOCK, 2, false, VEC>);
-          if (V == 4) return go(&norm_kernel<Tx, Ts, BLOCK, 4, false, VEC>);
           return go(&norm_kernel<Tx, Ts, BLOCK, 0, false, VEC>);
         });
       });

@@ -24,6 +24,7 @@ constexpr int kTileK = 256;       // codes of a K tile: the 128 bytes of a swizz
 constexpr int kTileM = 128;       // features of a tile
 constexpr int kThreads = 192;     // four warps for the sums, one to load, one to multiply
 constexpr int kMostSplits = 8;    // CTAs of a cluster that share a tile's K
+constexpr int kAhead = 8;         // K tiles of the weight that a CTA asks for ahead of its turn
 
 struct LinearArgs {
   const uint8_t *w_scales, *x_scales;
@@ -38,38 +39,58 @@ struct LinearArgs {
 // ---------------------------------------------------------------------------------------------
 // Instructions
 // ---------------------------------------------------------------------------------------------
+// The same box to L2 only.  Before the kernel in front has ended, too: L2 is where that kernel's writes arrive.
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void bulk_prefetch(const void* p, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
                "r"(x), "r"(y), "r"(smem_addr(bar))
                : "memory");
 }
+// One lane of a converged warp, in a form that the compiler knows to be one: what it issues takes its operands from uniform registers as they are,
+// where behind `lane == 0` every one of these instructions waits for a lane to be picked for its operands.
+__device__ __forceinline__ bool one_lane() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
 // Shared-memory descriptors: start address and stride of 8 rows in 16 bytes, version 1, swizzle (2: 128 bytes; 0: none)
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t stride, uint64_t swizzle) {
   return (uint64_t)((addr & 0x3ffffu) >> 4) | 1ull << 16 | (uint64_t)(stride >> 4) << 32 | 1ull << 46 | swizzle << 61;
 }
-// 32 lanes x 16 bytes of shared memory to 4 columns, for all four warps' lanes
+// 32 lanes x 16 bytes of shared memory to 4 columns, for all four warps' lanes; of a pair (PAIR), each CTA from its own memory
+template <bool PAIR>
 __device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+  if constexpr (PAIR)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
 // Instruction descriptor: e2m1 times e2m1, fp32 sums, both operands along K; the scales' type (1: e8m0) and the bytes of a word of scales to begin with
 __host__ __device__ constexpr uint32_t instruction(int M, int N, bool e8m0, int byte) {
   return 1u << 7 | 1u << 10 | (uint32_t)(N >> 3) << 17 | (e8m0 ? 1u << 23 : 0u) | (uint32_t)(M >> 4) << 24 | (uint32_t)byte << 29 | (uint32_t)byte << 4;
 }
-template <int BLOCK>
+#define GNB200_MMA(group, kind)                                                                                                         \
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"                                                                        \
+               "tcgen05.mma.cta_group::" group ".kind::" kind " [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(acc),                      \
+               "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(a_scales), "r"(b_scales)                                                        \
+               : "memory")
+template <int BLOCK, bool PAIR>
 __device__ __forceinline__ void multiply(uint32_t acc, uint64_t a, uint64_t b, uint32_t idesc, uint32_t a_scales, uint32_t b_scales, uint32_t add) {
-  if constexpr (BLOCK == 16)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(acc),
-        "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(a_scales), "r"(b_scales)
-        : "memory");
+  if constexpr (BLOCK == 16 && PAIR)
+    GNB200_MMA("2", "mxf4nvf4.block_scale.scale_vec::4X");
+  else if constexpr (BLOCK == 16)
+    GNB200_MMA("1", "mxf4nvf4.block_scale.scale_vec::4X");
+  else if constexpr (PAIR)
+    GNB200_MMA("2", "mxf4.block_scale.scale_vec::2X");
   else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(acc),
-        "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(a_scales), "r"(b_scales)
-        : "memory");
+    GNB200_MMA("1", "mxf4.block_scale.scale_vec::2X");
 }
+#undef GNB200_MMA
 __device__ __forceinline__ void commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
@@ -82,6 +103,19 @@ __device__ __forceinline__ void tmem_load16(uint32_t col, float (&f)[16]) {
     f[4 * k] = __uint_as_float(v[k].x), f[4 * k + 1] = __uint_as_float(v[k].y);
     f[4 * k + 2] = __uint_as_float(v[k].z), f[4 * k + 3] = __uint_as_float(v[k].w);
   }
+}
+// 32 words; on their way until tmem_wait
+__device__ __forceinline__ void tmem_ask32(uint32_t col, float* f) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7]), "=f"(f[8]), "=f"(f[9]), "=f"(f[10]), "=f"(f[11]), "=f"(f[12]), "=f"(f[13]), "=f"(f[14]), "=f"(f[15]), "=f"(f[16]), "=f"(f[17]), "=f"(f[18]), "=f"(f[19]), "=f"(f[20]), "=f"(f[21]), "=f"(f[22]), "=f"(f[23]), "=f"(f[24]), "=f"(f[25]), "=f"(f[26]), "=f"(f[27]), "=f"(f[28]), "=f"(f[29]), "=f"(f[30]), "=f"(f[31])
+      : "r"(col)
+      : "memory");
+}
+template <int N>
+__device__ __forceinline__ void tmem_wait(float (&f)[N]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  pin_regs(f);  // (no use of them moves in front)
 }
 __device__ __forceinline__ float peer_float(uint32_t addr, unsigned rank) {
   uint32_t there;
@@ -96,6 +130,7 @@ __device__ __forceinline__ float peer_float(uint32_t addr, unsigned rank) {
 // ---------------------------------------------------------------------------------------------
 // Shared and tensor memory of a CTA.  The scales of a stage have columns of their own: they are written anew only when the stage is,
 // behind the barrier that its products have passed.  Half of either memory at most: two CTAs share an SM.
+// NT: 128, or enough for all tokens; a tile of tokens begins with a tile of scales, whose columns of tensor memory the products take from the first one on.
 template <int NT, int BLOCK>
 struct Layout {
   static constexpr int kChunks = kTileK / (4 * BLOCK);  // tiles of scales to a K tile
@@ -119,7 +154,7 @@ __global__ void __launch_bounds__(kThreads, 2) linear4_kernel(const __grid_const
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up;
   char* const stages = raw + (-smem_addr(raw) & 1023u);  // (swizzled tiles begin on 1024 bytes)
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const unsigned splits = cluster_nctarank(), rank = cluster_ctarank();
   const int m0 = (int)(blockIdx.x / splits) * kTileM, n0 = (int)blockIdx.y * NT;
   if (threadIdx.x == 0) {
@@ -141,11 +176,18 @@ __global__ void __launch_bounds__(kThreads, 2) linear4_kernel(const __grid_const
   // this CTA's K tiles
   const int ktiles = (p.K + kTileK - 1) / kTileK;
   const int k_begin = (int)((long long)ktiles * rank / splits), k_count = (int)((long long)ktiles * (rank + 1) / splits) - k_begin;
+  const uint8_t* const ws = p.w_scales + (long long)(m0 / 128) * p.tiles * kScaleTile;
+  if (warp == 4 && one_lane()) {  // the weight's way from memory is the longest: it begins while the kernel that makes the tokens' codes runs
+    for (int k = k_begin; k < k_begin + min(k_count, kAhead); ++k) {
+      tma_prefetch_2d(&w_map, k * 128, m0);
+      bulk_prefetch(ws + (long long)k * L::kScales, min(L::kChunks, p.tiles - k * L::kChunks) * kScaleTile);
+    }
+  }
+  __syncwarp();
   grid_dep_wait();
   bool whole = true;
   if (warp == 4) {
-    if (lane == 0) {
-      const uint8_t* ws = p.w_scales + (long long)(m0 / 128) * p.tiles * kScaleTile;
+    if (one_lane()) {
       const uint8_t* xs = p.x_scales + (long long)(n0 / 128) * p.tiles * kScaleTile;
       int issued = 0;
       for (; issued < k_count; ++issued) {
@@ -168,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 2) linear4_kernel(const __grid_const
     }
     __syncwarp();
   } else if (warp == 5) {
-    if (lane == 0) {
+    if (one_lane()) {
       for (int i = 0; i < k_count; ++i) {
         const int s = i % L::kStages, k = k_begin + i;
         producer_wait(&full[s], (i / L::kStages) & 1, &gave_up, p.wait);
@@ -178,15 +220,14 @@ __global__ void __launch_bounds__(kThreads, 2) linear4_kernel(const __grid_const
         const uint32_t ws = scales_at + s * 2 * L::kColumns, xs = ws + L::kColumns;
         const int chunks = min(L::kChunks, p.tiles - k * L::kChunks);
         for (int c = 0; c < chunks; ++c) {
-          copy_scales(ws + 4 * c, smem_desc(at + L::kA + L::kB + c * kScaleTile, 128, 0));
-          copy_scales(xs + 4 * c, smem_desc(at + L::kA + L::kB + L::kScales + c * kScaleTile, 128, 0));
+          copy_scales<false>(ws + 4 * c, smem_desc(at + L::kA + L::kB + c * kScaleTile, 128, 0));
+          copy_scales<false>(xs + 4 * c, smem_desc(at + L::kA + L::kB + L::kScales + c * kScaleTile, 128, 0));
         }
-        const uint32_t xs_tile = xs + (n0 % 128) / 32;
         const int steps = min(4, (p.K - k * kTileK + 63) / 64);
         for (int j = 0; j < steps; ++j) {  // 64 codes of K, 32 bytes of a row
           const int c = BLOCK == 16 ? j : j / 2, byte = BLOCK == 16 ? 0 : j % 2 * 2;
-          multiply<BLOCK>(acc, smem_desc(at + j * 32, 1024, 2), smem_desc(at + L::kA + j * 32, 1024, 2), instruction(kTileM, NT, BLOCK == 32, byte), ws + 4 * c,
-                          xs_tile + 4 * c, i + j > 0);
+          multiply<BLOCK, false>(acc, smem_desc(at + j * 32, 1024, 2), smem_desc(at + L::kA + j * 32, 1024, 2), instruction(kTileM, NT, BLOCK == 32, byte), ws + 4 * c,
+                          xs + 4 * c, i + j > 0);
         }
         commit(&empty[s]);
       }
@@ -223,8 +264,11 @@ __global__ void __launch_bounds__(kThreads, 2) linear4_kernel(const __grid_const
       asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
       cluster_wait();
       for (int j = rank; j < count; j += splits) {
-        float t = 0.f;
-        for (unsigned q = 0; q < splits; ++q) t += peer_float(smem_addr(red + j * kTileM), q);
+        float part[kMostSplits], t = 0.f;
+#pragma unroll
+        for (unsigned q = 0; q < kMostSplits; ++q) part[q] = q < splits ? peer_float(smem_addr(red + j * kTileM), q) : 0.f;  // (on their way together)
+#pragma unroll
+        for (unsigned q = 0; q < kMostSplits; ++q) t += part[q];
         if (inside) out[(long long)j * p.features] = store_param<T>(fmaf(t, alpha, bias));
       }
       asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -241,6 +285,219 @@ __global__ void __launch_bounds__(kThreads, 2) linear4_kernel(const __grid_const
   fence_after();
   __syncwarp();
   if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(acc), "r"(L::kTmem) : "memory");
+}
+
+// ---------------------------------------------------------------------------------------------
+// Many tokens: pairs of CTAs
+// ---------------------------------------------------------------------------------------------
+// A pair of SMs multiplies 256 tokens (A, 128 of them an SM) by 256 features (B, half of them in either SM's shared memory), so that an SM brings
+// half of what a tile of its own of 128 x 256 would take.  Persistent: the loads run ahead into the next tile, whose products begin as soon as
+// eight warps have the sums in registers; these round and store them meanwhile, rows of 256 bytes, through a corner of shared memory of each
+// warp's own.
+constexpr int kPairThreads = 320;  // eight warps for the sums, one to load, one to multiply
+constexpr int kPairTile = 256;     // tokens and features of a pair's tile
+constexpr int kPairStages = 4;
+
+template <int BLOCK>
+struct PairLayout {
+  static constexpr int kChunks = kTileK / (4 * BLOCK);
+  static constexpr int kRows = 128 * 128, kScales = kChunks * kScaleTile;  // bytes of an operand's half, of the scales of 128 rows
+  static constexpr int kStage = 2 * kRows + 3 * kScales, kStageAt = (kStage + 1023) / 1024 * 1024;
+  static constexpr int kColumns = 3 * 4 * kChunks;  // of tensor memory, for a stage's scales
+  static constexpr int kPitch = 256 + 16;           // bytes of a row on its way out: 16-byte accesses of eight lanes meet different banks
+  static constexpr int kOut = 32 * kPitch;          // a warp's
+  static constexpr int kSmem = kPairStages * kStageAt + 8 * kOut + 1024;
+  static_assert(kPairTile + kPairStages * kColumns <= 512, "tensor memory");
+};
+
+struct PairArgs {
+  LinearArgs l;
+  int token_tiles, feature_tiles, stores;  // stores: whole 16 bytes
+};
+
+__device__ __forceinline__ uint32_t leaders(const void* mine) {
+  uint32_t there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"(smem_addr(mine)));
+  return there;
+}
+// into this CTA's shared memory, counted on the leader's barrier
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+               "l"(map), "r"(x), "r"(y), "r"(bar)
+               : "memory");
+}
+// on the barriers of both CTAs, when all products so far are done
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(bar)),
+               "h"((uint16_t)3)
+               : "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Tiles in the order of their work: bands of 8 tiles of tokens, along the features, so that the pairs that run at a time share what L2 holds.
+__device__ __forceinline__ void tile_at(const PairArgs& p, int t, int& token, int& feature) {
+  constexpr int kBand = 8;
+  const int per_band = kBand * p.feature_tiles, band = t / per_band, in = t - band * per_band;
+  const int high = min(kBand, p.token_tiles - band * kBand);
+  token = (band * kBand + in % high) * kPairTile;
+  feature = in / high * kPairTile;
+}
+
+template <typename T, int BLOCK>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    linear4_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap xs_map,
+                        const __grid_constant__ CUtensorMap ws_map, const PairArgs p) {
+  using L = PairLayout<BLOCK>;
+  extern __shared__ char raw[];
+  __shared__ __align__(8) uint64_t full[kPairStages], empty[kPairStages], sums, taken;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int gave_up;
+  char* const stages = raw + (-smem_addr(raw) & 1023u);
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rank = (int)cluster_ctarank();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+    mbar_init(&sums, 1);
+    mbar_init(&taken, 16);  // the warps of both CTAs
+    gave_up = 0;
+    fence_mbar_init_cluster();
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // the peer's barriers are there
+  cluster_wait();
+  fence_after();
+  grid_dep_launch_dependents();
+  const uint32_t acc = tmem_slot, scales_at = acc + kPairTile;
+  const int ktiles = (p.l.K + kTileK - 1) / kTileK, tiles = p.token_tiles * p.feature_tiles, pairs = (int)gridDim.x / 2, first = (int)blockIdx.x / 2;
+  grid_dep_wait();
+  if (warp == 8) {
+    if (one_lane()) {
+      int n = 0;
+      for (int t = first; t < tiles; t += pairs) {
+        int token, feature;
+        tile_at(p, t, token, feature);
+        for (int k = 0; k < ktiles; ++k, ++n) {
+          const int s = n % kPairStages;
+          if (n >= kPairStages) {
+            producer_wait(&empty[s], (n / kPairStages - 1) & 1, &gave_up, p.l.wait);
+            if (*(volatile int*)&gave_up) goto drain;
+          }
+          const uint32_t at = smem_addr(stages) + s * L::kStageAt, bar = leaders(&full[s]);
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * L::kStage);
+          tma_load_pair(at, &x_map, k * 128, token + rank * 128, bar);
+          tma_load_pair(at + L::kRows, &w_map, k * 128, feature + rank * 128, bar);
+          tma_load_pair(at + 2 * L::kRows, &xs_map, k * (L::kScales / 8), token / 128 + rank, bar);
+          tma_load_pair(at + 2 * L::kRows + L::kScales, &ws_map, k * (L::kScales / 8), feature / 128, bar);
+        }
+      }
+    drain:
+      // (the leader sees both CTAs' loads land before the pair ends, given up or not)
+      if (rank == 0)
+        for (int k = max(0, n - kPairStages); k < n; ++k)
+          if (!mbar_wait_bounded(&full[k % kPairStages], (k / kPairStages) & 1, p.l.wait)) gave_up = 1;
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    if (rank == 0 && one_lane()) {
+      int n = 0, turn = 0;
+      for (int t = first; t < tiles; t += pairs, ++turn) {
+        if (turn > 0) {
+          producer_wait(&taken, (turn - 1) & 1, &gave_up, p.l.wait);
+          if (*(volatile int*)&gave_up) break;
+          fence_after();
+        }
+        for (int k = 0; k < ktiles; ++k, ++n) {
+          const int s = n % kPairStages;
+          producer_wait(&full[s], (n / kPairStages) & 1, &gave_up, p.l.wait);
+          if (*(volatile int*)&gave_up) break;
+          fence_after();
+          const uint32_t at = smem_addr(stages) + s * L::kStageAt;
+          const uint32_t xs = scales_at + s * L::kColumns, ws = xs + 4 * L::kChunks;
+          const int steps = min(4, (p.l.K - k * kTileK + 63) / 64);
+#pragma unroll
+          for (int c = 0; c < L::kChunks; ++c) {
+            const uint32_t from = at + 2 * L::kRows + c * kScaleTile;
+            copy_scales<true>(xs + 4 * c, smem_desc(from, 128, 0));
+            copy_scales<true>(ws + 8 * c, smem_desc(from + L::kScales, 128, 0));
+            copy_scales<true>(ws + 8 * c + 4, smem_desc(from + 2 * L::kScales, 128, 0));
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int c = BLOCK == 16 ? j : j / 2, byte = BLOCK == 16 ? 0 : j % 2 * 2;
+            if (j < steps)
+              multiply<BLOCK, true>(acc, smem_desc(at + j * 32, 1024, 2), smem_desc(at + L::kRows + j * 32, 1024, 2),
+                                    instruction(256, kPairTile, BLOCK == 32, byte), xs + 4 * c, ws + 8 * c, k + j > 0);
+          }
+          commit_pair(&empty[s]);
+        }
+        commit_pair(&sums);
+      }
+    }
+    __syncwarp();
+  } else {
+    const uint32_t own = acc + ((uint32_t)(warp & 3) << 21) + (uint32_t)(warp >> 2) * 128;
+    const uint32_t taken_at = leaders(&taken);
+    const float alpha = (p.l.x_scale ? *p.l.x_scale : 1.f) * (p.l.w_scale ? *p.l.w_scale : 1.f);
+    char* const corner = stages + kPairStages * L::kStageAt + warp * L::kOut;
+    constexpr int VE = 16 / sizeof(T), kCols = 256 / sizeof(T);  // columns of a row on its way out
+    int turn = 0;
+    for (int t = first; t < tiles; t += pairs, ++turn) {
+      int token, feature;
+      tile_at(p, t, token, feature);
+      token += rank * 128 + (warp & 3) * 32;
+      feature += (warp >> 2) * 128;
+      const bool whole = consumer_wait(&sums, turn & 1, &gave_up, p.l.wait);
+      fence_after();
+      __syncwarp();
+      float f[128];
+#pragma unroll
+      for (int j = 0; j < 128; j += 32) tmem_ask32(own + j, f + j);
+      tmem_wait(f);
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      if (lane == 0) arrive_at(taken_at);
+      const float factor = whole ? alpha : kNaN;
+      if (p.l.bias) {
+#pragma unroll
+        for (int j = 0; j < 128; ++j) f[j] = fmaf(f[j], factor, feature + j < p.l.features ? param_at(p.l.bias, p.l.bias_dtype, feature + j, 0.f) : 0.f);
+      } else {
+        scale_each(f, factor);
+      }
+#pragma unroll
+      for (int from = 0; from < 128; from += kCols) {
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < kCols; j += VE)
+          *reinterpret_cast<Pack<T, VE>*>(corner + lane * L::kPitch + j * sizeof(T)) = pack<T, VE>(*reinterpret_cast<float(*)[VE]>(f + from + j));
+        __syncwarp();
+        if (p.stores) {
+          const int column = feature + from + lane % 16 * VE;
+#pragma unroll 4
+          for (int r = lane / 16; r < 32; r += 2) {
+            const uint4 v = *reinterpret_cast<const uint4*>(corner + r * L::kPitch + lane % 16 * 16);
+            if (token + r < p.l.tokens && column < p.l.features) *reinterpret_cast<uint4*>(static_cast<T*>(p.l.out) + (long long)(token + r) * p.l.features + column) = v;
+          }
+        } else {
+          for (int r = 0; r < 32 && token + r < p.l.tokens; ++r)
+            for (int j = lane; j < kCols && feature + from + j < p.l.features; j += 32)
+              static_cast<T*>(p.l.out)[(long long)(token + r) * p.l.features + feature + from + j] = reinterpret_cast<const T*>(corner + r * L::kPitch)[j];
+        }
+      }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  }
+  __syncthreads();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // neither CTA's memory is used any more
+  cluster_wait();
+  fence_after();
+  __syncwarp();
+  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(acc), "r"(512) : "memory");
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -275,6 +532,53 @@ cudaError_t codes_map(CUtensorMap* map, const void* base, int64_t rows, int64_t 
   return rc == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+// tiles of scales of rows in blocks of 128, as words of 8 bytes: `tiles` of them and `high` blocks of rows a box, zeros outside
+cudaError_t scales_map(CUtensorMap* map, const void* base, int64_t rows, int64_t tiles, int box_tiles, int high) {
+  EncodeTiledFn enc = nullptr;
+  const cudaError_t err = encode_fn(&enc);
+  if (err != cudaSuccess) return err;
+  const cuuint64_t dims[2] = {(cuuint64_t)tiles * (kScaleTile / 8), (cuuint64_t)((rows + 127) / 128)}, strides[1] = {(cuuint64_t)tiles * kScaleTile};
+  const cuuint32_t boxes[2] = {(cuuint32_t)(box_tiles * (kScaleTile / 8)), (cuuint32_t)high}, steps[2] = {1, 1};
+  const CUresult rc = enc(map, CU_TENSOR_MAP_DATA_TYPE_INT64, 2, const_cast<void*>(base), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return rc == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+template <typename T, int BLOCK>
+cudaError_t launch_pairs(const LinearArgs& l, const void* w_codes, const void* x_codes, cudaStream_t stream) {
+  using L = PairLayout<BLOCK>;
+  auto kernel = &linear4_pair_kernel<T, BLOCK>;
+  CUtensorMap x_map, w_map, xs_map, ws_map;
+  cudaError_t err = codes_map(&x_map, x_codes, l.tokens, l.K, 128);
+  if (err == cudaSuccess) err = codes_map(&w_map, w_codes, l.features, l.K, 128);
+  if (err == cudaSuccess) err = scales_map(&xs_map, l.x_scales, l.tokens, l.tiles, L::kChunks, 1);
+  if (err == cudaSuccess) err = scales_map(&ws_map, l.w_scales, l.features, l.tiles, L::kChunks, 2);
+  if (err == cudaSuccess) err = ensure_kernel_attributes((const void*)kernel, L::kSmem, false);
+  if (err != cudaSuccess) return err;
+  PairArgs p = {};
+  p.l = l;
+  p.token_tiles = (l.tokens + kPairTile - 1) / kPairTile, p.feature_tiles = (l.features + kPairTile - 1) / kPairTile;
+  p.stores = reinterpret_cast<uintptr_t>(l.out) % 16 == 0 && l.features % (16 / (int)sizeof(T)) == 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = L::kSmem;
+  cfg.stream = stream;
+  cfg.gridDim = dim3(2);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int pairs = 0;
+  err = resident_clusters((const void*)kernel, &cfg, &pairs);
+  if (err != cudaSuccess) return err;
+  cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(pairs, (int64_t)p.token_tiles * p.feature_tiles)));
+  cfg.numAttrs = chain_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, x_map, w_map, xs_map, ws_map, p);
+}
+
 template <typename T, int NT, int BLOCK>
 cudaError_t launch_tiles(const LinearArgs& p, const CUtensorMap& w_map, const CUtensorMap& x_map, int splits, cudaStream_t stream) {
   using L = Layout<NT, BLOCK>;
@@ -298,6 +602,7 @@ cudaError_t launch_tiles(const LinearArgs& p, const CUtensorMap& w_map, const CU
 
 template <typename T, int BLOCK>
 cudaError_t launch_linear(const LinearArgs& p, const void* w_codes, const void* x_codes, cudaStream_t stream) {
+  if (p.tokens > 128 && p.features > 128) return launch_pairs<T, BLOCK>(p, w_codes, x_codes, stream);
   const int NT = p.tokens <= 16 ? 16 : p.tokens <= 32 ? 32 : p.tokens <= 64 ? 64 : 128;
   CUtensorMap w_map, x_map;
   cudaError_t err = codes_map(&w_map, w_codes, p.features, p.K, kTileM);

@@ -240,9 +240,9 @@ def test_module_and_nothing():
     assert pkg.dropout_add(x[0, 0], p=0.0).shape == ()
 
 
-def test_far_elements():
-    """Elements counted in more than 32 bits."""
-    n = 2 ** 32 + 4096
+@pytest.mark.parametrize("n", [2 ** 32 + 4096, 2 ** 34 + 4104])
+def test_far_elements(n):
+    """Elements, and counters, of more than 32 bits."""
     x = torch.empty(n, device="cuda", dtype=BF16)
     x[-8192:] = 1.0
     s = pkg.dropout_add(x, None, 0.5, 77)
