@@ -13,8 +13,8 @@
 namespace gnb200 {
 namespace {
 
-constexpr int VE = 8, kThreads = 256;
-constexpr long long kNear = 1ll << 33;  // elements up to which 32 bits count the vectors and the counters, the grid's last steps included
+constexpr int kThreads = 256;
+constexpr long long kNear = 1ll << 33;  // elements up to which 32 bits count the counters, the grid's last steps included
 
 struct DropoutArgs {
   const void *in, *residual;
@@ -47,27 +47,22 @@ struct Philox {
   }
 };
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&f)[VE]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-  } else {
-    unpack<T, VE>(load_vec<T, VE>(p), f);
-  }
-}
-
 // acc + x * scale where the word is large enough, else acc; x * scale or zero
 __device__ __forceinline__ float add_kept(float acc, float x, float scale, uint32_t word, uint32_t least) {
   asm("{\n\t.reg .pred p;\n\tsetp.hs.u32 p, %3, %4;\n\t@p fma.rn.f32 %0, %1, %2, %0;\n\t}" : "+f"(acc) : "f"(x), "f"(scale), "r"(word), "r"(least));
   return acc;
 }
 
-// VEC: tensors begin on 16 bytes and are taken 8 elements a thread, but for their end; otherwise element by element.  I: an index of vectors and
-// of counters, two a vector.
+// Vectors of 16 bytes of the wider type, 8 elements or 4, and 16 elements that a thread has under way: four chains of products hide their latency.
+template <typename Ti, typename To>
+constexpr int kVector = sizeof(Ti) == 4 || sizeof(To) == 4 ? 4 : 8;
+
+// VEC: tensors begin on vector boundaries and are taken a vector at a time, but for their end; otherwise element by element.  I: an index of counters.
+// What a thread needs from memory is asked for in front of its words and unpacked behind them (unpacked in front: bf16 with a residual 83 us, so 66).
+// Bound by HBM with a residual (16384 x 4096 bf16 66 us of 61, fp32 123 of 123); without one, in 16 bits, by the products: 62 us of 41.
 template <typename Ti, typename To, bool RES, bool VEC, typename I>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropoutArgs p) {
-  constexpr int AT_ONCE = VEC ? 2 : 1;  // vectors that a thread has under way: four chains of products hide their latency, two did not (bf16 without a residual 78 us)
+  constexpr int VE = kVector<Ti, To>, AT_ONCE = VEC ? 16 / VE : 1;
   const Ti* in = static_cast<const Ti*>(p.in);
   const To* res = static_cast<const To*>(p.residual);
   To* out = static_cast<To*>(p.out);
@@ -76,40 +71,36 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropoutArgs p) 
   const float scale = p.scale;
   const uint32_t least = p.least;
   for (I v = blockIdx.x * kThreads + threadIdx.x; v < vectors; v += AT_ONCE * step) {
-    float f[AT_ONCE][VE], r[AT_ONCE][VE];
-    bool whole[AT_ONCE];
+    Pack<Ti, VE> x[AT_ONCE];
+    Pack<To, VE> r[AT_ONCE];
 #pragma unroll
     for (int k = 0; k < AT_ONCE; ++k) {
       const long long first = (long long)(v + k * step) * VE;
-      whole[k] = VEC && first + VE <= p.n;
-      if (whole[k]) {
-        load8<Ti>(in + first, f[k]);
-        if constexpr (RES) load8<To>(res + first, r[k]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          f[k][e] = first + e < p.n ? load_param<Ti>(in + first, e) : 0.f;
-          if constexpr (RES) r[k][e] = first + e < p.n ? load_param<To>(res + first, e) : 0.f;
-        }
+      if (VEC && first + VE <= p.n) {
+        x[k] = load_vec<Ti, VE>(in + first);
+        if constexpr (RES) r[k] = load_vec<To, VE>(res + first);
       }
     }
-    uint32_t w[AT_ONCE][2][4];
+    uint32_t w[AT_ONCE][VE / 4][4];
 #pragma unroll
-    for (int k = 0; k < AT_ONCE; ++k) {
-      philox.words<I>(2 * (v + k * step), w[k][0]);
-      philox.words<I>(2 * (v + k * step) + 1, w[k][1]);
-    }
+    for (int k = 0; k < AT_ONCE; ++k)
+#pragma unroll
+      for (int c = 0; c < VE / 4; ++c) philox.words<I>(VE / 4 * (v + k * step) + c, w[k][c]);
 #pragma unroll
     for (int k = 0; k < AT_ONCE; ++k) {
       const long long first = (long long)(v + k * step) * VE;
+      if (VEC && first + VE <= p.n) {
+        float f[VE], sum[VE];
+        unpack<Ti, VE>(x[k], f);
+        if constexpr (RES) unpack<To, VE>(r[k], sum);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) f[k][e] = add_kept(RES ? r[k][e] : 0.f, f[k][e], scale, w[k][e / 4][e % 4], least);
-      if (whole[k]) {
-        store_vec<To, VE>(out + first, pack<To, VE>(f[k]));
+        for (int e = 0; e < VE; ++e) sum[e] = add_kept(RES ? sum[e] : 0.f, f[e], scale, w[k][e / 4][e % 4], least);
+        store_vec<To, VE>(out + first, pack<To, VE>(sum));
       } else {
 #pragma unroll
         for (int e = 0; e < VE; ++e)
-          if (first + e < p.n) out[first + e] = store_param<To>(f[k][e]);
+          if (first + e < p.n)
+            out[first + e] = store_param<To>(add_kept(RES ? load_param<To>(res + first, e) : 0.f, load_param<Ti>(in + first, e), scale, w[k][e / 4][e % 4], least));
       }
     }
   }
@@ -130,11 +121,12 @@ cudaError_t launch_dropout(const DropoutArgs& p, cudaStream_t stream) {
     Residency r = {};
     const cudaError_t err = residency((const void*)kernel, kThreads, 0, &r);
     if (err != cudaSuccess) return err;
+    constexpr int VE = kVector<Ti, To>;
     const long long need = ((p.n + VE - 1) / VE + kThreads - 1) / kThreads;
     kernel<<<(unsigned)std::min<long long>(need, (long long)r.per_sm * r.sms), kThreads, 0, stream>>>(p);
     return cudaGetLastError();
   };
-  const bool vec = on16(p.in) && on16(p.residual) && on16(p.out);
+  const bool vec = on16(p.in) && on16(p.residual) && on16(p.out);  // (8 bytes do for the narrow side of two types)
   if (p.n < kNear) return vec ? go(&dropout_kernel<Ti, To, RES, true, uint32_t>) : go(&dropout_kernel<Ti, To, RES, false, uint32_t>);
   return vec ? go(&dropout_kernel<Ti, To, RES, true, unsigned long long>) : go(&dropout_kernel<Ti, To, RES, false, unsigned long long>);
 }

@@ -23,73 +23,6 @@ struct FourRows {
   int C, wide, tiles;
 };
 
-// ---------------------------------------------------------------------------------------------
-// Codes and scales
-// ---------------------------------------------------------------------------------------------
-// Quotients are those of a division: with 16-bit inputs y / d lies midway between two codes often enough that a quotient one unit off shows.  The
-// reciprocal is the correctly rounded one (a Newton step from the hardware's), a quotient is corrected by its remainder (Markstein's theorem).
-__device__ __forceinline__ float reciprocal(float d) {
-  float near;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(near) : "f"(d));
-  return fmaf(fmaf(-d, near, 1.f), near, near);
-}
-__device__ __forceinline__ float scale_value(uint32_t byte, int block) {
-  if (block == 16) return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
-  return byte == 0xff ? __uint_as_float(0x7fc00000u) : byte == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);  // (2^-127 is subnormal)
-}
-// The tensor's scale and what is made of it once
-struct TensorScale {
-  float g, six, inverse;  // 6 g and its reciprocal
-  __device__ __forceinline__ TensorScale(const float* at) {
-    g = at ? *at : 1.f;
-    six = 6.f * g;
-    inverse = reciprocal(six);
-  }
-};
-struct Step {
-  float value, inverse;
-  uint32_t byte;
-};
-template <int BLOCK>
-__device__ __forceinline__ Step step_of(float most, const TensorScale& t) {
-  Step step;
-  const bool finite = most < __uint_as_float(0x7f800000u);  // (no NaN either)
-  if constexpr (BLOCK == 16) {
-    const float q = most * t.inverse;
-    const float s = q >= 448.f ? 448.f : fmaxf(fmaf(-t.inverse, fmaf(q, t.six, -most), q), 0.001953125f);
-    step.byte = finite ? __nv_cvt_float_to_fp8(s, __NV_SATFINITE, __NV_E4M3) : 0x7fu;
-    step.value = scale_value(step.byte, 16) * t.g;
-    step.inverse = reciprocal(step.value);
-  } else {
-    const int e = max((int)(__float_as_uint(most) >> 23) - 2, 0);
-    step.byte = finite ? (uint32_t)e : 0xffu;
-    step.value = 0.f;  // (a product with the inverse, a power of two, is the quotient)
-    step.inverse = __uint_as_float((uint32_t)(254 - min(e, 252)) << 23);
-  }
-  return step;
-}
-// 8 codes
-template <int BLOCK>
-__device__ __forceinline__ uint32_t codes_of(const float* y, const Step& step) {
-  float q[8];
-#pragma unroll
-  for (int e = 0; e < 8; e += 2) {
-    mul2(q[e], q[e + 1], y[e], y[e + 1], step.inverse, step.inverse);
-    if constexpr (BLOCK == 16) {
-      float r0, r1;
-      fma2(r0, r1, q[e], q[e + 1], step.value, step.value, -y[e], -y[e + 1]);
-      fma2(q[e], q[e + 1], r0, r1, -step.inverse, -step.inverse, q[e], q[e + 1]);
-    }
-  }
-  uint32_t word;
-  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
-      "mov.b32 %0, {a, b, c, d};\n\t}"
-      : "=r"(word)
-      : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
-  return word;
-}
 // Codes of the 16 channels y of vector v of a row (zeros where it has none) and the scales that its lanes share; by whole warps.
 template <int BLOCK>
 __device__ __forceinline__ void put(const FourRows& p, long long row, int v, bool live, const float (&y)[VE], const TensorScale& t) {
@@ -98,31 +31,16 @@ __device__ __forceinline__ void put(const FourRows& p, long long row, int v, boo
 #pragma unroll
   for (int e = 0; e < VE; ++e) most = larger(most, fabsf(y[e]));
   if constexpr (LANES > 1) most = larger(most, __shfl_xor_sync(0xffffffffu, most, 1));
-  const Step step = step_of<BLOCK>(most, t);
-  const uint2 words = make_uint2(codes_of<BLOCK>(y, step), codes_of<BLOCK>(y + 8, step));
+  const FourStep step = four_step<BLOCK>(most, t);
+  const uint2 words = make_uint2(codes8<BLOCK>(y, step), codes8<BLOCK>(y + 8, step));
   const bool inside = v * VE < p.wide;
   if (live && inside) *reinterpret_cast<uint2*>(p.codes + (row * (p.wide / VE) + v) * 8) = words;
   const int block = v / LANES;
   uint32_t scales = inside ? step.byte << (8 * (block & 3)) : 0;
   scales |= __shfl_xor_sync(0xffffffffu, scales, LANES);
   scales |= __shfl_xor_sync(0xffffffffu, scales, 2 * LANES);
-  if (live && v % (4 * LANES) == 0) {
-    uint32_t* const at = reinterpret_cast<uint32_t*>(p.scales + four_scale_at(row, block >> 2, p.tiles));
-    at[0] = scales;
-    // zeros for the rows of this lane's 16 bytes that are not there
-    if (row + 32 >= p.rows)
-      for (int k = 1; k < 4 - (int)(row >> 5 & 3); ++k) at[k] = 0;
-  }
+  if (live && v % (4 * LANES) == 0) put_scales(p.scales, row, p.rows, block >> 2, p.tiles, scales);
 }
-// The scales of the lanes of the last tile that have no row at all, by all threads of the grid.
-__device__ __forceinline__ void clear_behind(const FourRows& p, unsigned thread, unsigned threads) {
-  const unsigned rows = (unsigned)(p.rows & 127);
-  if (rows == 0 || rows >= 32) return;
-  uint8_t* const last = p.scales + (p.rows >> 7) * p.tiles * kScaleTile;
-  const unsigned lanes = 32 - rows, all = lanes * (unsigned)p.tiles;
-  for (unsigned i = thread; i < all; i += threads) *reinterpret_cast<uint4*>(last + (size_t)(i / lanes) * kScaleTile + (rows + i % lanes) * 16) = make_uint4(0, 0, 0, 0);
-}
-
 // ---------------------------------------------------------------------------------------------
 // 16 channels of a row
 // ---------------------------------------------------------------------------------------------
@@ -205,38 +123,67 @@ __device__ __forceinline__ void zero(float (&f)[VE]) {
   for (int e = 0; e < VE; ++e) f[e] = 0.f;
 }
 
+// 16 channels as they lie in an aligned row
+template <typename T>
+struct Raw {
+  uint4 q[sizeof(T)];
+  __device__ __forceinline__ void load(const T* row, int v, int C) {
+#pragma unroll
+    for (int k = 0; k < (int)sizeof(T); ++k) {
+      q[k] = make_uint4(0, 0, 0, 0);
+      if (v * VE + k * (int)(16 / sizeof(T)) < C) q[k] = reinterpret_cast<const uint4*>(row + v * VE)[k];
+    }
+  }
+  __device__ __forceinline__ void unpack(float (&f)[VE]) const {
+    constexpr int W = 16 / sizeof(T);
+#pragma unroll
+    for (int k = 0; k < (int)sizeof(T); ++k) {
+      float part[W];
+      unpack16<T, W>(q[k], part);
+#pragma unroll
+      for (int e = 0; e < W; ++e) f[k * W + e] = part[e];
+    }
+  }
+};
+
 // ---------------------------------------------------------------------------------------------
 // Rows to four bits and back
 // ---------------------------------------------------------------------------------------------
 constexpr int kThreads = 256;
 
-// 2^shift threads share a row's piece; the grid's second axis shares a row out.
+// 2^shift threads share a row's piece; the grid's second axis shares a row out.  Aligned rows: a lane asks for its next 16 channels before it works on these.
 template <typename T, int BLOCK, bool VEC>
 __global__ void __launch_bounds__(kThreads) quantize_kernel(const T* x, long long x_stride, const Bounds bounds, const FourRows p, int shift) {
-  constexpr int AT_ONCE = sizeof(T) == 2 ? 2 : 1;  // vectors that a thread has under way
   grid_dep_launch_dependents();
   const int lanes = 1 << shift, per_cta = kThreads >> shift, lane = threadIdx.x & (lanes - 1), vectors = p.tiles * 4 * kLanes<BLOCK>, step = gridDim.y << shift;
   const TensorScale t(BLOCK == 16 ? p.tensor_scale : nullptr);
-  for (long long base = (long long)blockIdx.x * per_cta; base < p.rows; base += (long long)gridDim.x * per_cta) {
-    const long long row = base + (threadIdx.x >> shift);
-    const bool live = row < p.rows;
-    const T* from = x + row * x_stride;
-    for (int first = blockIdx.y << shift; first < vectors; first += AT_ONCE * step) {
-      float y[AT_ONCE][VE];
-#pragma unroll
-      for (int k = 0; k < AT_ONCE; ++k) {
-        zero(y[k]);
-        const int v = first + k * step + lane;
-        if (live && v * VE < p.C) load16<T, VEC>(from, v, p.C, bounds, y[k]);
-      }
-#pragma unroll
-      for (int k = 0; k < AT_ONCE; ++k) {
-        const int v = first + k * step + lane;
-        put<BLOCK>(p, row, v, live && v < vectors, y[k], t);
-      }
+  const long long rows_step = (long long)gridDim.x * per_cta;
+  const int begin = blockIdx.y << shift;
+  long long base = (long long)blockIdx.x * per_cta, row = base + (threadIdx.x >> shift);  // (base and first: the same for the warp)
+  int first = begin;
+  Raw<T> next;
+  const auto ask = [&]() {
+    if (VEC && row < p.rows && (first + lane) * VE < p.C) next.load(x + row * x_stride, first + lane, p.C);
+  };
+  ask();
+  while (base < p.rows) {
+    const long long here = row;
+    const int v = first + lane;
+    const bool live = here < p.rows;
+    float y[VE];
+    zero(y);
+    if (live && v * VE < p.C) {
+      if constexpr (VEC)
+        next.unpack(y);
+      else
+        load16<T, false>(x + here * x_stride, v, p.C, bounds, y);
     }
+    first += step;
+    if (first >= vectors) first = begin, base += rows_step, row += rows_step;
+    if (base < p.rows) ask();
+    put<BLOCK>(p, here, v, live && v < vectors, y, t);
   }
-  clear_behind(p, (blockIdx.y * gridDim.x + blockIdx.x) * kThreads + threadIdx.x, gridDim.x * gridDim.y * kThreads);
+  clear_behind(p.scales, p.rows, p.tiles, (blockIdx.y * gridDim.x + blockIdx.x) * kThreads + threadIdx.x, gridDim.x * gridDim.y * kThreads);
 }
 
 __device__ __forceinline__ void values_of(uint32_t word, float (&f)[8]) {
@@ -259,17 +206,31 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const FourRows p, 
     const uint8_t* const codes = p.codes + row * (p.wide / 2);
     T* const to = out + row * p.C;
     if constexpr (VEC) {
-      for (int v = (blockIdx.y << shift) + lane; v * VE < p.C; v += step) {
-        const uint2 words = *reinterpret_cast<const uint2*>(codes + v * 8);
-        const float scale = scale_at(row, v * VE);
-        float f[VE], low[8], high[8];
-        values_of(words.x, low);
-        values_of(words.y, high);
+      // a vector of the output a lane, so that a warp's stores lie side by side (16 codes a lane: 16384 x 8192 bf16 90 us); two under way
+      constexpr int W = 16 / sizeof(T);
+      for (int v = (blockIdx.y << shift) + lane; v * W < p.C; v += 2 * step) {
+        uint32_t word[2];
+        float scale[2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = low[e], f[8 + e] = high[e];
-        scale_each(f, scale);
-        if constexpr (BLOCK == 16) scale_each(f, g);
-        store16<T, true>(to, v, p.C, f);
+        for (int k = 0; k < 2; ++k) {
+          const int at = (v + k * step) * W;
+          word[k] = 0, scale[k] = 0.f;
+          if (at < p.C) {
+            word[k] = W == 8 ? *reinterpret_cast<const uint32_t*>(codes + at / 2) : *reinterpret_cast<const uint16_t*>(codes + at / 2);
+            scale[k] = scale_at(row, at);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int at = (v + k * step) * W;
+          float f[8], o[W];
+          values_of(word[k], f);
+#pragma unroll
+          for (int e = 0; e < W; ++e) o[e] = f[e];
+          scale_each(o, scale[k]);
+          if constexpr (BLOCK == 16) scale_each(o, g);
+          if (at < p.C) store_vec<T, W>(to + at, pack<T, W>(o));
+        }
       }
     } else {
       // in the frame of the output's 16-byte vectors, whose first and last have elements of the rows beside this one; 8 codes from any one on
@@ -330,77 +291,97 @@ __device__ __forceinline__ void weight16(const NormArgs& a, int v, int C, float 
   for (int e = 0; e < VE; ++e) w[e] += a.offset;
 }
 
-// A row to a warp (WARP) or a CTA, V vectors a thread in registers; V = 0: rows of any length, read twice.
-template <typename Tx, typename Ts, int BLOCK, int V, bool WARP, bool VEC>
+// A row to a warp (WARP) or a CTA, V vectors a thread in registers; V = 0: rows of any length, read twice.  The CTAs that are resident walk over the
+// rows; of an aligned row with one vector a thread the next one's vectors are asked for before this one's sum.
+template <typename Tx, typename Ts, int BLOCK, int V, bool WARP, bool VEC, bool RES>
 __global__ void __launch_bounds__(WARP ? 128 : V == 1 ? 512 : 1024) norm_kernel(const NormArgs a, const FourRows p) {
   constexpr int HELD = V > 0 ? V : 1;
+  constexpr bool AHEAD = VEC && V == 1;
   __shared__ TeamSlots slots;
   grid_dep_launch_dependents();
   const int threads = WARP ? 32 : (int)blockDim.x, at = WARP ? (int)threadIdx.x & 31 : (int)threadIdx.x;
-  const long long row = WARP ? (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
-  const bool live = row < p.rows;
+  const int per_cta = WARP ? (int)blockDim.x >> 5 : 1;
   const int vectors = p.tiles * 4 * kLanes<BLOCK>;
-  const Tx* x = static_cast<const Tx*>(a.x) + row * a.x_stride;
-  const Ts* r = a.residual ? static_cast<const Ts*>(a.residual) + row * a.r_stride : nullptr;
   if constexpr (!WARP) clear<false>(slots, threads, 0, at);
-  auto sum_of = [&](int v, float (&s)[VE]) {
-    zero(s);
-    if (live && v * VE < p.C) {
-      load16<Tx, VEC>(x, v, p.C, a.x_bounds, s);
-      if (r) {
-        float f[VE];
-        load16<Ts, VEC>(r, v, p.C, a.r_bounds, f);
-        add_each(s, f);
-      }
-    }
-  };
-  float s[HELD][VE], sq[2] = {0.f, 0.f};
-  if constexpr (V > 0) {
-#pragma unroll
-    for (int k = 0; k < V; ++k) sum_of(at + k * threads, s[k]);
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const int v = at + k * threads;
-      if (r && live && v * VE < p.C) store16<Ts, VEC>(static_cast<Ts*>(a.sum) + row * p.C, v, p.C, s[k]);
-      dot_each(sq, s[k], s[k]);
-    }
-  } else {
-    for (int v = at; v * VE < p.C; v += threads) {
-      sum_of(v, s[0]);
-      dot_each(sq, s[0], s[0]);
-    }
-  }
   const TensorScale t(BLOCK == 16 ? p.tensor_scale : nullptr);
   int turn = 0;
-  const float all = WARP ? lanes_sum(sq[0] + sq[1], 32) : team_sum<false>(sq[0] + sq[1], slots, turn, threads, 0);
-  const float rstd = __frsqrt_rn(fmaf(all, a.inv_c, a.eps));
-  auto finish = [&](int v, float (&y)[VE]) {
-    if (v * VE < p.C) {
-      scale_each(y, rstd);
-      if (a.weight) {
-        float w[VE];
-        weight16<VEC>(a, v, p.C, w);
-        mul_each(y, w);
+  Raw<Tx> next_x;
+  Raw<Ts> next_r;
+  const auto ask = [&](long long row) {
+    if (row < p.rows && at * VE < p.C) {
+      next_x.load(static_cast<const Tx*>(a.x) + row * a.x_stride, at, p.C);
+      if constexpr (RES) next_r.load(static_cast<const Ts*>(a.residual) + row * a.r_stride, at, p.C);
+    }
+  };
+  long long row = (long long)blockIdx.x * per_cta + (WARP ? (int)threadIdx.x >> 5 : 0);
+  if constexpr (AHEAD) ask(row);
+  for (; row < p.rows; row += (long long)gridDim.x * per_cta) {  // (whole warps)
+    const Tx* x = static_cast<const Tx*>(a.x) + row * a.x_stride;
+    const Ts* r = RES ? static_cast<const Ts*>(a.residual) + row * a.r_stride : nullptr;
+    auto sum_of = [&](int v, float (&s)[VE]) {
+      zero(s);
+      if (v * VE < p.C) {
+        if constexpr (AHEAD)
+          next_x.unpack(s);
+        else
+          load16<Tx, VEC>(x, v, p.C, a.x_bounds, s);
+        if constexpr (RES) {
+          float f[VE];
+          if constexpr (AHEAD)
+            next_r.unpack(f);
+          else
+            load16<Ts, VEC>(r, v, p.C, a.r_bounds, f);
+          add_each(s, f);
+        }
       }
-      if (v * VE + VE > p.C) {  // (behind the row a NaN rstd would leave NaN in the zeros)
+    };
+    float s[HELD][VE], sq[2] = {0.f, 0.f};
+    if constexpr (V > 0) {
 #pragma unroll
-        for (int e = 0; e < VE; ++e)
-          if (v * VE + e >= p.C) y[e] = 0.f;
+      for (int k = 0; k < V; ++k) sum_of(at + k * threads, s[k]);
+      if constexpr (AHEAD) ask(row + (long long)gridDim.x * per_cta);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const int v = at + k * threads;
+        if (RES && v * VE < p.C) store16<Ts, VEC>(static_cast<Ts*>(a.sum) + row * p.C, v, p.C, s[k]);
+        dot_each(sq, s[k], s[k]);
+      }
+    } else {
+      for (int v = at; v * VE < p.C; v += threads) {
+        sum_of(v, s[0]);
+        dot_each(sq, s[0], s[0]);
       }
     }
-    put<BLOCK>(p, row, v, live && v < vectors, y, t);
-  };
-  if constexpr (V > 0) {
+    const float all = WARP ? lanes_sum(sq[0] + sq[1], 32) : team_sum<false>(sq[0] + sq[1], slots, turn, threads, 0);
+    const float rstd = __frsqrt_rn(fmaf(all, a.inv_c, a.eps));
+    auto finish = [&](int v, float (&y)[VE]) {
+      if (v * VE < p.C) {
+        scale_each(y, rstd);
+        if (a.weight) {
+          float w[VE];
+          weight16<VEC>(a, v, p.C, w);
+          mul_each(y, w);
+        }
+        if (v * VE + VE > p.C) {  // (behind the row a NaN rstd would leave NaN in the zeros)
 #pragma unroll
-    for (int k = 0; k < V; ++k) finish(at + k * threads, s[k]);
-  } else {
-    for (int first = 0; first < vectors; first += threads) {
-      sum_of(first + at, s[0]);  // (the last look at these: the sum may be the residual's own buffer)
-      if (r && (first + at) * VE < p.C) store16<Ts, VEC>(static_cast<Ts*>(a.sum) + row * p.C, first + at, p.C, s[0]);
-      finish(first + at, s[0]);
+          for (int e = 0; e < VE; ++e)
+            if (v * VE + e >= p.C) y[e] = 0.f;
+        }
+      }
+      put<BLOCK>(p, row, v, v < vectors, y, t);
+    };
+    if constexpr (V > 0) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) finish(at + k * threads, s[k]);
+    } else {
+      for (int first = 0; first < vectors; first += threads) {
+        sum_of(first + at, s[0]);  // (the last look at these: the sum may be the residual's own buffer)
+        if (RES && (first + at) * VE < p.C) store16<Ts, VEC>(static_cast<Ts*>(a.sum) + row * p.C, first + at, p.C, s[0]);
+        finish(first + at, s[0]);
+      }
     }
   }
-  clear_behind(p, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
+  clear_behind(p.scales, p.rows, p.tiles, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -526,7 +507,7 @@ int gnb200_dequantize_4bit(const void* codes, const void* scales, int64_t rows, 
       return with_flag(vec, [&](auto v) {
         auto kernel = &dequantize_kernel<T, decltype(b)::value, decltype(v)::value>;
         Shares s;
-        const cudaError_t err = share_out(rows, vec ? (C + VE - 1) / VE : C / width + 1, 4, (const void*)kernel, &s);
+        const cudaError_t err = share_out(rows, C / width + 1, 4, (const void*)kernel, &s);
         if (err != cudaSuccess) return err;
         kernel<<<s.grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p, static_cast<T*>(out), s.shift);
         return cudaGetLastError();
@@ -550,6 +531,9 @@ int gnb200_rms_fwd_4bit(const void* x, int64_t x_stride, const void* residual, i
   if (!x || !codes || !scales || (residual && !sum)) return report_error(GNB200_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
   if (!on16(codes) || !on16(scales)) return report_error(GNB200_ERR_INVALID_ARGUMENT, "%s: codes and scales begin on 16 bytes", name);
   const FourRows p = four_rows(rows, C, block, tensor_scale, codes, scales);
+  const FourNorm n = {x, residual, weight, sum, p.codes, p.scales, tensor_scale, rows, x_stride, residual_stride, (int)C, block, dtype, residual_dtype, weight_dtype, eps, offset};
+  const cudaError_t how = launch_rms_4bit(n, static_cast<cudaStream_t>(stream));
+  if (how != cudaErrorInvalidValue) return launched(name, how);
   NormArgs a = {};
   a.x = x, a.residual = residual, a.weight = weight, a.sum = sum, a.x_stride = x_stride, a.r_stride = residual_stride, a.w_dtype = weight_dtype;
   a.eps = (float)eps, a.offset = (float)offset, a.inv_c = (float)(1.0 / (double)C);
@@ -568,33 +552,37 @@ int gnb200_rms_fwd_4bit(const void* x, int64_t x_stride, const void* residual, i
     V = vectors <= 512 ? 1 : vectors <= 2048 ? 2 : 0;
     threads = V == 0 ? 1024 : (int)((vectors + V - 1) / V + 31) / 32 * 32;
   }
-  const int64_t grid = warp ? (rows + 3) / 4 : rows;
   return launched(name, with_type(dtype, [&](auto t) {
     using Tx = decltype(t);
-    const auto typed = [&](auto u) {
+    const auto typed = [&](auto u, auto is_res) {
       using Ts = decltype(u);
       return with_block(block, [&](auto b) {
         return with_flag(vec, [&](auto is_vec) {
           constexpr int BLOCK = decltype(b)::value;
-          constexpr bool VEC = decltype(is_vec)::value;
-          const auto go = [&](auto kernel) {
-            kernel<<<(unsigned)grid, threads, 0, static_cast<cudaStream_t>(stream)>>>(a, p);
+          constexpr bool VEC = decltype(is_vec)::value, RES = decltype(is_res)::value;
+          const auto go = [&](void (*kernel)(const NormArgs, const FourRows)) {
+            Residency r = {};
+            const cudaError_t err = residency((const void*)kernel, threads, 0, &r);
+            if (err != cudaSuccess) return err;
+            const int64_t need = warp ? (rows + 3) / 4 : rows;
+            kernel<<<(unsigned)std::min<int64_t>(need, (int64_t)r.per_sm * r.sms), threads, 0, static_cast<cudaStream_t>(stream)>>>(a, p);
             return cudaGetLastError();
           };
           if (warp) {
-            if (V == 1) return go(&norm_kernel<Tx, Ts, BLOCK, 1, true, VEC>);
-            if (V == 2) return go(&norm_kernel<Tx, Ts, BLOCK, 2, true, VEC>);
-            return go(&norm_kernel<Tx, Ts, BLOCK, 4, true, VEC>);
+            if (V == 1) return go(&norm_kernel<Tx, Ts, BLOCK, 1, true, VEC, RES>);
+            if (V == 2) return go(&norm_kernel<Tx, Ts, BLOCK, 2, true, VEC, RES>);
+            return go(&norm_kernel<Tx, Ts, BLOCK, 4, true, VEC, RES>);
           }
-          if (V == 1) return go(&norm_kernel<Tx, Ts, BLOCK, 1, false, VEC>);
-          if (V == 2) return go(&norm_kernel<Tx, Ts, BLOCK, 2, false, VEC>);
-          return go(&norm_kernel<Tx, Ts, BLOCK, 0, false, VEC>);
+          if (V == 1) return go(&norm_kernel<Tx, Ts, BLOCK, 1, false, VEC, RES>);
+          if (V == 2) return go(&norm_kernel<Tx, Ts, BLOCK, 2, false, VEC, RES>);
+          return go(&norm_kernel<Tx, Ts, BLOCK, 0, false, VEC, RES>);
         });
       });
     };
+    if (!residual) return typed(Tx(), std::false_type());
     if constexpr (!std::is_same<Tx, float>::value)
-      if (residual_dtype == GNB200_F32) return typed(float());
-    return typed(Tx());
+      if (residual_dtype == GNB200_F32) return typed(float(), std::true_type());
+    return typed(Tx(), std::true_type());
   }));
 }
 

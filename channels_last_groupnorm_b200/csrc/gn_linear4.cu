@@ -3,8 +3,7 @@
 //
 // tcgen05.mma with block scales: the weight is the A operand, so that a tile has 128 features by any number of tokens, and few tokens cost
 // little.  A producer thread brings K tiles of 256 codes (128 bytes a row, swizzled) by TMA and their scales by bulk copies; one thread
-// copies the scales of a stage to tensor memory and multiplies; four warps take the sums out, a feature a lane, so that a warp's stores
-// lie side by side at any width of the output.
+// copies the scales of a stage to tensor memory and multiplies; four warps take the sums out.
 // Where a grid of tiles leaves SMs idle the K tiles are shared out over a cluster, whose sums are added over distributed shared memory in
 // the order of their ranks.
 #include <cuda.h>
@@ -33,6 +32,7 @@ struct LinearArgs {
   void* out;
   int tokens, features, K, tiles;  // tiles: of scales, along K
   int bias_dtype;
+  int stores;  // features and output allow vectors (few tokens: of 4 features; many: of 16 bytes)
   WaitLimit wait;
 };
 
@@ -117,16 +117,17 @@ __device__ __forceinline__ void tmem_wait(float (&f)[N]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
   pin_regs(f);  // (no use of them moves in front)
 }
-__device__ __forceinline__ float peer_float(uint32_t addr, unsigned rank) {
+// 16 bytes of shared memory of a CTA of the cluster, at this CTA's address
+__device__ __forceinline__ float4 peer_floats(uint32_t addr, unsigned rank) {
   uint32_t there;
-  float v;
+  float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(there) : "memory");
   return v;
 }
 
 // ---------------------------------------------------------------------------------------------
-// Kernel
+// Few tokens: a tile to a CTA, or to a cluster
 // ---------------------------------------------------------------------------------------------
 // Shared and tensor memory of a CTA.  The scales of a stage have columns of their own: they are written anew only when the stage is,
 // behind the barrier that its products have passed.  Half of either memory at most: two CTAs share an SM.
@@ -241,43 +242,63 @@ __global__ void __launch_bounds__(kThreads, 2) linear4_kernel(const __grid_const
   fence_after();
   whole = whole && *(volatile int*)&gave_up == 0;
   if (warp < 4) {
-    const int feature = m0 + warp * 32 + lane, count = min(NT, p.tokens - n0);
-    const bool inside = feature < p.features;
-    const float alpha = (p.x_scale ? *p.x_scale : 1.f) * (p.w_scale ? *p.w_scale : 1.f);
-    const float bias = p.bias && inside ? param_at(p.bias, p.bias_dtype, feature, 0.f) : 0.f;
-    T* const out = static_cast<T*>(p.out) + (long long)n0 * p.features + feature;
+    const int count = min(NT, p.tokens - n0);
     const uint32_t own = acc + ((uint32_t)warp << 21);
-    float* const red = reinterpret_cast<float*>(stages) + warp * 32 + lane;
+    float* const red = reinterpret_cast<float*>(stages);
     for (int j = 0; j < count; j += 16) {
       float f[16];
       tmem_load16(own + j, f);
-      if (splits == 1) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (inside && j + e < count) out[(long long)(j + e) * p.features] = store_param<T>(whole ? fmaf(f[e], alpha, bias) : kNaN);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) red[(j + e) * kTileM] = whole ? f[e] : kNaN;
-      }
+      for (int e = 0; e < 16; ++e) red[(j + e) * kTileM + warp * 32 + lane] = whole ? f[e] : kNaN;
     }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     if (splits > 1) {
       asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
       cluster_wait();
-      for (int j = rank; j < count; j += splits) {
-        float part[kMostSplits], t = 0.f;
-#pragma unroll
-        for (unsigned q = 0; q < kMostSplits; ++q) part[q] = q < splits ? peer_float(smem_addr(red + j * kTileM), q) : 0.f;  // (on their way together)
-#pragma unroll
-        for (unsigned q = 0; q < kMostSplits; ++q) t += part[q];
-        if (inside) out[(long long)j * p.features] = store_param<T>(fmaf(t, alpha, bias));
-      }
-      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-      cluster_wait();
+    } else {
+      asm volatile("barrier.sync 1, 128;" ::: "memory");
     }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    // a token to a warp, 4 features a lane; of the tokens of a tile that several CTAs share, each adds its part
+    const int feature = m0 + lane * 4, there = p.features - feature;
+    const float alpha = (p.x_scale ? *p.x_scale : 1.f) * (p.w_scale ? *p.w_scale : 1.f);
+    float bias[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bias[e] = p.bias && e < there ? param_at(p.bias, p.bias_dtype, feature + e, 0.f) : 0.f;
+    constexpr int AT_ONCE = 2;  // tokens under way
+    for (int first = rank + splits * warp; first < count; first += AT_ONCE * 4 * splits) {
+      float4 part[AT_ONCE][kMostSplits];
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const uint32_t at = smem_addr(red + min(first + k * 4 * (int)splits, count - 1) * kTileM + lane * 4);
+#pragma unroll
+        for (unsigned q = 0; q < kMostSplits; ++q) part[k][q] = q < splits ? peer_floats(at, q) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const int j = first + k * 4 * (int)splits;
+        float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (unsigned q = 0; q < kMostSplits; ++q) t[0] += part[k][q].x, t[1] += part[k][q].y, t[2] += part[k][q].z, t[3] += part[k][q].w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = fmaf(t[e], alpha, bias[e]);
+        T* const out = static_cast<T*>(p.out) + (long long)(n0 + j) * p.features + feature;
+        if (j < count) {
+          if (p.stores && there > 0) {
+            *reinterpret_cast<Pack<T, 4>*>(out) = pack<T, 4>(t);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (e < there) out[e] = store_param<T>(t[e]);
+          }
+        }
+      }
+    }
   } else if (splits > 1) {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     cluster_wait();
+  }
+  if (splits > 1) {  // (the others have read what this CTA holds)
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     cluster_wait();
   }
@@ -295,24 +316,25 @@ __global__ void __launch_bounds__(kThreads, 2) linear4_kernel(const __grid_const
 // eight warps have the sums in registers; these round and store them meanwhile, rows of 256 bytes, through a corner of shared memory of each
 // warp's own.
 constexpr int kPairThreads = 320;  // eight warps for the sums, one to load, one to multiply
-constexpr int kPairTile = 256;     // tokens and features of a pair's tile
+constexpr int kPairTokens = 256;   // of a pair's tile
 constexpr int kPairStages = 4;
 
-template <int BLOCK>
+template <int BLOCK, int NF>  // NF: features of a pair's tile, 256 or 128
 struct PairLayout {
   static constexpr int kChunks = kTileK / (4 * BLOCK);
-  static constexpr int kRows = 128 * 128, kScales = kChunks * kScaleTile;  // bytes of an operand's half, of the scales of 128 rows
-  static constexpr int kStage = 2 * kRows + 3 * kScales, kStageAt = (kStage + 1023) / 1024 * 1024;
-  static constexpr int kColumns = 3 * 4 * kChunks;  // of tensor memory, for a stage's scales
+  static constexpr int kHigh = NF / 128;  // blocks of 128 features
+  static constexpr int kA = 128 * 128, kB = NF / 2 * 128, kScales = kChunks * kScaleTile;  // bytes of the operands' halves, of the scales of 128 rows
+  static constexpr int kStage = kA + kB + (1 + kHigh) * kScales, kStageAt = (kStage + 1023) / 1024 * 1024;
+  static constexpr int kColumns = (1 + kHigh) * 4 * kChunks;  // of tensor memory, for a stage's scales
   static constexpr int kPitch = 256 + 16;           // bytes of a row on its way out: 16-byte accesses of eight lanes meet different banks
   static constexpr int kOut = 32 * kPitch;          // a warp's
   static constexpr int kSmem = kPairStages * kStageAt + 8 * kOut + 1024;
-  static_assert(kPairTile + kPairStages * kColumns <= 512, "tensor memory");
+  static_assert(NF + kPairStages * kColumns <= 512, "tensor memory");
 };
 
 struct PairArgs {
   LinearArgs l;
-  int token_tiles, feature_tiles, stores;  // stores: whole 16 bytes
+  int token_tiles, feature_tiles;
 };
 
 __device__ __forceinline__ uint32_t leaders(const void* mine) {
@@ -337,19 +359,20 @@ __device__ __forceinline__ void arrive_at(uint32_t bar) {
 }
 
 // Tiles in the order of their work: bands of 8 tiles of tokens, along the features, so that the pairs that run at a time share what L2 holds.
+template <int NF>
 __device__ __forceinline__ void tile_at(const PairArgs& p, int t, int& token, int& feature) {
   constexpr int kBand = 8;
   const int per_band = kBand * p.feature_tiles, band = t / per_band, in = t - band * per_band;
   const int high = min(kBand, p.token_tiles - band * kBand);
-  token = (band * kBand + in % high) * kPairTile;
-  feature = in / high * kPairTile;
+  token = (band * kBand + in % high) * kPairTokens;
+  feature = in / high * NF;
 }
 
-template <typename T, int BLOCK>
+template <typename T, int BLOCK, int NF>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     linear4_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap xs_map,
                         const __grid_constant__ CUtensorMap ws_map, const PairArgs p) {
-  using L = PairLayout<BLOCK>;
+  using L = PairLayout<BLOCK, NF>;
   extern __shared__ char raw[];
   __shared__ __align__(8) uint64_t full[kPairStages], empty[kPairStages], sums, taken;
   __shared__ uint32_t tmem_slot;
@@ -374,7 +397,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   cluster_wait();
   fence_after();
   grid_dep_launch_dependents();
-  const uint32_t acc = tmem_slot, scales_at = acc + kPairTile;
+  const uint32_t acc = tmem_slot, scales_at = acc + NF;
   const int ktiles = (p.l.K + kTileK - 1) / kTileK, tiles = p.token_tiles * p.feature_tiles, pairs = (int)gridDim.x / 2, first = (int)blockIdx.x / 2;
   grid_dep_wait();
   if (warp == 8) {
@@ -382,7 +405,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       int n = 0;
       for (int t = first; t < tiles; t += pairs) {
         int token, feature;
-        tile_at(p, t, token, feature);
+        tile_at<NF>(p, t, token, feature);
         for (int k = 0; k < ktiles; ++k, ++n) {
           const int s = n % kPairStages;
           if (n >= kPairStages) {
@@ -392,9 +415,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           const uint32_t at = smem_addr(stages) + s * L::kStageAt, bar = leaders(&full[s]);
           if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * L::kStage);
           tma_load_pair(at, &x_map, k * 128, token + rank * 128, bar);
-          tma_load_pair(at + L::kRows, &w_map, k * 128, feature + rank * 128, bar);
-          tma_load_pair(at + 2 * L::kRows, &xs_map, k * (L::kScales / 8), token / 128 + rank, bar);
-          tma_load_pair(at + 2 * L::kRows + L::kScales, &ws_map, k * (L::kScales / 8), feature / 128, bar);
+          tma_load_pair(at + L::kA, &w_map, k * 128, feature + rank * (NF / 2), bar);
+          tma_load_pair(at + L::kA + L::kB, &xs_map, k * (L::kScales / 8), token / 128 + rank, bar);
+          tma_load_pair(at + L::kA + L::kB + L::kScales, &ws_map, k * (L::kScales / 8), feature / 128, bar);
         }
       }
     drain:
@@ -423,17 +446,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           const int steps = min(4, (p.l.K - k * kTileK + 63) / 64);
 #pragma unroll
           for (int c = 0; c < L::kChunks; ++c) {
-            const uint32_t from = at + 2 * L::kRows + c * kScaleTile;
+            const uint32_t from = at + L::kA + L::kB + c * kScaleTile;
             copy_scales<true>(xs + 4 * c, smem_desc(from, 128, 0));
-            copy_scales<true>(ws + 8 * c, smem_desc(from + L::kScales, 128, 0));
-            copy_scales<true>(ws + 8 * c + 4, smem_desc(from + 2 * L::kScales, 128, 0));
+#pragma unroll
+            for (int h = 0; h < L::kHigh; ++h) copy_scales<true>(ws + 4 * (L::kHigh * c + h), smem_desc(from + (1 + h) * L::kScales, 128, 0));
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int c = BLOCK == 16 ? j : j / 2, byte = BLOCK == 16 ? 0 : j % 2 * 2;
             if (j < steps)
-              multiply<BLOCK, true>(acc, smem_desc(at + j * 32, 1024, 2), smem_desc(at + L::kRows + j * 32, 1024, 2),
-                                    instruction(256, kPairTile, BLOCK == 32, byte), xs + 4 * c, ws + 8 * c, k + j > 0);
+              multiply<BLOCK, true>(acc, smem_desc(at + j * 32, 1024, 2), smem_desc(at + L::kA + j * 32, 1024, 2),
+                                    instruction(256, NF, BLOCK == 32, byte), xs + 4 * c, ws + 4 * L::kHigh * c, k + j > 0);
           }
           commit_pair(&empty[s]);
         }
@@ -442,45 +465,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     }
     __syncwarp();
   } else {
-    const uint32_t own = acc + ((uint32_t)(warp & 3) << 21) + (uint32_t)(warp >> 2) * 128;
+    constexpr int MINE = NF / 2;  // features of a warp
+    const uint32_t own = acc + ((uint32_t)(warp & 3) << 21) + (uint32_t)(warp >> 2) * MINE;
     const uint32_t taken_at = leaders(&taken);
     const float alpha = (p.l.x_scale ? *p.l.x_scale : 1.f) * (p.l.w_scale ? *p.l.w_scale : 1.f);
     char* const corner = stages + kPairStages * L::kStageAt + warp * L::kOut;
-    constexpr int VE = 16 / sizeof(T), kCols = 256 / sizeof(T);  // columns of a row on its way out
+    constexpr int VE = 16 / sizeof(T), kCols = MINE < 256 / (int)sizeof(T) ? MINE : 256 / (int)sizeof(T);  // columns of a row on its way out
     int turn = 0;
     for (int t = first; t < tiles; t += pairs, ++turn) {
       int token, feature;
-      tile_at(p, t, token, feature);
+      tile_at<NF>(p, t, token, feature);
       token += rank * 128 + (warp & 3) * 32;
-      feature += (warp >> 2) * 128;
+      feature += (warp >> 2) * MINE;
       const bool whole = consumer_wait(&sums, turn & 1, &gave_up, p.l.wait);
       fence_after();
       __syncwarp();
-      float f[128];
+      float f[MINE];
 #pragma unroll
-      for (int j = 0; j < 128; j += 32) tmem_ask32(own + j, f + j);
+      for (int j = 0; j < MINE; j += 32) tmem_ask32(own + j, f + j);
       tmem_wait(f);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       if (lane == 0) arrive_at(taken_at);
       const float factor = whole ? alpha : kNaN;
       if (p.l.bias) {
 #pragma unroll
-        for (int j = 0; j < 128; ++j) f[j] = fmaf(f[j], factor, feature + j < p.l.features ? param_at(p.l.bias, p.l.bias_dtype, feature + j, 0.f) : 0.f);
+        for (int j = 0; j < MINE; ++j) f[j] = fmaf(f[j], factor, feature + j < p.l.features ? param_at(p.l.bias, p.l.bias_dtype, feature + j, 0.f) : 0.f);
       } else {
         scale_each(f, factor);
       }
 #pragma unroll
-      for (int from = 0; from < 128; from += kCols) {
+      for (int from = 0; from < MINE; from += kCols) {
         __syncwarp();
 #pragma unroll
         for (int j = 0; j < kCols; j += VE)
           *reinterpret_cast<Pack<T, VE>*>(corner + lane * L::kPitch + j * sizeof(T)) = pack<T, VE>(*reinterpret_cast<float(*)[VE]>(f + from + j));
         __syncwarp();
-        if (p.stores) {
-          const int column = feature + from + lane % 16 * VE;
+        if (p.l.stores) {
+          constexpr int kEach = kCols / VE;  // lanes of a row
+          const int column = feature + from + lane % kEach * VE;
 #pragma unroll 4
-          for (int r = lane / 16; r < 32; r += 2) {
-            const uint4 v = *reinterpret_cast<const uint4*>(corner + r * L::kPitch + lane % 16 * 16);
+          for (int r = lane / kEach; r < 32; r += 32 / kEach) {
+            const uint4 v = *reinterpret_cast<const uint4*>(corner + r * L::kPitch + lane % kEach * 16);
             if (token + r < p.l.tokens && column < p.l.features) *reinterpret_cast<uint4*>(static_cast<T*>(p.l.out) + (long long)(token + r) * p.l.features + column) = v;
           }
         } else {
@@ -544,21 +569,21 @@ cudaError_t scales_map(CUtensorMap* map, const void* base, int64_t rows, int64_t
   return rc == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-template <typename T, int BLOCK>
+template <typename T, int BLOCK, int NF>
 cudaError_t launch_pairs(const LinearArgs& l, const void* w_codes, const void* x_codes, cudaStream_t stream) {
-  using L = PairLayout<BLOCK>;
-  auto kernel = &linear4_pair_kernel<T, BLOCK>;
+  using L = PairLayout<BLOCK, NF>;
+  auto kernel = &linear4_pair_kernel<T, BLOCK, NF>;
   CUtensorMap x_map, w_map, xs_map, ws_map;
   cudaError_t err = codes_map(&x_map, x_codes, l.tokens, l.K, 128);
-  if (err == cudaSuccess) err = codes_map(&w_map, w_codes, l.features, l.K, 128);
+  if (err == cudaSuccess) err = codes_map(&w_map, w_codes, l.features, l.K, NF / 2);
   if (err == cudaSuccess) err = scales_map(&xs_map, l.x_scales, l.tokens, l.tiles, L::kChunks, 1);
-  if (err == cudaSuccess) err = scales_map(&ws_map, l.w_scales, l.features, l.tiles, L::kChunks, 2);
+  if (err == cudaSuccess) err = scales_map(&ws_map, l.w_scales, l.features, l.tiles, L::kChunks, L::kHigh);
   if (err == cudaSuccess) err = ensure_kernel_attributes((const void*)kernel, L::kSmem, false);
   if (err != cudaSuccess) return err;
   PairArgs p = {};
   p.l = l;
-  p.token_tiles = (l.tokens + kPairTile - 1) / kPairTile, p.feature_tiles = (l.features + kPairTile - 1) / kPairTile;
-  p.stores = reinterpret_cast<uintptr_t>(l.out) % 16 == 0 && l.features % (16 / (int)sizeof(T)) == 0;
+  p.token_tiles = (l.tokens + kPairTokens - 1) / kPairTokens, p.feature_tiles = (l.features + NF - 1) / NF;
+  p.l.stores = reinterpret_cast<uintptr_t>(l.out) % 16 == 0 && l.features % (16 / (int)sizeof(T)) == 0;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kPairThreads);
   cfg.dynamicSmemBytes = L::kSmem;
@@ -601,16 +626,29 @@ cudaError_t launch_tiles(const LinearArgs& p, const CUtensorMap& w_map, const CU
 }
 
 template <typename T, int BLOCK>
-cudaError_t launch_linear(const LinearArgs& p, const void* w_codes, const void* x_codes, cudaStream_t stream) {
-  if (p.tokens > 128 && p.features > 128) return launch_pairs<T, BLOCK>(p, w_codes, x_codes, stream);
+cudaError_t launch_linear(LinearArgs p, const void* w_codes, const void* x_codes, cudaStream_t stream) {
+  const int64_t ktiles = (p.K + kTileK - 1) / kTileK;
+  Residency r = {};
+  cudaError_t err = residency((const void*)&linear4_kernel<T, 16, BLOCK>, kThreads, 0, &r);  // (asked for the number of SMs)
+  if (err != cudaSuccess) return err;
+  // Pairs for more than a tile of tokens, in tiles of 128 features where those are one wave (1024 x 4096 x 2048 11.3 us, 256 features 12.2; 777 x 1344 x 4096, two
+  // waves, 10.4 and 8.6); but with fewer tiles than two fifths of the pairs and a K that is worth sharing out, clusters (300 x 4096 x 1111 8.9 us, pairs
+  // 12.7; 1024 x 1024 x 1024, four K tiles, 7.6 and 5.6).
+  if (p.tokens > 128 && p.features > 128) {
+    const int64_t high = (p.tokens + kPairTokens - 1) / kPairTokens, tiles = high * ((p.features + 127) / 128), pairs = r.sms / 2;
+    if (tiles > pairs) return launch_pairs<T, BLOCK, 256>(p, w_codes, x_codes, stream);
+    if (ktiles <= 4 || 5 * tiles >= 2 * pairs) return launch_pairs<T, BLOCK, 128>(p, w_codes, x_codes, stream);
+  }
+  p.stores = p.features % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % (4 * sizeof(T)) == 0;
   const int NT = p.tokens <= 16 ? 16 : p.tokens <= 32 ? 32 : p.tokens <= 64 ? 64 : 128;
   CUtensorMap w_map, x_map;
-  cudaError_t err = codes_map(&w_map, w_codes, p.features, p.K, kTileM);
+  err = codes_map(&w_map, w_codes, p.features, p.K, kTileM);
   if (err == cudaSuccess) err = codes_map(&x_map, x_codes, p.tokens, p.K, NT);
   if (err != cudaSuccess) return err;
-  const int64_t tiles = (int64_t)((p.features + kTileM - 1) / kTileM) * ((p.tokens + NT - 1) / NT), ktiles = (p.K + kTileK - 1) / kTileK;
+  const int64_t tiles = (int64_t)((p.features + kTileM - 1) / kTileM) * ((p.tokens + NT - 1) / NT);
+  // K is shared out until there are CTAs for the SMs and a third more (32 x 4096 x 4096 in clusters of 4 6.4 us, of 2 7.7, of 8 8.0; 8 x 4096 x 6144 6.8, 8.1, 10.6)
   int splits = 1;
-  while (splits < kMostSplits && splits * 2 <= ktiles && tiles * splits * 2 <= 296) splits *= 2;
+  while (splits < kMostSplits && splits * 2 <= ktiles && tiles * splits * 2 * 3 <= 4 * r.sms) splits *= 2;
   if (NT == 16) return launch_tiles<T, 16, BLOCK>(p, w_map, x_map, splits, stream);
   if (NT == 32) return launch_tiles<T, 32, BLOCK>(p, w_map, x_map, splits, stream);
   if (NT == 64) return launch_tiles<T, 64, BLOCK>(p, w_map, x_map, splits, stream);

@@ -25,6 +25,7 @@
 #include <initializer_list>
 
 #include "../../include/gnb200.h"
+#include "gn_four.cuh"
 #include "gn_kernels.h"
 #include "gn_rows.h"
 #include "gn_tokens.cuh"
@@ -283,16 +284,19 @@ struct Place {
 template <typename Tx, typename Ts, int VE, int V, int THREADS>
 constexpr bool kStaged = THREADS > kWarpThreads && (THREADS > 512 || V * VE * (sizeof(Tx) + sizeof(Ts)) > 64);
 constexpr int kMostBlocks = 512;  // of the rows that these kernels take
+enum Output { kPlain = 0, kCodes8 = 1, kCodes4 = 2 };
 
 // THREADS: the CTA's at most; kWarpThreads where a row has a group of lanes, otherwise a row has the CTA
-template <typename Tx, typename Ts, int VE, int V, int THREADS, bool Q, bool RES, bool RAGGED>
+// OUT: y in x's type, 8-bit codes, 4-bit codes (aligned rows of whole blocks of 32 channels; `rstd` is the tensor's scale then, `blocks` the tiles of scales along a row)
+template <typename Tx, typename Ts, int VE, int V, int THREADS, int OUT, bool RES, bool RAGGED>
 __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
   constexpr bool WARP = THREADS == kWarpThreads, STAGED = kStaged<Tx, Ts, VE, V, THREADS>;
   extern __shared__ __align__(16) char smem[];
   __shared__ TeamSlots slots;
   __shared__ uint32_t most[32];
-  __shared__ uint2 blocks[Q && RAGGED ? kMostBlocks : 1];  // maxima of a block's own vectors, of the channels before them
+  __shared__ uint2 blocks[OUT == kCodes8 && RAGGED ? kMostBlocks : 1];  // maxima of a block's own vectors, of the channels before them
   const Place<WARP, false> at(p.lanes, p.stage_bytes, p.stages, line_bytes(p.C, VE, RAGGED), smem);
+  if constexpr (OUT == kCodes4) grid_dep_launch_dependents();  // (the product that takes the codes)
   const int lanes = at.lanes, first = at.first;
   const Tx* next_x = static_cast<const Tx*>(p.x) + at.row * p.x_stride;  // the next row to be asked for
   const Ts* next_r = RES ? static_cast<const Ts*>(p.residual) + at.row * p.r_stride : nullptr;
@@ -394,17 +398,51 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
     ask();  // (a lane's own vectors: read, so free)
     const float all_sq = WARP ? lanes_sum(sq[0] + sq[1], lanes) : team_sum<false>(sq[0] + sq[1], slots, turn, lanes, 0);
     const float rstd = __frsqrt_rn(fmaf(all_sq, p.inv_c, p.eps));
-    if (p.rstd && live && first == 0) p.rstd[row] = rstd;
+    if (OUT != kCodes4 && p.rstd && live && first == 0) p.rstd[row] = rstd;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       scale_each(s[v], rstd);
       mul_each(s[v], w[v]);
     }
-    if constexpr (!Q) {
+    if constexpr (OUT == kPlain) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const int i = first + v * lanes;
         if (live && i < nvec) frame.store(static_cast<Tx*>(p.y) + out_at, i, s[v]);
+      }
+    } else if constexpr (OUT == kCodes4) {
+      const TensorScale tensor(p.block == 16 ? p.rstd : nullptr);
+      const int share = p.block / VE;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int i = first + v * lanes;
+        const bool inside = live && i < nvec;
+        float most = 0.f;
+        if (i < nvec) {  // (beyond the row a NaN rstd would leave NaN in the zeros)
+#pragma unroll
+          for (int e = 0; e < VE; ++e) most = larger(most, fabsf(s[v][e]));
+        }
+        const float all = __uint_as_float(lanes_max(magnitude(most), share));
+        const FourStep step = p.block == 16 ? four_step<16>(all, tensor) : four_step<32>(all, tensor);
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = e < VE ? s[v][e] : 0.f;
+        const uint32_t word = p.block == 16 ? codes8<16>(y, step) : codes8<32>(y, step);
+        uint8_t* const to = static_cast<uint8_t*>(p.y) + (row * nvec + i) * (VE / 2);
+        if (inside) {
+          if constexpr (VE == 8)
+            *reinterpret_cast<uint32_t*>(to) = word;
+          else
+            *reinterpret_cast<uint16_t*>(to) = (uint16_t)word;
+        }
+        const int block = i / share;
+        uint32_t four = i < nvec ? step.byte << (8 * (block & 3)) : 0;
+#pragma unroll
+        for (int k = 1; k <= 2; ++k) {  // of four blocks, where the row has them in this group
+          const uint32_t other = __shfl_xor_sync(0xffffffffu, four, k * share);
+          if (k * share < lanes) four |= other;
+        }
+        if (inside && (i & (4 * share - 1)) == 0) put_scales(reinterpret_cast<uint8_t*>(p.scale), row, p.rows, block >> 2, p.blocks, four);
       }
     } else {
       uint8_t* const out = static_cast<uint8_t*>(p.y) + out_at;
@@ -480,6 +518,7 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
       }
     }
   }
+  if constexpr (OUT == kCodes4) clear_behind(reinterpret_cast<uint8_t*>(p.scale), p.rows, p.blocks, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
 }
 
 // Rows of any length: one CTA per row, element by element, read once for the sum and once more for each thing that needs it.  Outputs are
@@ -916,7 +955,7 @@ cudaError_t with_geometry(const RmsGeom& g, F&& f) {
   }
 }
 
-template <bool Q>
+template <int OUT>
 cudaError_t launch_rms_fwd(RmsFwd p, int dtype, int sum_dtype, Rows rows, cudaStream_t stream) {
   return with_types(dtype, sum_dtype, [&](auto tx, auto ts) {
     using Tx = decltype(tx);
@@ -938,15 +977,21 @@ cudaError_t launch_rms_fwd(RmsFwd p, int dtype, int sum_dtype, Rows rows, cudaSt
         constexpr int VE = decltype(ve)::value, V = decltype(v)::value, THREADS = decltype(most)::value;
         constexpr bool RAGGED = decltype(ragged)::value;
         staged = kStaged<Tx, Ts, VE, V, THREADS>;
-        if constexpr (std::is_same<Tx, Ts>::value)
-          if (!p.residual) return go(&rms_fwd_kernel<Tx, Ts, VE, V, THREADS, Q, false, RAGGED>);
-        return go(&rms_fwd_kernel<Tx, Ts, VE, V, THREADS, Q, true, RAGGED>);
+        if constexpr (OUT == kCodes4 && RAGGED) return cudaErrorInvalidValue;
+        else {
+          if constexpr (std::is_same<Tx, Ts>::value)
+            if (!p.residual) return go(&rms_fwd_kernel<Tx, Ts, VE, V, THREADS, OUT, false, RAGGED>);
+          return go(&rms_fwd_kernel<Tx, Ts, VE, V, THREADS, OUT, true, RAGGED>);
+        }
       });
-      if (err != cudaErrorInvalidValue) return err;
+      if (OUT == kCodes4 || err != cudaErrorInvalidValue) return err;
       g = RmsGeom{1, 0, kMostThreads, kMostThreads, false, false, 0};
       staged = false;
     }
-    return go(&rms_fwd_any_kernel<Tx, Ts, Q>);
+    if constexpr (OUT == kCodes4)
+      return cudaErrorInvalidValue;
+    else
+      return go(&rms_fwd_any_kernel<Tx, Ts, OUT == kCodes8>);
   });
 }
 
@@ -1034,6 +1079,21 @@ int launched(const char* name, cudaError_t err) {
 
 }  // namespace
 
+cudaError_t launch_rms_4bit(const FourNorm& n, cudaStream_t stream) {
+  if (n.C % kFourUnit != 0) return cudaErrorInvalidValue;
+  const int size = size_of(n.dtype), wide = size_of(n.residual_dtype);
+  if (rows_of(n.dtype == GNB200_F32 ? 4 : 8, n.C, n.rows, n.weight,
+              {{n.x, n.x_stride, size}, {n.residual, n.r_stride, wide}, {n.sum, n.C, wide}}) != kAligned)
+    return cudaErrorInvalidValue;
+  RmsFwd p = {};
+  p.x = n.x, p.residual = n.residual, p.weight = n.weight, p.y = n.codes, p.sum = n.sum;
+  p.rstd = const_cast<float*>(n.tensor_scale), p.scale = reinterpret_cast<float*>(n.scales);
+  p.rows = n.rows, p.x_stride = n.x_stride, p.r_stride = n.r_stride;
+  p.C = n.C, p.w_dtype = n.weight_dtype, p.block = n.block, p.blocks = (int)four_tiles(n.C, n.block);
+  p.eps = (float)n.eps, p.offset = (float)n.offset, p.inv_c = (float)(1.0 / (double)n.C);
+  return launch_rms_fwd<kCodes4>(p, n.dtype, n.residual_dtype, kAligned, stream);
+}
+
 cudaError_t launch_column_sums(const ColumnSums& p, int sets, cudaStream_t stream, bool chained) {
   return launch_chained(&column_sums_kernel, (unsigned)((p.C + 31) / 32 * sets), dim3(32 * kSumWarps), 0, stream, chained && chain_enabled(), p);
 }
@@ -1068,8 +1128,8 @@ static int rms_forward(const char* name, const void* x, int64_t x_stride, const 
                            {{x, x_stride, size}, {residual, residual_stride, wide}, {y, C, codes ? 1 : size}, {sum, C, wide}});
   p.edge = edge_of(width, {{x, x_stride, size}, {residual, residual_stride, wide}});
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return launched(name, codes ? launch_rms_fwd<true>(p, dtype, residual_dtype, how, s)
-                              : launch_rms_fwd<false>(p, dtype, residual_dtype, how, s));
+  return launched(name, codes ? launch_rms_fwd<kCodes8>(p, dtype, residual_dtype, how, s)
+                              : launch_rms_fwd<kPlain>(p, dtype, residual_dtype, how, s));
 }
 
 int gnb200_rms_fwd(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight, int64_t rows,
