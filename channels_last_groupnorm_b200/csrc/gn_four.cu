@@ -151,39 +151,57 @@ struct Raw {
 // ---------------------------------------------------------------------------------------------
 constexpr int kThreads = 256;
 
-// 2^shift threads share a row's piece; the grid's second axis shares a row out.  Aligned rows: a lane asks for its next 16 channels before it works on these.
+// Work in units: 2^shift lanes a row, one vector a lane.  A row has `pieces` of these; the units of all rows are dealt out one by one, so that CTAs have the
+// same number of them but for one (whole rows to a warp: 8192 x 8192 on 740 CTAs, one row or two a warp, 36 us).
+struct Units {
+  int shift, pieces;
+  int over, rest;  // what a step of the whole grid is: rows of CTAs, pieces
+};
+struct Unit {
+  long long base;  // rows of CTAs
+  int piece;
+  __device__ __forceinline__ Unit(const Units& u) {
+    base = blockIdx.x / u.pieces;
+    piece = blockIdx.x % u.pieces;
+  }
+  __device__ __forceinline__ void step(const Units& u) {
+    base += u.over;
+    piece += u.rest;
+    if (piece >= u.pieces) piece -= u.pieces, ++base;
+  }
+};
+
+// Aligned rows: a lane asks for its next 16 channels before it works on these.
 template <typename T, int BLOCK, bool VEC>
-__global__ void __launch_bounds__(kThreads) quantize_kernel(const T* x, long long x_stride, const Bounds bounds, const FourRows p, int shift) {
+__global__ void __launch_bounds__(kThreads) quantize_kernel(const T* x, long long x_stride, const Bounds bounds, const FourRows p, const Units u) {
   grid_dep_launch_dependents();
-  const int lanes = 1 << shift, per_cta = kThreads >> shift, lane = threadIdx.x & (lanes - 1), vectors = p.tiles * 4 * kLanes<BLOCK>, step = gridDim.y << shift;
+  const int per_cta = kThreads >> u.shift, own_row = threadIdx.x >> u.shift, lane = threadIdx.x & ((1 << u.shift) - 1), vectors = p.tiles * 4 * kLanes<BLOCK>;
   const TensorScale t(BLOCK == 16 ? p.tensor_scale : nullptr);
-  const long long rows_step = (long long)gridDim.x * per_cta;
-  const int begin = blockIdx.y << shift;
-  long long base = (long long)blockIdx.x * per_cta, row = base + (threadIdx.x >> shift);  // (base and first: the same for the warp)
-  int first = begin;
+  Unit unit(u);
   Raw<T> next;
   const auto ask = [&]() {
-    if (VEC && row < p.rows && (first + lane) * VE < p.C) next.load(x + row * x_stride, first + lane, p.C);
+    const long long row = unit.base * per_cta + own_row;
+    const int v = (unit.piece << u.shift) + lane;
+    if (VEC && row < p.rows && v * VE < p.C) next.load(x + row * x_stride, v, p.C);
   };
   ask();
-  while (base < p.rows) {
-    const long long here = row;
-    const int v = first + lane;
-    const bool live = here < p.rows;
+  while (unit.base * per_cta < p.rows) {
+    const long long row = unit.base * per_cta + own_row;
+    const int v = (unit.piece << u.shift) + lane;
+    const bool live = row < p.rows;
     float y[VE];
     zero(y);
     if (live && v * VE < p.C) {
       if constexpr (VEC)
         next.unpack(y);
       else
-        load16<T, false>(x + here * x_stride, v, p.C, bounds, y);
+        load16<T, false>(x + row * x_stride, v, p.C, bounds, y);
     }
-    first += step;
-    if (first >= vectors) first = begin, base += rows_step, row += rows_step;
-    if (base < p.rows) ask();
-    put<BLOCK>(p, here, v, live && v < vectors, y, t);
+    unit.step(u);
+    ask();
+    put<BLOCK>(p, row, v, live && v < vectors, y, t);
   }
-  clear_behind(p.scales, p.rows, p.tiles, (blockIdx.y * gridDim.x + blockIdx.x) * kThreads + threadIdx.x, gridDim.x * gridDim.y * kThreads);
+  clear_behind(p.scales, p.rows, p.tiles, blockIdx.x * kThreads + threadIdx.x, gridDim.x * kThreads);
 }
 
 __device__ __forceinline__ void values_of(uint32_t word, float (&f)[8]) {
@@ -193,69 +211,74 @@ __device__ __forceinline__ void values_of(uint32_t word, float (&f)[8]) {
     f[e] = two.x, f[e + 1] = two.y;
   }
 }
-// VEC: output rows of whole 16-byte vectors on their boundaries.
+// VEC: output rows of whole 16-byte vectors on their boundaries; a vector a lane, so that a warp's stores lie side by side (16 codes a lane: 16384 x 8192 bf16
+// 90 us).
 template <typename T, int BLOCK, bool VEC>
-__global__ void __launch_bounds__(kThreads) dequantize_kernel(const FourRows p, T* out, int shift) {
-  const int lanes = 1 << shift, per_cta = kThreads >> shift, lane = threadIdx.x & (lanes - 1), step = gridDim.y << shift;
+__global__ void __launch_bounds__(kThreads) dequantize_kernel(const FourRows p, T* out, const Units u) {
+  constexpr int W = 16 / sizeof(T), AT_ONCE = VEC ? 4 : 1;
+  const int per_cta = kThreads >> u.shift, own_row = threadIdx.x >> u.shift, lane = threadIdx.x & ((1 << u.shift) - 1);
   const float g = BLOCK == 16 && p.tensor_scale ? *p.tensor_scale : 1.f;
   const auto scale_at = [&](long long row, int channel) {
     const int block = channel / BLOCK;
     return scale_value(p.scales[four_scale_at(row, block >> 2, p.tiles) + (block & 3)], BLOCK);
   };
-  for (long long row = (long long)blockIdx.x * per_cta + (threadIdx.x >> shift); row < p.rows; row += (long long)gridDim.x * per_cta) {
-    const uint8_t* const codes = p.codes + row * (p.wide / 2);
-    T* const to = out + row * p.C;
+  Unit unit(u);
+  while (unit.base * per_cta < p.rows) {
     if constexpr (VEC) {
-      // a vector of the output a lane, so that a warp's stores lie side by side (16 codes a lane: 16384 x 8192 bf16 90 us); two under way
-      constexpr int W = 16 / sizeof(T);
-      for (int v = (blockIdx.y << shift) + lane; v * W < p.C; v += 2 * step) {
-        uint32_t word[2];
-        float scale[2];
+      uint32_t word[AT_ONCE];
+      float scale[AT_ONCE];
+      T* to[AT_ONCE];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int at = (v + k * step) * W;
-          word[k] = 0, scale[k] = 0.f;
-          if (at < p.C) {
-            word[k] = W == 8 ? *reinterpret_cast<const uint32_t*>(codes + at / 2) : *reinterpret_cast<const uint16_t*>(codes + at / 2);
-            scale[k] = scale_at(row, at);
-          }
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const long long row = unit.base * per_cta + own_row;
+        const int at = ((unit.piece << u.shift) + lane) * W;
+        to[k] = row < p.rows && at < p.C ? out + row * p.C + at : nullptr;
+        if (to[k]) {
+          const uint8_t* const from = p.codes + row * (p.wide / 2) + at / 2;
+          word[k] = W == 8 ? *reinterpret_cast<const uint32_t*>(from) : *reinterpret_cast<const uint16_t*>(from);
+          scale[k] = scale_at(row, at);
         }
+        unit.step(u);
+      }
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int at = (v + k * step) * W;
+      for (int k = 0; k < AT_ONCE; ++k) {
+        if (to[k]) {
           float f[8], o[W];
           values_of(word[k], f);
 #pragma unroll
           for (int e = 0; e < W; ++e) o[e] = f[e];
           scale_each(o, scale[k]);
           if constexpr (BLOCK == 16) scale_each(o, g);
-          if (at < p.C) store_vec<T, W>(to + at, pack<T, W>(o));
+          store_vec<T, W>(to[k], pack<T, W>(o));
         }
       }
     } else {
       // in the frame of the output's 16-byte vectors, whose first and last have elements of the rows beside this one; 8 codes from any one on
-      constexpr int W = 16 / sizeof(T);
-      const int skew = (int)(reinterpret_cast<uintptr_t>(to) / sizeof(T) % W), count = (p.C + skew + W - 1) / W, words = p.wide / 8;
-      for (int v = (blockIdx.y << shift) + lane; v < count; v += step) {
-        const int c = v * W - skew, at = c < 0 ? -1 : c / 8;
-        const uint32_t* const w = reinterpret_cast<const uint32_t*>(codes);
-        const uint32_t below = at >= 0 ? w[at] : 0, above = at + 1 < words ? w[at + 1] : 0;
-        float f[8];
-        values_of(__funnelshift_r(below, above, 4 * (c & 7)), f);
-        const int border = ((c + W - 1) / BLOCK) * BLOCK;  // channels from here on have the last one's scale
-        const float last = scale_at(row, min(c + W - 1, p.C - 1)), first = c >= 0 && c < border ? scale_at(row, c) : last;
-        const bool whole = c >= 0 && c + W <= p.C;
-        float o[W];
+      const long long row = unit.base * per_cta + own_row;
+      if (row < p.rows) {
+        T* const to = out + row * p.C;
+        const int skew = (int)(reinterpret_cast<uintptr_t>(to) / sizeof(T) % W), words = p.wide / 8;
+        const int c = ((unit.piece << u.shift) + lane) * W - skew, at = c < 0 ? -1 : c / 8;
+        if (c < p.C) {
+          const uint32_t* const w = reinterpret_cast<const uint32_t*>(p.codes + row * (p.wide / 2));
+          const uint32_t below = at >= 0 ? w[at] : 0, above = at + 1 < words ? w[at + 1] : 0;
+          float f[8];
+          values_of(__funnelshift_r(below, above, 4 * (c & 7)), f);
+          const int border = ((c + W - 1) / BLOCK) * BLOCK;  // channels from here on have the last one's scale
+          const float last = scale_at(row, min(c + W - 1, p.C - 1)), first = c >= 0 && c < border ? scale_at(row, c) : last;
+          float o[W];
 #pragma unroll
-        for (int e = 0; e < W; ++e) o[e] = f[e] * (c + e < border ? first : last) * g;
-        if (whole) {
-          store_vec<T, W>(to + c, pack<T, W>(o));
-        } else {
+          for (int e = 0; e < W; ++e) o[e] = f[e] * (c + e < border ? first : last) * g;
+          if (c >= 0 && c + W <= p.C) {
+            store_vec<T, W>(to + c, pack<T, W>(o));
+          } else {
 #pragma unroll
-          for (int e = 0; e < W; ++e)
-            if ((unsigned)(c + e) < (unsigned)p.C) to[c + e] = store_param<T>(o[e]);
+            for (int e = 0; e < W; ++e)
+              if ((unsigned)(c + e) < (unsigned)p.C) to[c + e] = store_param<T>(o[e]);
+          }
         }
       }
+      unit.step(u);
     }
   }
 }
@@ -272,116 +295,51 @@ struct NormArgs {
   float eps, offset, inv_c;
 };
 
-// (offset + w) of 16 channels, from addresses on 16 bytes (VEC) or any
-template <bool VEC>
-__device__ __forceinline__ void weight16(const NormArgs& a, int v, int C, float (&w)[VE]) {
-  if constexpr (VEC) {
-    const Bounds none = {};
-    if (a.w_dtype == 0)
-      load16<float, true>(static_cast<const float*>(a.weight), v, C, none, w);
-    else if (a.w_dtype == 1)
-      load16<__half, true>(static_cast<const __half*>(a.weight), v, C, none, w);
-    else
-      load16<__nv_bfloat16, true>(static_cast<const __nv_bfloat16*>(a.weight), v, C, none, w);
-  } else {
-#pragma unroll
-    for (int e = 0; e < VE; ++e) w[e] = v * VE + e < C ? param_at(a.weight, a.w_dtype, v * VE + e, 1.f) : 0.f;
-  }
-#pragma unroll
-  for (int e = 0; e < VE; ++e) w[e] += a.offset;
-}
-
-// A row to a warp (WARP) or a CTA, V vectors a thread in registers; V = 0: rows of any length, read twice.  The CTAs that are resident walk over the
-// rows; of an aligned row with one vector a thread the next one's vectors are asked for before this one's sum.
-template <typename Tx, typename Ts, int BLOCK, int V, bool WARP, bool VEC, bool RES>
-__global__ void __launch_bounds__(WARP ? 128 : V == 1 ? 512 : 1024) norm_kernel(const NormArgs a, const FourRows p) {
-  constexpr int HELD = V > 0 ? V : 1;
-  constexpr bool AHEAD = VEC && V == 1;
+// Rows that the kernels of gn_rms.cu do not take: tensors without a common frame, rows of more channels than a CTA holds.  A CTA to a row, which it
+// reads twice.
+constexpr int kNormThreads = 512;
+template <typename Tx, typename Ts, int BLOCK, bool VEC>
+__global__ void __launch_bounds__(kNormThreads) norm_any_kernel(const NormArgs a, const FourRows p) {
   __shared__ TeamSlots slots;
   grid_dep_launch_dependents();
-  const int threads = WARP ? 32 : (int)blockDim.x, at = WARP ? (int)threadIdx.x & 31 : (int)threadIdx.x;
-  const int per_cta = WARP ? (int)blockDim.x >> 5 : 1;
-  const int vectors = p.tiles * 4 * kLanes<BLOCK>;
-  if constexpr (!WARP) clear<false>(slots, threads, 0, at);
+  const int at = threadIdx.x, vectors = p.tiles * 4 * kLanes<BLOCK>;
   const TensorScale t(BLOCK == 16 ? p.tensor_scale : nullptr);
+  clear<false>(slots, kNormThreads, 0, at);
   int turn = 0;
-  Raw<Tx> next_x;
-  Raw<Ts> next_r;
-  const auto ask = [&](long long row) {
-    if (row < p.rows && at * VE < p.C) {
-      next_x.load(static_cast<const Tx*>(a.x) + row * a.x_stride, at, p.C);
-      if constexpr (RES) next_r.load(static_cast<const Ts*>(a.residual) + row * a.r_stride, at, p.C);
-    }
-  };
-  long long row = (long long)blockIdx.x * per_cta + (WARP ? (int)threadIdx.x >> 5 : 0);
-  if constexpr (AHEAD) ask(row);
-  for (; row < p.rows; row += (long long)gridDim.x * per_cta) {  // (whole warps)
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const Tx* x = static_cast<const Tx*>(a.x) + row * a.x_stride;
-    const Ts* r = RES ? static_cast<const Ts*>(a.residual) + row * a.r_stride : nullptr;
+    const Ts* r = a.residual ? static_cast<const Ts*>(a.residual) + row * a.r_stride : nullptr;
     auto sum_of = [&](int v, float (&s)[VE]) {
       zero(s);
       if (v * VE < p.C) {
-        if constexpr (AHEAD)
-          next_x.unpack(s);
-        else
-          load16<Tx, VEC>(x, v, p.C, a.x_bounds, s);
-        if constexpr (RES) {
+        load16<Tx, VEC>(x, v, p.C, a.x_bounds, s);
+        if (r) {
           float f[VE];
-          if constexpr (AHEAD)
-            next_r.unpack(f);
-          else
-            load16<Ts, VEC>(r, v, p.C, a.r_bounds, f);
+          load16<Ts, VEC>(r, v, p.C, a.r_bounds, f);
           add_each(s, f);
         }
       }
     };
-    float s[HELD][VE], sq[2] = {0.f, 0.f};
-    if constexpr (V > 0) {
-#pragma unroll
-      for (int k = 0; k < V; ++k) sum_of(at + k * threads, s[k]);
-      if constexpr (AHEAD) ask(row + (long long)gridDim.x * per_cta);
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const int v = at + k * threads;
-        if (RES && v * VE < p.C) store16<Ts, VEC>(static_cast<Ts*>(a.sum) + row * p.C, v, p.C, s[k]);
-        dot_each(sq, s[k], s[k]);
-      }
-    } else {
-      for (int v = at; v * VE < p.C; v += threads) {
-        sum_of(v, s[0]);
-        dot_each(sq, s[0], s[0]);
-      }
+    float s[VE], sq[2] = {0.f, 0.f};
+    for (int v = at; v * VE < p.C; v += kNormThreads) {
+      sum_of(v, s);
+      dot_each(sq, s, s);
     }
-    const float all = WARP ? lanes_sum(sq[0] + sq[1], 32) : team_sum<false>(sq[0] + sq[1], slots, turn, threads, 0);
-    const float rstd = __frsqrt_rn(fmaf(all, a.inv_c, a.eps));
-    auto finish = [&](int v, float (&y)[VE]) {
+    const float rstd = __frsqrt_rn(fmaf(team_sum<false>(sq[0] + sq[1], slots, turn, kNormThreads, 0), a.inv_c, a.eps));
+    for (int first = 0; first < vectors; first += kNormThreads) {
+      const int v = first + at;
+      sum_of(v, s);  // (the last look at these: the sum may be the residual's own buffer)
       if (v * VE < p.C) {
-        scale_each(y, rstd);
-        if (a.weight) {
-          float w[VE];
-          weight16<VEC>(a, v, p.C, w);
-          mul_each(y, w);
-        }
-        if (v * VE + VE > p.C) {  // (behind the row a NaN rstd would leave NaN in the zeros)
+        if (r) store16<Ts, VEC>(static_cast<Ts*>(a.sum) + row * p.C, v, p.C, s);
+        scale_each(s, rstd);
 #pragma unroll
-          for (int e = 0; e < VE; ++e)
-            if (v * VE + e >= p.C) y[e] = 0.f;
-        }
+        for (int e = 0; e < VE; ++e)  // (behind the row a NaN rstd would leave NaN in the zeros)
+          s[e] = v * VE + e >= p.C ? 0.f : a.weight ? s[e] * (a.offset + param_at(a.weight, a.w_dtype, v * VE + e, 1.f)) : s[e];
       }
-      put<BLOCK>(p, row, v, v < vectors, y, t);
-    };
-    if constexpr (V > 0) {
-#pragma unroll
-      for (int k = 0; k < V; ++k) finish(at + k * threads, s[k]);
-    } else {
-      for (int first = 0; first < vectors; first += threads) {
-        sum_of(first + at, s[0]);  // (the last look at these: the sum may be the residual's own buffer)
-        if (RES && (first + at) * VE < p.C) store16<Ts, VEC>(static_cast<Ts*>(a.sum) + row * p.C, first + at, p.C, s[0]);
-        finish(first + at, s[0]);
-      }
+      put<BLOCK>(p, row, v, v < vectors, s, t);
     }
   }
-  clear_behind(p.scales, p.rows, p.tiles, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
+  clear_behind(p.scales, p.rows, p.tiles, blockIdx.x * kNormThreads + threadIdx.x, gridDim.x * kNormThreads);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -409,23 +367,22 @@ Bounds bounds_of(const void* p, int64_t rows, int64_t stride, int64_t C, int siz
   return p && stride >= 0 ? Bounds{begin, begin + ((rows - 1) * stride + C) * size} : Bounds{};
 }
 
-struct Shares {
-  int shift;
-  dim3 grid;
-};
-// Lanes of a row's piece: a row's vectors where they are few, a warp's where there are rows enough to fill the GPU with warps, otherwise the
-// CTA; the rest of a row goes round, or to other CTAs while there are SMs without one.
-cudaError_t share_out(int64_t rows, int64_t vectors, int least, const void* kernel, Shares* out) {
+// `vectors` a row, at least `least` lanes (a power of two) to it.  A row's vectors go to as many lanes, up to a warp's; more where the call is too small for all CTAs.
+cudaError_t share_out(int64_t rows, int64_t vectors, int least, const void* kernel, Units* u, unsigned* grid) {
   Residency r = {};
   const cudaError_t err = residency(kernel, kThreads, 0, &r);
   if (err != cudaSuccess) return err;
   const int64_t resident = (int64_t)r.per_sm * r.sms;
-  const int most = rows * 32 >= resident * kThreads ? 5 : 8;
   int shift = 0;
-  while (1 << shift < least || (shift < most && 1 << shift < vectors)) ++shift;
-  const int64_t need = (rows + (kThreads >> shift) - 1) / (kThreads >> shift), pieces = (vectors + (1 << shift) - 1) >> shift;
-  out->shift = shift;
-  out->grid = dim3((unsigned)std::min(need, resident), (unsigned)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(pieces, 65535), resident / need)));
+  while (1 << shift < least || (shift < 5 && 1 << shift < vectors)) ++shift;
+  // (few rows leave lanes of a CTA without one)
+  while (shift < 8 && rows < kThreads >> shift && 1 << shift < vectors) ++shift;
+  const int64_t high = (rows + (kThreads >> shift) - 1) / (kThreads >> shift);
+  u->shift = shift;
+  u->pieces = (int)((vectors + (1 << shift) - 1) >> shift);
+  *grid = (unsigned)std::min<int64_t>(high * u->pieces, resident);
+  u->over = (int)(*grid / u->pieces);
+  u->rest = (int)(*grid % u->pieces);
   return cudaSuccess;
 }
 
@@ -480,10 +437,11 @@ int gnb200_quantize_4bit(const void* x, int64_t x_stride, int64_t rows, int64_t 
       return with_flag(vec, [&](auto v) {
         constexpr int BLOCK = decltype(b)::value;
         auto kernel = &quantize_kernel<T, BLOCK, decltype(v)::value>;
-        Shares s;
-        const cudaError_t err = share_out(rows, (int64_t)p.tiles * 4 * kLanes<BLOCK>, 4 * kLanes<BLOCK>, (const void*)kernel, &s);
+        Units u;
+        unsigned grid = 0;
+        const cudaError_t err = share_out(rows, (int64_t)p.tiles * 4 * kLanes<BLOCK>, 4 * kLanes<BLOCK>, (const void*)kernel, &u, &grid);
         if (err != cudaSuccess) return err;
-        kernel<<<s.grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const T*>(x), x_stride, bounds_of(x, rows, x_stride, C, sizeof(T)), p, s.shift);
+        kernel<<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const T*>(x), x_stride, bounds_of(x, rows, x_stride, C, sizeof(T)), p, u);
         return cudaGetLastError();
       });
     });
@@ -506,10 +464,11 @@ int gnb200_dequantize_4bit(const void* codes, const void* scales, int64_t rows, 
     return with_block(block, [&](auto b) {
       return with_flag(vec, [&](auto v) {
         auto kernel = &dequantize_kernel<T, decltype(b)::value, decltype(v)::value>;
-        Shares s;
-        const cudaError_t err = share_out(rows, C / width + 1, 4, (const void*)kernel, &s);
+        Units u;
+        unsigned grid = 0;
+        const cudaError_t err = share_out(rows, vec ? C / width : (C + 2 * width - 2) / width, 4, (const void*)kernel, &u, &grid);
         if (err != cudaSuccess) return err;
-        kernel<<<s.grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p, static_cast<T*>(out), s.shift);
+        kernel<<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p, static_cast<T*>(out), u);
         return cudaGetLastError();
       });
     });
@@ -538,51 +497,26 @@ int gnb200_rms_fwd_4bit(const void* x, int64_t x_stride, const void* residual, i
   a.x = x, a.residual = residual, a.weight = weight, a.sum = sum, a.x_stride = x_stride, a.r_stride = residual_stride, a.w_dtype = weight_dtype;
   a.eps = (float)eps, a.offset = (float)offset, a.inv_c = (float)(1.0 / (double)C);
   a.x_bounds = bounds_of(x, rows, x_stride, C, size_of(dtype)), a.r_bounds = bounds_of(residual, rows, residual_stride, C, size_of(residual_dtype));
-  const bool vec = C % 8 == 0 && on16(x) && on16(residual) && on16(weight) && on16(sum) &&
+  const bool vec = C % 8 == 0 && on16(x) && on16(residual) && on16(sum) &&
                    (rows == 1 || (x_stride * size_of(dtype) % 16 == 0 && (!residual || residual_stride * size_of(residual_dtype) % 16 == 0)));
-  const int64_t vectors = (int64_t)p.tiles * 4 * (block / VE);
-  // a warp to a row of four vectors a lane at most, where there are rows for the SMs' warps; else a CTA with one vector a thread, two above 8192
-  // channels; longer rows are read twice
-  const bool warp = vectors <= 128 && rows >= 148 * 8;
-  int V, threads;
-  if (warp) {
-    V = vectors <= 32 ? 1 : vectors <= 64 ? 2 : 4;
-    threads = 128;
-  } else {
-    V = vectors <= 512 ? 1 : vectors <= 2048 ? 2 : 0;
-    threads = V == 0 ? 1024 : (int)((vectors + V - 1) / V + 31) / 32 * 32;
-  }
   return launched(name, with_type(dtype, [&](auto t) {
     using Tx = decltype(t);
-    const auto typed = [&](auto u, auto is_res) {
+    const auto typed = [&](auto u) {
       using Ts = decltype(u);
       return with_block(block, [&](auto b) {
         return with_flag(vec, [&](auto is_vec) {
-          constexpr int BLOCK = decltype(b)::value;
-          constexpr bool VEC = decltype(is_vec)::value, RES = decltype(is_res)::value;
-          const auto go = [&](void (*kernel)(const NormArgs, const FourRows)) {
-            Residency r = {};
-            const cudaError_t err = residency((const void*)kernel, threads, 0, &r);
-            if (err != cudaSuccess) return err;
-            const int64_t need = warp ? (rows + 3) / 4 : rows;
-            kernel<<<(unsigned)std::min<int64_t>(need, (int64_t)r.per_sm * r.sms), threads, 0, static_cast<cudaStream_t>(stream)>>>(a, p);
-            return cudaGetLastError();
-          };
-          if (warp) {
-            if (V == 1) return go(&norm_kernel<Tx, Ts, BLOCK, 1, true, VEC, RES>);
-            if (V == 2) return go(&norm_kernel<Tx, Ts, BLOCK, 2, true, VEC, RES>);
-            return go(&norm_kernel<Tx, Ts, BLOCK, 4, true, VEC, RES>);
-          }
-          if (V == 1) return go(&norm_kernel<Tx, Ts, BLOCK, 1, false, VEC, RES>);
-          if (V == 2) return go(&norm_kernel<Tx, Ts, BLOCK, 2, false, VEC, RES>);
-          return go(&norm_kernel<Tx, Ts, BLOCK, 0, false, VEC, RES>);
+          auto kernel = &norm_any_kernel<Tx, Ts, decltype(b)::value, decltype(is_vec)::value>;
+          Residency r = {};
+          const cudaError_t err = residency((const void*)kernel, kNormThreads, 0, &r);
+          if (err != cudaSuccess) return err;
+          kernel<<<(unsigned)std::min<int64_t>(rows, (int64_t)r.per_sm * r.sms), kNormThreads, 0, static_cast<cudaStream_t>(stream)>>>(a, p);
+          return cudaGetLastError();
         });
       });
     };
-    if (!residual) return typed(Tx(), std::false_type());
     if constexpr (!std::is_same<Tx, float>::value)
-      if (residual_dtype == GNB200_F32) return typed(float(), std::true_type());
-    return typed(Tx(), std::true_type());
+      if (residual && residual_dtype == GNB200_F32) return typed(float());
+    return typed(Tx());
   }));
 }
 

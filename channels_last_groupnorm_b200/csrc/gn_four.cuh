@@ -111,7 +111,7 @@ __device__ __forceinline__ void clear_behind(uint8_t* scales, long long all_rows
   for (unsigned i = thread; i < all; i += threads) *reinterpret_cast<uint4*>(last + (size_t)(i / lanes) * kScaleTile + (rows + i % lanes) * 16) = make_uint4(0, 0, 0, 0);
 }
 
-// gnb200_rms_fwd_4bit of aligned rows of whole blocks of 32 channels on the kernels of gn_rms.cu; cudaErrorInvalidValue: not rows of theirs
+// gnb200_rms_fwd_4bit on the kernels of gn_rms.cu; cudaErrorInvalidValue: rows without a common frame or longer than these hold
 struct FourNorm {
   const void *x, *residual, *weight;
   void* sum;

@@ -287,7 +287,8 @@ constexpr int kMostBlocks = 512;  // of the rows that these kernels take
 enum Output { kPlain = 0, kCodes8 = 1, kCodes4 = 2 };
 
 // THREADS: the CTA's at most; kWarpThreads where a row has a group of lanes, otherwise a row has the CTA
-// OUT: y in x's type, 8-bit codes, 4-bit codes (aligned rows of whole blocks of 32 channels; `rstd` is the tensor's scale then, `blocks` the tiles of scales along a row)
+// OUT: y in x's type, 8-bit codes, 4-bit codes (`rstd` is the tensor's scale then, `scale` the tiles, `blocks` how many lie along a row).  Blocks of 4-bit codes
+// begin at channel 0: of a ragged row they are taken out of the line that its sum went through.
 template <typename Tx, typename Ts, int VE, int V, int THREADS, int OUT, bool RES, bool RAGGED>
 __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
   constexpr bool WARP = THREADS == kWarpThreads, STAGED = kStaged<Tx, Ts, VE, V, THREADS>;
@@ -339,7 +340,9 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
   if constexpr (STAGED)
     for (int i = 1; i < p.stages; ++i) ask();
   float w[V][VE];
-  fetch_weight<VE, V, RAGGED>(w, p.weight, p.w_dtype, p.offset, frame, first, lanes);
+  Frame<VE, RAGGED> weights = frame;
+  if constexpr (OUT == kCodes4) weights.skew = 0, weights.nvec = (p.C + VE - 1) / VE;
+  fetch_weight<VE, V, RAGGED>(w, p.weight, p.w_dtype, p.offset, weights, first, lanes);
   if constexpr (!WARP) clear<false>(slots, lanes, 0, first);
   int turn = 0;
   long long row = at.row;
@@ -399,6 +402,16 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
     const float all_sq = WARP ? lanes_sum(sq[0] + sq[1], lanes) : team_sum<false>(sq[0] + sq[1], slots, turn, lanes, 0);
     const float rstd = __frsqrt_rn(fmaf(all_sq, p.inv_c, p.eps));
     if (OUT != kCodes4 && p.rstd && live && first == 0) p.rstd[row] = rstd;
+    if constexpr (OUT == kCodes4 && RAGGED) {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const int c = (first + v * lanes) * VE + e;
+          s[v][e] = live && c < p.C ? at.line[frame.skew + c] : 0.f;
+        }
+      at.meet();  // (the next row's line is written behind these looks at it)
+    }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       scale_each(s[v], rstd);
@@ -412,23 +425,20 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
       }
     } else if constexpr (OUT == kCodes4) {
       const TensorScale tensor(p.block == 16 ? p.rstd : nullptr);
-      const int share = p.block / VE;
+      const int share = p.block / VE, wide = (int)four_wide(p.C) / VE;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const int i = first + v * lanes;
-        const bool inside = live && i < nvec;
-        float most = 0.f;
-        if (i < nvec) {  // (beyond the row a NaN rstd would leave NaN in the zeros)
+        const bool inside = live && i < wide;
+        float y[8], most = 0.f;
 #pragma unroll
-          for (int e = 0; e < VE; ++e) most = larger(most, fabsf(s[v][e]));
-        }
+        for (int e = 0; e < 8; ++e) y[e] = e < VE && (RAGGED ? i * VE + e < p.C : i < nvec) ? s[v][e] : 0.f;  // (beyond the row a NaN rstd would leave NaN in the zeros)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) most = larger(most, fabsf(y[e]));
         const float all = __uint_as_float(lanes_max(magnitude(most), share));
         const FourStep step = p.block == 16 ? four_step<16>(all, tensor) : four_step<32>(all, tensor);
-        float y[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = e < VE ? s[v][e] : 0.f;
         const uint32_t word = p.block == 16 ? codes8<16>(y, step) : codes8<32>(y, step);
-        uint8_t* const to = static_cast<uint8_t*>(p.y) + (row * nvec + i) * (VE / 2);
+        uint8_t* const to = static_cast<uint8_t*>(p.y) + (row * wide + i) * (VE / 2);
         if (inside) {
           if constexpr (VE == 8)
             *reinterpret_cast<uint32_t*>(to) = word;
@@ -436,7 +446,7 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
             *reinterpret_cast<uint16_t*>(to) = (uint16_t)word;
         }
         const int block = i / share;
-        uint32_t four = i < nvec ? step.byte << (8 * (block & 3)) : 0;
+        uint32_t four = i < wide ? step.byte << (8 * (block & 3)) : 0;
 #pragma unroll
         for (int k = 1; k <= 2; ++k) {  // of four blocks, where the row has them in this group
           const uint32_t other = __shfl_xor_sync(0xffffffffu, four, k * share);
@@ -960,7 +970,9 @@ cudaError_t launch_rms_fwd(RmsFwd p, int dtype, int sum_dtype, Rows rows, cudaSt
   return with_types(dtype, sum_dtype, [&](auto tx, auto ts) {
     using Tx = decltype(tx);
     using Ts = decltype(ts);
-    RmsGeom g = rms_geometry(p.C, dtype, rows, false);
+    int64_t lanes_for = p.C;  // channels that a row's lanes have to do with
+    if (OUT == kCodes4) lanes_for = std::max<int64_t>(p.C, four_wide(p.C) - (rows == kRagged ? 2 * (16 / (int)sizeof(Tx)) - 2 : 0));
+    RmsGeom g = rms_geometry(lanes_for, dtype, rows, false);
     bool staged = false;
     auto go = [&](void (*kernel)(const RmsFwd)) {
       RmsLaunch l = {};
@@ -977,12 +989,9 @@ cudaError_t launch_rms_fwd(RmsFwd p, int dtype, int sum_dtype, Rows rows, cudaSt
         constexpr int VE = decltype(ve)::value, V = decltype(v)::value, THREADS = decltype(most)::value;
         constexpr bool RAGGED = decltype(ragged)::value;
         staged = kStaged<Tx, Ts, VE, V, THREADS>;
-        if constexpr (OUT == kCodes4 && RAGGED) return cudaErrorInvalidValue;
-        else {
-          if constexpr (std::is_same<Tx, Ts>::value)
-            if (!p.residual) return go(&rms_fwd_kernel<Tx, Ts, VE, V, THREADS, OUT, false, RAGGED>);
-          return go(&rms_fwd_kernel<Tx, Ts, VE, V, THREADS, OUT, true, RAGGED>);
-        }
+        if constexpr (std::is_same<Tx, Ts>::value)
+          if (!p.residual) return go(&rms_fwd_kernel<Tx, Ts, VE, V, THREADS, OUT, false, RAGGED>);
+        return go(&rms_fwd_kernel<Tx, Ts, VE, V, THREADS, OUT, true, RAGGED>);
       });
       if (OUT == kCodes4 || err != cudaErrorInvalidValue) return err;
       g = RmsGeom{1, 0, kMostThreads, kMostThreads, false, false, 0};
@@ -1080,18 +1089,17 @@ int launched(const char* name, cudaError_t err) {
 }  // namespace
 
 cudaError_t launch_rms_4bit(const FourNorm& n, cudaStream_t stream) {
-  if (n.C % kFourUnit != 0) return cudaErrorInvalidValue;
-  const int size = size_of(n.dtype), wide = size_of(n.residual_dtype);
-  if (rows_of(n.dtype == GNB200_F32 ? 4 : 8, n.C, n.rows, n.weight,
-              {{n.x, n.x_stride, size}, {n.residual, n.r_stride, wide}, {n.sum, n.C, wide}}) != kAligned)
-    return cudaErrorInvalidValue;
+  const int size = size_of(n.dtype), wide = size_of(n.residual_dtype), width = n.dtype == GNB200_F32 ? 4 : 8;
+  const Rows how = rows_of(width, n.C, n.rows, n.weight, {{n.x, n.x_stride, size}, {n.residual, n.r_stride, wide}, {n.sum, n.C, wide}});
+  if (how == kAny) return cudaErrorInvalidValue;
   RmsFwd p = {};
   p.x = n.x, p.residual = n.residual, p.weight = n.weight, p.y = n.codes, p.sum = n.sum;
   p.rstd = const_cast<float*>(n.tensor_scale), p.scale = reinterpret_cast<float*>(n.scales);
   p.rows = n.rows, p.x_stride = n.x_stride, p.r_stride = n.r_stride;
   p.C = n.C, p.w_dtype = n.weight_dtype, p.block = n.block, p.blocks = (int)four_tiles(n.C, n.block);
   p.eps = (float)n.eps, p.offset = (float)n.offset, p.inv_c = (float)(1.0 / (double)n.C);
-  return launch_rms_fwd<kCodes4>(p, n.dtype, n.residual_dtype, kAligned, stream);
+  p.edge = edge_of(width, {{n.x, n.x_stride, size}, {n.residual, n.r_stride, wide}});
+  return launch_rms_fwd<kCodes4>(p, n.dtype, n.residual_dtype, how, stream);
 }
 
 cudaError_t launch_column_sums(const ColumnSums& p, int sets, cudaStream_t stream, bool chained) {
