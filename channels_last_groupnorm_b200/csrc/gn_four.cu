@@ -29,7 +29,7 @@ __device__ __forceinline__ void put(const FourRows& p, long long row, int v, boo
   constexpr int LANES = kLanes<BLOCK>;
   float most = 0.f;
 #pragma unroll
-  for (int e = 0; e < VE; ++e) most = larger(most, fabsf(y[e]));
+  for (int e = 0; e < VE; e += 2) most = largest(most, y[e], y[e + 1]);
   if constexpr (LANES > 1) most = larger(most, __shfl_xor_sync(0xffffffffu, most, 1));
   const FourStep step = four_step<BLOCK>(most, t);
   const uint2 words = make_uint2(codes8<BLOCK>(y, step), codes8<BLOCK>(y + 8, step));

@@ -42,6 +42,12 @@ __device__ __forceinline__ float scale_value(uint32_t byte, int block) {
   if (block == 16) return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
   return byte == 0xff ? __uint_as_float(0x7fc00000u) : byte == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);  // (2^-127 is subnormal)
 }
+// the largest magnitude of three, or NaN where one is
+__device__ __forceinline__ float largest(float a, float b, float c) {
+  float m;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
+}
 // The tensor's scale and what is made of it once
 struct TensorScale {
   float g, six, inverse;  // 6 g and its reciprocal

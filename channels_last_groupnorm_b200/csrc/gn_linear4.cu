@@ -431,11 +431,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     if (rank == 0 && one_lane()) {
       int n = 0, turn = 0;
       for (int t = first; t < tiles; t += pairs, ++turn) {
-        if (turn > 0) {
-          producer_wait(&taken, (turn - 1) & 1, &gave_up, p.l.wait);
-          if (*(volatile int*)&gave_up) break;
-          fence_after();
-        }
         for (int k = 0; k < ktiles; ++k, ++n) {
           const int s = n % kPairStages;
           producer_wait(&full[s], (n / kPairStages) & 1, &gave_up, p.l.wait);
@@ -450,6 +445,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             copy_scales<true>(xs + 4 * c, smem_desc(from, 128, 0));
 #pragma unroll
             for (int h = 0; h < L::kHigh; ++h) copy_scales<true>(ws + 4 * (L::kHigh * c + h), smem_desc(from + (1 + h) * L::kScales, 128, 0));
+          }
+          if (k == 0 && turn > 0) {  // the sums of the tile before are in registers
+            producer_wait(&taken, (turn - 1) & 1, &gave_up, p.l.wait);
+            if (*(volatile int*)&gave_up) break;
+            fence_after();
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -477,7 +477,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       tile_at<NF>(p, t, token, feature);
       token += rank * 128 + (warp & 3) * 32;
       feature += (warp >> 2) * MINE;
-      const bool whole = consumer_wait(&sums, turn & 1, &gave_up, p.l.wait);
+      bool whole = false;
+      for (int tries = 0; tries < 64 && !whole; ++tries) whole = __all_sync(0xffffffffu, mbar_try_wait(&sums, turn & 1));  // (all lanes: one poll less than by way of lane 0)
+      if (!whole) whole = consumer_wait(&sums, turn & 1, &gave_up, p.l.wait);
       fence_after();
       __syncwarp();
       float f[MINE];

@@ -284,20 +284,23 @@ struct Place {
 template <typename Tx, typename Ts, int VE, int V, int THREADS>
 constexpr bool kStaged = THREADS > kWarpThreads && (THREADS > 512 || V * VE * (sizeof(Tx) + sizeof(Ts)) > 64);
 constexpr int kMostBlocks = 512;  // of the rows that these kernels take
-enum Output { kPlain = 0, kCodes8 = 1, kCodes4 = 2 };
+enum Output { kPlain = 0, kCodes8 = 1, kCodes4Of16 = 2, kCodes4Of32 = 3 };  // (4-bit codes in blocks of 16 or 32)
+__host__ __device__ constexpr bool is_four(int out) { return out >= kCodes4Of16; }
 
 // THREADS: the CTA's at most; kWarpThreads where a row has a group of lanes, otherwise a row has the CTA
 // OUT: y in x's type, 8-bit codes, 4-bit codes (`rstd` is the tensor's scale then, `scale` the tiles, `blocks` how many lie along a row).  Blocks of 4-bit codes
 // begin at channel 0: of a ragged row they are taken out of the line that its sum went through.
+// (4-bit codes: the compiler is held to two CTAs of 512 threads, three or five of 128; 0 leaves it free as no second bound does; left to itself it took 100 registers for the 50 of before a smaller change, and
+// 8192 x 8192 over fp32 158 us in place of 127.)
 template <typename Tx, typename Ts, int VE, int V, int THREADS, int OUT, bool RES, bool RAGGED>
-__global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
+__global__ void __launch_bounds__(THREADS, !is_four(OUT) || THREADS == 1024 ? 0 : THREADS == 512 ? 2 : V == 4 ? 3 : 5) rms_fwd_kernel(const RmsFwd p) {
   constexpr bool WARP = THREADS == kWarpThreads, STAGED = kStaged<Tx, Ts, VE, V, THREADS>;
   extern __shared__ __align__(16) char smem[];
   __shared__ TeamSlots slots;
   __shared__ uint32_t most[32];
   __shared__ uint2 blocks[OUT == kCodes8 && RAGGED ? kMostBlocks : 1];  // maxima of a block's own vectors, of the channels before them
   const Place<WARP, false> at(p.lanes, p.stage_bytes, p.stages, line_bytes(p.C, VE, RAGGED), smem);
-  if constexpr (OUT == kCodes4) grid_dep_launch_dependents();  // (the product that takes the codes)
+  if constexpr (is_four(OUT)) grid_dep_launch_dependents();  // (the product that takes the codes)
   const int lanes = at.lanes, first = at.first;
   const Tx* next_x = static_cast<const Tx*>(p.x) + at.row * p.x_stride;  // the next row to be asked for
   const Ts* next_r = RES ? static_cast<const Ts*>(p.residual) + at.row * p.r_stride : nullptr;
@@ -341,7 +344,7 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
     for (int i = 1; i < p.stages; ++i) ask();
   float w[V][VE];
   Frame<VE, RAGGED> weights = frame;
-  if constexpr (OUT == kCodes4) weights.skew = 0, weights.nvec = (p.C + VE - 1) / VE;
+  if constexpr (is_four(OUT)) weights.skew = 0, weights.nvec = (p.C + VE - 1) / VE;
   fetch_weight<VE, V, RAGGED>(w, p.weight, p.w_dtype, p.offset, weights, first, lanes);
   if constexpr (!WARP) clear<false>(slots, lanes, 0, first);
   int turn = 0;
@@ -401,8 +404,8 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
     ask();  // (a lane's own vectors: read, so free)
     const float all_sq = WARP ? lanes_sum(sq[0] + sq[1], lanes) : team_sum<false>(sq[0] + sq[1], slots, turn, lanes, 0);
     const float rstd = __frsqrt_rn(fmaf(all_sq, p.inv_c, p.eps));
-    if (OUT != kCodes4 && p.rstd && live && first == 0) p.rstd[row] = rstd;
-    if constexpr (OUT == kCodes4 && RAGGED) {
+    if (!is_four(OUT) && p.rstd && live && first == 0) p.rstd[row] = rstd;
+    if constexpr (is_four(OUT) && RAGGED) {
 #pragma unroll
       for (int v = 0; v < V; ++v)
 #pragma unroll
@@ -423,21 +426,24 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
         const int i = first + v * lanes;
         if (live && i < nvec) frame.store(static_cast<Tx*>(p.y) + out_at, i, s[v]);
       }
-    } else if constexpr (OUT == kCodes4) {
-      const TensorScale tensor(p.block == 16 ? p.rstd : nullptr);
-      const int share = p.block / VE, wide = (int)four_wide(p.C) / VE;
+    } else if constexpr (is_four(OUT)) {
+      // (A row whose sum is NaN has NaN for all its scales, those of the channels that fill its last unit up among them.)
+      constexpr int BLOCK = OUT == kCodes4Of16 ? 16 : 32, share = BLOCK / VE;
+      const TensorScale tensor(BLOCK == 16 ? p.rstd : nullptr);
+      const int wide = (int)four_wide(p.C) / VE;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const int i = first + v * lanes;
         const bool inside = live && i < wide;
         float y[8], most = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = e < VE && (RAGGED ? i * VE + e < p.C : i < nvec) ? s[v][e] : 0.f;  // (beyond the row a NaN rstd would leave NaN in the zeros)
+        for (int e = 0; e < 8; ++e) y[e] = e < VE ? s[v][e] : 0.f;
 #pragma unroll
-        for (int e = 0; e < VE; ++e) most = larger(most, fabsf(y[e]));
-        const float all = __uint_as_float(lanes_max(magnitude(most), share));
-        const FourStep step = p.block == 16 ? four_step<16>(all, tensor) : four_step<32>(all, tensor);
-        const uint32_t word = p.block == 16 ? codes8<16>(y, step) : codes8<32>(y, step);
+        for (int e = 0; e < VE; e += 2) most = largest(most, y[e], y[e + 1]);
+#pragma unroll
+        for (int delta = 1; delta < share; delta *= 2) most = larger(most, __shfl_xor_sync(0xffffffffu, most, delta));
+        const FourStep step = four_step<BLOCK>(most, tensor);
+        const uint32_t word = codes8<BLOCK>(y, step);
         uint8_t* const to = static_cast<uint8_t*>(p.y) + (row * wide + i) * (VE / 2);
         if (inside) {
           if constexpr (VE == 8)
@@ -528,7 +534,7 @@ __global__ void __launch_bounds__(THREADS) rms_fwd_kernel(const RmsFwd p) {
       }
     }
   }
-  if constexpr (OUT == kCodes4) clear_behind(reinterpret_cast<uint8_t*>(p.scale), p.rows, p.blocks, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
+  if constexpr (is_four(OUT)) clear_behind(reinterpret_cast<uint8_t*>(p.scale), p.rows, p.blocks, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
 }
 
 // Rows of any length: one CTA per row, element by element, read once for the sum and once more for each thing that needs it.  Outputs are
@@ -971,7 +977,7 @@ cudaError_t launch_rms_fwd(RmsFwd p, int dtype, int sum_dtype, Rows rows, cudaSt
     using Tx = decltype(tx);
     using Ts = decltype(ts);
     int64_t lanes_for = p.C;  // channels that a row's lanes have to do with
-    if (OUT == kCodes4) lanes_for = std::max<int64_t>(p.C, four_wide(p.C) - (rows == kRagged ? 2 * (16 / (int)sizeof(Tx)) - 2 : 0));
+    if (is_four(OUT)) lanes_for = std::max<int64_t>(p.C, four_wide(p.C) - (rows == kRagged ? 2 * (16 / (int)sizeof(Tx)) - 2 : 0));
     RmsGeom g = rms_geometry(lanes_for, dtype, rows, false);
     bool staged = false;
     auto go = [&](void (*kernel)(const RmsFwd)) {
@@ -993,11 +999,11 @@ cudaError_t launch_rms_fwd(RmsFwd p, int dtype, int sum_dtype, Rows rows, cudaSt
           if (!p.residual) return go(&rms_fwd_kernel<Tx, Ts, VE, V, THREADS, OUT, false, RAGGED>);
         return go(&rms_fwd_kernel<Tx, Ts, VE, V, THREADS, OUT, true, RAGGED>);
       });
-      if (OUT == kCodes4 || err != cudaErrorInvalidValue) return err;
+      if (is_four(OUT) || err != cudaErrorInvalidValue) return err;
       g = RmsGeom{1, 0, kMostThreads, kMostThreads, false, false, 0};
       staged = false;
     }
-    if constexpr (OUT == kCodes4)
+    if constexpr (is_four(OUT))
       return cudaErrorInvalidValue;
     else
       return go(&rms_fwd_any_kernel<Tx, Ts, OUT == kCodes8>);
@@ -1099,7 +1105,7 @@ cudaError_t launch_rms_4bit(const FourNorm& n, cudaStream_t stream) {
   p.C = n.C, p.w_dtype = n.weight_dtype, p.block = n.block, p.blocks = (int)four_tiles(n.C, n.block);
   p.eps = (float)n.eps, p.offset = (float)n.offset, p.inv_c = (float)(1.0 / (double)n.C);
   p.edge = edge_of(width, {{n.x, n.x_stride, size}, {n.residual, n.r_stride, wide}});
-  return launch_rms_fwd<kCodes4>(p, n.dtype, n.residual_dtype, how, stream);
+  return n.block == 16 ? launch_rms_fwd<kCodes4Of16>(p, n.dtype, n.residual_dtype, how, stream) : launch_rms_fwd<kCodes4Of32>(p, n.dtype, n.residual_dtype, how, stream);
 }
 
 cudaError_t launch_column_sums(const ColumnSums& p, int sets, cudaStream_t stream, bool chained) {
