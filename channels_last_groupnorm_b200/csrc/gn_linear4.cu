@@ -648,9 +648,10 @@ cudaError_t launch_linear(LinearArgs p, const void* w_codes, const void* x_codes
   if (err == cudaSuccess) err = codes_map(&x_map, x_codes, p.tokens, p.K, NT);
   if (err != cudaSuccess) return err;
   const int64_t tiles = (int64_t)((p.features + kTileM - 1) / kTileM) * ((p.tokens + NT - 1) / NT);
-  // K is shared out until there are CTAs for the SMs and a third more (32 x 4096 x 4096 in clusters of 4 6.4 us, of 2 7.7, of 8 8.0; 8 x 4096 x 6144 6.8, 8.1, 10.6)
+  // K is shared out by two and by four while all CTAs are resident, two an SM (32 x 8192 x 8192 in clusters of 1, 2, 4, 8: 19.4, 14.4, 13.2, 19.5 us; 16 x 4096 x 16384
+  // 13.4, 12.5, 16.5, 25.2), by eight while there is one for two thirds of them (32 x 4096 x 4096 10.7, 7.7, 6.4, 8.0; 4 x 5120 x 1280 11.1, 7.7, 5.5, 4.9).
   int splits = 1;
-  while (splits < kMostSplits && splits * 2 <= ktiles && tiles * splits * 2 * 3 <= 4 * r.sms) splits *= 2;
+  while (splits < kMostSplits && splits * 2 <= ktiles && tiles * splits * 2 <= (splits < 4 ? 2 * r.sms : 4 * r.sms / 3)) splits *= 2;
   if (NT == 16) return launch_tiles<T, 16, BLOCK>(p, w_map, x_map, splits, stream);
   if (NT == 32) return launch_tiles<T, 32, BLOCK>(p, w_map, x_map, splits, stream);
   if (NT == 64) return launch_tiles<T, 64, BLOCK>(p, w_map, x_map, splits, stream);
