@@ -354,6 +354,9 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {
                "h"((uint16_t)3)
                : "memory");
 }
+__device__ __forceinline__ void commit_leader(uint64_t* bar) {  // on this CTA's alone
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
 __device__ __forceinline__ void arrive_at(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -374,7 +377,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                         const __grid_constant__ CUtensorMap ws_map, const PairArgs p) {
   using L = PairLayout<BLOCK, NF>;
   extern __shared__ char raw[];
-  __shared__ __align__(8) uint64_t full[kPairStages], empty[kPairStages], sums, taken;
+  __shared__ __align__(8) uint64_t full[kPairStages], empty[kPairStages], sums, taken, last;
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up;
   char* const stages = raw + (-smem_addr(raw) & 1023u);
@@ -384,6 +387,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     for (int s = 0; s < kPairStages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
     mbar_init(&sums, 1);
     mbar_init(&taken, 16);  // the warps of both CTAs
+    mbar_init(&last, 1);
     gave_up = 0;
     fence_mbar_init_cluster();
   }
@@ -434,7 +438,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         for (int k = 0; k < ktiles; ++k, ++n) {
           const int s = n % kPairStages;
           producer_wait(&full[s], (n / kPairStages) & 1, &gave_up, p.l.wait);
-          if (*(volatile int*)&gave_up) break;
+          if (*(volatile int*)&gave_up) goto end;
           fence_after();
           const uint32_t at = smem_addr(stages) + s * L::kStageAt;
           const uint32_t xs = scales_at + s * L::kColumns, ws = xs + 4 * L::kChunks;
@@ -448,7 +452,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           }
           if (k == 0 && turn > 0) {  // the sums of the tile before are in registers
             producer_wait(&taken, (turn - 1) & 1, &gave_up, p.l.wait);
-            if (*(volatile int*)&gave_up) break;
+            if (*(volatile int*)&gave_up) goto end;
             fence_after();
           }
 #pragma unroll
@@ -462,6 +466,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         }
         commit_pair(&sums);
       }
+    end:
+      // (given up, the sums are not announced: both CTAs' warps give up too and store NaN; no product runs any more when the pair ends)
+      commit_leader(&last);
+      if (!mbar_wait_bounded(&last, 0, p.l.wait)) gave_up = 1;
     }
     __syncwarp();
   } else {

@@ -294,3 +294,33 @@ def test_far_rows():
     assert torch.equal(byte, R.untiled(tiles, 160, c // 32)[-32:])
     y = pkg.dequantize_4bit(codes, scales, c)
     assert torch.equal(y[-32:], pkg.dequantize_4bit(want, tiles, c)[-32:])
+
+
+def test_codes_of_another_maker():
+    """Codes and tiles laid out as documented, without the kernels, are read back and normed rows agree with them after a round trip."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for block in (16, 32):
+        codes = torch.randint(0, 16, (77, 96), device="cuda", generator=g, dtype=torch.uint8)
+        byte = torch.randint(0x30, 0x50, (77, 96 // block), device="cuda", generator=g).to(torch.uint8)
+        kind = torch.float8_e4m3fn if block == 16 else torch.float8_e8m0fnu
+        rows, tiles = R.packed(codes).view(torch.float4_e2m1fn_x2), R.tiled(byte).view(kind)
+        y = pkg.dequantize_4bit(rows, tiles, 96, dtype=F32)
+        assert torch.equal(y.double(), R.values(rows, tiles))
+
+
+def test_rows_behind_the_last_are_left():
+    """Through the C ABI: codes and tiles of a call, and nothing behind them."""
+    from channels_last_groupnorm_b200 import _native as nt
+
+    for rows, c in ((5, 100), (130, 64), (33, 1111)):
+        x = _rows(rows, c, BF16, 1)
+        want = pkg.quantize_4bit(x)
+        norm = pkg.rms_norm_quant_4bit(x)
+        n, m = nt.lib.gnb200_4bit_code_bytes(rows, c), nt.lib.gnb200_4bit_scale_bytes(rows, c, 16)
+        stream = torch.cuda.current_stream().cuda_stream
+        for expect, call in ((want, lambda a, b: nt.lib.gnb200_quantize_4bit(x.data_ptr(), c, rows, c, 2, 16, None, a, b, stream)),
+                             (norm, lambda a, b: nt.lib.gnb200_rms_fwd_4bit(x.data_ptr(), c, None, c, None, rows, c, 1e-6, 0.0, 2, 2, 2, 16, None, a, b, None, stream))):
+            codes, tiles = (torch.full((k + 1024,), 0xA5, dtype=torch.uint8, device="cuda") for k in (n, m))
+            assert call(codes.data_ptr(), tiles.data_ptr()) == 0
+            assert torch.equal(codes[:n], expect[0].view(torch.uint8).reshape(-1)) and torch.equal(tiles[:m], expect[1].view(torch.uint8).reshape(-1))
+            assert (codes[n:] == 0xA5).all() and (tiles[m:] == 0xA5).all()

@@ -211,3 +211,58 @@ def test_module(block):
             assert four.half().weight_scale.dtype == F32 and torch.equal(four.weight_scale, kept)
     with pytest.raises(ValueError, match="expected input"):
         four(x[..., :199])
+
+
+# pairs with tiles of 256 and of 128 features, clusters, single CTAs; outputs whose rows begin anywhere
+@pytest.mark.parametrize("tokens,features,k", [(3000, 1111, 1344), (2100, 1536, 512), (777, 1111, 320), (300, 1110, 2080), (70, 1113, 1056), (9, 2500, 96)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("bias", [False, True])
+def test_sixteen_bits(tokens, features, k, dtype, bias):
+    x, w = _exact(tokens, k, 16, tokens), _exact(features, k, 16, features + 1)
+    b = torch.randint(-64, 64, (features,), device="cuda").to(dtype) if bias else None
+    got = pkg.linear_4bit(*x, *w, bias=b, dtype=dtype)
+    want = R.values(*x) @ R.values(*w).t() + (b.double() if bias else 0.0)
+    assert torch.equal(got, want.to(dtype))  # exact in 32 bits, rounded once
+
+
+def test_outputs_of_any_address():
+    """Through the C ABI: an output that begins off a vector, and what lies around it as it was."""
+    for tokens, features in ((300, 512), (20, 512), (2100, 1536)):
+        x, w = _exact(tokens, 512, 16, 1), _exact(features, 512, 16, 2)
+        want = pkg.linear_4bit(*x, *w)
+        room = torch.full((tokens * features + 64,), 7.0, device="cuda", dtype=BF16)
+        rc = nt.lib.gnb200_linear_4bit(x[0].data_ptr(), x[1].data_ptr(), None, w[0].data_ptr(), w[1].data_ptr(), None, None, tokens, features, 512, 16, 0, 2,
+                                       room.data_ptr() + 2, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        assert torch.equal(room[1:1 + tokens * features].view(tokens, features), want)
+        assert (room[0] == 7).all() and (room[1 + tokens * features:] == 7).all()
+
+
+def test_nothing_is_written_behind():
+    """Rows and features that fill up a tile leave what lies behind the output as it was."""
+    for tokens, features, k in ((130, 131, 256), (1, 1, 32), (17, 129, 544), (2000, 1111, 256)):
+        x, w = _exact(tokens, k, 32, 1), _exact(features, k, 32, 2)
+        room = torch.full((tokens * features + 4096,), 7.0, device="cuda")
+        rc = nt.lib.gnb200_linear_4bit(x[0].data_ptr(), x[1].data_ptr(), None, w[0].data_ptr(), w[1].data_ptr(), None, None, tokens, features, k, 32, 0, 0,
+                                       room.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        assert torch.equal(room[:tokens * features].view(tokens, features).double(), R.values(*x) @ R.values(*w).t())
+        assert (room[tokens * features:] == 7).all()
+
+
+def test_several_streams_at_once():
+    """Calls of all kernels side by side on four streams: the bits of calls one by one."""
+    shapes = [(300, 512, 512), (8, 4096, 2048), (2100, 1536, 512), (64, 1000, 4096)]
+    calls = [(_exact(t, k, 16, t), _exact(n, k, 16, n)) for t, n, k in shapes]
+    want = [pkg.linear_4bit(*x, *w) for x, w in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [[] for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for i, ((x, w), s) in enumerate(zip(calls, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(pkg.linear_4bit(*x, *w))
+    torch.cuda.synchronize()
+    for one, outs in zip(want, got):
+        assert all(torch.equal(one, o) for o in outs)
+    assert nt.wait_timeouts() == 0
