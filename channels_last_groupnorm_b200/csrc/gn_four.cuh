@@ -82,14 +82,16 @@ __device__ __forceinline__ FourStep four_step(float most, const TensorScale& t) 
 // 8 codes
 template <int BLOCK>
 __device__ __forceinline__ uint32_t codes8(const float* y, const FourStep& step) {
+  // (block 16: of the negative quotient, so that its correction takes the remainder y - q d with no sign to be turned for each, and a zero keeps its own)
+  const float inverse = BLOCK == 16 ? -step.inverse : step.inverse;
   float q[8];
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
-    mul2(q[e], q[e + 1], y[e], y[e + 1], step.inverse, step.inverse);
+    mul2(q[e], q[e + 1], y[e], y[e + 1], inverse, inverse);
     if constexpr (BLOCK == 16) {
       float r0, r1;
-      fma2(r0, r1, q[e], q[e + 1], step.value, step.value, -y[e], -y[e + 1]);
-      fma2(q[e], q[e + 1], r0, r1, -step.inverse, -step.inverse, q[e], q[e + 1]);
+      fma2(r0, r1, q[e], q[e + 1], step.value, step.value, y[e], y[e + 1]);
+      fma2(q[e], q[e + 1], r0, r1, inverse, inverse, q[e], q[e + 1]);
     }
   }
   uint32_t word;
@@ -99,7 +101,7 @@ __device__ __forceinline__ uint32_t codes8(const float* y, const FourStep& step)
       "mov.b32 %0, {a, b, c, d};\n\t}"
       : "=r"(word)
       : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
-  return word;
+  return BLOCK == 16 ? word ^ 0x88888888u : word;
 }
 // The scales of four blocks, one word, of row `row` and tile `tile`; zeros for the rows of its 16 bytes that are not there.
 __device__ __forceinline__ void put_scales(uint8_t* scales, long long row, long long rows, int tile, int tiles, uint32_t word) {
