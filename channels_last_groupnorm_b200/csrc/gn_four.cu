@@ -367,8 +367,9 @@ Bounds bounds_of(const void* p, int64_t rows, int64_t stride, int64_t C, int siz
   return p && stride >= 0 ? Bounds{begin, begin + ((rows - 1) * stride + C) * size} : Bounds{};
 }
 
-// `vectors` a row, at least `least` lanes (a power of two) to it.  A row's vectors go to as many lanes, up to a warp's; more where the call is too small for all CTAs.
-cudaError_t share_out(int64_t rows, int64_t vectors, int least, const void* kernel, Units* u, unsigned* grid) {
+// `vectors` a row, at least `least` lanes (a power of two) to it; `waves` times the CTAs that are resident, which evens out what the SMs differ in (to four bits 16384 x 8192
+// bf16 in blocks of 16 72 us with one, 65 with three, 66 with eight; back one is the best).  A row's vectors go to as many lanes, up to a warp's; more where the call is too small for all CTAs.
+cudaError_t share_out(int64_t rows, int64_t vectors, int least, int waves, const void* kernel, Units* u, unsigned* grid) {
   Residency r = {};
   const cudaError_t err = residency(kernel, kThreads, 0, &r);
   if (err != cudaSuccess) return err;
@@ -380,7 +381,7 @@ cudaError_t share_out(int64_t rows, int64_t vectors, int least, const void* kern
   const int64_t high = (rows + (kThreads >> shift) - 1) / (kThreads >> shift);
   u->shift = shift;
   u->pieces = (int)((vectors + (1 << shift) - 1) >> shift);
-  *grid = (unsigned)std::min<int64_t>(high * u->pieces, resident);
+  *grid = (unsigned)std::min<int64_t>(high * u->pieces, waves * resident);
   u->over = (int)(*grid / u->pieces);
   u->rest = (int)(*grid % u->pieces);
   return cudaSuccess;
@@ -439,7 +440,7 @@ int gnb200_quantize_4bit(const void* x, int64_t x_stride, int64_t rows, int64_t 
         auto kernel = &quantize_kernel<T, BLOCK, decltype(v)::value>;
         Units u;
         unsigned grid = 0;
-        const cudaError_t err = share_out(rows, (int64_t)p.tiles * 4 * kLanes<BLOCK>, 4 * kLanes<BLOCK>, (const void*)kernel, &u, &grid);
+        const cudaError_t err = share_out(rows, (int64_t)p.tiles * 4 * kLanes<BLOCK>, 4 * kLanes<BLOCK>, 3, (const void*)kernel, &u, &grid);
         if (err != cudaSuccess) return err;
         kernel<<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const T*>(x), x_stride, bounds_of(x, rows, x_stride, C, sizeof(T)), p, u);
         return cudaGetLastError();
@@ -466,7 +467,7 @@ int gnb200_dequantize_4bit(const void* codes, const void* scales, int64_t rows, 
         auto kernel = &dequantize_kernel<T, decltype(b)::value, decltype(v)::value>;
         Units u;
         unsigned grid = 0;
-        const cudaError_t err = share_out(rows, vec ? C / width : (C + 2 * width - 2) / width, 4, (const void*)kernel, &u, &grid);
+        const cudaError_t err = share_out(rows, vec ? C / width : (C + 2 * width - 2) / width, 4, 1, (const void*)kernel, &u, &grid);
         if (err != cudaSuccess) return err;
         kernel<<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p, static_cast<T*>(out), u);
         return cudaGetLastError();
