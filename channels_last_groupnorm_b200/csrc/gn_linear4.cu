@@ -1,11 +1,15 @@
 // Product of two matrices in four bits (layout: gn_four.cuh): out[token][feature] = alpha * sum over k of x[token][k] w[feature][k] + bias, sums in
 // fp32 in tensor memory, alpha the product of the two tensors' own scales, one rounding at the end.
 //
-// tcgen05.mma with block scales: the weight is the A operand, so that a tile has 128 features by any number of tokens, and few tokens cost
-// little.  A producer thread brings K tiles of 256 codes (128 bytes a row, swizzled) by TMA and their scales by bulk copies; one thread
-// copies the scales of a stage to tensor memory and multiplies; four warps take the sums out.
-// Where a grid of tiles leaves SMs idle the K tiles are shared out over a cluster, whose sums are added over distributed shared memory in
-// the order of their ranks.
+// Products of e2m1 codes with their block scales on tcgen05.mma, operands by TMA in K tiles of 256 codes (128 bytes a row, swizzled), block scales by
+// copies of their 512-byte tiles to tensor memory, sums in tensor memory.  One thread loads, one multiplies, the others take the sums out.  Two kernels:
+//
+//   few tokens    the weight is the A operand: a tile has 128 features by all tokens up to 128, and what it costs is the weight's bytes.  Bound by HBM where the
+//                 weight is large (8 x 5120 x 20480 14.3 us, 4.1 TB/s; floor 9.1), by the way there and back where it is not (1 x 4096 x 4096 5.6 us, floor 1.4): launch,
+//                 one trip to memory, the cluster's meeting.  Where the tiles leave SMs idle, the K tiles are shared out over a cluster, whose sums are added over
+//                 distributed shared memory in the order of their ranks; the weight's first K tiles are asked into L2 while the kernel before still runs.
+//   many tokens   pairs of CTAs, 256 tokens by 256 or 128 features (below).  8192^3 226 us = 4.9 PFLOP/s in a short run, of 5.9 that the vendor's library reaches; at
+//                 length the GPU's 1000 W bound it, 262 us at 1.49 GHz (the library 217).  The products alone would take 136.
 #include <cuda.h>
 
 #include <algorithm>
@@ -314,7 +318,9 @@ __global__ void __launch_bounds__(kThreads, 2) linear4_kernel(const __grid_const
 // A pair of SMs multiplies 256 tokens (A, 128 of them an SM) by 256 features (B, half of them in either SM's shared memory), so that an SM brings
 // half of what a tile of its own of 128 x 256 would take.  Persistent: the loads run ahead into the next tile, whose products begin as soon as
 // eight warps have the sums in registers; these round and store them meanwhile, rows of 256 bytes, through a corner of shared memory of each
-// warp's own.
+// warp's own.  Tensor memory holds one tile's sums (256 columns) and the scales of four stages (192), not two tiles' sums: a tile's 13 us at K = 8192 have some
+// 1 us in which the sums are on their way out and nothing is multiplied.
+// ns a K tile of 256 (8192^3 in blocks of 16, parts left out to time the others): products 303, with the scales' copies 360, with the loads 420.
 constexpr int kPairThreads = 320;  // eight warps for the sums, one to load, one to multiply
 constexpr int kPairTokens = 256;   // of a pair's tile
 constexpr int kPairStages = 4;
