@@ -13,7 +13,6 @@
 namespace gnb200 {
 namespace {
 
-constexpr int kThreads = 256;
 constexpr long long kNear = 1ll << 33;  // elements up to which 32 bits count the counters, the grid's last steps included
 
 struct DropoutArgs {
@@ -56,21 +55,26 @@ __device__ __forceinline__ float add_kept(float acc, float x, float scale, uint3
 // Vectors of 16 bytes of the wider type, 8 elements or 4, and 16 elements that a thread has under way: four chains of products hide their latency.
 template <typename Ti, typename To>
 constexpr int kVector = sizeof(Ti) == 4 || sizeof(To) == 4 ? 4 : 8;
+// Threads of a CTA at most: 16384 x 4096 bf16 with and without a residual 69.5 and 65 us with 256, 65 and 62 with 512, 64.5 and 60 with 1024; fp32 127, 124.5, 141.
+// Small calls take 256, to reach more SMs.
+template <typename Ti, typename To>
+constexpr int kMostThreads = kVector<Ti, To> == 8 ? 1024 : 512;
+constexpr int kFewThreads = 256;
 
 // VEC: tensors begin on vector boundaries and are taken a vector at a time, but for their end; otherwise element by element.  I: an index of counters.
 // What a thread needs from memory is asked for in front of its words and unpacked behind them (unpacked in front: bf16 with a residual 83 us, so 66).
-// Bound by HBM with a residual (16384 x 4096 bf16 66 us of 61, fp32 123 of 123); without one, in 16 bits, by the products: 62 us of 41.
+// Bound by HBM with a residual (16384 x 4096 bf16 61 us of 61, fp32 123 of 123); without one, in 16 bits, by the products: 56 us of 41.
 template <typename Ti, typename To, bool RES, bool VEC, typename I>
-__global__ void __launch_bounds__(kThreads) dropout_kernel(const DropoutArgs p) {
+__global__ void __launch_bounds__(kMostThreads<Ti, To>) dropout_kernel(const DropoutArgs p) {
   constexpr int VE = kVector<Ti, To>, AT_ONCE = VEC ? 16 / VE : 1;
   const Ti* in = static_cast<const Ti*>(p.in);
   const To* res = static_cast<const To*>(p.residual);
   To* out = static_cast<To*>(p.out);
   const Philox philox(p.seed_at ? *p.seed_at : p.seed, p.layer);
-  const I vectors = (I)((p.n + VE - 1) / VE), step = gridDim.x * kThreads;
+  const I vectors = (I)((p.n + VE - 1) / VE), step = gridDim.x * blockDim.x;
   const float scale = p.scale;
   const uint32_t least = p.least;
-  for (I v = blockIdx.x * kThreads + threadIdx.x; v < vectors; v += AT_ONCE * step) {
+  for (I v = blockIdx.x * blockDim.x + threadIdx.x; v < vectors; v += AT_ONCE * step) {
     Pack<Ti, VE> x[AT_ONCE];
     Pack<To, VE> r[AT_ONCE];
 #pragma unroll
@@ -118,12 +122,14 @@ bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 template <typename Ti, typename To, bool RES>
 cudaError_t launch_dropout(const DropoutArgs& p, cudaStream_t stream) {
   const auto go = [&](void (*kernel)(const DropoutArgs)) {
+    constexpr int VE = kVector<Ti, To>, most = kMostThreads<Ti, To>;
     Residency r = {};
-    const cudaError_t err = residency((const void*)kernel, kThreads, 0, &r);
+    cudaError_t err = residency((const void*)kernel, most, 0, &r);
     if (err != cudaSuccess) return err;
-    constexpr int VE = kVector<Ti, To>;
-    const long long need = ((p.n + VE - 1) / VE + kThreads - 1) / kThreads;
-    kernel<<<(unsigned)std::min<long long>(need, (long long)r.per_sm * r.sms), kThreads, 0, stream>>>(p);
+    const long long vectors = (p.n + VE - 1) / VE;
+    const int threads = vectors >= (long long)r.per_sm * r.sms * most ? most : kFewThreads;
+    if (threads != most && (err = residency((const void*)kernel, threads, 0, &r)) != cudaSuccess) return err;
+    kernel<<<(unsigned)std::min<long long>((vectors + threads - 1) / threads, (long long)r.per_sm * r.sms), threads, 0, stream>>>(p);
     return cudaGetLastError();
   };
   const bool vec = on16(p.in) && on16(p.residual) && on16(p.out);  // (8 bytes do for the narrow side of two types)
