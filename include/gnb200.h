@@ -310,7 +310,8 @@ int gnb200_rotary_bwd(const gnb200_rotary_args* args, const void* dq, const int6
  * for 128 rows and 4 blocks, byte (r % 32) * 16 + r % 128 / 32 * 4 + b % 4 of a tile; a row's tiles lie behind one another, then come those of the
  * next 128 rows; zeros for rows and blocks that are not there (gnb200_4bit_scale_bytes for all of them).  Codes and scales begin on 16 bytes.
  * gnb200_quantize_4bit: rows of x, x_stride elements apart.  gnb200_dequantize_4bit: contiguous rows of C values code * s * g, rounded once.
- * gnb200_rms_fwd_4bit: gnb200_rms_fwd (in place as there) with its y, not rounded before, as codes and scales.
+ * gnb200_rms_fwd_4bit: gnb200_rms_fwd (`sum` in place as there) with its y, not rounded before, as codes and scales.  A row whose sum is NaN has NaN scales
+ *   throughout, those of the channels that fill its last unit of 32 up among them.
  * gnb200_linear_4bit: out[tokens][features] = sum over channels of x * w, + bias (NULL: none; any of the three types): both operands codes and scales of
  *   the same block, sums in fp32, one rounding to dtype.  It waits inside the kernel as the group norm does (bounded; see below).
  */
