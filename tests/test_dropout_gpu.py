@@ -240,6 +240,35 @@ def test_module_and_nothing():
     assert pkg.dropout_add(x[0, 0], p=0.0).shape == ()
 
 
+def test_one_tensor_in_both_places():
+    x, _, ds = _inputs((9, 40), F32, F32)
+    x.requires_grad_(True)
+    g, = torch.autograd.grad(pkg.dropout_add(x, x, 0.25, 3), x, ds)
+    kept = D.kept(x.numel(), 0.25, 3, device="cuda").view(x.shape)
+    want = ds.double() + torch.where(kept, ds.double() / 0.75, 0.0)
+    ref.within(g, want, 6 * ref.U32 * want.abs() + 6 * ref.U32 * ds.double().abs())
+
+
+def test_graphs_that_are_kept_and_dropped():
+    """Twice through a graph that is kept; an error the second time where the seed, which it holds, is gone; hooks on what is saved; a checkpoint."""
+    from torch.utils.checkpoint import checkpoint
+
+    x, r, ds = _inputs((9, 40), BF16, BF16)
+    x.requires_grad_(True)
+    seed = torch.tensor([6], device="cuda")
+    want, = torch.autograd.grad(pkg.dropout_add(x, r, 0.25, 6, 1), x, ds)
+    s = pkg.dropout_add(x, r, 0.25, seed, 1)
+    for keep in (True, False):
+        assert torch.equal(torch.autograd.grad(s, x, ds, retain_graph=keep)[0], want)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(s, x, ds)
+    with torch.autograd.graph.save_on_cpu():
+        s = pkg.dropout_add(x, r, 0.25, seed, 1)
+    assert torch.equal(torch.autograd.grad(s, x, ds)[0], want)
+    s = checkpoint(lambda t: pkg.dropout_add(t, r, 0.25, seed, 1), x, use_reentrant=False)
+    assert torch.equal(torch.autograd.grad(s, x, ds)[0], want)
+
+
 @pytest.mark.parametrize("n", [2 ** 32 + 4096, 2 ** 34 + 4104])
 def test_far_elements(n):
     """Elements, and counters, of more than 32 bits."""
