@@ -1,7 +1,7 @@
 // Rows in four bits, shared by the kernels that make them (gn_four.cu) and multiply them (gn_linear4.cu): e2m1 codes, two a byte, the first
 // one low, and block scales in tiles.
 //
-//   block 16: scale s in e4m3, d = s * g with the tensor's own scale g in fp32:  s = e4m3(max |y| / (6 g)), in 2^-9 .. 448
+//   block 16: scale s in e4m3, d = s * g with the tensor's own scale g in fp32, 2^-100 .. 2^117:  s = e4m3(max |y| / (6 g)), in 2^-9 .. 448
 //   block 32: scale d = 2^(floor(log2 max |y|) - 2) in e8m0, no g
 //   code = e2m1(y / d), nearest, ties to the even code, at most 6 in magnitude; a block with a NaN or an infinity has a NaN for its scale
 //
@@ -60,6 +60,7 @@ struct TensorScale {
 struct FourStep {
   float value, inverse;
   uint32_t byte;
+  bool cut;  // the scale is the largest there is: quotients may be infinite
 };
 template <int BLOCK>
 __device__ __forceinline__ FourStep four_step(float most, const TensorScale& t) {
@@ -71,11 +72,13 @@ __device__ __forceinline__ FourStep four_step(float most, const TensorScale& t) 
     step.byte = finite ? __nv_cvt_float_to_fp8(s, __NV_SATFINITE, __NV_E4M3) : 0x7fu;
     step.value = scale_value(step.byte, 16) * t.g;
     step.inverse = reciprocal(step.value);
+    step.cut = q >= 448.f;
   } else {
     const int e = max((int)(__float_as_uint(most) >> 23) - 2, 0);
     step.byte = finite ? (uint32_t)e : 0xffu;
     step.value = 0.f;  // (a product with the inverse, a power of two, is the quotient)
     step.inverse = __uint_as_float((uint32_t)(254 - min(e, 252)) << 23);
+    step.cut = false;
   }
   return step;
 }
@@ -84,13 +87,20 @@ template <int BLOCK>
 __device__ __forceinline__ uint32_t codes8(const float* y, const FourStep& step) {
   // (block 16: of the negative quotient, so that its correction takes the remainder y - q d with no sign to be turned for each, and a zero keeps its own)
   const float inverse = BLOCK == 16 ? -step.inverse : step.inverse;
-  float q[8];
+  float q[8], x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = y[e];
+  if (BLOCK == 16 && step.cut) {  // (what is beyond 8 d has the largest code; an infinite quotient would have a NaN for its correction)
+    const float most = 8.f * step.value;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = fminf(fmaxf(x[e], -most), most);
+  }
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
-    mul2(q[e], q[e + 1], y[e], y[e + 1], inverse, inverse);
+    mul2(q[e], q[e + 1], x[e], x[e + 1], inverse, inverse);
     if constexpr (BLOCK == 16) {
       float r0, r1;
-      fma2(r0, r1, q[e], q[e + 1], step.value, step.value, y[e], y[e + 1]);
+      fma2(r0, r1, q[e], q[e + 1], step.value, step.value, x[e], x[e + 1]);
       fma2(q[e], q[e + 1], r0, r1, inverse, inverse, q[e], q[e + 1]);
     }
   }

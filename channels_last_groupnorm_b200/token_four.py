@@ -67,7 +67,7 @@ def quantize_4bit(x, block=16, scale=None):
     """Rows as 4-bit codes and block scales: (codes, scales).
 
     x: (*, channels) in float32, float16 or bfloat16, read in place as by `rms_norm`.  block 16: the scale of a block is its largest magnitude over 6 *
-    scale, rounded to e4m3, 2^-9 to 448; `scale`, one float32 on the device (None: 1), belongs to the whole tensor.  block 32: the scale
+    scale, rounded to e4m3, 2^-9 to 448; `scale`, one float32 on the device (None: 1) from 2^-100 to 2^117, belongs to the whole tensor.  block 32: the scale
     is 2^(floor(log2(largest magnitude)) - 2), and there is no `scale`.  A code is that of x over its scales, the nearest one, ties to the even
     code, saturating.  A NaN or an infinity makes the scale of its block NaN.  No gradient: it refuses to run where one would be recorded.
     """

@@ -302,8 +302,9 @@ int gnb200_rotary_bwd(const gnb200_rotary_args* args, const void* dq, const int6
 
 /*
  * Rows in four bits: e2m1 codes, two a byte (the first channel in the low half), with a scale for each block of 16 or 32 channels.
- *   block 16: a scale s in e4m3 beside a scale g of the whole tensor, one float on the device (NULL: 1; s * g must not be subnormal).  s = max |x| /
- *     (6 g), at least 2^-9, at most 448, rounded to e4m3; codes are those of x / (s g), product and quotient in fp32 as IEEE rounds them.
+ *   block 16: a scale s in e4m3 beside a scale g of the whole tensor, one float on the device (NULL: 1), from 2^-100 to 2^117: beyond these the
+ *     codes are not specified.  s = max |x| / (6 g), at least 2^-9, at most 448, rounded to e4m3; codes are those of x / (s g), product and quotient in
+ *     fp32 as IEEE rounds them.
  *   block 32: the scale is the power of two 2^(floor(log2 max |x|) - 2), in e8m0, at least 2^-127; no scale of the tensor (NULL).
  *   Codes go to the nearest value, ties to the even code, and saturate at 6.  A NaN or an infinity makes the scale of its block NaN.
  * Codes lie in rows of ceil(C / 32) * 16 bytes (gnb200_4bit_code_bytes for all rows), zeros behind the channels.  Scales lie in tiles of 512 bytes
