@@ -26,7 +26,7 @@ PYTHON_LIB = os.path.join(LIB_DIR, "gnb200_python.so")
 CUDA_SOURCES = ["gn_fwd.cu", "gn_bwd.cu", "gn_wave.cu", "gn_resident.cu", "gn_nchw.cu", "gn_f64.cu", "gn_rms.cu", "gn_rotary.cu", "gn_four.cu", "gn_linear4.cu", "gn_dropout.cu", "gn_plan.cu", "gn_capi.cu", "gn_static_scratch.cu"]
 TORCH_SOURCES = ["gn_torch.cpp", "gn_torch_tokens.cpp", "gn_torch_four.cpp", "gn_torch_dropout.cpp"]
 TORCH_HEADERS = ["gn_torch.h", "gn_torch_rows.h"]
-CUDA_HEADERS = ["gn_common.cuh", "gn_math.cuh", "gn_async.cuh", "gn_reduce.cuh", "gn_peer.cuh", "gn_tokens.cuh", "gn_four.cuh", "gn_rows.h", "gn_kernels.h", os.path.join(INCLUDE_DIR, "gnb200.h")]
+CUDA_HEADERS = ["gn_common.cuh", "gn_math.cuh", "gn_async.cuh", "gn_reduce.cuh", "gn_peer.cuh", "gn_tokens.cuh", "gn_four.cuh", "gn_rows.h", "gn_turns.h", "gn_kernels.h", os.path.join(INCLUDE_DIR, "gnb200.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC"]
 

@@ -19,6 +19,7 @@
 #include "gn_async.cuh"
 #include "gn_four.cuh"
 #include "gn_kernels.h"
+#include "gn_turns.h"
 
 namespace gnb200 {
 namespace {
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 2) linear4_kernel(const __grid_const
         bulk_load(at + L::kA + L::kB, ws + (long long)k * L::kScales, chunks * kScaleTile, &full[s]);
         bulk_load(at + L::kA + L::kB + L::kScales, xs + (long long)k * L::kScales, chunks * kScaleTile, &full[s]);
       }
-      // (nothing is in flight when the CTA ends, given up or not)
+      // (the copies have landed when the CTA ends, given up or not, unless this wait runs out too)
       for (int k = max(0, issued - L::kStages); k < issued; ++k)
         if (!mbar_wait_bounded(&full[k % L::kStages], (k / L::kStages) & 1, p.wait)) gave_up = 1;
     }
@@ -354,11 +355,21 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m
                "l"(map), "r"(x), "r"(y), "r"(bar)
                : "memory");
 }
+// half of a stage's bytes that never come
+__device__ __forceinline__ void mbar_complete_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
+}
 // on the barriers of both CTAs, when all products so far are done
 __device__ __forceinline__ void commit_pair(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(bar)),
                "h"((uint16_t)3)
                : "memory");
+}
+// a word of the peer's shared memory, at the place that it has in this CTA's
+__device__ __forceinline__ void tell_peer(const int* mine, int rank, int value) {
+  uint32_t there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(smem_addr(mine)), "r"(rank ^ 1));
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there), "r"(value) : "memory");
 }
 __device__ __forceinline__ void commit_leader(uint64_t* bar) {  // on this CTA's alone
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
@@ -385,7 +396,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   extern __shared__ char raw[];
   __shared__ __align__(8) uint64_t full[kPairStages], empty[kPairStages], sums, taken, last;
   __shared__ uint32_t tmem_slot;
-  __shared__ int gave_up;
+  __shared__ int gave_up, peer_gave_up;
+  __shared__ PairEnd end;
   char* const stages = raw + (-smem_addr(raw) & 1023u);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = (int)cluster_ctarank();
@@ -394,7 +406,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     mbar_init(&sums, 1);
     mbar_init(&taken, 16);  // the warps of both CTAs
     mbar_init(&last, 1);
-    gave_up = 0;
+    gave_up = peer_gave_up = 0;
     fence_mbar_init_cluster();
   }
   if (warp == 9) {
@@ -420,7 +432,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           const int s = n % kPairStages;
           if (n >= kPairStages) {
             producer_wait(&empty[s], (n / kPairStages - 1) & 1, &gave_up, p.l.wait);
-            if (*(volatile int*)&gave_up) goto drain;
+            if (*(volatile int*)&gave_up) goto stop;
           }
           const uint32_t at = smem_addr(stages) + s * L::kStageAt, bar = leaders(&full[s]);
           if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * L::kStage);
@@ -430,16 +442,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           tma_load_pair(at + L::kA + L::kB + L::kScales, &ws_map, k * (L::kScales / 8), feature / 128, bar);
         }
       }
-    drain:
-      // (the leader sees both CTAs' loads land before the pair ends, given up or not)
-      if (rank == 0)
-        for (int k = max(0, n - kPairStages); k < n; ++k)
-          if (!mbar_wait_bounded(&full[k % kPairStages], (k / kPairStages) & 1, p.l.wait)) gave_up = 1;
+      // the products' last arrivals at this CTA's barriers; those before were waited for
+      for (int k = drain_begin(n, kPairStages); k < n; ++k) producer_wait(&empty[k % kPairStages], (k / kPairStages) & 1, &gave_up, p.l.wait);
+    stop:
+      end.loads[rank] = n;
     }
     __syncwarp();
   } else if (warp == 9) {
     if (rank == 0 && one_lane()) {
-      int n = 0, turn = 0;
+      int n = 0, turn = 0, told = 0;
       for (int t = first; t < tiles; t += pairs, ++turn) {
         for (int k = 0; k < ktiles; ++k, ++n) {
           const int s = n % kPairStages;
@@ -471,8 +482,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           commit_pair(&empty[s]);
         }
         commit_pair(&sums);
+        ++told;
       }
     end:
+      end.multiplied = n, end.announced = told;
       // (given up, the sums are not announced: both CTAs' warps give up too and store NaN; no product runs any more when the pair ends)
       commit_leader(&last);
       if (!mbar_wait_bounded(&last, 0, p.l.wait)) gave_up = 1;
@@ -486,14 +499,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     char* const corner = stages + kPairStages * L::kStageAt + warp * L::kOut;
     constexpr int VE = 16 / sizeof(T), kCols = MINE < 256 / (int)sizeof(T) ? MINE : 256 / (int)sizeof(T);  // columns of a row on its way out
     int turn = 0;
+    Turns turns;
     for (int t = first; t < tiles; t += pairs, ++turn) {
       int token, feature;
       tile_at<NF>(p, t, token, feature);
       token += rank * 128 + (warp & 3) * 32;
       feature += (warp >> 2) * MINE;
       bool whole = false;
-      for (int tries = 0; tries < 64 && !whole; ++tries) whole = __all_sync(0xffffffffu, mbar_try_wait(&sums, turn & 1));  // (all lanes: one poll less than by way of lane 0)
-      if (!whole) whole = consumer_wait(&sums, turn & 1, &gave_up, p.l.wait);
+      if (!turns.gone) {
+        for (int tries = 0; tries < 64 && !whole; ++tries) whole = __all_sync(0xffffffffu, mbar_try_wait(&sums, turn & 1));  // (all lanes: one poll less than by way of lane 0)
+        if (!whole) whole = consumer_wait(&sums, turn & 1, &gave_up, p.l.wait);
+      }
+      whole = turns.take(whole);
       fence_after();
       __syncwarp();
       float f[MINE];
@@ -501,7 +518,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       for (int j = 0; j < MINE; j += 32) tmem_ask32(own + j, f + j);
       tmem_wait(f);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      if (lane == 0) arrive_at(taken_at);
+      if (lane == 0 && whole) arrive_at(taken_at);
       const float factor = whole ? alpha : kNaN;
       if (p.l.bias) {
 #pragma unroll
@@ -562,8 +579,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   }
   __syncthreads();
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // neither CTA's memory is used any more
+  const bool mine = *(volatile int*)&gave_up != 0;
+  if (mine && threadIdx.x == 0) tell_peer(&peer_gave_up, rank, 1);
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // neither CTA's memory is used by the other's threads any more ...
   cluster_wait();
+  // ... nor by what they started: the products have waited for all copies, the loaders and the others for all of the products' arrivals.  Where a wait gave up, that is
+  // done here, unless these waits run out too.
+  if (mine || *(volatile int*)&peer_gave_up) {
+    if (threadIdx.x == 0) {
+      tell_peer(&end.loads[rank], rank, end.loads[rank]);
+      if (rank == 0) tell_peer(&end.multiplied, rank, end.multiplied), tell_peer(&end.announced, rank, end.announced);
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    cluster_wait();
+    if (threadIdx.x == 0) {
+      for (int k = drain_begin(end.multiplied, kPairStages); k < end.multiplied; ++k)
+        if (!mbar_wait_bounded(&empty[k % kPairStages], (k / kPairStages) & 1, p.l.wait)) break;
+      if (end.announced > 0) mbar_wait_bounded(&sums, (end.announced - 1) & 1, p.l.wait);
+      for (int k = drain_begin(end.loads[0], kPairStages); rank == 0 && k < drain_end(end.loads[0], end.loads[1]); ++k) {
+        const Missing missing = missing_of(k, end.loads[0], end.loads[1]);
+        if (missing == kAnnouncement) mbar_arrive_expect_tx(&full[k % kPairStages], L::kStage);
+        if (missing == kPeersBytes) mbar_complete_tx(&full[k % kPairStages], L::kStage);
+        if (!mbar_wait_bounded(&full[k % kPairStages], (k / kPairStages) & 1, p.l.wait)) break;
+      }
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    cluster_wait();
+  }
   fence_after();
   __syncwarp();
   if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(acc), "r"(512) : "memory");
