@@ -244,8 +244,12 @@ __global__ void __launch_bounds__(kThreads, 2) linear4_kernel(const __grid_const
     whole = consumer_wait(&done, 0, &gave_up, p.wait);
   }
   __syncthreads();
+  if (*(volatile int*)&gave_up) {  // no product runs any more when memory is used anew and given back, unless this wait runs out too
+    if (threadIdx.x == 0) mbar_wait_bounded(&done, 0, p.wait);
+    __syncthreads();
+    whole = false;
+  }
   fence_after();
-  whole = whole && *(volatile int*)&gave_up == 0;
   if (warp < 4) {
     const int count = min(NT, p.tokens - n0);
     const uint32_t own = acc + ((uint32_t)warp << 21);
