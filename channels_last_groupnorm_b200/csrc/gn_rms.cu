@@ -418,8 +418,18 @@ __global__ void __launch_bounds__(THREADS, !is_four(OUT) || THREADS == 1024 ? 0 
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      scale_each(s[v], rstd);
+      // (4-bit codes: zeros behind the channels, which NaN would change; here a vector at a time, below element by element)
+      scale_each(s[v], is_four(OUT) && !RAGGED && first + v * lanes >= nvec ? 0.f : rstd);
       mul_each(s[v], w[v]);
+    }
+    if constexpr (is_four(OUT) && RAGGED) {
+      if (!(rstd < __uint_as_float(0x7f800000u))) {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+          for (int e = 0; e < VE; ++e)
+            if ((first + v * lanes) * VE + e >= p.C) s[v][e] = 0.f;
+      }
     }
     if constexpr (OUT == kPlain) {
 #pragma unroll
@@ -428,7 +438,6 @@ __global__ void __launch_bounds__(THREADS, !is_four(OUT) || THREADS == 1024 ? 0 
         if (live && i < nvec) frame.store(static_cast<Tx*>(p.y) + out_at, i, s[v]);
       }
     } else if constexpr (is_four(OUT)) {
-      // (A row whose sum is NaN has NaN for all its scales, those of the channels that fill its last unit up among them.)
       constexpr int BLOCK = OUT == kCodes4Of16 ? 16 : 32, share = BLOCK / VE;
       const TensorScale tensor(BLOCK == 16 ? p.rstd : nullptr);
       const int wide = (int)four_wide(p.C) / VE;
