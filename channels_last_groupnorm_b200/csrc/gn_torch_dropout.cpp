@@ -63,7 +63,9 @@ struct DropoutBackward : torch::autograd::Node {
     if (!ds.defined()) return out;
     const Tensor seed_tensor = has_seed ? seed_at.unpack(shared_from_this()) : Tensor();
     if (task_should_compute_output(0)) {
-      if (c10::GradMode::is_enabled()) {  // a graph of the backward is asked for: through the dispatcher, which has the mask's own gradient
+      // Through the dispatcher where a graph of the backward is asked for, as it has the mask's own gradient, and where somebody else looks at the
+      // gradient: a batch of them, a dispatch mode.
+      if (c10::GradMode::is_enabled() || !plain({&ds, &seed_tensor})) {
         out[0] = dropout_mask_handle().call(ds, p, opt(seed_tensor), seed, layer, x_type);
       } else {
         at::AutoDispatchBelowADInplaceOrView guard;
