@@ -156,7 +156,8 @@ struct RmsFunction : torch::autograd::Function<RmsFunction> {
       }
       return out;
     }
-    if (c10::GradMode::is_enabled()) {  // a graph of the backward is asked for: through the dispatcher, whose formula refuses a second derivative
+    // through the dispatcher, whose formula refuses a second derivative, where a graph of the backward is asked for or somebody else looks at the gradients
+    if (c10::GradMode::is_enabled() || !plain({&dy, &dsum, &sum, &addend, &weight, &rstd})) {
       auto [dx, ds, dw] = rms_bwd_handle().call(dy, opt(dsum), sum, opt(addend), opt(weight), rstd, offset);
       out[0] = dx;
       if (want_dsum) out[1] = sum.scalar_type() == x_type ? dx : ds;
@@ -392,7 +393,8 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
     if (!dq.defined() && !dk.defined()) return out;
     const double eps = ctx->saved_data["eps"].toDouble(), offset = ctx->saved_data["offset"].toDouble();
     const bool interleaved = ctx->saved_data["interleaved"].toBool();
-    if (c10::GradMode::is_enabled()) {  // through the dispatcher, whose formula refuses a second derivative
+    // (as in RmsFunction)
+    if (c10::GradMode::is_enabled() || !plain({&dq, &dk, &saved[0], &saved[1], &saved[2], &saved[3], &saved[4], &saved[5]})) {
       const auto& op = rotary_bwd_handle();
       if (!dq.defined()) {  // (the keys alone, in the queries' place)
         auto [gk, none, gkw, no_weight] = op.call(dk, OptTensor(), saved[1].defined() ? saved[1] : dk, OptTensor(), saved[4], saved[5], sections,
