@@ -34,10 +34,12 @@ Tensor dropout(const Tensor& x_in, const Tensor& residual_in, double p, const Te
 
 Tensor dropout_add_op(const Tensor& x, const OptTensor& residual, double p, const OptTensor& seed_at, int64_t seed, int64_t layer) {
   if (const char* why = refusal_of_dropout(x, value(residual), p, value(seed_at))) TORCH_CHECK(false, "gnb200: ", why);
+  refuse_tangents("dropout_add", {x, value(residual)});
   return dropout(x, value(residual), p, value(seed_at), seed, layer, residual.has_value() ? residual->scalar_type() : x.scalar_type());
 }
 Tensor dropout_mask_op(const Tensor& t, double p, const OptTensor& seed_at, int64_t seed, int64_t layer, at::ScalarType dtype) {
   if (const char* why = refusal_of_dropout(t, Tensor(), p, value(seed_at))) TORCH_CHECK(false, "gnb200: ", why);
+  refuse_tangents("dropout_add", {t});
   TORCH_CHECK(dtype == t.scalar_type() || dtype == at::kFloat || (t.scalar_type() == at::kFloat && dtype_code(dtype) >= 0),
               "gnb200: dtype must be that of t, or one of them float32");
   return dropout(t, Tensor(), p, value(seed_at), seed, layer, dtype);

@@ -127,22 +127,26 @@ Tensor linear(const Tensor& codes, const Tensor& scales, const Tensor& w_codes, 
 
 std::tuple<Tensor, Tensor> quantize_op(const Tensor& x, int64_t block, const OptTensor& scale) {
   if (const char* why = refusal_of_quant(x, Tensor(), Tensor(), block, value(scale))) TORCH_CHECK(false, "gnb200: ", why);
+  refuse_tangents("quantize_4bit", {x, value(scale)});
   Four f = quantize(x, Tensor(), Tensor(), 0.0, 0.0, block, value(scale), false);
   return {f.codes, f.scales};
 }
 std::tuple<Tensor, Tensor, Tensor> rms_quant_4bit_op(const Tensor& x, const OptTensor& residual, const OptTensor& weight, double eps, double offset, int64_t block,
                                                      const OptTensor& scale) {
   if (const char* why = refusal_of_quant(x, value(weight), value(residual), block, value(scale))) TORCH_CHECK(false, "gnb200: ", why);
+  refuse_tangents("rms_norm_quant_4bit", {x, value(weight), value(residual), value(scale)});
   Four f = quantize(x, value(weight), value(residual), eps, offset, block, value(scale), true);
   return {f.codes, f.scales, f.sum.defined() ? f.sum : none_of(x)};
 }
 Tensor dequantize_op(const Tensor& codes, const Tensor& scales, int64_t channels, const OptTensor& scale, at::ScalarType dtype) {
   if (const char* why = refusal_of_dequantize(codes, scales, channels, value(scale), dtype)) TORCH_CHECK(false, "gnb200: ", why);
+  refuse_tangents("dequantize_4bit", {value(scale)});
   return dequantize(codes, scales, channels, value(scale), dtype);
 }
 Tensor linear_op(const Tensor& codes, const Tensor& scales, const Tensor& w_codes, const Tensor& w_scales, const OptTensor& scale, const OptTensor& w_scale,
                  const OptTensor& bias, at::ScalarType dtype) {
   if (const char* why = refusal_of_linear(codes, scales, w_codes, w_scales, value(scale), value(w_scale), value(bias), dtype)) TORCH_CHECK(false, "gnb200: ", why);
+  refuse_tangents("linear_4bit", {value(scale), value(w_scale), value(bias)});
   return linear(codes, scales, w_codes, w_scales, value(scale), value(w_scale), value(bias), dtype);
 }
 

@@ -94,6 +94,12 @@ bool wants_graph(std::initializer_list<const Tensor*> tensors) {
 // The gradients' own gradients: an error, where an op without a formula would leave its term out.
 void refuse_second(const char* name) { TORCH_CHECK(false, "gnb200: ", name, " is differentiable once; a gradient of its gradient was asked for"); }
 
+// Tangents of forward mode: an error too, where the kernels would leave them out.
+void refuse_tangents(const char* name, std::initializer_list<Tensor> tensors) {
+  for (const Tensor& t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), "gnb200: ", name, " has no derivative in forward mode");
+}
+
 bool plain(std::initializer_list<const Tensor*> tensors) {
   if (!gnb200_ops::only_cuda_sees(tensors)) return false;
   for (const Tensor* t : tensors)

@@ -99,17 +99,20 @@ RmsGrads rms_backward(const Tensor& dy, const Tensor& dsum, const Tensor& sum, c
 }
 
 std::tuple<Tensor, Tensor, Tensor> rms_fwd_op(const Tensor& x, const OptTensor& residual, const OptTensor& weight, double eps, double offset) {
+  refuse_tangents("rms_norm", {x, value(weight), value(residual)});
   RmsOut o = rms_forward(x, value(weight), value(residual), eps, offset, true, 0, -1);
   return {o.y, o.sum.defined() ? o.sum : none_of(x), o.rstd};
 }
 std::tuple<Tensor, Tensor, Tensor> rms_bwd_op(const Tensor& dy, const OptTensor& dsum, const Tensor& sum, const OptTensor& addend,
                                               const OptTensor& weight, const Tensor& rstd, double offset) {
+  refuse_tangents("rms_norm", {dy, value(dsum), sum, value(addend), value(weight), rstd});
   RmsGrads g = rms_backward(dy, value(dsum), sum, value(addend), value(weight), rstd, offset, true, true);
   return {g.dx, g.dsum.defined() ? g.dsum : none_of(sum), g.dweight.defined() ? g.dweight : none_of(sum)};
 }
 std::tuple<Tensor, Tensor, Tensor> rms_quant_op(const Tensor& x, const OptTensor& residual, const OptTensor& weight, double eps, double offset,
                                                 int64_t block, int64_t format) {
   TORCH_CHECK(format == GNB200_E4M3 || format == GNB200_INT8, "gnb200: unknown format code ", format, " (0 e4m3, 1 int8)");
+  refuse_tangents("rms_norm_quant", {x, value(weight), value(residual)});
   RmsOut o = rms_forward(x, value(weight), value(residual), eps, offset, false, block, (int)format);
   return {o.y, o.scale, o.sum.defined() ? o.sum : none_of(x)};
 }
@@ -349,6 +352,7 @@ RotaryGrads rotary_backward(const Tensor& dq_in, const Tensor& dk_in, const Tens
 std::tuple<Tensor, Tensor> rotary_op(const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& inv_freq,
                                      at::IntArrayRef sections, const OptTensor& q_weight, const OptTensor& k_weight, double eps, double offset,
                                      bool interleaved) {
+  refuse_tangents("rotary", {q, value(k), positions, inv_freq, value(q_weight), value(k_weight)});
   auto [qo, ko] = rotary_forward(q, value(k), positions, inv_freq, sections, value(q_weight), value(k_weight), eps, offset, interleaved);
   return {qo, ko.defined() ? ko : none_of(q)};
 }
@@ -358,6 +362,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rotary_bwd_op(const Tensor& dq, const
                                                          bool interleaved) {
   if (const char* why = refusal_of_heads(dq, value(dk), positions, inv_freq, sections, value(q_weight), value(k_weight)))
     TORCH_CHECK(false, "gnb200: (gradients) ", why);
+  refuse_tangents("rotary", {dq, value(dk), q, value(k), positions, inv_freq, value(q_weight), value(k_weight)});
   RotaryGrads g = rotary_backward(dq, value(dk), q, value(k), positions, inv_freq, sections, value(q_weight), value(k_weight), eps, offset,
                                   interleaved);
   const auto filled = [&](const Tensor& t) { return t.defined() ? t : none_of(dq); };

@@ -7,7 +7,7 @@ import torch
 import torch.nn as nn
 
 from . import _native
-from .token_rows import check_rows
+from .token_rows import check_rows, refuse_tangents
 
 _dropout_add = _native.python_module.dropout_add
 
@@ -42,6 +42,7 @@ def dropout_add(x, residual=None, p=0.1, seed=0, layer=0):
     if at is not None and (at.numel() != 1 or at.dtype != torch.int64 or at.device != x.device):
         raise ValueError("dropout_add: a seed that is a tensor must have one element, int64, on the device of x, got %s %s on %s"
                          % (tuple(at.shape), at.dtype, at.device))
+    refuse_tangents("dropout_add", x, residual)
     return torch.ops.gnb200.dropout_add(x, residual, p, at, 0 if at is not None else _signed("seed", seed), _signed("layer", layer))
 
 

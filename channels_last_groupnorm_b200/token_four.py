@@ -13,7 +13,7 @@ import torch
 import torch.nn as nn
 
 from . import _native
-from .token_rows import TYPES, check_rows
+from .token_rows import TYPES, check_rows, refuse_tangents
 
 _quantize = _native.python_module.quantize_4bit
 _dequantize = _native.python_module.dequantize_4bit
@@ -37,6 +37,7 @@ def _check_block(name, block, scale, device):
 def _refuse_grad(name, *tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise ValueError("%s has no gradient: call it under torch.no_grad()" % name)
+    refuse_tangents(name, *tensors)
 
 
 def _up(n, to):

@@ -9,7 +9,7 @@ import torch.nn as nn
 
 from . import _native
 from .token_four import rms_norm_quant_4bit
-from .token_rows import check_rows
+from .token_rows import check_rows, refuse_tangents
 
 _rms_norm = _native.python_module.rms_norm
 _rms_quant = _native.python_module.rms_quant
@@ -33,6 +33,7 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6, offset=0.0):
         if out is not None:
             return out
     check_rows("rms_norm", x, weight, residual)
+    refuse_tangents("rms_norm", x, weight, residual)
     if weight is not None:
         weight = weight.contiguous()
     y, s, _ = torch.ops.gnb200.rms_fwd(x, residual, weight, float(eps), float(offset))
@@ -55,6 +56,7 @@ def rms_norm_quant(x, weight=None, residual=None, eps=1e-6, offset=0.0, block=0,
         if out is not None:
             return out
     check_rows("rms_norm_quant", x, weight, residual)
+    refuse_tangents("rms_norm_quant", x, weight, residual)
     if block not in (0, 32, 64, 128):
         raise ValueError("rms_norm_quant: block must be 0 (one scale per row), 32, 64 or 128, got %s" % (block,))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):

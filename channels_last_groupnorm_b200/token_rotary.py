@@ -8,6 +8,7 @@ import torch
 import torch.nn as nn
 
 from . import _native
+from .token_rows import refuse_tangents
 
 _rotary = _native.python_module.rotary
 _TYPES = (torch.float32, torch.float16, torch.bfloat16)
@@ -68,6 +69,7 @@ def rotary(q, k, positions, inv_freq, sections, q_weight=None, k_weight=None, ep
             return out
     sections = [int(s) for s in sections]
     _check(q, k, positions, inv_freq, sections, q_weight, k_weight)
+    refuse_tangents("rotary", q, k, positions, inv_freq, q_weight, k_weight)
     q_weight, k_weight = (w if w is None else w.contiguous() for w in (q_weight, k_weight))
     out = torch.ops.gnb200.rotary(q, k, positions, inv_freq.contiguous(), sections, q_weight, k_weight, float(eps), float(offset), bool(interleaved))
     return out[0], (None if k is None else out[1])

@@ -1,5 +1,6 @@
 """What the operators on token rows ask of their arguments."""
 import torch
+from torch.autograd import forward_ad
 
 TYPES = (torch.float32, torch.float16, torch.bfloat16)
 
@@ -23,3 +24,10 @@ def check_rows(name, x, weight, residual):
                              % (name, x.shape[-1], tuple(weight.shape), weight.device))
         if weight.dtype not in (x.dtype, torch.float32):
             raise ValueError("%s: weight must have the dtype of x or float32, got %s for %s" % (name, weight.dtype, x.dtype))
+
+
+def refuse_tangents(name, *tensors):
+    """Forward mode, torch.func.jvp too, whose wrapped tensors the ops do not see: an error where its tangents would be left out."""
+    if not torch.compiler.is_compiling() and forward_ad._current_level >= 0:
+        if any(t is not None and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+            raise NotImplementedError("%s has no derivative in forward mode" % name)
