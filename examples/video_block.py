@@ -56,8 +56,8 @@ class VideoBlock(nn.Module):
         frames, channels, height, width = like.shape
         return tokens.view(frames, height, width, channels).permute(0, 3, 1, 2)
 
-    def forward(self, maps, seed=0):
-        """seed: of the step's dropout, a number or a tensor of one int64 on the device."""
+    def forward(self, maps, seed=None):
+        """seed: of the step's dropout, a number or a tensor of one int64 on the device; training with dropout needs it."""
         positions = self.positions(maps.shape[0], maps.shape[2], maps.shape[3], maps.device)
         stream = self.tokens_of(maps)
         attended = self.out(self.attention(self.qkv(self.norm1(stream)), positions))
