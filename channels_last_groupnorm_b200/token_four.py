@@ -153,8 +153,8 @@ class Linear4bit(nn.Module):
     """Linear4bit(weight, bias=None, block=16): a trained `nn.Linear`'s weight in four bits, for serving.
 
     `forward(x, scale=None)` quantises x and multiplies; `forward((codes, scales), scale)` takes what `RMSNorm.quantize_4bit` made with the same
-    block and scale.  In blocks of 16 the weight's own scale is its largest magnitude over 6 * 448, so that the largest block scale is the
-    largest e4m3.  `dtype`: that of the result for codes (x's own for x); the weight's by default.
+    block and scale.  In blocks of 16 the weight's own scale is its largest finite magnitude over 6 * 448, so that the largest block scale is
+    the largest e4m3.  `dtype`: that of the result for codes (x's own for x); the weight's by default.
     """
 
     def __init__(self, weight, bias=None, block=16, dtype=None):
@@ -165,7 +165,9 @@ class Linear4bit(nn.Module):
         with torch.no_grad():
             scale = None
             if self.block == 16:
-                scale = (weight.abs().amax().float() / (6 * 448)).clamp_min(2.0 ** -100).reshape(1)
+                # (of the finite ones: a NaN or an infinity makes its own feature NaN, not all of them)
+                most = weight.abs().nan_to_num_(nan=0.0, posinf=0.0).amax() if weight.numel() else weight.new_zeros(())
+                scale = (most.float() / (6 * 448)).clamp_min(2.0 ** -100).reshape(1)
             codes, scales = quantize_4bit(weight.detach(), self.block, scale)
         self.register_buffer("weight_codes", codes.view(torch.uint8))  # (the packed type has neither copies nor checkpoints)
         self.register_buffer("weight_scales", scales.view(torch.uint8))

@@ -34,6 +34,42 @@ def test_compiled_module(block, bias):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("block", [16, 32])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
+def test_module_of_a_broken_weight(block, what):
+    """A NaN or an infinity among the weights makes its feature NaN and leaves the others as they are."""
+    torch.manual_seed(0)
+    weight = torch.randn(72, 200, device="cuda").bfloat16()
+    weight[9, :4] = 0.01
+    x = torch.randn(5, 200, device="cuda").bfloat16()
+    broken = weight.clone()
+    broken[9, 3] = what
+    with torch.no_grad():
+        want, got = pkg.Linear4bit(weight, block=block)(x), pkg.Linear4bit(broken, block=block)(x)
+    assert torch.isnan(got[:, 9]).all()
+    rest = torch.arange(72, device="cuda") != 9
+    assert torch.equal(got[:, rest], want[:, rest])
+
+
+@pytest.mark.parametrize("size", [2.0 ** -110, 2.0 ** -60, 2.0 ** 100])
+def test_module_of_far_weights(size):
+    """Weights far from one, down to where the weight's own scale is cut off: as near as weights of one."""
+    torch.manual_seed(0)
+    weight, x = torch.randn(72, 200, device="cuda"), torch.randn(5, 200, device="cuda")
+    with torch.no_grad():
+        near, far = pkg.Linear4bit(weight)(x).double(), pkg.Linear4bit(weight * size)(x).double() / size
+    if size < 2.0 ** -100:  # block scales have fewer bits there, but no sum is lost
+        want = x.double() @ weight.double().t()
+        assert (far - want).norm() <= 0.3 * want.norm()
+    else:
+        assert torch.equal(far, near)
+
+
+def test_module_without_features():
+    four = pkg.Linear4bit(torch.zeros(0, 200, device="cuda").bfloat16())
+    assert four(torch.ones(3, 200, device="cuda").bfloat16()).shape == (3, 0)
+
+
 def test_replay_on_another_stream():
     """A captured product follows its inputs on the stream of the replay."""
     rows, weights = torch.randn(40, 1024, device="cuda"), torch.randn(300, 1024, device="cuda")
