@@ -2,8 +2,8 @@
 // gn_four.cuh; the norm is that of gn_rms.cu: s = x + r in fp32, y = s * rsqrt(mean(s^2) + eps) * (offset + w), y not rounded before its codes).
 //
 // A lane holds 16 channels: a block of 16, or half of one of 32, whose largest magnitude a shuffle completes; 8 bytes of codes a lane; the scales
-// of four blocks become one word.  To four bits bound by HBM and instructions (10 an element): 16384 x 8192 bf16 56 us in blocks of 32, 65 of 16 (the scales' words, which go to
-// tiles of their own, take 10 of these), floor 52; back by the writes: 71 us, where filling the output alone takes 69.  The norm runs on the kernels of gn_rms.cu, which
+// of four blocks become one word.  To four bits bound by HBM and instructions (12 to 14 for 32 elements): 16384 x 8192 bf16 55 us in blocks of 32, 63 of 16 (the scales' words, which go to
+// tiles of their own, take most of the difference), floor 52; back by the writes: 71 us, where filling the output alone takes 69.  The norm runs on the kernels of gn_rms.cu, which
 // hand a row's 16-byte vectors out; here are the rows that these do not take.
 #include <algorithm>
 

@@ -5,11 +5,11 @@
 // copies of their 512-byte tiles to tensor memory, sums in tensor memory.  One thread loads, one multiplies, the others take the sums out.  Two kernels:
 //
 //   few tokens    the weight is the A operand: a tile has 128 features by all tokens up to 128, and what it costs is the weight's bytes.  Bound by HBM where the
-//                 weight is large (8 x 5120 x 20480 14.3 us, 4.1 TB/s; floor 9.1), by the way there and back where it is not (1 x 4096 x 4096 5.6 us, floor 1.4): launch,
+//                 weight is large (8 x 5120 x 20480 14.1 us, 4.2 TB/s; floor 9.1), by the way there and back where it is not (1 x 4096 x 4096 5.5 us, floor 1.4): launch,
 //                 one trip to memory, the cluster's meeting.  Where the tiles leave SMs idle, the K tiles are shared out over a cluster, whose sums are added over
 //                 distributed shared memory in the order of their ranks; the weight's first K tiles are asked into L2 while the kernel before still runs.
-//   many tokens   pairs of CTAs, 256 tokens by 256 or 128 features (below).  8192^3 226 us = 4.9 PFLOP/s in a short run, of 5.9 that the vendor's library reaches; at
-//                 length the GPU's 1000 W bound it, 262 us at 1.49 GHz (the library 217).  The products alone would take 136.
+//   many tokens   pairs of CTAs, 256 tokens by 256 or 128 features (below).  8192^3 224 us = 4.9 PFLOP/s in a short run, of 6.1 that the vendor's library reaches; at
+//                 length the GPU's 1000 W bound it, 262 us at 1.49 GHz (the library 215).  The products alone would take 136.
 #include <cuda.h>
 
 #include <algorithm>

@@ -11,8 +11,8 @@
 // the output, and the only traffic beside them is a row of partial sums per CTA in the backward.  Bound by HBM where there are rows enough:
 // 16384 x 4096 bf16 with the residual, forward 89 us = 6.0 TB/s, backward (four tensors read, one written) 107 us = 6.3 TB/s, 92 and
 // 96 % of a copy's rate; 8192 x 8192 bf16 over an fp32 stream to 8 bits 115 us = 6.4 TB/s.  A call of one row takes 2.2 us, of 8 rows in
-// 8 bits 3: launch, first load and one reduction.  With 4-bit codes (gn_four.cuh): 8192 x 8192 bf16 over an fp32 stream 117 - 120 us, bf16 alone 71 = 6.2 TB/s, 2048 x 4096
-// over fp32 18, odd rows 36 (9001 x 1111).
+// 8 bits 3: launch, first load and one reduction.  With 4-bit codes (gn_four.cuh): 8192 x 8192 bf16 over an fp32 stream 115 us in blocks of 32, 120 of 16, over bf16 73 = 6.0 TB/s, 2048 x 4096
+// over fp32 20, odd rows 36 (9001 x 1111).
 //
 // Rows of up to four vectors a lane belong to a group of lanes of one warp (shuffles only), longer ones to a CTA, or in the backward to a
 // team of warps, of which a CTA has several so that fewer partial rows are left to add up; rows longer than those (more than 16384

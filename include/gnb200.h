@@ -310,11 +310,12 @@ int gnb200_rotary_bwd(const gnb200_rotary_args* args, const void* dq, const int6
  * Codes lie in rows of ceil(C / 32) * 16 bytes (gnb200_4bit_code_bytes for all rows), zeros behind the channels whatever a row holds.  Scales lie in tiles of 512 bytes
  * for 128 rows and 4 blocks, byte (r % 32) * 16 + r % 128 / 32 * 4 + b % 4 of a tile; a row's tiles lie behind one another, then come those of the
  * next 128 rows; zeros for rows and blocks that are not there (gnb200_4bit_scale_bytes for all of them).  Codes and scales begin on 16 bytes.
- * gnb200_quantize_4bit: rows of x, x_stride elements apart.  gnb200_dequantize_4bit: contiguous rows of C values code * s * g, rounded once.
+ * gnb200_quantize_4bit: rows of x, x_stride elements apart.  gnb200_dequantize_4bit: contiguous rows of C values code * s * g in fp32, then in dtype.
  * gnb200_rms_fwd_4bit: gnb200_rms_fwd (`sum` in place as there) with its y, not rounded before, as codes and scales.  A row whose sum is NaN has a NaN for the scale
  *   of each block that holds one of its channels.
  * gnb200_linear_4bit: out[tokens][features] = sum over channels of x * w, + bias (NULL: none; any of the three types): both operands codes and scales of
- *   the same block, sums in fp32, one rounding to dtype.  It waits inside the kernel as the group norm does (bounded; see below).
+ *   the same block, sums in fp32, times the product of the two g in fp32 (2^-126 to 2^127), one rounding to dtype.  It waits inside the kernel as the
+ *   group norm does (bounded; see below).
  */
 size_t gnb200_4bit_code_bytes(int64_t rows, int64_t C);
 size_t gnb200_4bit_scale_bytes(int64_t rows, int64_t C, int block);
